@@ -389,6 +389,105 @@ int qwattn_layer_attention_qsa(qwattn_ctx* ctx, void* stream, int slot, const vo
                                const void* v, int in_dtype, const float* qn, const float* kn, float* out,
                                int pos, int n, int n_split, const uint32_t* key_bits, int kb_words);
 
+/* ---- The operators of the other layers: linear attention and experts ------------------------------------
+ * The rest of a hybrid layer stack around the projections (qwattn_mat): a linear-attention layer is
+ * qwattn_conv_silu on its projected q, k, v channels, then qwattn_delta_rule; an expert layer is
+ * qwattn_moe_route on the router's logits, then qwattn_moe. Reference dispatches: shaders/conv1d.comp,
+ * shaders/deltanet.comp, shaders/gated_norm.comp, shaders/moe_route.comp, shaders/moe_group.comp,
+ * shaders/moe_combine.comp.
+ *
+ * Calls of these four use no state of the context but its device and rms_eps, so calls on different streams
+ * may overlap as long as their states, outputs and workspaces differ. They allocate nothing, clear what they
+ * need by kernels of their own and read no device data on the host, so they can be captured into a graph;
+ * calls (or captured graphs) that may overlap need workspaces of their own. Outputs and states must not
+ * overlap inputs or each other.
+ *
+ * Sequences: n_seq of them, n rows each (row b * n + t is token t of sequence b). `lens` (device int32 [n_seq],
+ * NULL: n everywhere) shortens them: sequence b has min(max(lens[b], 0), n) tokens; rows past them are neither
+ * used nor written, and the state is that after the last token. */
+
+/* Short causal depthwise convolution with SiLU: y[t][c] = silu(bias[c] + sum_j w[c][j] x[t - taps + 1 + j][c]),
+ * rows before the first token from `state`, which then receives the last taps - 1 rows. fp32 sums, one rounding
+ * to dtype. */
+typedef struct qwattn_conv {
+    int n_seq, n;
+    int channels;         /* a multiple of 8 */
+    int taps;             /* 2, 3 or 4 */
+    int dtype;            /* of x and y: QWATTN_F32 or QWATTN_BF16 */
+    const int32_t* lens;  /* device [n_seq] or NULL */
+    const void* x;        /* [n_seq * n] rows of x_stride elements (>= channels, a multiple of 8), 16-byte aligned */
+    int64_t x_stride;
+    const float* w;       /* [channels][taps], 16-byte aligned */
+    const float* bias;    /* [channels], 16-byte aligned, or NULL */
+    float* state;         /* [n_seq][taps - 1][channels], oldest row first, 16-byte aligned */
+    float* snap;          /* NULL, or [n_seq][n][taps - 1][channels]: the state after each token (rollback of
+                             rejected drafts: copy row accepted - 1 back into the state) */
+    void* y;              /* [n_seq * n] rows of y_stride elements (as x_stride) */
+    int64_t y_stride;
+} qwattn_conv;
+int qwattn_conv_silu(qwattn_ctx* ctx, void* stream, const qwattn_conv* args);
+
+/* The gated delta rule. Per token and value head h, with its key head's q and k divided by their 2-norms
+ * (x / sqrt(sum x^2 + rms_eps); q also by sqrt(key_dim)), decay = exp(g) and a state S [key_dim][val_dim]:
+ *   S <- decay S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q
+ * with g = a and beta = b as given, or, with a_coef and dt_bias, g = a_coef[h] softplus(a + dt_bias[h]) and
+ * beta = 1 / (1 + e^-b). With z and gamma the output is o rsqrt(mean o^2 + rms_eps) gamma silu(z), else o.
+ * fp32 arithmetic (chunks of many tokens: products of fp32 accuracy on the matrix cores), one rounding to dtype.
+ * Few tokens run token by token; more run in chunks of 64 tokens whose chunk-internal part is computed for all
+ * chunks at once (that form needs the workspace). Results do not depend on timing. */
+typedef struct qwattn_delta {
+    int n_seq, n;
+    int k_heads, v_heads; /* v_heads a multiple of k_heads */
+    int key_dim, val_dim; /* 64 or 128 each */
+    int tiled;            /* value head h uses key head h / (v_heads / k_heads) (0) or h % k_heads (1) */
+    int dtype;            /* of q, k, v, z and out: QWATTN_F32 or QWATTN_BF16 */
+    const int32_t* lens;  /* device [n_seq] or NULL */
+    const void *q, *k, *v; /* rows of k_heads * key_dim (q, k) and v_heads * val_dim (v) elements at strides that are
+                              multiples of 8; 16-byte aligned */
+    int64_t q_stride, k_stride, v_stride;
+    const float *a, *b;   /* [n_seq * n][v_heads] */
+    const float *a_coef, *dt_bias; /* [v_heads], both or neither */
+    float* state;         /* [n_seq][v_heads][key_dim][val_dim], updated; 16-byte aligned */
+    float* snap;          /* NULL, or [n_seq][n][v_heads][key_dim][val_dim]: the state after each token, 16-byte
+                             aligned (runs token by token) */
+    const void* z;        /* NULL, or rows of v_heads * val_dim elements at z_stride (as v) */
+    int64_t z_stride;
+    const float* gamma;   /* [val_dim], with z */
+    void* out;            /* rows of v_heads * val_dim elements at out_stride (as v) */
+    int64_t out_stride;
+    void* workspace;      /* qwattn_delta_workspace bytes, 256-byte aligned (NULL where that is 0) */
+    size_t workspace_bytes;
+} qwattn_delta;
+int qwattn_delta_rule(qwattn_ctx* ctx, void* stream, const qwattn_delta* args);
+/* The workspace of such a call (only sizes, dtype, snap and z of *args are looked at). */
+int qwattn_delta_workspace(const qwattn_delta* args, size_t* bytes);
+
+/* The router: per row of logits[n][logits_stride] (n_experts used) the top_k largest, largest first, the lower
+ * index first among equal ones, into ids[n][top_k], and their weights[n][top_k]: the softmax over all experts,
+ * divided by the selected ones' sum when renorm != 0. A logit of -inf or NaN is no choice: a row with fewer
+ * choices than top_k ends with ids of -1 and weights of 0. n_experts <= 1024, top_k <= 64. */
+int qwattn_moe_route(qwattn_ctx* ctx, void* stream, const float* logits, int logits_stride, int n, int n_experts,
+                     int top_k, int renorm, int32_t* ids, float* weights);
+
+/* One layer's SwiGLU experts, planar Q8_0 as in qwattn_mat: gate and up int8 [n_experts][ffn][hidden] with scales
+ * [n_experts][ffn][hidden / 32], down [n_experts][hidden][ffn] with [n_experts][hidden][ffn / 32]. Device
+ * pointers, the int8 ones 16-byte aligned; hidden and ffn multiples of 32. */
+typedef struct qwattn_moe_layer {
+    int n_experts, hidden, ffn;
+    const int8_t *w_gate, *w_up, *w_down;
+    const float *s_gate, *s_up, *s_down;
+} qwattn_moe_layer;
+
+/* y[t] = sum_j weights[t][j] W_down (silu(W_gate x[t]) * (W_up x[t])) of expert ids[t][j], j < top_k <= 64. An id
+ * outside [0, n_experts) is skipped (a free place of a batch: its row of y is then zero); the same expert may
+ * occur twice. x and y are dtype (QWATTN_F32 or QWATTN_BF16) rows at strides that are multiples of 8, x 16-byte
+ * aligned; fp32 accuracy, one rounding to dtype. The result of a row does not depend on the other rows nor on
+ * timing. workspace: qwattn_moe_workspace bytes, 256-byte aligned. */
+int qwattn_moe(qwattn_ctx* ctx, void* stream, const qwattn_moe_layer* layer, const void* x, int dtype,
+               int64_t x_stride, const int32_t* ids, const float* weights, int top_k, void* y, int64_t y_stride, int n,
+               void* workspace, size_t workspace_bytes);
+int qwattn_moe_workspace(const qwattn_moe_layer* layer, int dtype, int n, int top_k, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -112,6 +112,30 @@ public:
               "qwattn_layer_attention_qsa");
     }
 
+    // The operators of linear-attention and expert layers (arguments and formulas: qwattn.h).
+    void conv_silu(void* stream, const qwattn_conv& a) { check(ctx_, qwattn_conv_silu(ctx_, stream, &a), "qwattn_conv_silu"); }
+    static size_t delta_workspace(const qwattn_delta& a) {
+        size_t bytes = 0;
+        check(nullptr, qwattn_delta_workspace(&a, &bytes), "qwattn_delta_workspace");
+        return bytes;
+    }
+    void delta_rule(void* stream, const qwattn_delta& a) { check(ctx_, qwattn_delta_rule(ctx_, stream, &a), "qwattn_delta_rule"); }
+    void moe_route(void* stream, const float* logits, int logits_stride, int n, int n_experts, int top_k, bool renorm,
+                   int32_t* ids, float* weights) {
+        check(ctx_, qwattn_moe_route(ctx_, stream, logits, logits_stride, n, n_experts, top_k, renorm ? 1 : 0, ids, weights),
+              "qwattn_moe_route");
+    }
+    static size_t moe_workspace(const qwattn_moe_layer& l, int dtype, int n, int top_k) {
+        size_t bytes = 0;
+        check(nullptr, qwattn_moe_workspace(&l, dtype, n, top_k, &bytes), "qwattn_moe_workspace");
+        return bytes;
+    }
+    void moe(void* stream, const qwattn_moe_layer& l, const void* x, int dtype, int64_t x_stride, const int32_t* ids,
+             const float* weights, int top_k, void* y, int64_t y_stride, int n, void* workspace, size_t workspace_bytes) {
+        check(ctx_, qwattn_moe(ctx_, stream, &l, x, dtype, x_stride, ids, weights, top_k, y, y_stride, n, workspace,
+                               workspace_bytes), "qwattn_moe");
+    }
+
     // Waits for `stream` and throws if a bounded in-kernel wait of an earlier decode launch gave up.
     void sync(void* stream) { check(ctx_, qwattn_sync_status(ctx_, stream), "qwattn_sync_status"); }
 

@@ -9,6 +9,7 @@ The package directory name carries a hyphen, so it is loaded by path (see load_p
 tests/conftest.py, bench.py and __graft_entry__.py) under the module name `qwattn_amd`.
 """
 import ctypes
+import functools
 import os
 import struct
 
@@ -45,6 +46,12 @@ class MatOut(ctypes.Structure):
 
 _MAT_OUT = struct.Struct("@PPI4xPIif4x")  # MatOut's layout; packing it costs a quarter of a ctypes.Structure
 assert _MAT_OUT.size == ctypes.sizeof(MatOut)
+
+
+# qwattn_conv, qwattn_delta and qwattn_moe_layer as the C ABI lays them out
+_CONV = struct.Struct("@5i4xPPqPPPPPq")
+_DELTA = struct.Struct("@8iPPPPqqqPPPPPPPqPPqPN")
+_MOE_LAYER = struct.Struct("@3i4xPPPPPP")
 
 
 _lib = None
@@ -93,6 +100,12 @@ def load_library():
         "qwattn_layer_attention_qsa": [_P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _I],
         "qwattn_decode_noalloc": [_I, _P, ctypes.POINTER(Config), _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _P, _I, _I,
                                   _I, _P, ctypes.POINTER(_I)],
+        "qwattn_conv_silu": [_P, _P, _P],
+        "qwattn_delta_rule": [_P, _P, _P],
+        "qwattn_delta_workspace": [_P, _P],
+        "qwattn_moe_route": [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P],
+        "qwattn_moe": [_P, _P, _P, _P, _I, ctypes.c_int64, _P, _P, _I, _P, ctypes.c_int64, _I, _P, ctypes.c_size_t],
+        "qwattn_moe_workspace": [_P, _I, _I, _I, _P],
         "qwattn_set_wait_limits": [_P, _I, _I],
         "qwattn_set_alloc_fault": [_P, _I],
     }
@@ -182,6 +195,31 @@ def _check_rows(t, name, width, n=None):
     if n is not None and shape[0] < n:
         raise ValueError(f"{name} has {shape[0]} rows, needs >= {n}")
     return shape[0], stride[0]
+
+
+_ROW_DT = {torch.float32: F32, torch.bfloat16: BF16}
+
+
+def _check_seq_rows(t, name, shape, dtype):
+    """Row stride of a [n_seq, n, ...] operand of the linear-attention operators: `shape`, dtype, its rows (all but the
+    first two dims) contiguous, row b * n + t at one stride."""
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    stride, inner = t.stride(), 1
+    for d in range(len(shape) - 1, 1, -1):
+        if stride[d] != inner and shape[d] != 1:
+            raise ValueError(f"{name}: the elements of a row must be contiguous, got strides {stride}")
+        inner *= shape[d]
+    row = stride[1] if shape[1] > 1 else stride[0] if shape[0] > 1 else inner
+    if shape[0] > 1 and shape[1] > 1 and stride[0] != shape[1] * row:
+        raise ValueError(f"{name}: row b * n + t must be at (b * n + t) times one stride, got strides {stride}")
+    return row
+
+
+def _check_whole(t, name, shape, dtype=torch.float32):
+    """A contiguous operand of exactly `shape` and dtype."""
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
 BLK = 32  # positions per cache block
@@ -368,6 +406,126 @@ class Attention:
         self._check(self.lib.qwattn_mat_multi(self.h, _stream(stream), bytes(mats), len(outs), int(q8), cols,
                                               x.data_ptr(), x_stride, n))
 
+    # ---- linear attention and experts -------------------------------------------------------------------
+
+    def _on_device(self, tensors, stream):
+        """The stream's handle, once every operand is known to be on this context's GPU (the device's current stream
+        where none is given)."""
+        for t in tensors:
+            if t is not None and (not t.is_cuda or t.get_device() != self.device):
+                raise ValueError(f"operands must be on cuda:{self.device}, got one on {t.device}")
+        if stream is not None:
+            return stream.cuda_stream
+        return _raw_stream(self.device) if _raw_stream else torch.cuda.current_stream(self.device).cuda_stream
+
+    def _workspace(self, size, given, stream):
+        """(address, bytes) of the caller's workspace tensor, or of one from torch's allocator, and the tensor itself,
+        which must live until the call is made."""
+        if given is not None:
+            if not given.is_contiguous():
+                raise ValueError("the workspace must be contiguous")
+            return given.data_ptr(), given.numel() * given.element_size(), given
+        if not size:
+            return 0, 0, None
+        t = torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
+        if stream is not None:
+            t.record_stream(stream)
+        return t.data_ptr(), size, t
+
+    def conv_silu(self, x, w, state, y, bias=None, lens=None, snap=None, stream=None):
+        """Short causal depthwise convolution + SiLU of x [n_seq, n, channels] into y, rows before the first from
+        state [n_seq, taps - 1, channels], which becomes the last rows; w [channels, taps], bias [channels]; lens
+        [n_seq] int32 shortens sequences; snap [n_seq, n, taps - 1, channels] gets the state after each token."""
+        if x.dtype not in _ROW_DT or len(x.shape) != 3 or len(w.shape) != 2:
+            raise ValueError(f"x must be float32 or bfloat16 [n_seq, n, channels] and w [channels, taps], got {x.dtype} "
+                             f"{tuple(x.shape)} and {tuple(w.shape)}")
+        (n_seq, n, ch), taps = x.shape, w.shape[1]
+        x_stride = _check_seq_rows(x, "x", x.shape, x.dtype)
+        y_stride = _check_seq_rows(y, "y", x.shape, x.dtype)
+        _check_whole(w, "w", (ch, taps))
+        _check_whole(state, "state", (n_seq, taps - 1, ch))
+        if bias is not None:
+            _check_whole(bias, "bias", (ch,))
+        if lens is not None:
+            _check_whole(lens, "lens", (n_seq,), torch.int32)
+        if snap is not None:
+            _check_whole(snap, "snap", (n_seq, n, taps - 1, ch))
+        s = self._on_device((x, w, state, y, bias, lens, snap), stream)
+        args = _CONV.pack(n_seq, n, ch, taps, _ROW_DT[x.dtype], _ptr(lens) or 0, x.data_ptr(), x_stride, w.data_ptr(),
+                          _ptr(bias) or 0, state.data_ptr(), _ptr(snap) or 0, y.data_ptr(), y_stride)
+        self._check(self.lib.qwattn_conv_silu(self.h, s, args))
+
+    def delta_rule(self, q, k, v, a, b, state, out, a_coef=None, dt_bias=None, z=None, gamma=None, lens=None, snap=None,
+                   tiled=False, workspace=None, stream=None):
+        """The gated delta rule over n tokens of n_seq sequences: q, k [n_seq, n, k_heads, key_dim], v, z and out
+        [n_seq, n, v_heads, val_dim] of one dtype, gates a, b [n_seq, n, v_heads], state [n_seq, v_heads, key_dim,
+        val_dim] updated in place, snap [n_seq, n, v_heads, key_dim, val_dim] the state after each token; formulas in
+        include/qwattn.h. workspace: a tensor of delta_workspace() bytes (None: from torch's allocator)."""
+        if v.dtype not in _ROW_DT or len(v.shape) != 4 or len(k.shape) != 4:
+            raise ValueError(f"k and v must be float32 or bfloat16 [n_seq, n, heads, dim], got {v.dtype}, "
+                             f"{tuple(k.shape)}, {tuple(v.shape)}")
+        n_seq, n, hv, dv = v.shape
+        hk, dk = k.shape[2], k.shape[3]
+        qk = (n_seq, n, hk, dk)
+        q_stride, k_stride = _check_seq_rows(q, "q", qk, v.dtype), _check_seq_rows(k, "k", qk, v.dtype)
+        v_stride = _check_seq_rows(v, "v", v.shape, v.dtype)
+        out_stride = _check_seq_rows(out, "out", v.shape, v.dtype)
+        z_stride = _check_seq_rows(z, "z", v.shape, v.dtype) if z is not None else 0
+        _check_whole(a, "a", (n_seq, n, hv))
+        _check_whole(b, "b", (n_seq, n, hv))
+        _check_whole(state, "state", (n_seq, hv, dk, dv))
+        for t, name, shape in ((a_coef, "a_coef", (hv,)), (dt_bias, "dt_bias", (hv,)), (gamma, "gamma", (dv,)),
+                               (snap, "snap", (n_seq, n, hv, dk, dv))):
+            if t is not None:
+                _check_whole(t, name, shape)
+        if lens is not None:
+            _check_whole(lens, "lens", (n_seq,), torch.int32)
+        s = self._on_device((q, k, v, a, b, state, out, a_coef, dt_bias, z, gamma, lens, snap, workspace), stream)
+        size = delta_workspace(n_seq, n, hk, hv, dk, dv, v.dtype, z is not None, snap is not None)
+        ws, ws_bytes, keep = self._workspace(size, workspace, stream)
+        args = _DELTA.pack(n_seq, n, hk, hv, dk, dv, int(tiled), _ROW_DT[v.dtype], _ptr(lens) or 0, q.data_ptr(),
+                           k.data_ptr(), v.data_ptr(), q_stride, k_stride, v_stride, a.data_ptr(), b.data_ptr(),
+                           _ptr(a_coef) or 0, _ptr(dt_bias) or 0, state.data_ptr(), _ptr(snap) or 0, _ptr(z) or 0,
+                           z_stride, _ptr(gamma) or 0, out.data_ptr(), out_stride, ws, ws_bytes)
+        self._check(self.lib.qwattn_delta_rule(self.h, s, args))
+
+    def moe_route(self, logits, ids, weights, renorm=True, stream=None):
+        """The top_k experts of each row of logits [n, >= n_experts] (its columns are the experts) into ids [n, top_k]
+        int32 and weights [n, top_k]: softmax weights, divided by the selected ones' sum with renorm."""
+        n, stride = _check_rows(logits, "logits", 1)
+        if len(ids.shape) != 2 or ids.shape[0] != n:
+            raise ValueError(f"ids must be [{n}, top_k], got {tuple(ids.shape)}")
+        top_k, experts = ids.shape[1], logits.shape[1]
+        _check_whole(ids, "ids", (n, top_k), torch.int32)
+        _check_whole(weights, "weights", (n, top_k))
+        s = self._on_device((logits, ids, weights), stream)
+        self._check(self.lib.qwattn_moe_route(self.h, s, logits.data_ptr(), stride if n > 1 else experts, n, experts, top_k,
+                                              int(renorm), ids.data_ptr(), weights.data_ptr()))
+
+    def moe(self, x, ids, weights, gate, up, down, y, workspace=None, stream=None):
+        """SwiGLU experts over x [n, hidden] into y: each token's ids [n, top_k] int32 (outside the experts: skipped) with
+        weights [n, top_k]; gate, up (int8 [n_experts, ffn, hidden], scales [n_experts, ffn, hidden / 32]) and down
+        ([n_experts, hidden, ffn], [n_experts, hidden, ffn / 32]) pairs. workspace as in delta_rule (moe_workspace())."""
+        w = gate[0]
+        if x.dtype not in _ROW_DT or len(x.shape) != 2 or len(ids.shape) != 2 or len(w.shape) != 3:
+            raise ValueError(f"x must be float32 or bfloat16 [n, hidden], ids [n, top_k] and gate [n_experts, ffn, hidden], "
+                             f"got {x.dtype} {tuple(x.shape)}, {tuple(ids.shape)}, {tuple(w.shape)}")
+        (n, top_k), (experts, ffn, hidden) = ids.shape, w.shape
+        for (q, s), name, r, c in ((gate, "gate", ffn, hidden), (up, "up", ffn, hidden), (down, "down", hidden, ffn)):
+            _check_whole(q, name, (experts, r, c), _I8)
+            _check_whole(s, f"{name}'s scales", (experts, r, c // 32))
+        x_stride = _check_seq_rows(x[None], "x", (1, n, hidden), x.dtype)
+        y_stride = _check_seq_rows(y[None], "y", (1, n, hidden), x.dtype)
+        _check_whole(ids, "ids", (n, top_k), torch.int32)
+        _check_whole(weights, "weights", (n, top_k))
+        s = self._on_device((x, ids, weights, *gate, *up, *down, y, workspace), stream)
+        size = moe_workspace(experts, hidden, ffn, x.dtype, n, top_k)
+        ws, ws_bytes, keep = self._workspace(size, workspace, stream)
+        layer = _MOE_LAYER.pack(experts, hidden, ffn, gate[0].data_ptr(), up[0].data_ptr(), down[0].data_ptr(),
+                                gate[1].data_ptr(), up[1].data_ptr(), down[1].data_ptr())
+        self._check(self.lib.qwattn_moe(self.h, s, layer, x.data_ptr(), _ROW_DT[x.dtype], x_stride, ids.data_ptr(),
+                                        weights.data_ptr(), top_k, y.data_ptr(), y_stride, n, ws, ws_bytes))
+
     def qsa_key_bits(self, mask, cr, pos, n, key_bits, stream=None):
         """Per-key visibility bits [n, kb_words] from a block mask [n, mask_words] (shaders/attention.comp:35-43)."""
         self._check(self.lib.qwattn_qsa_key_bits(self.h, _stream(stream), _ptr(mask), mask.shape[-1], cr, pos, n,
@@ -458,6 +616,30 @@ def decode_noalloc(cfg, qg, k, v, qn, kn, rope, kcache, vcache, kv_cap, out, pos
     if rc:
         raise QwattnError(rc, lib.qwattn_last_error(None).decode())
     return used.value
+
+
+@functools.lru_cache(maxsize=4096)
+def delta_workspace(n_seq, n, k_heads, v_heads, key_dim, val_dim, dtype, gated=False, snap=False):
+    """Bytes of workspace an Attention.delta_rule call of these sizes needs (gated: with z)."""
+    lib, size = load_library(), ctypes.c_size_t()
+    some = 256  # any address: only whether z and snap are set is looked at
+    args = _DELTA.pack(n_seq, n, k_heads, v_heads, key_dim, val_dim, 0, _ROW_DT[dtype], 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                       some if snap else 0, some if gated else 0, 0, 0, 0, 0, 0, 0)
+    rc = lib.qwattn_delta_workspace(args, ctypes.byref(size))
+    if rc:
+        raise QwattnError(rc, lib.qwattn_last_error(None).decode())
+    return size.value
+
+
+@functools.lru_cache(maxsize=4096)
+def moe_workspace(n_experts, hidden, ffn, dtype, n, top_k):
+    """Bytes of workspace an Attention.moe call of these sizes needs."""
+    lib, size = load_library(), ctypes.c_size_t()
+    rc = lib.qwattn_moe_workspace(_MOE_LAYER.pack(n_experts, hidden, ffn, 0, 0, 0, 0, 0, 0), _ROW_DT[dtype], n, top_k,
+                                  ctypes.byref(size))
+    if rc:
+        raise QwattnError(rc, lib.qwattn_last_error(None).decode())
+    return size.value
 
 
 class _DeviceArray:

@@ -290,4 +290,61 @@ __host__ __device__ constexpr unsigned gemm_s_off(int row, int j, int k, int nkb
 // Whether they stay below kFar, and below 2^32 with it added, over a tile's 256 rows and 128 tokens.
 constexpr bool gemm_offsets_fit(int cols, int x_stride) { return cols <= 1 << 22 && (127ll * x_stride + cols) * 4 < kFar; }
 
+// qwattn_conv_silu's arguments (include/qwattn.h)
+struct ConvArgs {
+    int n_seq, n, channels, taps;
+    const int32_t* lens;
+    const void* x;
+    size_t x_stride;
+    const float* w;
+    const float* bias;
+    float* state;
+    float* snap;
+    void* y;
+    size_t y_stride;
+    int tile;  // tokens a workgroup walks (set by the launcher)
+};
+hipError_t launch_conv_silu(ConvArgs a, bool bf16, hipStream_t s);
+
+// qwattn_delta_rule's (include/qwattn.h)
+struct DeltaArgs {
+    int n_seq, n, k_heads, v_heads, key_dim, val_dim, tiled;
+    float eps;
+    const int32_t* lens;
+    const void *q, *k, *v, *z;
+    size_t q_stride, k_stride, v_stride, z_stride, out_stride;
+    const float *a, *b, *a_coef, *dt_bias, *gamma;
+    float* state;
+    float* snap;
+    void* out;
+    void* ws;
+};
+// Bytes of workspace that launch_delta needs (0: none); only sizes, z and snap of `a` are looked at.
+size_t delta_workspace(const DeltaArgs& a, bool bf16);
+hipError_t launch_delta(const DeltaArgs& a, bool bf16, hipStream_t s);
+
+struct RouteArgs {
+    const float* logits;
+    int stride, n, n_experts, top_k, renorm;
+    int32_t* ids;
+    float* weights;
+};
+hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s);
+
+// qwattn_moe's (include/qwattn.h)
+struct MoeArgs {
+    int n_experts, hidden, ffn, n, top_k;
+    const int8_t *w_gate, *w_up, *w_down;
+    const float *s_gate, *s_up, *s_down;
+    const void* x;
+    size_t x_stride;
+    const int32_t* ids;
+    const float* weights;
+    void* y;
+    size_t y_stride;
+    float* h;  // workspace: [n * top_k][ffn]
+};
+size_t moe_workspace(const MoeArgs& a, bool bf16);
+hipError_t launch_moe(MoeArgs a, bool bf16, void* workspace, hipStream_t s);
+
 }  // namespace qw

@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "../../include/qwattn.h"
+#include "checks.hpp"
 #include "kernels.hpp"
 
 struct qwattn_ctx {
@@ -217,6 +218,26 @@ qw::DecodeArgs decode_args(const qwattn_ctx* c, const void* q, const void* knew,
     return a;
 }
 
+
+qw::DeltaArgs delta_args(const qwattn_delta& p, float eps) {
+    qw::DeltaArgs a{};
+    a.n_seq = p.n_seq, a.n = p.n, a.k_heads = p.k_heads, a.v_heads = p.v_heads, a.key_dim = p.key_dim;
+    a.val_dim = p.val_dim, a.tiled = p.tiled, a.eps = eps, a.lens = p.lens;
+    a.q = p.q, a.k = p.k, a.v = p.v, a.z = p.z, a.out = p.out;
+    a.q_stride = (size_t)p.q_stride, a.k_stride = (size_t)p.k_stride, a.v_stride = (size_t)p.v_stride;
+    a.z_stride = (size_t)p.z_stride, a.out_stride = (size_t)p.out_stride;
+    a.a = p.a, a.b = p.b, a.a_coef = p.a_coef, a.dt_bias = p.dt_bias, a.gamma = p.gamma;
+    a.state = p.state, a.snap = p.snap, a.ws = p.workspace;
+    return a;
+}
+
+qw::MoeArgs moe_args(const qwattn_moe_layer& l, int n, int top_k) {
+    qw::MoeArgs a{};
+    a.n_experts = l.n_experts, a.hidden = l.hidden, a.ffn = l.ffn, a.n = n, a.top_k = top_k;
+    a.w_gate = l.w_gate, a.w_up = l.w_up, a.w_down = l.w_down;
+    a.s_gate = l.s_gate, a.s_up = l.s_up, a.s_down = l.s_down;
+    return a;
+}
 
 }  // namespace
 
@@ -1116,6 +1137,74 @@ int qwattn_qsa_key_bits(qwattn_ctx* c, void* stream, const uint32_t* mask, int m
     DeviceGuard dg(c->device);
     qw::QsaKeyBitsArgs a{mask, key_bits, mask_words, kb_words, pos, n, cr};
     HIP_TRY(c, qw::launch_qsa_key_bits(a, (hipStream_t)stream));
+    return QWATTN_OK;
+}
+
+// ---- linear attention and experts (checks: checks.hpp) -------------------------------------------------
+
+int qwattn_conv_silu(qwattn_ctx* c, void* stream, const qwattn_conv* p) {
+    if (!c) return QWATTN_EINVAL;
+    qw::CheckText m;
+    if (int rc = qw::check_conv(p, m)) return fail(c, rc, "%s", m.text);
+    DeviceGuard dg(c->device);
+    const qw::ConvArgs a{p->n_seq, p->n,    p->channels, p->taps, p->lens, p->x, (size_t)p->x_stride, p->w,
+                         p->bias,  p->state, p->snap,     p->y,    (size_t)p->y_stride, 0};
+    HIP_TRY(c, qw::launch_conv_silu(a, p->dtype == QWATTN_BF16, (hipStream_t)stream));
+    return QWATTN_OK;
+}
+
+int qwattn_delta_workspace(const qwattn_delta* p, size_t* bytes) {
+    qw::CheckText m;
+    if (int rc = qw::check_delta_shape(p, m)) return fail(nullptr, rc, "%s", m.text);
+    if (!bytes) return fail(nullptr, QWATTN_EINVAL, "qwattn_delta_workspace: null pointer");
+    *bytes = qw::delta_workspace(delta_args(*p, 0.f), p->dtype == QWATTN_BF16);
+    return QWATTN_OK;
+}
+
+int qwattn_delta_rule(qwattn_ctx* c, void* stream, const qwattn_delta* p) {
+    if (!c) return QWATTN_EINVAL;
+    qw::CheckText m;
+    if (int rc = qw::check_delta_shape(p, m)) return fail(c, rc, "%s", m.text);
+    const qw::DeltaArgs a = delta_args(*p, c->cfg.rms_eps);
+    const bool bf16 = p->dtype == QWATTN_BF16;
+    if (int rc = qw::check_delta(p, qw::delta_workspace(a, bf16), m)) return fail(c, rc, "%s", m.text);
+    DeviceGuard dg(c->device);
+    HIP_TRY(c, qw::launch_delta(a, bf16, (hipStream_t)stream));
+    return QWATTN_OK;
+}
+
+int qwattn_moe_route(qwattn_ctx* c, void* stream, const float* logits, int logits_stride, int n, int n_experts,
+                     int top_k, int renorm, int32_t* ids, float* weights) {
+    if (!c) return QWATTN_EINVAL;
+    qw::CheckText m;
+    if (int rc = qw::check_route(logits, logits_stride, n, n_experts, top_k, ids, weights, m)) return fail(c, rc, "%s", m.text);
+    DeviceGuard dg(c->device);
+    HIP_TRY(c, qw::launch_moe_route({logits, logits_stride, n, n_experts, top_k, renorm, ids, weights}, (hipStream_t)stream));
+    return QWATTN_OK;
+}
+
+int qwattn_moe_workspace(const qwattn_moe_layer* l, int dtype, int n, int top_k, size_t* bytes) {
+    qw::CheckText m;
+    if (int rc = qw::check_moe_layer(l, dtype, n, top_k, m)) return fail(nullptr, rc, "%s", m.text);
+    if (!bytes) return fail(nullptr, QWATTN_EINVAL, "qwattn_moe_workspace: null pointer");
+    *bytes = qw::moe_workspace(moe_args(*l, n, top_k), dtype == QWATTN_BF16);
+    return QWATTN_OK;
+}
+
+int qwattn_moe(qwattn_ctx* c, void* stream, const qwattn_moe_layer* l, const void* x, int dtype, int64_t x_stride,
+               const int32_t* ids, const float* weights, int top_k, void* y, int64_t y_stride, int n, void* workspace,
+               size_t workspace_bytes) {
+    if (!c) return QWATTN_EINVAL;
+    qw::CheckText m;
+    if (int rc = qw::check_moe_layer(l, dtype, n, top_k, m)) return fail(c, rc, "%s", m.text);
+    qw::MoeArgs a = moe_args(*l, n, top_k);
+    const bool bf16 = dtype == QWATTN_BF16;
+    const size_t need = qw::moe_workspace(a, bf16);
+    if (int rc = qw::check_moe(l, x, dtype, x_stride, ids, weights, top_k, y, y_stride, n, workspace, workspace_bytes, need, m))
+        return fail(c, rc, "%s", m.text);
+    a.x = x, a.x_stride = (size_t)x_stride, a.ids = ids, a.weights = weights, a.y = y, a.y_stride = (size_t)y_stride;
+    DeviceGuard dg(c->device);
+    HIP_TRY(c, qw::launch_moe(a, bf16, workspace, (hipStream_t)stream));
     return QWATTN_OK;
 }
 
