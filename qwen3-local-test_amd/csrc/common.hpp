@@ -12,6 +12,10 @@ typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // buffer load/store cache policy: device scope (sc1). Such stores reach the point every XCD reads from
 // once acknowledged, and such loads never return a stale line of the local L2: partial results written by
@@ -56,7 +60,6 @@ __device__ __forceinline__ void load_vec(const void* p, size_t off, float (&x)[N
         if constexpr (N % 8 == 0) {
 #pragma unroll
             for (int i = 0; i < N; i += 8) {
-                typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
                 const u32x4 v = *reinterpret_cast<const u32x4*>(b + i);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -125,6 +128,22 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // x below about -88 (e^-x overflows, its reciprocal is 0) and to 1 above
 __device__ __forceinline__ float sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
+}
+
+// Two values as bf16, rounded: one v_cvt_pk_bf16_f32
+__device__ __forceinline__ uint32_t pk_bf16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+
+// What the bf16 pair w = pk_bf16(v0, v1) leaves of v0 (E = 0) or v1 (E = 1), exactly, in one v_dot2_f32_bf16 with
+// (-1, 0) or (0, -1) (an infinity in either makes both NaN). The pair is made opaque: as a constant the compiler
+// writes the first as the inline operand -1.0, which the instruction reads as the second.
+template <int E>
+__device__ __forceinline__ float rest_bf16(uint32_t w, float v) {
+    uint32_t m;
+    if constexpr (E == 0) asm("s_mov_b32 %0, 0xbf80" : "=s"(m));
+    else asm("s_mov_b32 %0, 0xbf800000" : "=s"(m));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, m), v, false);
 }
 
 // Compile-time loop: f(std::integral_constant<int, I>) for I = B .. E-1, each body a separate

@@ -19,7 +19,6 @@ __device__ __forceinline__ void store8(void* p, size_t i, const float (&v)[8]) {
         *reinterpret_cast<f32x4*>(f) = f32x4{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4*>(f + 4) = f32x4{v[4], v[5], v[6], v[7]};
     } else {
-        typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
         bf16x8 o;
 #pragma unroll
         for (int k = 0; k < 8; k++) o[k] = (__bf16)v[k];

@@ -25,11 +25,6 @@ namespace qw {
 
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kMatNTP = 4;  // tokens a workgroup (f32 weights)
 
 // Sum over the 64 lanes, in every lane.
@@ -227,21 +222,6 @@ __device__ __forceinline__ void split_bf16(const float (&v)[8], bf16x8& hi, bf16
 // fp32 sums), for the token counts below 16. bf16 ends at 2^-133, so the last part of an |x| below 2^-109 loses bits:
 // rows whose values are all that small keep 1.2e-6 at 2^-115 and 4e-5 at 2^-120 of their outputs, with two parts
 // 2.8e-6 and 4e-5.
-__device__ __forceinline__ uint32_t pk_bf16(float a, float b) {  // one v_cvt_pk_bf16_f32
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
-}
-
-// What the bf16 pair w = pk_bf16(v0, v1) leaves of v0 (E = 0) or v1 (E = 1), exactly, in one v_dot2_f32_bf16 with
-// (-1, 0) or (0, -1) (an infinity in either makes both NaN). The pair is made opaque: as a constant the compiler
-// writes the first as the inline operand -1.0, which the instruction reads as the second.
-template <int E>
-__device__ __forceinline__ float rest_bf16(uint32_t w, float v) {
-    uint32_t m;
-    if constexpr (E == 0) asm("s_mov_b32 %0, 0xbf80" : "=s"(m));
-    else asm("s_mov_b32 %0, 0xbf800000" : "=s"(m));
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, m), v, false);
-}
-
 // Eight int8 weights (two words) as bf16, exactly.
 __device__ __forceinline__ bf16x8 weights_bf16(uint32_t lo, uint32_t hi) {
     u32x4 w;

@@ -5,8 +5,6 @@
 
 namespace qw {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 __device__ __forceinline__ float moe_wave_sum(float x) {
     x = sum32(x);
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
