@@ -178,6 +178,8 @@ static hipError_t delta_step(const DeltaArgs& a, hipStream_t s) {
 //                                            tiles of S are then the next product's operand fragment as they stand
 //   per (sequence, chunk, value head): T, P  [part][6: the 32-token steps of each 16-token row tile that it reaches]
 //                                      five vectors: beta, and the row scales of K S, Q S and K^T U; e^(G_end)
+// Where tokens are the summed index (K^T, T, P and the X and U beside them) lane group g of a 32-token step holds the
+// tokens 4 g .. 4 g + 3 of its first 16 and of its second 16: accumulator registers again.
 constexpr int kChunk = 64, kTriFrags = 6, kVec = 320;
 
 struct DeltaWs {
@@ -193,20 +195,22 @@ struct KqUnit {
 };
 constexpr int kTpOne = 3 * kTriFrags * 1024, kTpBytes = 2 * kTpOne;
 
-// The six (or, with one part on the left, three) part products, smallest first.
+// The six (or, with one part on the left, three) part products. Those of one order of magnitude share an accumulator:
+// three short chains instead of one long one, whose steps would wait for each other (a wave has no other on its SIMD to
+// fill the gaps).
 template <int NP>
-__device__ __forceinline__ f32x4 mfma_parts(const bf16x8 (&a)[NP], const bf16x8 (&b)[3], f32x4 c) {
+__device__ __forceinline__ void mfma_parts(const bf16x8 (&a)[NP], const bf16x8 (&b)[3], f32x4 (&c)[3]) {
+    c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[2], c[2], 0, 0, 0);
+    c[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[1], c[1], 0, 0, 0);
+    c[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[0], c[0], 0, 0, 0);
     if constexpr (NP == 3) {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[2], b[0], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[1], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[2], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[0], c, 0, 0, 0);
-    } else {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[2], c, 0, 0, 0);
+        c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[1], c[2], 0, 0, 0);
+        c[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[0], c[1], 0, 0, 0);
+        c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[2], b[0], c[2], 0, 0, 0);
     }
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[1], c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[0], c, 0, 0, 0);
 }
+__device__ __forceinline__ void zero(f32x4 (&c)[3]) { c[0] = c[1] = c[2] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+__device__ __forceinline__ float sum(const f32x4 (&c)[3], int i) { return (c[2][i] + c[1][i]) + c[0][i]; }
 
 // Three bf16 parts of a pair of values, a word each.
 __device__ __forceinline__ void split3(float v0, float v1, uint32_t (&w)[3]) {
@@ -227,9 +231,29 @@ __device__ __forceinline__ void split3(const float (&v)[8], u32x4 (&w)[3]) {
 // A barrier for LDS traffic alone: loads on their way to registers stay on it.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Running sum over the 64 lanes, in 64 bits: within rows of 16 lanes, then across them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double scan_step(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xF, true);
+    return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double scan64(double x) {
+    x = scan_step<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8 (zeros shifted in)
+    x = scan_step<0x112, 0xF>(x);
+    x = scan_step<0x114, 0xF>(x);
+    x = scan_step<0x118, 0xF>(x);
+    x = scan_step<0x142, 0xA>(x);  // lane 15 of rows 0 and 2 to rows 1 and 3
+    return scan_step<0x143, 0xC>(x);  // lane 31 to rows 2 and 3
+}
+
+// Lower triangle of 4 x 4 tiles: tile t of 10 is (row, column)
+constexpr int kTriRow[12] = {0, 1, 1, 2, 2, 2, 3, 3, 3, 3, 3, 3}, kTriCol[12] = {0, 0, 1, 0, 1, 2, 0, 1, 2, 3, 3, 3};
+
 template <int DT, int DK>
 __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a, DeltaWs ws, int c0, int ncs) {
-    constexpr int NP = DT ? 1 : 3, KS = DK / 32, DPT = DK / 4, LD = 68;  // LD: row length of the 64 x 64 matrices
+    constexpr int NP = DT ? 1 : 3, KS = DK / 32, LD = 68;  // LD: row length of the 64 x 64 matrices
     typedef KqUnit<DK, NP> Unit;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     uint8_t* fk = smem;                                        // K and Q fragments
@@ -237,9 +261,11 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a, DeltaWs ws, int
     float* sA = reinterpret_cast<float*>(fq + Unit::kOne);     // A
     float* sM = sA + 64 * LD;                                  // P, then T
     float* sD = sM + 64 * LD;                                  // the inverses of A's diagonal blocks, rows of 20
-    double* sG = reinterpret_cast<double*>(sD + 4 * 16 * 20);  // G
-    float* sBeta = reinterpret_cast<float*>(sG + 64);
-    float* sRk = sBeta + 64;
+    double* sG = reinterpret_cast<double*>(sD + 4 * 16 * 20);  // of four value heads: G (log2 units), beta
+    float* sBeta = reinterpret_cast<float*>(sG + 4 * 64);
+    float* sEnd = sBeta + 4 * 64;                              // of the head at work: e^(G_i - G at its row tile's end
+    float* sSince = sEnd + 3 * 64;                             // before) and e^(that - G_j), a row a row tile 1 .. 3
+    float* sRk = sSince + 64;
     float* sRq = sRk + 64;
 
     const int cl = blockIdx.x, kh = blockIdx.y, b = blockIdx.z;
@@ -250,135 +276,171 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a, DeltaWs ws, int
     const int c = lane & 15, g = lane >> 4;
     uint8_t* kq = ws.kq + ((size_t)(b * ncs + cl) * a.k_heads + kh) * Unit::kBytes;
 
-    {  // four lanes a row: norms, parts, fragments (zeros past the last token)
-        const int row = tid >> 2, dim0 = (tid & 3) * DPT;
-        const size_t r = (size_t)b * a.n + t0 + row;
-        float k2 = 0.f, q2 = 0.f;
+    {  // DK / 8 lanes a row, 8 dims a lane: norms, parts, fragments (zeros past the last token). In the LDS a fragment's
+       // piece of row r sits at row r ^ (4 step + group): the pieces that a wave writes at once lie on different banks.
+        constexpr int LPR = DK / 8, RPP = 256 / LPR;  // lanes a row, rows a pass
+        const int d = (tid % LPR) * 8, s = d >> 5, dg = (d >> 3) & 3;
+        float k[64 / RPP][8], q[64 / RPP][8];
 #pragma unroll
-        for (int p = 0; p < DPT / 8; p++) {
-            const int d = dim0 + 8 * p;
-            float k[8] = {}, q[8] = {};
-            if (row < nt) {
-                load_vec<DT, 8>(a.k, r * a.k_stride + kh * DK + d, k);
-                load_vec<DT, 8>(a.q, r * a.q_stride + kh * DK + d, q);
+        for (int p = 0; p < 64 / RPP; p++) {
+            const size_t r = (size_t)b * a.n + t0 + min(p * RPP + tid / LPR, nt - 1);
+            load_vec<DT, 8>(a.k, r * a.k_stride + kh * DK + d, k[p]);
+            load_vec<DT, 8>(a.q, r * a.q_stride + kh * DK + d, q[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < 64 / RPP; p++) {
+            const int row = p * RPP + tid / LPR;
+            float k2 = 0.f, q2 = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if (row >= nt) k[p][e] = q[p][e] = 0.f;
+                k2 = fmaf(k[p][e], k[p][e], k2), q2 = fmaf(q[p][e], q[p][e], q2);
             }
-#pragma unroll
-            for (int e = 0; e < 8; e++) k2 = fmaf(k[e], k[e], k2), q2 = fmaf(q[e], q[e], q2);
             u32x4 kp[3], qp[3];
-            split3(k, kp), split3(q, qp);
+            split3(k[p], kp), split3(q[p], qp);
 #pragma unroll
             for (int i = 0; i < NP; i++) {
-                const int at = ((i * 4 + (row >> 4)) * KS + (d >> 5)) * 1024 + ((row & 15) + 16 * ((d >> 3) & 3)) * 16;
-                *reinterpret_cast<u32x4*>(fk + at) = kp[i];
-                *reinterpret_cast<u32x4*>(fq + at) = qp[i];
+                const int frag = ((i * 4 + (row >> 4)) * KS + s) * 1024;
+                const int at = frag + ((row & 15) + 16 * dg) * 16, sw = frag + (((row & 15) ^ (4 * s + dg)) + 16 * dg) * 16;
+                *reinterpret_cast<u32x4*>(fk + sw) = kp[i];
+                *reinterpret_cast<u32x4*>(fq + sw) = qp[i];
                 *reinterpret_cast<u32x4*>(kq + at) = kp[i];
                 *reinterpret_cast<u32x4*>(kq + Unit::kOne + at) = qp[i];
             }
-        }
-        k2 += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(k2), 0xB1, 0xF, 0xF, false));
-        k2 += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(k2), 0x4E, 0xF, 0xF, false));
-        q2 += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(q2), 0xB1, 0xF, 0xF, false));
-        q2 += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(q2), 0x4E, 0xF, 0xF, false));
-        if ((tid & 3) == 0) {
-            sRk[row] = row < nt ? rsqrtf(k2 + a.eps) : 0.f;
-            sRq[row] = (row < nt ? rsqrtf(q2 + a.eps) : 0.f) * (DK == 128 ? 0.08838834764831845f : 0.125f);
+            auto row_sum = [](float x) {  // over the row's lanes
+                x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xB1, 0xF, 0xF, false));
+                x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x4E, 0xF, 0xF, false));
+                x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x141, 0xF, 0xF, false));
+                if (LPR == 16) x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x140, 0xF, 0xF, false));
+                return x;
+            };
+            k2 = row_sum(k2), q2 = row_sum(q2);
+            if (d == 0) {
+                sRk[row] = row < nt ? rsqrtf(k2 + a.eps) : 0.f;
+                sRq[row] = (row < nt ? rsqrtf(q2 + a.eps) : 0.f) * (DK == 128 ? 0.08838834764831845f : 0.125f);
+            }
         }
     }
+    const int R = a.v_heads / a.k_heads;
+    auto head = [&](int hi) { return a.tiled ? kh + hi * a.k_heads : kh * R + hi; };
     __syncthreads();
-    // K^T: eight tokens of one dim a piece
-    for (int i = tid; i < NP * 8 * DK; i += 256) {
-        const int l = i & 63, f = i >> 6;  // f: [part][step][tile][token step]
-        const int u = f & 1, j = (f >> 1) & 1, s = (f >> 2) % KS, part = (f >> 2) / KS;
-        const int d = 8 * ((l & 15) >> 2) + 4 * j + (l & 3), t = 32 * u + 8 * (l >> 4);
-        const uint8_t* from = fk + ((part * 4 + (t >> 4)) * KS + s) * 1024 + ((t & 15) + 16 * (d >> 3)) * 16 + (d & 7) * 2;
-        u32x4 w;
+    auto frag = [&](const uint8_t* f, int part, int tile, int s) {
+        return *reinterpret_cast<const bf16x8*>(f + ((part * 4 + tile) * KS + s) * 1024 + ((c ^ (4 * s + g)) + 16 * g) * 16);
+    };
+    // K^T of the row tile `wave`, by products with the unit matrix (exact): its accumulators hold four tokens of a dim
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            w[e] = *reinterpret_cast<const uint16_t*>(from + 32 * e) |
-                   (uint32_t)*reinterpret_cast<const uint16_t*>(from + 32 * e + 16) << 16;
-        *reinterpret_cast<u32x4*>(kq + 2 * Unit::kOne + f * 1024 + l * 16) = w;
-    }
-    // K K^T and Q K^T, wave w the row tile w
-    f32x4 kk[4], qk[4];
-    static_for<0, 4>([&](auto j_) {
-        constexpr int j = j_;
-        if (j <= wave) {
-            kk[j] = qk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 2; j++) {
+        bf16x8 unit;
+#pragma unroll
+        for (int e = 0; e < 8; e++) unit[e] = 8 * g + e == 8 * (c >> 2) + 4 * j + (c & 3) ? (__bf16)1.f : (__bf16)0.f;
+#pragma unroll
+        for (int p = 0; p < NP; p++)
 #pragma unroll
             for (int s = 0; s < KS; s++) {
-                bf16x8 ak[NP], aq[NP], bk[3];
+                const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+                const f32x4 v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(fk, p, wave, s), unit, z, 0, 0, 0);
+                *reinterpret_cast<u32x2*>(kq + 2 * Unit::kOne + (((p * KS + s) * 2 + j) * 2 + (wave >> 1)) * 1024 + lane * 16 +
+                                          (wave & 1) * 8) = u32x2{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
+            }
+    }
+    // K K^T and Q K^T: tiles wave, wave + 4, wave + 8 of the lower triangle's ten
+    f32x4 kk[3], qk[3];
 #pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    ak[p] = *reinterpret_cast<const bf16x8*>(fk + ((p * 4 + wave) * KS + s) * 1024 + lane * 16);
-                    aq[p] = *reinterpret_cast<const bf16x8*>(fq + ((p * 4 + wave) * KS + s) * 1024 + lane * 16);
-                    bk[p] = *reinterpret_cast<const bf16x8*>(fk + ((p * 4 + j) * KS + s) * 1024 + lane * 16);
-                }
-                if constexpr (NP == 3) {
-                    kk[j] = mfma_parts<3>(ak, bk, kk[j]);
-                    qk[j] = mfma_parts<3>(aq, bk, qk[j]);
-                } else {
-                    kk[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ak[0], bk[0], kk[j], 0, 0, 0);
-                    qk[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(aq[0], bk[0], qk[j], 0, 0, 0);
-                }
+    for (int m = 0; m < 3; m++) {
+        const int ti = kTriRow[wave + 4 * m], tj = kTriCol[wave + 4 * m];
+        kk[m] = qk[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (wave + 4 * m >= 10) break;
+        f32x4 ck[3], cq[3];
+        zero(ck), zero(cq);
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            bf16x8 ak[NP], aq[NP], bk[3];
+#pragma unroll
+            for (int p = 0; p < NP; p++) ak[p] = frag(fk, p, ti, s), aq[p] = frag(fq, p, ti, s), bk[p] = frag(fk, p, tj, s);
+            if constexpr (NP == 3) {
+                mfma_parts<3>(ak, bk, ck);
+                mfma_parts<3>(aq, bk, cq);
+            } else {
+                ck[s % 3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ak[0], bk[0], ck[s % 3], 0, 0, 0);
+                cq[s % 3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(aq[0], bk[0], cq[s % 3], 0, 0, 0);
             }
         }
-    });
+#pragma unroll
+        for (int i = 0; i < 4; i++) kk[m][i] = sum(ck, i), qk[m][i] = sum(cq, i);
+    }
 
-    const int R = a.v_heads / a.k_heads;
 #pragma unroll 1
     for (int hi = 0; hi < R; hi++) {
-        const int h = a.tiled ? kh + hi * a.k_heads : kh * R + hi;
-        const size_t unit = (size_t)(b * ncs + cl) * a.v_heads + h;
-        if (wave == 0) {  // lane: token. G in 64 bits (its differences are what counts), each g at least -2000 (e^g is 0
-                          // from -104 on; a sum of -inf would have no differences)
-            const size_t r = (size_t)b * a.n + t0 + lane;
-            const bool in = lane < nt;
-            double G = in ? (double)fmaxf(delta_log_decay(a, r, h), -2000.f) : 0.0;
-            const float beta = in ? delta_beta(a, r, h) : 0.f;
-#pragma unroll
-            for (int s = 1; s < 64; s *= 2) {
-                const double up = __shfl_up(G, s);
-                if (lane >= s) G += up;
+        const int slot = hi & 3;
+        const size_t unit = (size_t)(b * ncs + cl) * a.v_heads + head(hi);
+        if (slot == 0) {  // the gates of the next four heads, a wave a head, a lane a token. G in 64 bits (its differences
+                          // are what counts), each g at least -2000 (e^g is 0 from -104 on; sums of -inf have none)
+            if (hi + wave < R) {
+                const int h = head(hi + wave);
+                const size_t r = (size_t)b * a.n + t0 + min(lane, nt - 1);
+                const float lg = fmaxf(delta_log_decay(a, r, h), -2000.f), be = delta_beta(a, r, h);
+                const double G = scan64(lane < nt ? (double)lg * 1.4426950408889634074 : 0.0);
+                const uint64_t u = __builtin_bit_cast(uint64_t, G);
+                const double end = __builtin_bit_cast(
+                    double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), 63) << 32 |
+                                (uint32_t)__builtin_amdgcn_readlane((int)u, 63));
+                const float beta = lane < nt ? be : 0.f, since = exp2_fast((float)G), rk = sRk[lane];
+                sG[wave * 64 + lane] = G, sBeta[wave * 64 + lane] = beta;
+                float* v = ws.vec + ((size_t)(b * ncs + cl) * a.v_heads + h) * kVec + lane;
+                v[0] = beta;
+                v[64] = beta * since * rk;
+                v[128] = sRq[lane] * since;
+                v[192] = rk * exp2_fast((float)(end - G));
+                if (lane == 0) v[256] = exp2_fast((float)end);
             }
-            const double end = __shfl(G, 63);
-            const float since = expf((float)G), rk = sRk[lane];
-            sG[lane] = G, sBeta[lane] = beta;
-            float* v = ws.vec + unit * kVec + lane;
-            v[0] = beta;
-            v[64] = beta * since * rk;
-            v[128] = sRq[lane] * since;
-            v[192] = rk * expf((float)(end - G));
-            if (lane == 0) v[256] = expf((float)end);
+            __syncthreads();
+        }
+        {  // decays over more than a tile are a product of two, through the end of the tile before the row's
+            const double* G = sG + slot * 64;
+            if (wave < 3) sEnd[wave * 64 + lane] = lane < 16 * (wave + 1) ? exp2_fast((float)(G[16 * wave + 15] - G[lane])) : 0.f;
+            else sSince[lane] = lane < 16 ? 0.f : exp2_fast((float)(G[lane] - G[(lane & 48) - 1]));
         }
         __syncthreads();
-        static_for<0, 4>([&](auto j_) {
-            constexpr int j = j_;
-            const int col = 16 * j + c;
-            if (j <= wave) {
-                const double Gj = sG[col];
+        {
+            const double* G = sG + slot * 64;
+#pragma unroll
+            for (int m = 0; m < 3; m++) {
+                const int ti = kTriRow[wave + 4 * m], tj = kTriCol[wave + 4 * m];
+                if (wave + 4 * m >= 10) break;
+                const int col = 16 * tj + c, row0 = 16 * ti + 4 * g;
                 const float rkj = sRk[col];
+                const f32x4 be = *reinterpret_cast<const f32x4*>(sBeta + slot * 64 + row0);
+                const f32x4 rk = *reinterpret_cast<const f32x4*>(sRk + row0), rq = *reinterpret_cast<const f32x4*>(sRq + row0);
+                f32x4 d;
+                if (ti == tj) {
+                    const double Gj = G[col];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) d[i] = 4 * g + i >= c ? exp2_fast((float)(G[row0 + i] - Gj)) * rkj : 0.f;
+                } else {
+                    const f32x4 since = *reinterpret_cast<const f32x4*>(sSince + row0);
+                    const float e = sEnd[(ti - 1) * 64 + col] * rkj;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) d[i] = since[i] * e;
+                }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int row = 16 * wave + 4 * g + i;
-                    const float d = row >= col ? expf((float)(sG[row] - Gj)) * rkj : 0.f;
-                    sA[row * LD + col] = row > col ? sBeta[row] * sRk[row] * d * kk[j][i] : 0.f;
-                    sM[row * LD + col] = sRq[row] * d * qk[j][i];
+                    sA[(row0 + i) * LD + col] = ti > tj || 4 * g + i > c ? be[i] * rk[i] * d[i] * kk[m][i] : 0.f;
+                    sM[(row0 + i) * LD + col] = rq[i] * d[i] * qk[m][i];
                 }
-            } else if (j == wave + 1 && (wave & 1) == 0) {  // read as zeros by the row tile's 32-token step
+                if (ti == tj && (tj & 1))  // the tile above, read as zeros by its row tile's 32-token step
 #pragma unroll
-                for (int i = 0; i < 4; i++) sM[(16 * wave + 4 * g + i) * LD + col] = 0.f;
+                    for (int i = 0; i < 4; i++) sM[(row0 - 16 + i) * LD + col] = 0.f;
             }
-        });
+        }
         __syncthreads();
         uint8_t* tp = ws.tp + unit * kTpBytes;
         auto write_frags = [&](uint8_t* to) {
             for (int i = tid; i < kTriFrags * 64; i += 256) {
                 const int f = i >> 6, l = i & 63;
                 const int tile = f < 2 ? f : 1 + (f >> 1), step = f < 2 ? 0 : f & 1;
-                const float* from = sM + (16 * tile + (l & 15)) * LD + 32 * step + 8 * (l >> 4);
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = from[e];
+                const float* from = sM + (16 * tile + (l & 15)) * LD + 32 * step + 4 * (l >> 4);
+                const f32x4 v0 = *reinterpret_cast<const f32x4*>(from), v1 = *reinterpret_cast<const f32x4*>(from + 16);
+                const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
                 u32x4 w[3];
                 split3(v, w);
 #pragma unroll
@@ -440,11 +502,13 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a, DeltaWs ws, int
 
 template <int DT, int DK>
 constexpr size_t prep_lds() {
-    return 2 * KqUnit<DK, DT ? 1 : 3>::kOne + (2 * 64 * 68 + 4 * 16 * 20 + 3 * 64) * 4 + 64 * 8;
+    return 2 * KqUnit<DK, DT ? 1 : 3>::kOne + (2 * 64 * 68 + 4 * 16 * 20 + (4 + 3 + 1 + 2) * 64) * 4 + 4 * 64 * 8;
 }
 
+// Waves 0 .. 3 carry the state: row tile w of X and U, dims 32 w .. of S. Waves 4 .. 7, beside them on the same SIMDs,
+// compute and store the row tiles of the output, which nothing waits for.
 template <int DT, int DK, int DV, bool O32>  // O32: the output goes to the workspace, for the gated norm
-__global__ __launch_bounds__(256) void k_delta_chunks(DeltaArgs a, DeltaWs ws, int c0, int ncs) {
+__global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, int c0, int ncs) {
     constexpr int NP = DT ? 1 : 3, KS = DK / 32;
     typedef KqUnit<DK, NP> Unit;
     __shared__ __attribute__((aligned(16))) uint8_t sS[KS][3][1024], sX[2][3][1024], sU[2][3][1024], sW[2][3][1024];
@@ -454,168 +518,189 @@ __global__ __launch_bounds__(256) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
     const int len = a.lens ? min(max(a.lens[b], 0), a.n) : a.n;
     const int nc = min(ncs, (len + kChunk - 1) / kChunk - c0);
     if (nc <= 0) return;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const int c = lane & 15, g = lane >> 4, col = 16 * slice + c;
+    const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wave8 & 3, lane = threadIdx.x & 63;
+    const int c = lane & 15, g = lane >> 4;
     const int tok = 16 * wave + 4 * g;  // this lane's four tokens of a chunk
     const size_t row0 = (size_t)b * a.n + (size_t)c0 * kChunk;
     const int left = len - c0 * kChunk;
 
+    // A chunk's operands: each is loaded again for the next chunk right after its last use. Addresses are a uniform base
+    // that moves on by a chunk and a lane offset; no load is conditional (a wave without an operand loads one of
+    // another's), so that no branch waits for loads.
+    const uint32_t lane16 = lane * 16;
+    const size_t kq_step = (size_t)a.k_heads * Unit::kBytes, tp_step = (size_t)a.v_heads * kTpBytes, vec_step = (size_t)a.v_heads * kVec * 4;
+    const uint8_t* kq = ws.kq + ((size_t)b * ncs * a.k_heads + kh) * Unit::kBytes;
+    const uint8_t* tp = ws.tp + ((size_t)b * ncs * a.v_heads + h) * kTpBytes;
+    const uint8_t* vec = reinterpret_cast<const uint8_t*>(ws.vec + ((size_t)b * ncs * a.v_heads + h) * kVec);
+    auto frag = [&](const uint8_t* p) { return *reinterpret_cast<const bf16x8*>(p + lane16); };
+    auto vec4 = [&](int which) { return *reinterpret_cast<const f32x4*>(vec + 256 * which + (uint32_t)tok * 4); };
+    bf16x8 fR[KS][NP], fM[2][3];  // K and T, or Q and P
+    auto load_rows = [&](const uint8_t* p) {
+        p += wave * (KS * 1024);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int i = 0; i < NP; i++) fR[s][i] = frag(p + (i * 4 * KS + s) * 1024);
+    };
+    const int f0 = wave < 2 ? wave : 2 * (wave - 1), f1 = wave < 2 ? f0 : f0 + 1;  // this row tile's two steps
+    auto load_tri = [&](const uint8_t* p) {
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            fM[0][i] = frag(p + (i * kTriFrags + f0) * 1024);
+            fM[1][i] = frag(p + (i * kTriFrags + f1) * 1024);
+        }
+    };
+    auto get = [&](const uint8_t (&from)[3][1024], bf16x8 (&b)[3]) {
+#pragma unroll
+        for (int p = 0; p < 3; p++) b[p] = frag(from[p]);
+    };
+    auto rows_times_state = [&](f32x4 (&acc)[3]) {
+        zero(acc);
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            bf16x8 bs[3];
+            get(sS[s], bs);
+            mfma_parts<NP>(fR[s], bs, acc);
+        }
+    };
+    auto tri_times = [&](const uint8_t (&from)[2][3][1024], f32x4 (&acc)[3]) {
+        bf16x8 bx[3];
+        get(from[0], bx);
+        mfma_parts<3>(fM[0], bx, acc);
+        if (wave >= 2) {
+            get(from[1], bx);
+            mfma_parts<3>(fM[1], bx, acc);
+        }
+    };
+
+    if (wave8 >= 4) {
+        f32x4 vq, acc[3];
+        const size_t stride = O32 ? (size_t)a.v_heads * DV : a.out_stride;
+        size_t first = row0 * stride + h * DV + 16 * slice, at[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) at[i] = (tok + i) * stride + c;
+        load_rows(kq + Unit::kOne), load_tri(tp + kTpOne), vq = vec4(2);
+#pragma unroll 1
+        for (int ch = 0; ch < nc; ch++) {
+            if (ch + 1 < nc) kq += kq_step, tp += tp_step, vec += vec_step;
+            lds_barrier();
+            rows_times_state(acc);
+            load_rows(kq + Unit::kOne);
+            f32x4 qs;
+#pragma unroll
+            for (int i = 0; i < 4; i++) qs[i] = vq[i] * sum(acc, i);
+            lds_barrier();
+            vq = vec4(2);
+            zero(acc);
+            acc[0] = qs;
+            lds_barrier();
+            tri_times(sU, acc);
+            load_tri(tp + kTpOne);
+            const int more = left - ch * kChunk - tok;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i < more) {
+                    if constexpr (O32) ws.o[first + at[i]] = sum(acc, i);
+                    else store_out<DT>(a.out, first + at[i], sum(acc, i));
+                }
+            first += kChunk * stride;
+        }
+        return;
+    }
+
     f32x4 S[2];  // wave < KS: tile j, register i: dim 32 wave + 8 g + 4 j + i
-    float* state = a.state + ((size_t)b * a.v_heads + h) * (DK * DV) + col;
+    float* state = a.state + ((size_t)b * a.v_heads + h) * (DK * DV) + 16 * slice + c;
     if (wave < KS)
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
             for (int i = 0; i < 4; i++) S[j][i] = state[(32 * wave + 8 * g + 4 * j + i) * DV];
-
-    // a chunk's operands: each is loaded again for the next chunk right after its last use
-    bf16x8 fK[KS][NP], fQ[KS][NP], fKT[4][NP], fT[2][3], fP[2][3];
-    f32x4 vb, vk, vq, vw;
+    bf16x8 fKT[4][NP];
+    f32x4 vb, vk, vw;
     float end;
     uint32_t val[4];  // values as they lie in memory: nothing waits for them here
-    auto kq = [&](int ch) { return ws.kq + ((size_t)(b * ncs + ch) * a.k_heads + kh) * Unit::kBytes + lane * 16; };
-    auto tp = [&](int ch) { return ws.tp + ((size_t)(b * ncs + ch) * a.v_heads + h) * kTpBytes + lane * 16; };
-    auto vec = [&](int ch) { return ws.vec + ((size_t)(b * ncs + ch) * a.v_heads + h) * kVec; };
-    auto frag = [](const uint8_t* p) { return *reinterpret_cast<const bf16x8*>(p); };
-    auto load_kq = [&](int ch) {
-        const uint8_t* p = kq(ch);
+    size_t first = row0 * a.v_stride + h * DV + 16 * slice, at[4];
 #pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int i = 0; i < NP; i++) {
-                fK[s][i] = frag(p + ((i * 4 + wave) * KS + s) * 1024);
-                fQ[s][i] = frag(p + Unit::kOne + ((i * 4 + wave) * KS + s) * 1024);
-            }
-    };
-    // (no load is conditional: a wave without an operand loads one of another's, so that no branch waits for loads)
-    auto load_kt = [&](int ch) {
-        const uint8_t* p = kq(ch) + 2 * Unit::kOne;
+    for (int i = 0; i < 4; i++) at[i] = (tok + i) * a.v_stride + c;
+    auto load_kt = [&] {
+        const uint8_t* p = kq + 2 * Unit::kOne + wave % KS * 4096;
 #pragma unroll
         for (int f = 0; f < 4; f++)
 #pragma unroll
-            for (int i = 0; i < NP; i++) fKT[f][i] = frag(p + ((i * KS + wave % KS) * 4 + f) * 1024);
-    };
-    const int f0 = wave < 2 ? wave : 2 * (wave - 1), f1 = wave < 2 ? f0 : f0 + 1;  // this row tile's two steps
-    auto load_tri = [&](bf16x8 (&to)[2][3], const uint8_t* p) {
-#pragma unroll
-        for (int i = 0; i < 3; i++) {
-            to[0][i] = frag(p + (i * kTriFrags + f0) * 1024);
-            to[1][i] = frag(p + (i * kTriFrags + f1) * 1024);
-        }
+            for (int i = 0; i < NP; i++) fKT[f][i] = frag(p + (i * KS * 4 + f) * 1024);
+        vw = vec4(3);
+        end = *reinterpret_cast<const float*>(vec + 1024);
     };
     auto load_x = [&](int ch) {
-        vb = *reinterpret_cast<const f32x4*>(vec(ch) + tok);
-        vk = *reinterpret_cast<const f32x4*>(vec(ch) + 64 + tok);
+        vb = vec4(0), vk = vec4(1);
+        const int most = left - 1 - ch * kChunk;
+        if (most < kChunk - 1)  // past the last row: that one (beta is 0 there)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const size_t at = (row0 + min(ch * kChunk + tok + i, left - 1)) * a.v_stride + h * DV + col;
-            val[i] = DT ? static_cast<const uint16_t*>(a.v)[at] : static_cast<const uint32_t*>(a.v)[at];
-        }
+            for (int i = 0; i < 4; i++) at[i] = min(tok + i, most) * a.v_stride + c;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            val[i] = DT ? static_cast<const uint16_t*>(a.v)[first + at[i]] : static_cast<const uint32_t*>(a.v)[first + at[i]];
     };
-    auto load_o = [&](int ch) { vq = *reinterpret_cast<const f32x4*>(vec(ch) + 128 + tok); };
-    auto load_u = [&](int ch) {
-        vw = *reinterpret_cast<const f32x4*>(vec(ch) + 192 + tok);
-        end = vec(ch)[256];
-    };
-    load_kq(0), load_x(0), load_tri(fT, tp(0)), load_u(0), load_kt(0), load_o(0), load_tri(fP, tp(0) + kTpOne);
-
     auto put_state = [&] {
         if (KS == 4 || wave < KS) {
             const float v[8] = {S[0][0], S[0][1], S[0][2], S[0][3], S[1][0], S[1][1], S[1][2], S[1][3]};
             u32x4 w[3];
             split3(v, w);
 #pragma unroll
-            for (int p = 0; p < 3; p++) *reinterpret_cast<u32x4*>(sS[wave][p] + lane * 16) = w[p];
+            for (int p = 0; p < 3; p++) *reinterpret_cast<u32x4*>(sS[wave][p] + lane16) = w[p];
         }
     };
-    // four tokens of a column as the halves of a right operand's fragments (k: 32 tokens, column c)
-    const int put_at = (c + 16 * (2 * (wave & 1) + (g >> 1))) * 16 + (g & 1) * 8;
+    // four tokens of a column: half of a right operand's piece
     auto put_rows = [&](uint8_t (&to)[2][3][1024], const f32x4 v) {
         uint32_t lo[3], hi[3];
         split3(v[0], v[1], lo), split3(v[2], v[3], hi);
 #pragma unroll
-        for (int p = 0; p < 3; p++) *reinterpret_cast<u32x2*>(to[wave >> 1][p] + put_at) = u32x2{lo[p], hi[p]};
+        for (int p = 0; p < 3; p++)
+            *reinterpret_cast<u32x2*>(to[wave >> 1][p] + lane16 + (wave & 1) * 8) = u32x2{lo[p], hi[p]};
     };
-    auto get = [&](const uint8_t (&from)[3][1024], bf16x8 (&b)[3]) {
-#pragma unroll
-        for (int p = 0; p < 3; p++) b[p] = frag(from[p] + lane * 16);
-    };
+    load_rows(kq), load_x(0), load_tri(tp), load_kt();
     put_state();
 #pragma unroll 1
     for (int ch = 0; ch < nc; ch++) {
-        const int next = min(ch + 1, nc - 1);
+        if (ch + 1 < nc) kq += kq_step, tp += tp_step, vec += vec_step, first += kChunk * a.v_stride;
         lds_barrier();  // S is in the LDS
-        f32x4 ks[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, qs[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        f32x4 acc[3], x, w;
+        rows_times_state(acc);
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            bf16x8 bs[3];
-            get(sS[s], bs);
-            ks[s & 1] = mfma_parts<NP>(fK[s], bs, ks[s & 1]);
-            qs[s & 1] = mfma_parts<NP>(fQ[s], bs, qs[s & 1]);
-        }
-        load_kq(next);
-        f32x4 x;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float v = ch * kChunk + tok + i < left ? __uint_as_float(DT ? val[i] << 16 : val[i]) : 0.f;
-            x[i] = vb[i] * v - vk[i] * (ks[0][i] + ks[1][i]);
-        }
+        for (int i = 0; i < 4; i++) x[i] = vb[i] * __uint_as_float(DT ? val[i] << 16 : val[i]) - vk[i] * sum(acc, i);
         put_rows(sX, x);
-        load_x(next);
+        load_rows(kq), load_x(min(ch + 1, nc - 1));
         lds_barrier();  // X
-        f32x4 u = {0.f, 0.f, 0.f, 0.f};
-        {
-            bf16x8 bx[3];
-            get(sX[0], bx);
-            u = mfma_parts<3>(fT[0], bx, u);
-            if (wave >= 2) {
-                get(sX[1], bx);
-                u = mfma_parts<3>(fT[1], bx, u);
-            }
-        }
-        load_tri(fT, tp(next));
-        f32x4 w;
+        zero(acc);
+        tri_times(sX, acc);
+        load_tri(tp);
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = vw[i] * u[i];
+        for (int i = 0; i < 4; i++) x[i] = sum(acc, i), w[i] = vw[i] * x[i];
         put_rows(sW, w);
-        put_rows(sU, u);
+        put_rows(sU, x);
         lds_barrier();  // U, and with the scales of K^T's columns
         if (KS == 4 || wave < KS) {
-            bf16x8 bw[3];
+            f32x4 s[2][3];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                zero(s[j]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[j][0][i] = S[j][i] * end;
+            }
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                bf16x8 bw[3];
+                get(sW[st], bw);
+#pragma unroll
+                for (int j = 0; j < 2; j++) mfma_parts<NP>(fKT[2 * j + st], bw, s[j]);
+            }
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) S[j][i] *= end;
-#pragma unroll
-            for (int st = 0; st < 2; st++) {
-                get(sW[st], bw);
-#pragma unroll
-                for (int j = 0; j < 2; j++) S[j] = mfma_parts<NP>(fKT[2 * j + st], bw, S[j]);
-            }
+                for (int i = 0; i < 4; i++) S[j][i] = sum(s[j], i);
             put_state();  // (every wave has read the one before: it passed the barrier behind X)
         }
-        load_u(next), load_kt(next);
-        f32x4 o;
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = vq[i] * (qs[0][i] + qs[1][i]);
-        {
-            bf16x8 bu[3];
-            get(sU[0], bu);
-            o = mfma_parts<3>(fP[0], bu, o);
-            if (wave >= 2) {
-                get(sU[1], bu);
-                o = mfma_parts<3>(fP[1], bu, o);
-            }
-        }
-        load_o(next), load_tri(fP, tp(next) + kTpOne);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int t = ch * kChunk + tok + i;
-            if (t < left) {
-                if constexpr (O32) ws.o[((row0 + t) * a.v_heads + h) * DV + col] = o[i];
-                else store_out<DT>(a.out, (row0 + t) * a.out_stride + h * DV + col, o[i]);
-            }
-        }
+        load_kt();
     }
     if (wave < KS)
 #pragma unroll
@@ -688,8 +773,8 @@ static hipError_t delta_chunks(const DeltaArgs& a, hipStream_t s) {
         const int ncs = std::min(seg, nc - c0);
         k_delta_prep<DT, DK><<<dim3(ncs, a.k_heads, a.n_seq), 256, lds, s>>>(a, ws, c0, ncs);
         const int grid = a.v_heads * a.n_seq * (DV / 16);
-        if (a.z) k_delta_chunks<DT, DK, DV, true><<<grid, 256, 0, s>>>(a, ws, c0, ncs);
-        else k_delta_chunks<DT, DK, DV, false><<<grid, 256, 0, s>>>(a, ws, c0, ncs);
+        if (a.z) k_delta_chunks<DT, DK, DV, true><<<grid, 512, 0, s>>>(a, ws, c0, ncs);
+        else k_delta_chunks<DT, DK, DV, false><<<grid, 512, 0, s>>>(a, ws, c0, ncs);
     }
     if (a.z) {
         const size_t rows = (size_t)a.n_seq * a.n * a.v_heads;
