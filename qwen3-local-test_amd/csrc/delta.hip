@@ -252,7 +252,7 @@ __device__ __forceinline__ double scan64(double x) {
 constexpr int kTriRow[12] = {0, 1, 1, 2, 2, 2, 3, 3, 3, 3, 3, 3}, kTriCol[12] = {0, 0, 1, 0, 1, 2, 0, 1, 2, 3, 3, 3};
 
 template <int DT, int DK>
-__global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a, DeltaWs ws, int c0, int ncs) {
+__global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, int c0, int ncs) {
     constexpr int NP = DT ? 1 : 3, KS = DK / 32, LD = 68;  // LD: row length of the 64 x 64 matrices
     typedef KqUnit<DK, NP> Unit;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];

@@ -176,12 +176,14 @@ struct MoeTile {
 struct MoeWs {
     int* n_tiles;
     MoeTile* tiles;
-    int *row_pair, *pair_row;  // sorted row -> pair, pair -> sorted row (-1: no expert)
+    int *row_tok, *pair_row;   // sorted row -> token, pair -> sorted row (-1: no expert)
+    float* row_weight;         // sorted row -> its pair's weight
     int *x_shift, *h_shift;    // powers of two of the operand rows
     f16 *x16, *h16;            // operands [part][row][columns up to a multiple of 64]
     size_t x_part, h_part;     // elements of a part
     float* h;                  // [row][ffn]
     float* y;                  // [row][hidden]
+    int max_tiles;             // room in tiles
 };
 
 // One workgroup.
@@ -215,7 +217,8 @@ __global__ __launch_bounds__(1024) void k_moe_group(MoeArgs a, MoeWs ws, int bm)
         int r = -1;
         if (e >= 0 && e < a.n_experts) {
             r = atomicAdd(&count[e], 1);
-            ws.row_pair[r] = i;
+            ws.row_tok[r] = i / a.top_k;
+            ws.row_weight[r] = a.weights[i];
         }
         ws.pair_row[i] = r;
     }
@@ -270,97 +273,82 @@ __device__ __forceinline__ void weights_f16(uint32_t w, f16x2& a, f16x2& b) {
 }
 
 // P parts; WM x WN x WK waves (WK: the step's 32-column blocks shared out), MT x 2 tiles of 32 x 32 a wave; BKB blocks a step.
+// A stage of the LDS holds a step's operands as they come from memory, by direct loads two steps ahead: activations
+// [part][BM][RB bytes], weights [BN][RB / 2 bytes] in int8 (each wave converts the fragments it reads), scales [BN][BKB].
 template <int P, int WM, int WN, int WK, int MT, int BKB>
 struct MoeTileShape {
-    static constexpr int kThreads = 64 * WM * WN * WK, BM = WM * MT * 32, BN = WN * 64, RB = BKB * 64;  // RB: bytes of an LDS row
-    static constexpr int kA = P * BM * RB, kW = BN * RB, kS = BN * BKB * 4, kStage = kA + kW + kS;
-    static constexpr int AL = P * BM * BKB * 4 / kThreads, WL = BN * BKB * 2 / kThreads;
-    static constexpr int kLds = 2 * kStage + BM * 4;
-    static_assert(AL * kThreads == P * BM * BKB * 4 && WL * kThreads == BN * BKB * 2 && BN * BKB <= kThreads && BKB % WK == 0, "whole loads");
-    static_assert(WK == 1 || 2 * kStage >= WM * WN * MT * 2 * 16 * 256, "the blocks' sums meet in the stages");
+    static constexpr int kWaves = WM * WN * WK, kThreads = 64 * kWaves, BM = WM * MT * 32, BN = WN * 64, RB = BKB * 64;
+    static constexpr int kA = P * BM * RB, kW = BN * RB / 2, kS = kThreads * 4, kStage = kA + kW + kS, kStages = 3;
+    static constexpr int AL = kA / 1024 / kWaves, WL = kW / 1024 / kWaves;  // direct loads of a kilobyte a wave
+    static constexpr int kLds = kStages * kStage + BM * 8;
+    static_assert(AL * kWaves * 1024 == kA && WL * kWaves * 1024 == kW && BN * BKB <= kThreads && BKB % WK == 0, "whole loads");
+    static_assert(BKB == 1 || BKB == 2, "");
+    static_assert(WK == 1 || kStages * kStage >= WM * WN * MT * 2 * 16 * 256, "the blocks' sums meet in the stages");
 };
 
+// A lane's 16 (4) bytes to the LDS at `to` (uniform) + 16 (4) x lane
+__device__ __forceinline__ void load16_to_lds(const void* from, uint8_t* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+__device__ __forceinline__ void load4_to_lds(const void* from, uint8_t* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 4, 0, 0);
+}
+
 template <int P, int WM, int WN, int WK, int MT, int BKB, bool UP>
-__global__ __launch_bounds__(64 * WM * WN * WK) void k_moe_gemm(MoeArgs a, MoeWs ws) {
+__global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_moe_gemm(MoeArgs a, MoeWs ws) {
     typedef MoeTileShape<P, WM, WN, WK, MT, BKB> T;
-    constexpr int BM = T::BM, BN = T::BN, Q = BKB * 4;  // Q: 16-byte pieces of an LDS row
+    constexpr int BM = T::BM, BN = T::BN, Q = BKB * 4, QW = BKB * 2;  // Q, QW: 16-byte pieces of a row
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     // an M tile's column tiles on one XCD, one after the other: its rows come from that XCD's L2
     const int outs = UP ? a.ffn : a.hidden, cols = UP ? a.hidden : a.ffn, per = UP ? BN / 2 : BN;
     const int nn = (outs + per - 1) / per, seq = blockIdx.x >> 3;
     const int tile = seq / nn * 8 + (blockIdx.x & 7), n0 = seq % nn * per;
+    const MoeTile mt = ws.tiles[min(tile, ws.max_tiles - 1)];
     if (tile >= *ws.n_tiles) return;
-    const MoeTile mt = ws.tiles[tile];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c = lane & 31, h = lane >> 5;
     const int wk = wave % WK, wn = wave / WK % WN, wm = wave / WK / WN;
     const int padded = (cols + 63) & ~63, nkb = cols >> 5, steps = (nkb + BKB - 1) / BKB;
-    int* sShift = reinterpret_cast<int*>(smem + 2 * T::kStage);
-    for (int r = tid; r < BM; r += T::kThreads) {
-        const int row = mt.row + min(r, mt.rows - 1);
-        sShift[r] = -(UP ? ws.x_shift[ws.row_pair[row] / a.top_k] : ws.h_shift[row]);
-    }
 
-    // LDS rows of BKB * 64 bytes, 16-byte piece q of row r at q ^ (r >> SH) % Q: operand reads (16 rows' piece q) and writes
-    // spread over the banks
-    static_assert(BKB == 1 || BKB == 2, "");
-    constexpr int SH = BKB == 2 ? 1 : 2;
-    auto at = [](int r, int q) { return r * T::RB + ((q ^ ((r >> SH) & (Q - 1))) << 4); };
-    const f16* ap[T::AL];
-    int ald[T::AL];
-#pragma unroll
-    for (int i = 0; i < T::AL; i++) {
-        const int idx = tid + i * T::kThreads, q = idx % Q, r = idx / Q % BM, part = idx / Q / BM;
-        const int row = mt.row + min(r, mt.rows - 1);  // (rows past the tile's: the last one's, their results unused)
-        ap[i] = (UP ? ws.x16 + (size_t)(ws.row_pair[row] / a.top_k) * padded + (part ? ws.x_part : 0)
-                    : ws.h16 + (size_t)row * padded + (part ? ws.h_part : 0)) + q * 8;
-        ald[i] = part * BM * T::RB + at(r, q);
-    }
+    // 16-byte piece q of row r lies at q ^ (a few bits of r), so that operand reads (16 rows' piece q) spread over the banks
+    auto x_turn = [](int r) { return (r >> (BKB == 2 ? 1 : 2)) & (Q - 1); };
+    auto w_turn = [](int r) { return (r >> (BKB == 2 ? 2 : 3)) & (QW - 1); };
     // weight row r of the tile: UP: of each 64, 32 gate rows and the same 32 up rows
     auto weight_row = [&](int r) {
         const int o = UP ? n0 + (r >> 6) * 32 + (r & 31) : n0 + r;
         return (size_t)mt.expert * outs + min(o, outs - 1);
     };
+    const f16* ap[T::AL];
+#pragma unroll
+    for (int i = 0; i < T::AL; i++) {
+        const int piece = (wave * T::AL + i) * 64 + lane, r = piece / Q % BM, part = piece / Q / BM;
+        const int row = mt.row + min(r, mt.rows - 1);  // (rows past the tile's: the last one's, their results unused)
+        ap[i] = (UP ? ws.x16 + (size_t)ws.row_tok[row] * padded + (part ? ws.x_part : 0)
+                    : ws.h16 + (size_t)row * padded + (part ? ws.h_part : 0)) + ((piece % Q) ^ x_turn(r)) * 8;
+    }
     const int8_t* wp[T::WL];
-    int wld[T::WL];
-    const int wq = tid % (BKB * 2);  // (the same for every i: the thread count is a multiple)
+    int wcol[T::WL];
 #pragma unroll
     for (int i = 0; i < T::WL; i++) {
-        const int r = (tid + i * T::kThreads) / (BKB * 2);
+        const int piece = (wave * T::WL + i) * 64 + lane, r = piece / QW;
         wp[i] = (UP ? (r & 32 ? a.w_up : a.w_gate) : a.w_down) + weight_row(r) * cols;
-        wld[i] = r;
+        wcol[i] = ((piece % QW) ^ w_turn(r)) * 16;
     }
     const int sr = tid / BKB % BN, sb = tid % BKB;
     const float* sp = (UP ? (sr & 32 ? a.s_up : a.s_gate) : a.s_down) + weight_row(sr) * nkb;
-
-    u32x4 av[T::AL], wv[T::WL];
-    float sv;
-    auto load = [&](int k) {
+    auto load = [&](int k, uint8_t* S) {
         const int blk = k * BKB;
 #pragma unroll
-        for (int i = 0; i < T::AL; i++) av[i] = *reinterpret_cast<const u32x4*>(ap[i] + blk * 32);
-        // a block past the row: weights of its first one with a scale of zero, on the operands' zeros
-        const int wc = blk * 32 + 16 * wq, wcol = wc < cols ? wc : 0;
+        for (int i = 0; i < T::AL; i++) load16_to_lds(ap[i] + blk * 32, S + (wave * T::AL + i) * 1024);
+        // (a last step's second block may lie past the row: any weights and scales, on the operands' zeros)
 #pragma unroll
-        for (int i = 0; i < T::WL; i++) wv[i] = *reinterpret_cast<const u32x4*>(wp[i] + wcol);
-        sv = sp[min(blk + sb, nkb - 1)];
-        if (blk + sb >= nkb) sv = 0.f;
-    };
-    auto store = [&](uint8_t* S) {
-#pragma unroll
-        for (int i = 0; i < T::AL; i++) *reinterpret_cast<u32x4*>(S + ald[i]) = av[i];
-#pragma unroll
-        for (int i = 0; i < T::WL; i++)
-#pragma unroll
-            for (int p = 0; p < 2; p++) {
-                f16x2 v[4];
-                weights_f16(wv[i][2 * p], v[0], v[1]), weights_f16(wv[i][2 * p + 1], v[2], v[3]);
-                f16x8 o;
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[2 * e] = v[e][0], o[2 * e + 1] = v[e][1];
-                *reinterpret_cast<f16x8*>(S + T::kA + at(wld[i], 2 * wq + p)) = o;
-            }
-        if (tid < BN * BKB) reinterpret_cast<float*>(S + T::kA + T::kW)[sb * BN + sr] = sv;
+        for (int i = 0; i < T::WL; i++) {
+            const int col = blk * 32 + wcol[i];
+            load16_to_lds(wp[i] + (BKB == 1 || col < cols ? col : 0), S + T::kA + (wave * T::WL + i) * 1024);
+        }
+        load4_to_lds(sp + min(blk + sb, nkb - 1), S + T::kA + T::kW + wave * 256);
     };
 
     f32x16 acc[MT][2];
@@ -370,49 +358,77 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_moe_gemm(MoeArgs a, MoeWs
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[m][n][e] = 0.f;
-    load(0);
-    store(smem);
-    load(min(1, steps - 1));
-    __syncthreads();
+    load(0, smem);
+    load(min(1, steps - 1), smem + T::kStage);
+    // Of a row, for the results: its power of two and (down) its weight. After the first loads, before the last waits.
+    int* sShift = reinterpret_cast<int*>(smem + T::kStages * T::kStage);
+    float* sWeight = reinterpret_cast<float*>(sShift + BM);
+    if (tid < BM) {
+        const int row = mt.row + min(tid, mt.rows - 1);
+        sShift[tid] = -(UP ? ws.x_shift[ws.row_tok[row]] : ws.h_shift[row]);
+        if (!UP) sWeight[tid] = ws.row_weight[row];
+    }
+    f32x16 zero = {};
+    asm volatile("" : "+v"(zero));  // registers of zeros: a constant would be written into every accumulator anew
+    int at_stage = 0;
 #pragma unroll 1
     for (int k = 0; k < steps; k++) {
-        const uint8_t* S = smem + (k & 1) * T::kStage;
-        if (k + 1 < steps) store(smem + ((k + 1) & 1) * T::kStage);
-        load(min(k + 2, steps - 1));
+        // this step's loads have landed (the next one's may be on their way), in every wave; the last step's reads ended
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(T::AL + T::WL + 1) : "memory");
+        const uint8_t* S = smem + at_stage * T::kStage;
+        const int to = at_stage == 0 ? 2 : at_stage - 1;
+        load(min(k + 2, steps - 1), smem + to * T::kStage);
+        at_stage = at_stage == 2 ? 0 : at_stage + 1;
+        // Tile by tile of the step's blocks, the scaled sum of one behind the matrix instructions of the next, so that a
+        // wave's vector and matrix instructions run side by side.
+        constexpr int NJ = BKB / WK, NT = NJ * MT * 2;
+        f16x8 w[NJ][2][2], x[NJ][MT][P][2];
+        float sc[NJ][2];
+        f32x16 d[2];
 #pragma unroll
-        for (int jj = 0; jj < BKB / WK; jj++) {
+        for (int jj = 0; jj < NJ; jj++) {
             const int j = jj * WK + wk;
-            f16x8 w[2][2], x[MT][P][2];
-            float sc[2];
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const int r = wn * 64 + 32 * n + c;
-#pragma unroll
-                for (int q = 0; q < 2; q++) w[n][q] = *reinterpret_cast<const f16x8*>(S + T::kA + at(r, 4 * j + 2 * q + h));
-                sc[n] = reinterpret_cast<const float*>(S + T::kA + T::kW)[j * BN + r];
-            }
+            // lane half h takes 16 columns of the block, product q of the two their eights
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
                 for (int p = 0; p < P; p++)
 #pragma unroll
-                    for (int q = 0; q < 2; q++)
-                        x[m][p][q] = *reinterpret_cast<const f16x8*>(S + p * BM * T::RB + at((wm * MT + m) * 32 + c, 4 * j + 2 * q + h));
+                    for (int q = 0; q < 2; q++) {
+                        const int r = (wm * MT + m) * 32 + c;
+                        x[jj][m][p][q] = *reinterpret_cast<const f16x8*>(S + (p * BM + r) * T::RB + (((4 * j + 2 * h + q) ^ x_turn(r)) << 4));
+                    }
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+            for (int n = 0; n < 2; n++) {
+                const int r = wn * 64 + 32 * n + c;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(S + T::kA + r * (T::RB / 2) + (((2 * j + h) ^ w_turn(r)) << 4));
+                sc[jj][n] = reinterpret_cast<const float*>(S + T::kA + T::kW)[r * BKB + j];
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    f32x16 d = {};
+                for (int q = 0; q < 2; q++) {
+                    f16x2 p[4];
+                    weights_f16(v[2 * q], p[0], p[1]), weights_f16(v[2 * q + 1], p[2], p[3]);
 #pragma unroll
-                    for (int p = P - 1; p >= 0; p--)
-#pragma unroll
-                        for (int q = 0; q < 2; q++) d = mfma32h(x[m][p][q], w[n][q], d);
-#pragma unroll
-                    for (int e = 0; e < 16; e++) acc[m][n][e] = fmaf(sc[n], d[e], acc[m][n][e]);
+                    for (int e = 0; e < 4; e++) w[jj][n][q][2 * e] = p[e][0], w[jj][n][q][2 * e + 1] = p[e][1];
                 }
+            }
         }
-        __syncthreads();
+        static_for<0, NT + 1>([&](auto i_) {
+            constexpr int i = i_, jj = i / (MT * 2), m = i / 2 % MT, n = i % 2;
+            if constexpr (i < NT)
+#pragma unroll
+                for (int p = P - 1; p >= 0; p--)
+#pragma unroll
+                    for (int q = 0; q < 2; q++)
+                        d[i & 1] = mfma32h(x[jj][m][p][q], w[jj][n][q], p == P - 1 && q == 0 ? zero : d[i & 1]);
+            if constexpr (i > 0) {
+                constexpr int i1 = i - 1, j1 = i1 / (MT * 2), m1 = i1 / 2 % MT, n1 = i1 % 2;
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[m1][n1][e] = fmaf(sc[j1][n1], d[i1 & 1][e], acc[m1][n1][e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
     }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if constexpr (WK == 2) {
         float* meet = reinterpret_cast<float*>(smem) + (wm * WN + wn) * (MT * 2 * 16 * 64) + lane;
 #pragma unroll
@@ -431,25 +447,34 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_moe_gemm(MoeArgs a, MoeWs
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[m][n][e] += meet[((m * 2 + n) * 16 + e) * 64];
     }
-    // lane (c, h): weight row c of a tile, activation rows 8 (e / 4) + 4 h + e % 4
+    // lane (c, h): weight row c of a tile, activation rows 8 (e / 4) + 4 h + e % 4. Stores past the tile's rows, or past the
+    // last column, lie outside the resource.
+    float* out = (UP ? ws.h : ws.y) + (size_t)mt.row * outs;
+    const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(out, (short)0, mt.rows * outs * 4, 0x00020000);
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int r = (wm * MT + m) * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (r >= mt.rows) continue;
-            const int s = sShift[r];
-            const size_t row = mt.row + r;
-            if constexpr (UP) {
-                const int f = n0 + wn * 32 + c;
-                const float g = ldexpf(acc[m][0][e], s), u = ldexpf(acc[m][1][e], s);
-                if (f < outs) ws.h[row * outs + f] = g * sigmoid(g) * u;
-            } else {
-                const float wt = a.weights[ws.row_pair[row]];
+        for (int e4 = 0; e4 < 4; e4++) {
+            const int r0 = (wm * MT + m) * 32 + 8 * e4 + 4 * h;
+            typedef int i32x4 __attribute__((ext_vector_type(4)));
+            const i32x4 s = *reinterpret_cast<const i32x4*>(sShift + r0);
+            f32x4 wt;
+            if constexpr (!UP) wt = *reinterpret_cast<const f32x4*>(sWeight + r0);
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    const int o = n0 + wn * 64 + 32 * n + c;
-                    if (o < outs) ws.y[row * outs + o] = wt * ldexpf(acc[m][n][e], s);
+            for (int e = 0; e < 4; e++) {
+                const unsigned row_at = (unsigned)(r0 + e) * outs * 4u;
+                if constexpr (UP) {
+                    const int f = n0 + wn * 32 + c;
+                    const float g = ldexpf(acc[m][0][4 * e4 + e], s[e]), u = ldexpf(acc[m][1][4 * e4 + e], s[e]);
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(g * sigmoid(g) * u), ro,
+                                                          (int)(f < outs ? row_at + f * 4u : kFar), 0, 0);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const int o = n0 + wn * 64 + 32 * n + c;
+                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(wt[e] * ldexpf(acc[m][n][4 * e4 + e], s[e])), ro,
+                                                              (int)(o < outs ? row_at + o * 4u : kFar), 0, 0);
+                    }
                 }
             }
         }
@@ -492,8 +517,10 @@ static size_t lay_out(const MoeArgs& a, int parts, uint8_t* base, MoeWs& w) {
         p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(reinterpret_cast<uintptr_t>(base) + at);
         at += up256(bytes);
     };
-    take(w.n_tiles, 4), take(w.tiles, (pairs / 32 + a.n_experts + 1) * sizeof(MoeTile));
-    take(w.row_pair, pairs * 4), take(w.pair_row, pairs * 4), take(w.x_shift, n * 4), take(w.h_shift, pairs * 4);
+    take(w.n_tiles, 4);
+    w.max_tiles = (int)(pairs / 32) + a.n_experts + 1;
+    take(w.tiles, w.max_tiles * sizeof(MoeTile));
+    take(w.row_tok, pairs * 4), take(w.pair_row, pairs * 4), take(w.row_weight, pairs * 4), take(w.x_shift, n * 4), take(w.h_shift, pairs * 4);
     take(w.x16, parts * n * hp * 2), take(w.h16, 2 * pairs * fp * 2);
     w.x_part = n * hp, w.h_part = pairs * fp;
     take(w.y, pairs * std::max(a.hidden, a.ffn) * 4);
