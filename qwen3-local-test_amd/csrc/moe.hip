@@ -161,8 +161,8 @@ __global__ __launch_bounds__(256) void k_moe_pair_down(MoeArgs a) {
 }
 
 // ---- the experts, grouped: pairs sorted by expert, tiled products on the matrix cores ------------------------
-// k_moe_group sorts the pairs by expert and lists tiles of BM rows of one expert; k_moe_rows writes activations as fp16
-// operands; k_moe_gemm multiplies a tile's rows with 64 gate and the same 64 up rows of its expert's weights (or 128 down
+// k_moe_begin sorts the pairs by expert, lists tiles of BM rows of one expert and writes x as fp16 operands (k_moe_mid: h);
+// k_moe_gemm multiplies a tile's rows with 64 gate and the same 64 up rows of its expert's weights (or 128 down
 // rows); k_moe_combine sums a token's pairs in their order.
 //
 // Operands: an int8 weight is exact in fp16. A row of activations is scaled by the power of two that puts its largest
@@ -186,15 +186,29 @@ struct MoeWs {
     int max_tiles;             // room in tiles
 };
 
-// One workgroup.
-__global__ __launch_bounds__(1024) void k_moe_group(MoeArgs a, MoeWs ws, int bm) {
+// The pairs sorted by expert, by one workgroup. A lane's ids of 16 K pairs are loaded together: one after the other their
+// latencies took 46 us for 16,384 pairs.
+constexpr int kGroupIds = 16;
+
+__device__ __forceinline__ void moe_group(const MoeArgs& a, const MoeWs& ws, int bm) {
     __shared__ int count[1024], part[2][16];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, pairs = a.n * a.top_k;
+    int id[kGroupIds];
+    auto load = [&](int i0) {  // -1: no expert
+#pragma unroll
+        for (int u = 0; u < kGroupIds; u++) {
+            const int i = i0 + u * 1024 + tid, e = a.ids[min(i, pairs - 1)];
+            id[u] = i < pairs && e >= 0 && e < a.n_experts ? e : -1;
+        }
+    };
     count[tid] = 0;
+    load(0);
     __syncthreads();
-    for (int i = tid; i < pairs; i += 1024) {
-        const int e = a.ids[i];
-        if (e >= 0 && e < a.n_experts) atomicAdd(&count[e], 1);
+    for (int i0 = 0; i0 < pairs; i0 += kGroupIds * 1024) {
+        if (i0) load(i0);
+#pragma unroll
+        for (int u = 0; u < kGroupIds; u++)
+            if (id[u] >= 0) atomicAdd(&count[id[u]], 1);
     }
     __syncthreads();
     const int mine = count[tid], tiles = (mine + bm - 1) / bm;
@@ -212,39 +226,46 @@ __global__ __launch_bounds__(1024) void k_moe_group(MoeArgs a, MoeWs ws, int bm)
     if (tid == 1023) *ws.n_tiles = tile + tiles;
     count[tid] = rows;
     __syncthreads();
-    for (int i = tid; i < pairs; i += 1024) {
-        const int e = a.ids[i];
-        int r = -1;
-        if (e >= 0 && e < a.n_experts) {
-            r = atomicAdd(&count[e], 1);
-            ws.row_tok[r] = i / a.top_k;
-            ws.row_weight[r] = a.weights[i];
+    for (int i0 = 0; i0 < pairs; i0 += kGroupIds * 1024) {
+        if (pairs > kGroupIds * 1024) load(i0);
+        int r[kGroupIds];
+        float wt[kGroupIds];
+#pragma unroll
+        for (int u = 0; u < kGroupIds; u++) {
+            wt[u] = a.weights[min(i0 + u * 1024 + tid, pairs - 1)];
+            r[u] = id[u] >= 0 ? atomicAdd(&count[id[u]], 1) : -1;
         }
-        ws.pair_row[i] = r;
+#pragma unroll
+        for (int u = 0; u < kGroupIds; u++) {
+            const int i = i0 + u * 1024 + tid;
+            if (i >= pairs) break;
+            ws.pair_row[i] = r[u];
+            if (r[u] >= 0) ws.row_tok[r[u]] = i / a.top_k, ws.row_weight[r[u]] = wt[u];
+        }
     }
 }
 
-// A row of activations as fp16 operands: out[part][row][padded], zeros from `cols` on, and its power of two. A workgroup
-// a row.
+// A row of activations as fp16 operands: out[part][row][padded], zeros from `cols` on, and its power of two. 256 lanes a
+// row, `lane` of them this one; `most`: four floats of the LDS.
 template <int DT, int P>
-__global__ __launch_bounds__(256) void k_moe_rows(const void* x, size_t stride, int cols, int padded, f16* out, size_t part, int* shift) {
-    __shared__ float most[4];
-    const int tid = threadIdx.x;
-    const size_t row = blockIdx.x;
+__device__ __forceinline__ void moe_row(const void* x, size_t stride, int cols, int padded, f16* out, size_t part, int* shift,
+                                        size_t row, int lane, float* most, bool there) {
     float v[8], m = 0.f;
-    for (int c = tid * 8; c < cols; c += 2048) {
-        load_vec<DT, 8>(x, row * stride + c, v);
+    if (there)
+        for (int c = lane * 8; c < cols; c += 2048) {
+            load_vec<DT, 8>(x, row * stride + c, v);
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
-    }
+            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
+        }
     m = moe_wave_max(m);
-    if ((tid & 63) == 0) most[tid >> 6] = m;
+    if ((lane & 63) == 0) most[lane >> 6] = m;
     __syncthreads();
+    if (!there) return;
     m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
     // (a row with an infinity, or of zeros, is not scaled)
     const int up = m > 0.f && m < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
-    if (tid == 0) shift[row] = up;
-    for (int c = tid * 8; c < padded; c += 2048) {
+    if (lane == 0) shift[row] = up;
+    for (int c = lane * 8; c < padded; c += 2048) {
         f16x8 hi = {}, lo = {};
         if (c < cols) {
             load_vec<DT, 8>(x, row * stride + c, v);
@@ -260,6 +281,24 @@ __global__ __launch_bounds__(256) void k_moe_rows(const void* x, size_t stride, 
     }
 }
 
+// Workgroup 0 sorts; the others write four rows of x each.
+template <int DT, int P>
+__global__ __launch_bounds__(1024) void k_moe_begin(MoeArgs a, MoeWs ws, int bm) {
+    __shared__ float most[4][4];
+    if (blockIdx.x == 0) {
+        moe_group(a, ws, bm);
+        return;
+    }
+    const int sub = threadIdx.x >> 8, row = (blockIdx.x - 1) * 4 + sub;
+    moe_row<DT, P>(a.x, a.x_stride, a.hidden, (a.hidden + 63) & ~63, ws.x16, ws.x_part, ws.x_shift, row, threadIdx.x & 255,
+                   most[sub], row < a.n);
+}
+// Rows of h.
+__global__ __launch_bounds__(256) void k_moe_mid(MoeArgs a, MoeWs ws) {
+    __shared__ float most[4];
+    moe_row<0, 2>(ws.h, a.ffn, a.ffn, (a.ffn + 63) & ~63, ws.h16, ws.h_part, ws.h_shift, blockIdx.x, threadIdx.x, most, true);
+}
+
 __device__ __forceinline__ f32x16 mfma32h(f16x8 a, f16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
@@ -272,18 +311,21 @@ __device__ __forceinline__ void weights_f16(uint32_t w, f16x2& a, f16x2& b) {
     b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - off;
 }
 
-// P parts; WM x WN x WK waves (WK: the step's 32-column blocks shared out), MT x 2 tiles of 32 x 32 a wave; BKB blocks a step.
-// A stage of the LDS holds a step's operands as they come from memory, by direct loads two steps ahead: activations
-// [part][BM][RB bytes], weights [BN][RB / 2 bytes] in int8 (each wave converts the fragments it reads), scales [BN][BKB].
-template <int P, int WM, int WN, int WK, int MT, int BKB>
+constexpr int kMoeGroup = 4;  // M tiles whose column tiles follow each other on an XCD
+
+// P parts of the activations, tiles of MT x 32 rows by 128 weight rows, 64 columns a step. Four waves share out the weight
+// rows, 32 each, so that each int8 weight is converted by one wave. The LDS takes operands as they come from memory, by
+// direct loads: ST stages of activations [part][BM][128 bytes], ST - 1 steps ahead; two of int8 weights [BN][128 columns];
+// two of scales [BN][8 blocks]. Bound by the requests to L2 (one a cycle and channel, a line or less each), so rows are
+// read by whole lines where they can be: scales loaded two blocks a row at a time alone made as many as all the rest
+// (2,048 tokens of 8 of 128 experts, gate and up: 170 us).
+template <int P, int MT, int ST>
 struct MoeTileShape {
-    static constexpr int kWaves = WM * WN * WK, kThreads = 64 * kWaves, BM = WM * MT * 32, BN = WN * 64, RB = BKB * 64;
-    static constexpr int kA = P * BM * RB, kW = BN * RB / 2, kS = kThreads * 4, kStage = kA + kW + kS, kStages = 3;
-    static constexpr int AL = kA / 1024 / kWaves, WL = kW / 1024 / kWaves;  // direct loads of a kilobyte a wave
-    static constexpr int kLds = kStages * kStage + BM * 8;
-    static_assert(AL * kWaves * 1024 == kA && WL * kWaves * 1024 == kW && BN * BKB <= kThreads && BKB % WK == 0, "whole loads");
-    static_assert(BKB == 1 || BKB == 2, "");
-    static_assert(WK == 1 || kStages * kStage >= WM * WN * MT * 2 * 16 * 256, "the blocks' sums meet in the stages");
+    static constexpr int kThreads = 256, BM = MT * 32, BN = 128;
+    static constexpr int kA = P * BM * 128, kW = BN * 128, kS = BN * 8 * 4;
+    static constexpr int kAtW = ST * kA, kAtS = kAtW + 2 * kW, kAtRows = kAtS + 2 * kS, kLds = kAtRows + BM * 8;
+    static constexpr int AL = kA / 4096, WL = kW / 4096, SL = kS / 1024;  // direct loads a wave: 1 KB (scales: 256 bytes) each
+    static_assert(AL * 4096 == kA, "whole loads");
 };
 
 // A lane's 16 (4) bytes to the LDS at `to` (uniform) + 16 (4) x lane
@@ -296,72 +338,80 @@ __device__ __forceinline__ void load4_to_lds(const void* from, uint8_t* to) {
                                      (__attribute__((address_space(3))) void*)to, 4, 0, 0);
 }
 
-template <int P, int WM, int WN, int WK, int MT, int BKB, bool UP>
-__global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_moe_gemm(MoeArgs a, MoeWs ws) {
-    typedef MoeTileShape<P, WM, WN, WK, MT, BKB> T;
-    constexpr int BM = T::BM, BN = T::BN, Q = BKB * 4, QW = BKB * 2;  // Q, QW: 16-byte pieces of a row
+template <int P, int MT, int ST, bool UP>
+__global__ __launch_bounds__(256, 2) void k_moe_gemm(MoeArgs a, MoeWs ws) {
+    typedef MoeTileShape<P, MT, ST> T;
+    constexpr int BM = T::BM, BN = T::BN;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    // an M tile's column tiles on one XCD, one after the other: its rows come from that XCD's L2
+    // Groups of four M tiles (mostly one expert's) on one XCD, column tile after column tile: the group's weights come once
+    // from memory, its rows once, then from that XCD's L2.
     const int outs = UP ? a.ffn : a.hidden, cols = UP ? a.hidden : a.ffn, per = UP ? BN / 2 : BN;
-    const int nn = (outs + per - 1) / per, seq = blockIdx.x >> 3;
-    const int tile = seq / nn * 8 + (blockIdx.x & 7), n0 = seq % nn * per;
+    const int nn = (outs + per - 1) / per, seq = blockIdx.x >> 3, in = seq % (nn * kMoeGroup);
+    const int tile = (seq / (nn * kMoeGroup) * 8 + (blockIdx.x & 7)) * kMoeGroup + in % kMoeGroup, n0 = in / kMoeGroup * per;
     const MoeTile mt = ws.tiles[min(tile, ws.max_tiles - 1)];
     if (tile >= *ws.n_tiles) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c = lane & 31, h = lane >> 5;
-    const int wk = wave % WK, wn = wave / WK % WN, wm = wave / WK / WN;
-    const int padded = (cols + 63) & ~63, nkb = cols >> 5, steps = (nkb + BKB - 1) / BKB;
+    const int padded = (cols + 63) & ~63, nkb = cols >> 5, steps = padded >> 6;
 
-    // 16-byte piece q of row r lies at q ^ (a few bits of r), so that operand reads (16 rows' piece q) spread over the banks
-    auto x_turn = [](int r) { return (r >> (BKB == 2 ? 1 : 2)) & (Q - 1); };
-    auto w_turn = [](int r) { return (r >> (BKB == 2 ? 2 : 3)) & (QW - 1); };
-    // weight row r of the tile: UP: of each 64, 32 gate rows and the same 32 up rows
+    // 16-byte piece q of a 128-byte row r lies at q ^ (r / 2) % 8, so that operand reads (16 rows' piece q) spread over the
+    // banks; the eight lanes that fill a row load its line in that order
+    auto turn = [](int r) { return (r >> 1) & 7; };
+    const int lr = lane >> 3, lq = lane & 7;  // of a direct load: row and place
+    // weight row r of the tile: UP: of each 32, 16 gate rows and the same 16 up rows
     auto weight_row = [&](int r) {
-        const int o = UP ? n0 + (r >> 6) * 32 + (r & 31) : n0 + r;
+        const int o = UP ? n0 + (r >> 5) * 16 + (r & 15) : n0 + r;
         return (size_t)mt.expert * outs + min(o, outs - 1);
     };
     const f16* ap[T::AL];
 #pragma unroll
     for (int i = 0; i < T::AL; i++) {
-        const int piece = (wave * T::AL + i) * 64 + lane, r = piece / Q % BM, part = piece / Q / BM;
+        const int at = (wave * T::AL + i) * 8 + lr, r = at % BM, part = at / BM;
         const int row = mt.row + min(r, mt.rows - 1);  // (rows past the tile's: the last one's, their results unused)
         ap[i] = (UP ? ws.x16 + (size_t)ws.row_tok[row] * padded + (part ? ws.x_part : 0)
-                    : ws.h16 + (size_t)row * padded + (part ? ws.h_part : 0)) + ((piece % Q) ^ x_turn(r)) * 8;
+                    : ws.h16 + (size_t)row * padded + (part ? ws.h_part : 0)) + (lq ^ turn(r)) * 8;
     }
     const int8_t* wp[T::WL];
     int wcol[T::WL];
 #pragma unroll
     for (int i = 0; i < T::WL; i++) {
-        const int piece = (wave * T::WL + i) * 64 + lane, r = piece / QW;
-        wp[i] = (UP ? (r & 32 ? a.w_up : a.w_gate) : a.w_down) + weight_row(r) * cols;
-        wcol[i] = ((piece % QW) ^ w_turn(r)) * 16;
+        const int r = (wave * T::WL + i) * 8 + lr;
+        wp[i] = (UP ? (r & 16 ? a.w_up : a.w_gate) : a.w_down) + weight_row(r) * cols;
+        wcol[i] = (lq ^ turn(r)) * 16;
     }
-    const int sr = tid / BKB % BN, sb = tid % BKB;
-    const float* sp = (UP ? (sr & 32 ? a.s_up : a.s_gate) : a.s_down) + weight_row(sr) * nkb;
-    auto load = [&](int k, uint8_t* S) {
-        const int blk = k * BKB;
+    const float* sp[T::SL];
 #pragma unroll
-        for (int i = 0; i < T::AL; i++) load16_to_lds(ap[i] + blk * 32, S + (wave * T::AL + i) * 1024);
-        // (a last step's second block may lie past the row: any weights and scales, on the operands' zeros)
+    for (int i = 0; i < T::SL; i++) {
+        const int r = (wave * T::SL + i) * 8 + lr;
+        sp[i] = (UP ? (r & 16 ? a.s_up : a.s_gate) : a.s_down) + weight_row(r) * nkb;
+    }
+    auto load_a = [&](int k, int stage) {
+#pragma unroll
+        for (int i = 0; i < T::AL; i++) load16_to_lds(ap[i] + min(k, steps - 1) * 64, smem + stage * T::kA + (wave * T::AL + i) * 1024);
+    };
+    // (past the row: any weights and scales, on the operands' zeros or in steps that do not run)
+    auto load_w = [&](int m, int buffer) {  // columns 128 m ..
 #pragma unroll
         for (int i = 0; i < T::WL; i++) {
-            const int col = blk * 32 + wcol[i];
-            load16_to_lds(wp[i] + (BKB == 1 || col < cols ? col : 0), S + T::kA + (wave * T::WL + i) * 1024);
+            const int col = m * 128 + wcol[i];
+            load16_to_lds(wp[i] + (col < cols ? col : 0), smem + T::kAtW + buffer * T::kW + (wave * T::WL + i) * 1024);
         }
-        load4_to_lds(sp + min(blk + sb, nkb - 1), S + T::kA + T::kW + wave * 256);
+    };
+    auto load_s = [&](int m, int buffer) {  // blocks 8 m ..
+#pragma unroll
+        for (int i = 0; i < T::SL; i++)
+            load4_to_lds(sp[i] + min(m * 8 + lq, nkb - 1), smem + T::kAtS + buffer * T::kS + (wave * T::SL + i) * 256);
     };
 
-    f32x16 acc[MT][2];
+    f32x16 acc[MT];
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[m][n][e] = 0.f;
-    load(0, smem);
-    load(min(1, steps - 1), smem + T::kStage);
+        for (int e = 0; e < 16; e++) acc[m][e] = 0.f;
+    load_w(0, 0), load_s(0, 0), load_a(0, 0);
+    if (ST == 3) load_a(1, 1);
     // Of a row, for the results: its power of two and (down) its weight. After the first loads, before the last waits.
-    int* sShift = reinterpret_cast<int*>(smem + T::kStages * T::kStage);
+    int* sShift = reinterpret_cast<int*>(smem + T::kAtRows);
     float* sWeight = reinterpret_cast<float*>(sShift + BM);
     if (tid < BM) {
         const int row = mt.row + min(tid, mt.rows - 1);
@@ -370,112 +420,106 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_moe_gemm(MoeArgs a, Mo
     }
     f32x16 zero = {};
     asm volatile("" : "+v"(zero));  // registers of zeros: a constant would be written into every accumulator anew
-    int at_stage = 0;
+    // Four steps at a time (256 columns: a load of scales, two of weights). Step s loads activations first, then the next
+    // weights (s = 0, 2) and scales (s = 0): what of a step's loads may still be on its way at the next step's start is
+    // all of them (three stages) or those behind the activations.
+    constexpr int kNew[4] = {T::WL + T::SL, 0, T::WL, 0};
+    int stage = 0, sbuf = 0;
 #pragma unroll 1
-    for (int k = 0; k < steps; k++) {
-        // this step's loads have landed (the next one's may be on their way), in every wave; the last step's reads ended
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(T::AL + T::WL + 1) : "memory");
-        const uint8_t* S = smem + at_stage * T::kStage;
-        const int to = at_stage == 0 ? 2 : at_stage - 1;
-        load(min(k + 2, steps - 1), smem + to * T::kStage);
-        at_stage = at_stage == 2 ? 0 : at_stage + 1;
-        // Tile by tile of the step's blocks, the scaled sum of one behind the matrix instructions of the next, so that a
-        // wave's vector and matrix instructions run side by side.
-        constexpr int NJ = BKB / WK, NT = NJ * MT * 2;
-        f16x8 w[NJ][2][2], x[NJ][MT][P][2];
-        float sc[NJ][2];
-        f32x16 d[2];
+    for (int k0 = 0; k0 < steps; k0 += 4) {
+        static_for<0, 4>([&](auto s_) {
+            constexpr int s = s_, kFly = kNew[(s + 3) & 3] + (ST == 3 ? T::AL : 0);
+            const int k = k0 + s;
+            if (k >= steps) return;  // uniform
+            // this step's loads have landed, in every wave, and the last step's reads have ended
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kFly) : "memory");
+            const int to = ST == 3 ? (stage == 0 ? 2 : stage - 1) : stage ^ 1;
+            load_a(k + ST - 1, to);
+            if constexpr (s % 2 == 0) load_w((k >> 1) + 1, s == 0 ? 1 : 0);
+            if constexpr (s == 0) load_s((k >> 2) + 1, sbuf ^ 1);
+            const uint8_t* A = smem + stage * T::kA;
+            const uint8_t* W = smem + T::kAtW + (s >> 1) * T::kW;
+            const float* sS = reinterpret_cast<const float*>(smem + T::kAtS + sbuf * T::kS);
+            stage = ST == 3 ? (stage == 2 ? 0 : stage + 1) : stage ^ 1;
+            // Tile by tile of the step's two blocks, the scaled sum of one behind the matrix instructions of the next, so
+            // that a wave's vector and matrix instructions run side by side.
+            constexpr int NT = 2 * MT;
+            f16x8 w[2][2], x[2][MT][P][2];
+            float sc[2];
+            f32x16 d[2];
+            const int wr = wave * 32 + c;
 #pragma unroll
-        for (int jj = 0; jj < NJ; jj++) {
-            const int j = jj * WK + wk;
-            // lane half h takes 16 columns of the block, product q of the two their eights
+            for (int j = 0; j < 2; j++) {
+                // lane half h takes 16 columns of the block, product q of the two their eights
+                const u32x4 v = *reinterpret_cast<const u32x4*>(W + wr * 128 + (((4 * (s & 1) + 2 * j + h) ^ turn(wr)) << 4));
+                sc[j] = sS[wr * 8 + 2 * s + j];
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+                for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int p = 0; p < P; p++)
+                    for (int p = 0; p < P; p++)
 #pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        const int r = (wm * MT + m) * 32 + c;
-                        x[jj][m][p][q] = *reinterpret_cast<const f16x8*>(S + (p * BM + r) * T::RB + (((4 * j + 2 * h + q) ^ x_turn(r)) << 4));
-                    }
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const int r = wn * 64 + 32 * n + c;
-                const u32x4 v = *reinterpret_cast<const u32x4*>(S + T::kA + r * (T::RB / 2) + (((2 * j + h) ^ w_turn(r)) << 4));
-                sc[jj][n] = reinterpret_cast<const float*>(S + T::kA + T::kW)[r * BKB + j];
+                        for (int q = 0; q < 2; q++) {
+                            const int r = m * 32 + c;
+                            x[j][m][p][q] = *reinterpret_cast<const f16x8*>(A + (p * BM + r) * 128 + (((4 * j + 2 * h + q) ^ turn(r)) << 4));
+                        }
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
                     f16x2 p[4];
                     weights_f16(v[2 * q], p[0], p[1]), weights_f16(v[2 * q + 1], p[2], p[3]);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) w[jj][n][q][2 * e] = p[e][0], w[jj][n][q][2 * e + 1] = p[e][1];
+                    for (int e = 0; e < 4; e++) w[j][q][2 * e] = p[e][0], w[j][q][2 * e + 1] = p[e][1];
                 }
             }
-        }
-        static_for<0, NT + 1>([&](auto i_) {
-            constexpr int i = i_, jj = i / (MT * 2), m = i / 2 % MT, n = i % 2;
-            if constexpr (i < NT)
+            static_for<0, NT + 1>([&](auto i_) {
+                constexpr int i = i_, j = i / MT, m = i % MT;
+                if constexpr (i < NT)
 #pragma unroll
-                for (int p = P - 1; p >= 0; p--)
+                    for (int p = P - 1; p >= 0; p--)
 #pragma unroll
-                    for (int q = 0; q < 2; q++)
-                        d[i & 1] = mfma32h(x[jj][m][p][q], w[jj][n][q], p == P - 1 && q == 0 ? zero : d[i & 1]);
-            if constexpr (i > 0) {
-                constexpr int i1 = i - 1, j1 = i1 / (MT * 2), m1 = i1 / 2 % MT, n1 = i1 % 2;
+                        for (int q = 0; q < 2; q++)
+                            d[i & 1] = mfma32h(x[j][m][p][q], w[j][q], p == P - 1 && q == 0 ? zero : d[i & 1]);
+                if constexpr (i > 0) {
+                    constexpr int j1 = (i - 1) / MT, m1 = (i - 1) % MT;
 #pragma unroll
-                for (int e = 0; e < 16; e++) acc[m1][n1][e] = fmaf(sc[j1][n1], d[i1 & 1][e], acc[m1][n1][e]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
+                    for (int e = 0; e < 16; e++) acc[m1][e] = fmaf(sc[j1], d[(i - 1) & 1][e], acc[m1][e]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
         });
+        sbuf ^= 1;
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if constexpr (WK == 2) {
-        float* meet = reinterpret_cast<float*>(smem) + (wm * WN + wn) * (MT * 2 * 16 * 64) + lane;
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    if (wk) meet[((m * 2 + n) * 16 + e) * 64] = acc[m][n][e];
-        __syncthreads();
-        if (wk) return;
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[m][n][e] += meet[((m * 2 + n) * 16 + e) * 64];
-    }
     // lane (c, h): weight row c of a tile, activation rows 8 (e / 4) + 4 h + e % 4. Stores past the tile's rows, or past the
     // last column, lie outside the resource.
     float* out = (UP ? ws.h : ws.y) + (size_t)mt.row * outs;
     const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(out, (short)0, mt.rows * outs * 4, 0x00020000);
+    const int o = UP ? n0 + wave * 16 + (c & 15) : n0 + wave * 32 + c;
+    const unsigned col = o < outs ? o * 4u : kFar;
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int e4 = 0; e4 < 4; e4++) {
-            const int r0 = (wm * MT + m) * 32 + 8 * e4 + 4 * h;
             typedef int i32x4 __attribute__((ext_vector_type(4)));
+            const int r0 = m * 32 + 8 * e4 + 4 * h;
             const i32x4 s = *reinterpret_cast<const i32x4*>(sShift + r0);
-            f32x4 wt;
-            if constexpr (!UP) wt = *reinterpret_cast<const f32x4*>(sWeight + r0);
+            if constexpr (UP) {
+                // the lane pair (c, c + 16) holds a gate and an up value: the first takes one row of two, the second the other
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const unsigned row_at = (unsigned)(r0 + e) * outs * 4u;
-                if constexpr (UP) {
-                    const int f = n0 + wn * 32 + c;
-                    const float g = ldexpf(acc[m][0][4 * e4 + e], s[e]), u = ldexpf(acc[m][1][4 * e4 + e], s[e]);
+                for (int e = 0; e < 4; e += 2) {
+                    const auto p0 = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[m][4 * e4 + e]), __float_as_uint(acc[m][4 * e4 + e]), false, false);
+                    const auto p1 = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[m][4 * e4 + e + 1]), __float_as_uint(acc[m][4 * e4 + e + 1]), false, false);
+                    const bool odd = c & 16;
+                    const int sh = odd ? s[e + 1] : s[e];
+                    const float g = ldexpf(__uint_as_float(odd ? p1[0] : p0[0]), sh), u = ldexpf(__uint_as_float(odd ? p1[1] : p0[1]), sh);
                     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(g * sigmoid(g) * u), ro,
-                                                          (int)(f < outs ? row_at + f * 4u : kFar), 0, 0);
-                } else {
-#pragma unroll
-                    for (int n = 0; n < 2; n++) {
-                        const int o = n0 + wn * 64 + 32 * n + c;
-                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(wt[e] * ldexpf(acc[m][n][4 * e4 + e], s[e])), ro,
-                                                              (int)(o < outs ? row_at + o * 4u : kFar), 0, 0);
-                    }
+                                                          (int)((unsigned)(r0 + e + (odd ? 1 : 0)) * outs * 4u + col), 0, 0);
                 }
+            } else {
+                const f32x4 wt = *reinterpret_cast<const f32x4*>(sWeight + r0);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(wt[e] * ldexpf(acc[m][4 * e4 + e], s[e])), ro,
+                                                          (int)((unsigned)(r0 + e) * outs * 4u + col), 0, 0);
             }
         }
 }
@@ -542,27 +586,28 @@ static hipError_t moe_pairs(const MoeArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int P, int WM, int WN, int WK, int MT, int BKB, bool UP>
+template <int P, int MT, int ST, bool UP>
 static hipError_t moe_gemm(const MoeArgs& a, const MoeWs& w, hipStream_t s) {
-    typedef MoeTileShape<P, WM, WN, WK, MT, BKB> T;
+    typedef MoeTileShape<P, MT, ST> T;
     static std::atomic<uint64_t> raised{0};
-    const auto k = &k_moe_gemm<P, WM, WN, WK, MT, BKB, UP>;
+    const auto k = &k_moe_gemm<P, MT, ST, UP>;
     if (const hipError_t e = raise_lds(reinterpret_cast<const void*>(k), T::kLds, raised)) return e;
     // the most tiles that the pairs can make (workgroups past the real number end at once)
     const int pairs = a.n * a.top_k, tiles = std::min(pairs, pairs / T::BM + std::min(a.n_experts, pairs));
     const int outs = UP ? a.ffn : a.hidden, per = UP ? T::BN / 2 : T::BN;
-    k<<<(tiles + 7) / 8 * 8 * ((outs + per - 1) / per), T::kThreads, T::kLds, s>>>(a, w);
+    const int round = 8 * kMoeGroup;
+    k<<<(tiles + round - 1) / round * round * ((outs + per - 1) / per), T::kThreads, T::kLds, s>>>(a, w);
     return hipGetLastError();
 }
 
-template <int WM, int WN, int WK, int MT, int DT>
+template <int MT, int DT>
 static hipError_t moe_tiles(const MoeArgs& a, const MoeWs& w, hipStream_t s) {
-    constexpr int P = DT ? 1 : 2, BKB = WK == 2 || P == 1 ? 2 : 1, BKB2 = WK == 2 ? 2 : 1;  // (two parts of 64 columns: half the workgroups a CU)
-    k_moe_group<<<1, 1024, 0, s>>>(a, w, WM * MT * 32);
-    k_moe_rows<DT, P><<<a.n, 256, 0, s>>>(a.x, a.x_stride, a.hidden, (a.hidden + 63) & ~63, w.x16, w.x_part, w.x_shift);
-    if (const hipError_t e = moe_gemm<P, WM, WN, WK, MT, BKB, true>(a, w, s)) return e;
-    k_moe_rows<0, 2><<<a.n * a.top_k, 256, 0, s>>>(w.h, a.ffn, a.ffn, (a.ffn + 63) & ~63, w.h16, w.h_part, w.h_shift);
-    if (const hipError_t e = moe_gemm<2, WM, WN, WK, MT, BKB2, false>(a, w, s)) return e;
+    // as many stages of activations as leave a CU two workgroups
+    constexpr int P = DT ? 1 : 2, ST = P * MT > 2 ? 2 : 3, ST2 = MT > 1 ? 2 : 3;
+    k_moe_begin<DT, P><<<1 + (a.n + 3) / 4, 1024, 0, s>>>(a, w, MT * 32);
+    if (const hipError_t e = moe_gemm<P, MT, ST, true>(a, w, s)) return e;
+    k_moe_mid<<<a.n * a.top_k, 256, 0, s>>>(a, w);
+    if (const hipError_t e = moe_gemm<2, MT, ST2, false>(a, w, s)) return e;
     k_moe_combine<DT><<<dim3(a.n, (a.hidden + 1023) / 1024), 256, 0, s>>>(a, w);
     return hipGetLastError();
 }
@@ -581,9 +626,8 @@ static hipError_t moe_grouped(MoeArgs a, uint8_t* workspace, hipStream_t s) {
         b.ids = a.ids + (size_t)t * a.top_k, b.weights = a.weights + (size_t)t * a.top_k;
         const long long rows = (long long)b.n * a.top_k / a.n_experts;  // a mean expert's
         hipError_t e;
-        if (rows >= 96) e = moe_tiles<2, 2, 1, 2, DT>(b, w, s);
-        else if (rows >= 24) e = moe_tiles<2, 2, 1, 1, DT>(b, w, s);
-        else e = moe_tiles<1, 2, 2, 1, DT>(b, w, s);
+        if (rows >= 24) e = moe_tiles<2, DT>(b, w, s);
+        else e = moe_tiles<1, DT>(b, w, s);
         if (e) return e;
     }
     return hipSuccess;
