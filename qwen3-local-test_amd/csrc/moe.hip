@@ -168,13 +168,11 @@ __global__ __launch_bounds__(256) void k_moe_pair_down(MoeArgs a) {
 // Operands: an int8 weight is exact in fp16. A row of activations is scaled by the power of two that puts its largest
 // magnitude into [2^14, 2^15) and becomes the sum of two fp16 (within 2^-22, small values within 2^-39 of the row's
 // largest; one is enough for a bf16 x). The block scales multiply each 32-column product in fp32.
-// (an expert's rows in whatever order the sort's counters gave them: a row's result does not depend on the rows beside it)
 
 struct MoeTile {
     int expert, row, rows;
 };
 struct MoeWs {
-    int* n_tiles;
     MoeTile* tiles;
     int *row_tok, *pair_row;   // sorted row -> token, pair -> sorted row (-1: no expert)
     float* row_weight;         // sorted row -> its pair's weight
@@ -183,64 +181,56 @@ struct MoeWs {
     size_t x_part, h_part;     // elements of a part
     float* h;                  // [row][ffn]
     float* y;                  // [row][hidden]
-    int max_tiles;             // room in tiles
+    int max_tiles;             // tiles in use: pairs / BM + n_experts, some of them without rows
 };
 
-// The pairs sorted by expert, by one workgroup. A lane's ids of 16 K pairs are loaded together: one after the other their
-// latencies took 46 us for 16,384 pairs.
-constexpr int kGroupIds = 16;
+// The sort, a workgroup an expert: it counts the pairs of lower experts (its first row) and its own, and writes its own down
+// in their order; a wave goes through a quarter of the ids, 64 x kSortIds at a time. (One workgroup with counters in the
+// LDS took 28 us for 16,384 pairs.) An expert whose rows start at r has the tiles from r / BM + expert on: apart from
+// every other expert's without knowing their counts; the ones it does not need, up to the next expert's, get no rows.
+constexpr int kSortIds = 16;
 
-__device__ __forceinline__ void moe_group(const MoeArgs& a, const MoeWs& ws, int bm) {
-    __shared__ int count[1024], part[2][16];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, pairs = a.n * a.top_k;
-    int id[kGroupIds];
-    auto load = [&](int i0) {  // -1: no expert
+__device__ __forceinline__ void moe_sort(const MoeArgs& a, const MoeWs& ws, int bm, int e) {
+    __shared__ int own[4], low[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, pairs = a.n * a.top_k;
+    const int per = (pairs + 3) / 4, first = wave * per, last = min(first + per, pairs);
+    int id[kSortIds];
+    auto load = [&](int i0) {  // -1 past the wave's part
 #pragma unroll
-        for (int u = 0; u < kGroupIds; u++) {
-            const int i = i0 + u * 1024 + tid, e = a.ids[min(i, pairs - 1)];
-            id[u] = i < pairs && e >= 0 && e < a.n_experts ? e : -1;
+        for (int u = 0; u < kSortIds; u++) {
+            const int i = i0 + u * 64 + lane, v = a.ids[min(i, pairs - 1)];
+            id[u] = i < last ? v : -1;
         }
     };
-    count[tid] = 0;
-    load(0);
-    __syncthreads();
-    for (int i0 = 0; i0 < pairs; i0 += kGroupIds * 1024) {
-        if (i0) load(i0);
+    int n_own = 0, n_low = 0;
+    for (int i0 = first; i0 < last; i0 += 64 * kSortIds) {
+        load(i0);
 #pragma unroll
-        for (int u = 0; u < kGroupIds; u++)
-            if (id[u] >= 0) atomicAdd(&count[id[u]], 1);
-    }
-    __syncthreads();
-    const int mine = count[tid], tiles = (mine + bm - 1) / bm;
-    int rows = mine, tile = tiles;  // running sums over the experts
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) {
-        const int r = __shfl_up(rows, s), q = __shfl_up(tile, s);
-        if (lane >= s) rows += r, tile += q;
-    }
-    if (lane == 63) part[0][wave] = rows, part[1][wave] = tile;
-    __syncthreads();
-    for (int w = 0; w < wave; w++) rows += part[0][w], tile += part[1][w];
-    rows -= mine, tile -= tiles;
-    for (int i = 0; i < tiles; i++) ws.tiles[tile + i] = MoeTile{tid, rows + i * bm, min(bm, mine - i * bm)};
-    if (tid == 1023) *ws.n_tiles = tile + tiles;
-    count[tid] = rows;
-    __syncthreads();
-    for (int i0 = 0; i0 < pairs; i0 += kGroupIds * 1024) {
-        if (pairs > kGroupIds * 1024) load(i0);
-        int r[kGroupIds];
-        float wt[kGroupIds];
-#pragma unroll
-        for (int u = 0; u < kGroupIds; u++) {
-            wt[u] = a.weights[min(i0 + u * 1024 + tid, pairs - 1)];
-            r[u] = id[u] >= 0 ? atomicAdd(&count[id[u]], 1) : -1;
+        for (int u = 0; u < kSortIds; u++) {
+            n_own += __builtin_popcountll(__ballot(id[u] == e));
+            n_low += __builtin_popcountll(__ballot(id[u] >= 0 && id[u] < e));
         }
+    }
+    if (lane == 0) own[wave] = n_own, low[wave] = n_low;
+    __syncthreads();
+    const int row0 = low[0] + low[1] + low[2] + low[3], rows = own[0] + own[1] + own[2] + own[3];
+    int at = row0;
+    for (int w = 0; w < wave; w++) at += own[w];
+    const int t0 = row0 / bm + e, t1 = e == a.n_experts - 1 ? ws.max_tiles : (row0 + rows) / bm + e + 1;
+    for (int t = t0 + threadIdx.x; t < t1; t += 256)
+        ws.tiles[t] = MoeTile{e, row0 + (t - t0) * bm, max(0, min(bm, rows - (t - t0) * bm))};
+    if (rows == 0) return;
+    for (int i0 = first; i0 < last; i0 += 64 * kSortIds) {
+        if (last - first > 64 * kSortIds) load(i0);
 #pragma unroll
-        for (int u = 0; u < kGroupIds; u++) {
-            const int i = i0 + u * 1024 + tid;
-            if (i >= pairs) break;
-            ws.pair_row[i] = r[u];
-            if (r[u] >= 0) ws.row_tok[r[u]] = i / a.top_k, ws.row_weight[r[u]] = wt[u];
+        for (int u = 0; u < kSortIds; u++) {
+            const uint64_t hit = __ballot(id[u] == e);
+            if (hit == 0) continue;
+            if (id[u] == e) {
+                const int i = i0 + u * 64 + lane, r = at + __builtin_popcountll(hit & ((1ull << lane) - 1));
+                ws.pair_row[i] = r, ws.row_tok[r] = i / a.top_k, ws.row_weight[r] = a.weights[i];
+            }
+            at += __builtin_popcountll(hit);
         }
     }
 }
@@ -249,18 +239,16 @@ __device__ __forceinline__ void moe_group(const MoeArgs& a, const MoeWs& ws, int
 // row, `lane` of them this one; `most`: four floats of the LDS.
 template <int DT, int P>
 __device__ __forceinline__ void moe_row(const void* x, size_t stride, int cols, int padded, f16* out, size_t part, int* shift,
-                                        size_t row, int lane, float* most, bool there) {
+                                        size_t row, int lane, float* most) {
     float v[8], m = 0.f;
-    if (there)
-        for (int c = lane * 8; c < cols; c += 2048) {
-            load_vec<DT, 8>(x, row * stride + c, v);
+    for (int c = lane * 8; c < cols; c += 2048) {
+        load_vec<DT, 8>(x, row * stride + c, v);
 #pragma unroll
-            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
-        }
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
+    }
     m = moe_wave_max(m);
     if ((lane & 63) == 0) most[lane >> 6] = m;
     __syncthreads();
-    if (!there) return;
     m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
     // (a row with an infinity, or of zeros, is not scaled)
     const int up = m > 0.f && m < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
@@ -281,22 +269,25 @@ __device__ __forceinline__ void moe_row(const void* x, size_t stride, int cols, 
     }
 }
 
-// Workgroup 0 sorts; the others write four rows of x each.
+// The first n_experts workgroups sort; the others write a row of x each, and mark its pairs without an expert.
 template <int DT, int P>
-__global__ __launch_bounds__(1024) void k_moe_begin(MoeArgs a, MoeWs ws, int bm) {
-    __shared__ float most[4][4];
-    if (blockIdx.x == 0) {
-        moe_group(a, ws, bm);
+__global__ __launch_bounds__(256) void k_moe_begin(MoeArgs a, MoeWs ws, int bm) {
+    __shared__ float most[4];
+    if ((int)blockIdx.x < a.n_experts) {
+        moe_sort(a, ws, bm, blockIdx.x);
         return;
     }
-    const int sub = threadIdx.x >> 8, row = (blockIdx.x - 1) * 4 + sub;
-    moe_row<DT, P>(a.x, a.x_stride, a.hidden, (a.hidden + 63) & ~63, ws.x16, ws.x_part, ws.x_shift, row, threadIdx.x & 255,
-                   most[sub], row < a.n);
+    const size_t row = blockIdx.x - a.n_experts;
+    if ((int)threadIdx.x < a.top_k) {
+        const size_t i = row * a.top_k + threadIdx.x;
+        if (a.ids[i] < 0 || a.ids[i] >= a.n_experts) ws.pair_row[i] = -1;
+    }
+    moe_row<DT, P>(a.x, a.x_stride, a.hidden, (a.hidden + 63) & ~63, ws.x16, ws.x_part, ws.x_shift, row, threadIdx.x, most);
 }
 // Rows of h.
 __global__ __launch_bounds__(256) void k_moe_mid(MoeArgs a, MoeWs ws) {
     __shared__ float most[4];
-    moe_row<0, 2>(ws.h, a.ffn, a.ffn, (a.ffn + 63) & ~63, ws.h16, ws.h_part, ws.h_shift, blockIdx.x, threadIdx.x, most, true);
+    moe_row<0, 2>(ws.h, a.ffn, a.ffn, (a.ffn + 63) & ~63, ws.h16, ws.h_part, ws.h_shift, blockIdx.x, threadIdx.x, most);
 }
 
 __device__ __forceinline__ f32x16 mfma32h(f16x8 a, f16x8 b, f32x16 c) {
@@ -348,8 +339,9 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(MoeArgs a, MoeWs ws) {
     const int outs = UP ? a.ffn : a.hidden, cols = UP ? a.hidden : a.ffn, per = UP ? BN / 2 : BN;
     const int nn = (outs + per - 1) / per, seq = blockIdx.x >> 3, in = seq % (nn * kMoeGroup);
     const int tile = (seq / (nn * kMoeGroup) * 8 + (blockIdx.x & 7)) * kMoeGroup + in % kMoeGroup, n0 = in / kMoeGroup * per;
-    const MoeTile mt = ws.tiles[min(tile, ws.max_tiles - 1)];
-    if (tile >= *ws.n_tiles) return;
+    if (tile >= ws.max_tiles) return;
+    const MoeTile mt = ws.tiles[tile];
+    if (mt.rows == 0) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c = lane & 31, h = lane >> 5;
     const int padded = (cols + 63) & ~63, nkb = cols >> 5, steps = padded >> 6;
@@ -561,9 +553,7 @@ static size_t lay_out(const MoeArgs& a, int parts, uint8_t* base, MoeWs& w) {
         p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(reinterpret_cast<uintptr_t>(base) + at);
         at += up256(bytes);
     };
-    take(w.n_tiles, 4);
-    w.max_tiles = (int)(pairs / 32) + a.n_experts + 1;
-    take(w.tiles, w.max_tiles * sizeof(MoeTile));
+    take(w.tiles, (pairs / 32 + a.n_experts) * sizeof(MoeTile));
     take(w.row_tok, pairs * 4), take(w.pair_row, pairs * 4), take(w.row_weight, pairs * 4), take(w.x_shift, n * 4), take(w.h_shift, pairs * 4);
     take(w.x16, parts * n * hp * 2), take(w.h16, 2 * pairs * fp * 2);
     w.x_part = n * hp, w.h_part = pairs * fp;
@@ -592,19 +582,18 @@ static hipError_t moe_gemm(const MoeArgs& a, const MoeWs& w, hipStream_t s) {
     static std::atomic<uint64_t> raised{0};
     const auto k = &k_moe_gemm<P, MT, ST, UP>;
     if (const hipError_t e = raise_lds(reinterpret_cast<const void*>(k), T::kLds, raised)) return e;
-    // the most tiles that the pairs can make (workgroups past the real number end at once)
-    const int pairs = a.n * a.top_k, tiles = std::min(pairs, pairs / T::BM + std::min(a.n_experts, pairs));
     const int outs = UP ? a.ffn : a.hidden, per = UP ? T::BN / 2 : T::BN;
     const int round = 8 * kMoeGroup;
-    k<<<(tiles + round - 1) / round * round * ((outs + per - 1) / per), T::kThreads, T::kLds, s>>>(a, w);
+    k<<<(w.max_tiles + round - 1) / round * round * ((outs + per - 1) / per), T::kThreads, T::kLds, s>>>(a, w);
     return hipGetLastError();
 }
 
 template <int MT, int DT>
-static hipError_t moe_tiles(const MoeArgs& a, const MoeWs& w, hipStream_t s) {
+static hipError_t moe_tiles(const MoeArgs& a, MoeWs w, hipStream_t s) {
     // as many stages of activations as leave a CU two workgroups
     constexpr int P = DT ? 1 : 2, ST = P * MT > 2 ? 2 : 3, ST2 = MT > 1 ? 2 : 3;
-    k_moe_begin<DT, P><<<1 + (a.n + 3) / 4, 1024, 0, s>>>(a, w, MT * 32);
+    w.max_tiles = a.n * a.top_k / (MT * 32) + a.n_experts;
+    k_moe_begin<DT, P><<<a.n_experts + a.n, 256, 0, s>>>(a, w, MT * 32);
     if (const hipError_t e = moe_gemm<P, MT, ST, true>(a, w, s)) return e;
     k_moe_mid<<<a.n * a.top_k, 256, 0, s>>>(a, w);
     if (const hipError_t e = moe_gemm<2, MT, ST2, false>(a, w, s)) return e;
