@@ -203,9 +203,11 @@ _ROW_DT = {torch.float32: F32, torch.bfloat16: BF16}
 def _check_seq_rows(t, name, shape, dtype):
     """Row stride of a [n_seq, n, ...] operand of the linear-attention operators: `shape`, dtype, its rows (all but the
     first two dims) contiguous, row b * n + t at one stride."""
-    if t.dtype != dtype or t.shape != shape:
+    if t.dtype is not dtype or t.shape != shape:
         raise ValueError(f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
     stride, inner = t.stride(), 1
+    if len(stride) == 4 and stride[3] == 1 and stride[2] == shape[3] and stride[0] == shape[1] * stride[1]:
+        return stride[1]
     for d in range(len(shape) - 1, 1, -1):
         if stride[d] != inner and shape[d] != 1:
             raise ValueError(f"{name}: the elements of a row must be contiguous, got strides {stride}")
@@ -216,9 +218,17 @@ def _check_seq_rows(t, name, shape, dtype):
     return row
 
 
+def _check_matrix(t, name, shape, dtype):
+    """Row stride of a [n, width] operand of exactly `shape` and dtype with contiguous rows."""
+    stride = t.stride()
+    if t.dtype is not dtype or t.shape != shape or (stride[1] != 1 and shape[1] != 1):
+        raise ValueError(f"{name} must be {dtype} {shape} with contiguous rows, got {t.dtype} {tuple(t.shape)}")
+    return stride[0] if shape[0] > 1 else shape[1]
+
+
 def _check_whole(t, name, shape, dtype=torch.float32):
     """A contiguous operand of exactly `shape` and dtype."""
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -263,6 +273,7 @@ class Attention:
         self.cfg = Config(n_heads, n_kv_heads, head_dim, rope_dim, rope_theta, rms_eps, max_ctx, max_tokens,
                           max_splits)
         self.device = device
+        self._torch_device = torch.device("cuda", device)
         h = ctypes.c_void_p()
         rc = self.lib.qwattn_create(ctypes.byref(h), device, ctypes.byref(self.cfg))
         if rc:
@@ -411,12 +422,13 @@ class Attention:
     def _on_device(self, tensors, stream):
         """The stream's handle, once every operand is known to be on this context's GPU (the device's current stream
         where none is given)."""
+        device = self.device
         for t in tensors:
-            if t is not None and (not t.is_cuda or t.get_device() != self.device):
+            if t is not None and t.get_device() != device:  # (-1: the CPU)
                 raise ValueError(f"operands must be on cuda:{self.device}, got one on {t.device}")
         if stream is not None:
             return stream.cuda_stream
-        return _raw_stream(self.device) if _raw_stream else torch.cuda.current_stream(self.device).cuda_stream
+        return _raw_stream(device) if _raw_stream else torch.cuda.current_stream(self.device).cuda_stream
 
     def _workspace(self, size, given, stream):
         """(address, bytes) of the caller's workspace tensor, or of one from torch's allocator, and the tensor itself,
@@ -427,7 +439,7 @@ class Attention:
             return given.data_ptr(), given.numel() * given.element_size(), given
         if not size:
             return 0, 0, None
-        t = torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
+        t = torch.empty(size, dtype=torch.uint8, device=self._torch_device)
         if stream is not None:
             t.record_stream(stream)
         return t.data_ptr(), size, t
@@ -464,26 +476,32 @@ class Attention:
         if v.dtype not in _ROW_DT or len(v.shape) != 4 or len(k.shape) != 4:
             raise ValueError(f"k and v must be float32 or bfloat16 [n_seq, n, heads, dim], got {v.dtype}, "
                              f"{tuple(k.shape)}, {tuple(v.shape)}")
-        n_seq, n, hv, dv = v.shape
-        hk, dk = k.shape[2], k.shape[3]
+        shape, dtype = v.shape, v.dtype
+        n_seq, n, hv, dv = shape
+        _, _, hk, dk = k.shape
         qk = (n_seq, n, hk, dk)
-        q_stride, k_stride = _check_seq_rows(q, "q", qk, v.dtype), _check_seq_rows(k, "k", qk, v.dtype)
-        v_stride = _check_seq_rows(v, "v", v.shape, v.dtype)
-        out_stride = _check_seq_rows(out, "out", v.shape, v.dtype)
-        z_stride = _check_seq_rows(z, "z", v.shape, v.dtype) if z is not None else 0
-        _check_whole(a, "a", (n_seq, n, hv))
-        _check_whole(b, "b", (n_seq, n, hv))
+        q_stride, k_stride = _check_seq_rows(q, "q", qk, dtype), _check_seq_rows(k, "k", qk, dtype)
+        v_stride = _check_seq_rows(v, "v", shape, dtype)
+        out_stride = _check_seq_rows(out, "out", shape, dtype)
+        z_stride = _check_seq_rows(z, "z", shape, dtype) if z is not None else 0
+        gates, heads = (n_seq, n, hv), (hv,)
+        _check_whole(a, "a", gates)
+        _check_whole(b, "b", gates)
         _check_whole(state, "state", (n_seq, hv, dk, dv))
-        for t, name, shape in ((a_coef, "a_coef", (hv,)), (dt_bias, "dt_bias", (hv,)), (gamma, "gamma", (dv,)),
-                               (snap, "snap", (n_seq, n, hv, dk, dv))):
-            if t is not None:
-                _check_whole(t, name, shape)
+        if a_coef is not None:
+            _check_whole(a_coef, "a_coef", heads)
+        if dt_bias is not None:
+            _check_whole(dt_bias, "dt_bias", heads)
+        if gamma is not None:
+            _check_whole(gamma, "gamma", (dv,))
+        if snap is not None:
+            _check_whole(snap, "snap", (n_seq, n, hv, dk, dv))
         if lens is not None:
             _check_whole(lens, "lens", (n_seq,), torch.int32)
         s = self._on_device((q, k, v, a, b, state, out, a_coef, dt_bias, z, gamma, lens, snap, workspace), stream)
-        size = delta_workspace(n_seq, n, hk, hv, dk, dv, v.dtype, z is not None, snap is not None)
-        ws, ws_bytes, keep = self._workspace(size, workspace, stream)
-        args = _DELTA.pack(n_seq, n, hk, hv, dk, dv, int(tiled), _ROW_DT[v.dtype], _ptr(lens) or 0, q.data_ptr(),
+        size = delta_workspace(n_seq, n, hk, hv, dk, dv, dtype, z is not None, snap is not None)
+        ws, ws_bytes, keep = self._workspace(size, workspace, stream) if size or workspace is not None else (0, 0, None)
+        args = _DELTA.pack(n_seq, n, hk, hv, dk, dv, int(tiled), _ROW_DT[dtype], _ptr(lens) or 0, q.data_ptr(),
                            k.data_ptr(), v.data_ptr(), q_stride, k_stride, v_stride, a.data_ptr(), b.data_ptr(),
                            _ptr(a_coef) or 0, _ptr(dt_bias) or 0, state.data_ptr(), _ptr(snap) or 0, _ptr(z) or 0,
                            z_stride, _ptr(gamma) or 0, out.data_ptr(), out_stride, ws, ws_bytes)
@@ -511,19 +529,23 @@ class Attention:
             raise ValueError(f"x must be float32 or bfloat16 [n, hidden], ids [n, top_k] and gate [n_experts, ffn, hidden], "
                              f"got {x.dtype} {tuple(x.shape)}, {tuple(ids.shape)}, {tuple(w.shape)}")
         (n, top_k), (experts, ffn, hidden) = ids.shape, w.shape
-        for (q, s), name, r, c in ((gate, "gate", ffn, hidden), (up, "up", ffn, hidden), (down, "down", hidden, ffn)):
-            _check_whole(q, name, (experts, r, c), _I8)
-            _check_whole(s, f"{name}'s scales", (experts, r, c // 32))
-        x_stride = _check_seq_rows(x[None], "x", (1, n, hidden), x.dtype)
-        y_stride = _check_seq_rows(y[None], "y", (1, n, hidden), x.dtype)
+        wide, narrow = (experts, ffn, hidden), (experts, ffn, hidden // 32)
+        _check_whole(w, "gate", wide, _I8)
+        _check_whole(gate[1], "gate's scales", narrow)
+        _check_whole(up[0], "up", wide, _I8)
+        _check_whole(up[1], "up's scales", narrow)
+        _check_whole(down[0], "down", (experts, hidden, ffn), _I8)
+        _check_whole(down[1], "down's scales", (experts, hidden, ffn // 32))
+        dtype, rows = x.dtype, (n, hidden)
+        x_stride, y_stride = _check_matrix(x, "x", rows, dtype), _check_matrix(y, "y", rows, dtype)
         _check_whole(ids, "ids", (n, top_k), torch.int32)
         _check_whole(weights, "weights", (n, top_k))
         s = self._on_device((x, ids, weights, *gate, *up, *down, y, workspace), stream)
-        size = moe_workspace(experts, hidden, ffn, x.dtype, n, top_k)
+        size = moe_workspace(experts, hidden, ffn, dtype, n, top_k)
         ws, ws_bytes, keep = self._workspace(size, workspace, stream)
         layer = _MOE_LAYER.pack(experts, hidden, ffn, gate[0].data_ptr(), up[0].data_ptr(), down[0].data_ptr(),
                                 gate[1].data_ptr(), up[1].data_ptr(), down[1].data_ptr())
-        self._check(self.lib.qwattn_moe(self.h, s, layer, x.data_ptr(), _ROW_DT[x.dtype], x_stride, ids.data_ptr(),
+        self._check(self.lib.qwattn_moe(self.h, s, layer, x.data_ptr(), _ROW_DT[dtype], x_stride, ids.data_ptr(),
                                         weights.data_ptr(), top_k, y.data_ptr(), y_stride, n, ws, ws_bytes))
 
     def qsa_key_bits(self, mask, cr, pos, n, key_bits, stream=None):

@@ -185,15 +185,15 @@ struct MoeWs {
 };
 
 // The sort, a workgroup an expert: it counts the pairs of lower experts (its first row) and its own, and writes its own down
-// in their order; a wave goes through a quarter of the ids, 64 x kSortIds at a time. (One workgroup with counters in the
+// in their order; a wave goes through a sixteenth of the ids, 64 x kSortIds at a time. (One workgroup with counters in the
 // LDS took 28 us for 16,384 pairs.) An expert whose rows start at r has the tiles from r / BM + expert on: apart from
 // every other expert's without knowing their counts; the ones it does not need, up to the next expert's, get no rows.
 constexpr int kSortIds = 16;
 
 __device__ __forceinline__ void moe_sort(const MoeArgs& a, const MoeWs& ws, int bm, int e) {
-    __shared__ int own[4], low[4];
+    __shared__ int own[16], low[16];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, pairs = a.n * a.top_k;
-    const int per = (pairs + 3) / 4, first = wave * per, last = min(first + per, pairs);
+    const int per = (pairs + 15) / 16, first = wave * per, last = min(first + per, pairs);
     int id[kSortIds];
     auto load = [&](int i0) {  // -1 past the wave's part
 #pragma unroll
@@ -213,11 +213,15 @@ __device__ __forceinline__ void moe_sort(const MoeArgs& a, const MoeWs& ws, int 
     }
     if (lane == 0) own[wave] = n_own, low[wave] = n_low;
     __syncthreads();
-    const int row0 = low[0] + low[1] + low[2] + low[3], rows = own[0] + own[1] + own[2] + own[3];
-    int at = row0;
-    for (int w = 0; w < wave; w++) at += own[w];
+    int row0 = 0, rows = 0, at = 0;
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        row0 += low[w], rows += own[w];
+        if (w < wave) at += own[w];
+    }
+    at += row0;
     const int t0 = row0 / bm + e, t1 = e == a.n_experts - 1 ? ws.max_tiles : (row0 + rows) / bm + e + 1;
-    for (int t = t0 + threadIdx.x; t < t1; t += 256)
+    for (int t = t0 + threadIdx.x; t < t1; t += 1024)
         ws.tiles[t] = MoeTile{e, row0 + (t - t0) * bm, max(0, min(bm, rows - (t - t0) * bm))};
     if (rows == 0) return;
     for (int i0 = first; i0 < last; i0 += 64 * kSortIds) {
@@ -239,16 +243,18 @@ __device__ __forceinline__ void moe_sort(const MoeArgs& a, const MoeWs& ws, int 
 // row, `lane` of them this one; `most`: four floats of the LDS.
 template <int DT, int P>
 __device__ __forceinline__ void moe_row(const void* x, size_t stride, int cols, int padded, f16* out, size_t part, int* shift,
-                                        size_t row, int lane, float* most) {
+                                        size_t row, int lane, float* most, bool there) {
     float v[8], m = 0.f;
-    for (int c = lane * 8; c < cols; c += 2048) {
-        load_vec<DT, 8>(x, row * stride + c, v);
+    if (there)
+        for (int c = lane * 8; c < cols; c += 2048) {
+            load_vec<DT, 8>(x, row * stride + c, v);
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
-    }
+            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
+        }
     m = moe_wave_max(m);
     if ((lane & 63) == 0) most[lane >> 6] = m;
     __syncthreads();
+    if (!there) return;
     m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
     // (a row with an infinity, or of zeros, is not scaled)
     const int up = m > 0.f && m < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
@@ -269,25 +275,27 @@ __device__ __forceinline__ void moe_row(const void* x, size_t stride, int cols, 
     }
 }
 
-// The first n_experts workgroups sort; the others write a row of x each, and mark its pairs without an expert.
+// The first n_experts workgroups sort; the others write four rows of x each, and mark their pairs without an expert.
 template <int DT, int P>
-__global__ __launch_bounds__(256) void k_moe_begin(MoeArgs a, MoeWs ws, int bm) {
-    __shared__ float most[4];
+__global__ __launch_bounds__(1024) void k_moe_begin(MoeArgs a, MoeWs ws, int bm) {
+    __shared__ float most[4][4];
     if ((int)blockIdx.x < a.n_experts) {
         moe_sort(a, ws, bm, blockIdx.x);
         return;
     }
-    const size_t row = blockIdx.x - a.n_experts;
-    if ((int)threadIdx.x < a.top_k) {
-        const size_t i = row * a.top_k + threadIdx.x;
+    const int sub = threadIdx.x >> 8, lane = threadIdx.x & 255;
+    const size_t row = (size_t)(blockIdx.x - a.n_experts) * 4 + sub;
+    const bool there = row < (size_t)a.n;
+    if (there && lane < a.top_k) {
+        const size_t i = row * a.top_k + lane;
         if (a.ids[i] < 0 || a.ids[i] >= a.n_experts) ws.pair_row[i] = -1;
     }
-    moe_row<DT, P>(a.x, a.x_stride, a.hidden, (a.hidden + 63) & ~63, ws.x16, ws.x_part, ws.x_shift, row, threadIdx.x, most);
+    moe_row<DT, P>(a.x, a.x_stride, a.hidden, (a.hidden + 63) & ~63, ws.x16, ws.x_part, ws.x_shift, row, lane, most[sub], there);
 }
 // Rows of h.
 __global__ __launch_bounds__(256) void k_moe_mid(MoeArgs a, MoeWs ws) {
     __shared__ float most[4];
-    moe_row<0, 2>(ws.h, a.ffn, a.ffn, (a.ffn + 63) & ~63, ws.h16, ws.h_part, ws.h_shift, blockIdx.x, threadIdx.x, most);
+    moe_row<0, 2>(ws.h, a.ffn, a.ffn, (a.ffn + 63) & ~63, ws.h16, ws.h_part, ws.h_shift, blockIdx.x, threadIdx.x, most, true);
 }
 
 __device__ __forceinline__ f32x16 mfma32h(f16x8 a, f16x8 b, f32x16 c) {
@@ -593,7 +601,7 @@ static hipError_t moe_tiles(const MoeArgs& a, MoeWs w, hipStream_t s) {
     // as many stages of activations as leave a CU two workgroups
     constexpr int P = DT ? 1 : 2, ST = P * MT > 2 ? 2 : 3, ST2 = MT > 1 ? 2 : 3;
     w.max_tiles = a.n * a.top_k / (MT * 32) + a.n_experts;
-    k_moe_begin<DT, P><<<a.n_experts + a.n, 256, 0, s>>>(a, w, MT * 32);
+    k_moe_begin<DT, P><<<a.n_experts + (a.n + 3) / 4, 1024, 0, s>>>(a, w, MT * 32);
     if (const hipError_t e = moe_gemm<P, MT, ST, true>(a, w, s)) return e;
     k_moe_mid<<<a.n * a.top_k, 256, 0, s>>>(a, w);
     if (const hipError_t e = moe_gemm<2, MT, ST2, false>(a, w, s)) return e;
