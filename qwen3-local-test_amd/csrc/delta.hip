@@ -511,7 +511,8 @@ template <int DT, int DK, int DV, bool O32>  // O32: the output goes to the work
 __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, int c0, int ncs) {
     constexpr int NP = DT ? 1 : 3, KS = DK / 32;
     typedef KqUnit<DK, NP> Unit;
-    __shared__ __attribute__((aligned(16))) uint8_t sS[KS][3][1024], sX[2][3][1024], sU[2][3][1024], sW[2][3][1024];
+    __shared__ __attribute__((aligned(16))) uint8_t sS[KS][3][1024], sX[2][3][1024], sW[2][3][1024];
+    __shared__ f32x4 sU[4][64];  // U as it leaves the accumulators
     // a head's slices at block numbers apart by the number of heads: on one XCD where that is a multiple of eight
     const int units = a.v_heads * a.n_seq, hu = blockIdx.x % units, slice = blockIdx.x / units;
     const int h = hu % a.v_heads, b = hu / a.v_heads, kh = key_head(a, h);
@@ -554,23 +555,21 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
 #pragma unroll
         for (int p = 0; p < 3; p++) b[p] = frag(from[p]);
     };
-    auto rows_times_state = [&](f32x4 (&acc)[3]) {
+    // (selects: a branch between matrix instructions and the readers of their results was seen to lose the waits between)
+    auto move_on = [&](bool more) {
+        kq += more ? kq_step : 0, tp += more ? tp_step : 0, vec += more ? vec_step : 0;
+    };
+    const uint32_t later = wave < 2 ? 0 : 0xFFFFFFFFu;  // the second 32 tokens are behind row tiles 0 and 1: as zeros
+    // K S or Q S of this wave's row tile. The next loads that `meanwhile` issues go out while the LDS answers (here and
+    // below), not when another wave may wait for this one.
+    auto rows_times_state = [&](f32x4 (&acc)[3], auto meanwhile) {
+        bf16x8 bs[KS][3];
+#pragma unroll
+        for (int s = 0; s < KS; s++) get(sS[s], bs[s]);
+        meanwhile();
         zero(acc);
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            bf16x8 bs[3];
-            get(sS[s], bs);
-            mfma_parts<NP>(fR[s], bs, acc);
-        }
-    };
-    auto tri_times = [&](const uint8_t (&from)[2][3][1024], f32x4 (&acc)[3]) {
-        bf16x8 bx[3];
-        get(from[0], bx);
-        mfma_parts<3>(fM[0], bx, acc);
-        if (wave >= 2) {
-            get(from[1], bx);
-            mfma_parts<3>(fM[1], bx, acc);
-        }
+        for (int s = 0; s < KS; s++) mfma_parts<NP>(fR[s], bs[s], acc);
     };
 
     if (wave8 >= 4) {
@@ -582,9 +581,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         load_rows(kq + Unit::kOne), load_tri(tp + kTpOne), vq = vec4(2);
 #pragma unroll 1
         for (int ch = 0; ch < nc; ch++) {
-            if (ch + 1 < nc) kq += kq_step, tp += tp_step, vec += vec_step;
+            move_on(ch + 1 < nc);
             lds_barrier();
-            rows_times_state(acc);
+            rows_times_state(acc, [] {});
             load_rows(kq + Unit::kOne);
             f32x4 qs;
 #pragma unroll
@@ -594,7 +593,18 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
             zero(acc);
             acc[0] = qs;
             lds_barrier();
-            tri_times(sU, acc);
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                const f32x4 u0 = sU[2 * st][lane], u1 = sU[2 * st + 1][lane];
+                float v[8] = {u0[0], u0[1], u0[2], u0[3], u1[0], u1[1], u1[2], u1[3]};
+                if (st == 1)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = __uint_as_float(__float_as_uint(v[e]) & later);
+                u32x4 w[3];
+                split3(v, w);
+                const bf16x8 bu[3] = {__builtin_bit_cast(bf16x8, w[0]), __builtin_bit_cast(bf16x8, w[1]), __builtin_bit_cast(bf16x8, w[2])};
+                mfma_parts<3>(fM[st], bu, acc);
+            }
             load_tri(tp + kTpOne);
             const int more = left - ch * kChunk - tok;
 #pragma unroll
@@ -633,10 +643,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
     };
     auto load_x = [&](int ch) {
         vb = vec4(0), vk = vec4(1);
-        const int most = left - 1 - ch * kChunk;
-        if (most < kChunk - 1)  // past the last row: that one (beta is 0 there)
+        const int most = left - 1 - ch * kChunk;  // past the last row: that one (beta is 0 there)
 #pragma unroll
-            for (int i = 0; i < 4; i++) at[i] = min(tok + i, most) * a.v_stride + c;
+        for (int i = 0; i < 4; i++) at[i] = min(tok + i, most) * a.v_stride + c;
 #pragma unroll
         for (int i = 0; i < 4; i++)
             val[i] = DT ? static_cast<const uint16_t*>(a.v)[first + at[i]] : static_cast<const uint32_t*>(a.v)[first + at[i]];
@@ -658,27 +667,43 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         for (int p = 0; p < 3; p++)
             *reinterpret_cast<u32x2*>(to[wave >> 1][p] + lane16 + (wave & 1) * 8) = u32x2{lo[p], hi[p]};
     };
-    load_rows(kq), load_x(0), load_tri(tp), load_kt();
+    load_rows(kq), load_x(0), load_tri(tp);
     put_state();
+    __builtin_amdgcn_s_setprio(2);  // ahead of the output waves
 #pragma unroll 1
     for (int ch = 0; ch < nc; ch++) {
-        if (ch + 1 < nc) kq += kq_step, tp += tp_step, vec += vec_step, first += kChunk * a.v_stride;
         lds_barrier();  // S is in the LDS
         f32x4 acc[3], x, w;
-        rows_times_state(acc);
+        rows_times_state(acc, [&] {
+            load_kt();
+            move_on(ch + 1 < nc);
+            first += ch + 1 < nc ? kChunk * a.v_stride : 0;
+        });
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] = vb[i] * __uint_as_float(DT ? val[i] << 16 : val[i]) - vk[i] * sum(acc, i);
         put_rows(sX, x);
-        load_rows(kq), load_x(min(ch + 1, nc - 1));
         lds_barrier();  // X
+        bf16x8 bx[2][3];
+        get(sX[0], bx[0]), get(sX[1], bx[1]);
+        load_rows(kq), load_x(min(ch + 1, nc - 1));
+#pragma unroll
+        for (int p = 0; p < 3; p++) {
+            u32x4 v = __builtin_bit_cast(u32x4, bx[1][p]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] &= later;
+            bx[1][p] = __builtin_bit_cast(bf16x8, v);
+        }
         zero(acc);
-        tri_times(sX, acc);
-        load_tri(tp);
+        mfma_parts<3>(fM[0], bx[0], acc);
+        mfma_parts<3>(fM[1], bx[1], acc);
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] = sum(acc, i), w[i] = vw[i] * x[i];
         put_rows(sW, w);
-        put_rows(sU, x);
+        sU[wave][lane] = x;
         lds_barrier();  // U, and with the scales of K^T's columns
+        bf16x8 bw[2][3];
+        get(sW[0], bw[0]), get(sW[1], bw[1]);
+        load_tri(tp);
         if (KS == 4 || wave < KS) {
             f32x4 s[2][3];
 #pragma unroll
@@ -688,19 +713,15 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
                 for (int i = 0; i < 4; i++) s[j][0][i] = S[j][i] * end;
             }
 #pragma unroll
-            for (int st = 0; st < 2; st++) {
-                bf16x8 bw[3];
-                get(sW[st], bw);
+            for (int st = 0; st < 2; st++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) mfma_parts<NP>(fKT[2 * j + st], bw, s[j]);
-            }
+                for (int j = 0; j < 2; j++) mfma_parts<NP>(fKT[2 * j + st], bw[st], s[j]);
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) S[j][i] = sum(s[j], i);
             put_state();  // (every wave has read the one before: it passed the barrier behind X)
         }
-        load_kt();
     }
     if (wave < KS)
 #pragma unroll
