@@ -512,7 +512,8 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
     constexpr int NP = DT ? 1 : 3, KS = DK / 32;
     typedef KqUnit<DK, NP> Unit;
     __shared__ __attribute__((aligned(16))) uint8_t sS[KS][3][1024], sX[2][3][1024], sW[2][3][1024];
-    __shared__ f32x4 sU[4][64];  // U as it leaves the accumulators
+    __shared__ f32x4 sU[4][64];      // U as it leaves the accumulators
+    __shared__ f32x4 sK[KS][4][64];  // K S by parts: [dims' wave][row tile]
     // a head's slices at block numbers apart by the number of heads: on one XCD where that is a multiple of eight
     const int units = a.v_heads * a.n_seq, hu = blockIdx.x % units, slice = blockIdx.x / units;
     const int h = hu % a.v_heads, b = hu / a.v_heads, kh = key_head(a, h);
@@ -535,14 +536,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
     const uint8_t* vec = reinterpret_cast<const uint8_t*>(ws.vec + ((size_t)b * ncs * a.v_heads + h) * kVec);
     auto frag = [&](const uint8_t* p) { return *reinterpret_cast<const bf16x8*>(p + lane16); };
     auto vec4 = [&](int which) { return *reinterpret_cast<const f32x4*>(vec + 256 * which + (uint32_t)tok * 4); };
-    bf16x8 fR[KS][NP], fM[2][3];  // K and T, or Q and P
-    auto load_rows = [&](const uint8_t* p) {
-        p += wave * (KS * 1024);
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int i = 0; i < NP; i++) fR[s][i] = frag(p + (i * 4 * KS + s) * 1024);
-    };
+    bf16x8 fM[2][3];  // T or P
     const int f0 = wave < 2 ? wave : 2 * (wave - 1), f1 = wave < 2 ? f0 : f0 + 1;  // this row tile's two steps
     auto load_tri = [&](const uint8_t* p) {
 #pragma unroll
@@ -560,31 +554,33 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         kq += more ? kq_step : 0, tp += more ? tp_step : 0, vec += more ? vec_step : 0;
     };
     const uint32_t later = wave < 2 ? 0 : 0xFFFFFFFFu;  // the second 32 tokens are behind row tiles 0 and 1: as zeros
-    // K S or Q S of this wave's row tile. The next loads that `meanwhile` issues go out while the LDS answers (here and
-    // below), not when another wave may wait for this one.
-    auto rows_times_state = [&](f32x4 (&acc)[3], auto meanwhile) {
-        bf16x8 bs[KS][3];
-#pragma unroll
-        for (int s = 0; s < KS; s++) get(sS[s], bs[s]);
-        meanwhile();
-        zero(acc);
-#pragma unroll
-        for (int s = 0; s < KS; s++) mfma_parts<NP>(fR[s], bs[s], acc);
-    };
-
     if (wave8 >= 4) {
         f32x4 vq, acc[3];
+        bf16x8 fQ[KS][NP];
+        auto load_q = [&] {
+            const uint8_t* p = kq + Unit::kOne + wave * (KS * 1024);
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int i = 0; i < NP; i++) fQ[s][i] = frag(p + (i * 4 * KS + s) * 1024);
+        };
         const size_t stride = O32 ? (size_t)a.v_heads * DV : a.out_stride;
         size_t first = row0 * stride + h * DV + 16 * slice, at[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) at[i] = (tok + i) * stride + c;
-        load_rows(kq + Unit::kOne), load_tri(tp + kTpOne), vq = vec4(2);
+        load_q(), load_tri(tp + kTpOne), vq = vec4(2);
 #pragma unroll 1
         for (int ch = 0; ch < nc; ch++) {
             move_on(ch + 1 < nc);
             lds_barrier();
-            rows_times_state(acc, [] {});
-            load_rows(kq + Unit::kOne);
+            zero(acc);
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                bf16x8 bs[3];
+                get(sS[s], bs);
+                mfma_parts<NP>(fQ[s], bs, acc);
+            }
+            load_q();
             f32x4 qs;
 #pragma unroll
             for (int i = 0; i < 4; i++) qs[i] = vq[i] * sum(acc, i);
@@ -625,13 +621,20 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         for (int j = 0; j < 2; j++)
 #pragma unroll
             for (int i = 0; i < 4; i++) S[j][i] = state[(32 * wave + 8 * g + 4 * j + i) * DV];
-    bf16x8 fKT[4][NP];
+    bf16x8 fK[4][NP], fKT[4][NP], bS[3];  // K's row tiles in this wave's dims; S as an operand
     f32x4 vb, vk, vw;
     float end;
     uint32_t val[4];  // values as they lie in memory: nothing waits for them here
     size_t first = row0 * a.v_stride + h * DV + 16 * slice, at[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) at[i] = (tok + i) * a.v_stride + c;
+    auto load_k = [&] {
+        const uint8_t* p = kq + wave % KS * 1024;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int q = 0; q < NP; q++) fK[i][q] = frag(p + (q * 4 + i) * (KS * 1024));
+    };
     auto load_kt = [&] {
         const uint8_t* p = kq + 2 * Unit::kOne + wave % KS * 4096;
 #pragma unroll
@@ -656,7 +659,10 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
             u32x4 w[3];
             split3(v, w);
 #pragma unroll
-            for (int p = 0; p < 3; p++) *reinterpret_cast<u32x4*>(sS[wave][p] + lane16) = w[p];
+            for (int p = 0; p < 3; p++) {
+                *reinterpret_cast<u32x4*>(sS[wave][p] + lane16) = w[p];  // for Q S
+                bS[p] = __builtin_bit_cast(bf16x8, w[p]);
+            }
         }
     };
     // four tokens of a column: half of a right operand's piece
@@ -667,25 +673,45 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         for (int p = 0; p < 3; p++)
             *reinterpret_cast<u32x2*>(to[wave >> 1][p] + lane16 + (wave & 1) * 8) = u32x2{lo[p], hi[p]};
     };
-    load_rows(kq), load_x(0), load_tri(tp);
+    load_k(), load_x(0), load_tri(tp);
     put_state();
     __builtin_amdgcn_s_setprio(2);  // ahead of the output waves
 #pragma unroll 1
     for (int ch = 0; ch < nc; ch++) {
-        lds_barrier();  // S is in the LDS
-        f32x4 acc[3], x, w;
-        rows_times_state(acc, [&] {
-            load_kt();
-            move_on(ch + 1 < nc);
-            first += ch + 1 < nc ? kChunk * a.v_stride : 0;
-        });
+        // every row tile's K S over this wave's dims, whose rows of S are in its registers
+        if (KS == 4 || wave < KS) {
+            f32x4 part[4][3];
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = vb[i] * __uint_as_float(DT ? val[i] << 16 : val[i]) - vk[i] * sum(acc, i);
+            for (int i = 0; i < 4; i++) zero(part[i]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) mfma_parts<NP>(fK[i], bS, part[i]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = sum(part[i], e);
+                sK[wave][i][lane] = v;
+            }
+        }
+        lds_barrier();  // K S by parts, and S
+        f32x4 acc[3], x, w, ks = sK[0][wave][lane];
+#pragma unroll
+        for (int s = 1; s < KS; s++) {
+            const f32x4 v = sK[s][wave][lane];
+#pragma unroll
+            for (int e = 0; e < 4; e++) ks[e] += v[e];
+        }
+        // (the next loads go out while the LDS answers, here and below)
+        load_kt();
+        move_on(ch + 1 < nc);
+        first += ch + 1 < nc ? kChunk * a.v_stride : 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = vb[i] * __uint_as_float(DT ? val[i] << 16 : val[i]) - vk[i] * ks[i];
         put_rows(sX, x);
         lds_barrier();  // X
         bf16x8 bx[2][3];
         get(sX[0], bx[0]), get(sX[1], bx[1]);
-        load_rows(kq), load_x(min(ch + 1, nc - 1));
+        load_k(), load_x(min(ch + 1, nc - 1));
 #pragma unroll
         for (int p = 0; p < 3; p++) {
             u32x4 v = __builtin_bit_cast(u32x4, bx[1][p]);
