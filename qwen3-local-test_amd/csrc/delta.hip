@@ -172,7 +172,8 @@ static hipError_t delta_step(const DeltaArgs& a, hipStream_t s) {
 // keep fp32's range, so nothing is scaled beforehand.
 //
 // Every operand that k_delta_chunks reads lies in the workspace as matrix-core fragments, a contiguous kilobyte each:
-//   per (sequence, chunk, key head):   K, Q  [part][16-token tile][32-dim step]   rows tokens, k dims
+//   per (sequence, chunk, key head):   K, Q  [part][16-token tile][32-dim step]   rows tokens, k dims (fp32; bf16 rows are
+//                                            operands as they lie in q and k)
 //                                      K^T   [part][32-dim step][tile 0, 1][32-token step]; row r of tile j is the dim
 //                                            8 (r / 4) + 4 j + r % 4 of its step: accumulator registers of the two
 //                                            tiles of S are then the next product's operand fragment as they stand
@@ -180,6 +181,7 @@ static hipError_t delta_step(const DeltaArgs& a, hipStream_t s) {
 //                                      five vectors: beta, and the row scales of K S, Q S and K^T U; e^(G_end)
 // Where tokens are the summed index (K^T, T, P and the X and U beside them) lane group g of a 32-token step holds the
 // tokens 4 g .. 4 g + 3 of its first 16 and of its second 16: accumulator registers again.
+// What only the output takes part in (Q S and P U) has two parts where the output is bf16: within 2^-16 beside its 2^-9.
 constexpr int kChunk = 64, kTriFrags = 6, kVec = 320;
 
 struct DeltaWs {
@@ -191,22 +193,25 @@ struct DeltaWs {
 
 template <int DK, int NP>
 struct KqUnit {
-    static constexpr int kSteps = DK / 32, kOne = NP * 4 * kSteps * 1024, kBytes = 3 * kOne;
+    static constexpr int kSteps = DK / 32, kOne = NP * 4 * kSteps * 1024;
+    static constexpr int kQ = NP == 3 ? kOne : 0, kKT = NP == 3 ? 2 * kOne : 0, kBytes = kKT + kOne;  // (K at 0)
 };
-constexpr int kTpOne = 3 * kTriFrags * 1024, kTpBytes = 2 * kTpOne;
+constexpr int kTpOne = 3 * kTriFrags * 1024;
+constexpr int out_parts(int dt) { return dt ? 2 : 3; }
+constexpr int tp_bytes(int dt) { return kTpOne + out_parts(dt) * kTriFrags * 1024; }
 
 // The six (or, with one part on the left, three) part products. Those of one order of magnitude share an accumulator:
 // three short chains instead of one long one, whose steps would wait for each other (a wave has no other on its SIMD to
 // fill the gaps).
-template <int NP>
+template <int NP, int ORDERS = 3>  // ORDERS 2: without the smallest
 __device__ __forceinline__ void mfma_parts(const bf16x8 (&a)[NP], const bf16x8 (&b)[3], f32x4 (&c)[3]) {
-    c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[2], c[2], 0, 0, 0);
+    if constexpr (ORDERS == 3) c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[2], c[2], 0, 0, 0);
     c[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[1], c[1], 0, 0, 0);
     c[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[0], c[0], 0, 0, 0);
     if constexpr (NP == 3) {
-        c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[1], c[2], 0, 0, 0);
+        if constexpr (ORDERS == 3) c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[1], c[2], 0, 0, 0);
         c[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[0], c[1], 0, 0, 0);
-        c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[2], b[0], c[2], 0, 0, 0);
+        if constexpr (ORDERS == 3) c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[2], b[0], c[2], 0, 0, 0);
     }
 }
 __device__ __forceinline__ void zero(f32x4 (&c)[3]) { c[0] = c[1] = c[2] = f32x4{0.f, 0.f, 0.f, 0.f}; }
@@ -256,11 +261,12 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
     constexpr int NP = DT ? 1 : 3, KS = DK / 32, LD = 68;  // LD: row length of the 64 x 64 matrices
     typedef KqUnit<DK, NP> Unit;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    uint8_t* fk = smem;                                        // K and Q fragments
+    uint8_t* fk = smem;                                        // K and Q fragments, and in their place:
     uint8_t* fq = fk + Unit::kOne;
-    float* sA = reinterpret_cast<float*>(fq + Unit::kOne);     // A
+    float* sA = reinterpret_cast<float*>(smem);                // A
     float* sM = sA + 64 * LD;                                  // P, then T
-    float* sD = sM + 64 * LD;                                  // the inverses of A's diagonal blocks, rows of 20
+    constexpr int kFirst = 2 * Unit::kOne > 2 * 64 * LD * 4 ? 2 * Unit::kOne : 2 * 64 * LD * 4;
+    float* sD = reinterpret_cast<float*>(smem + kFirst);       // the inverses of A's diagonal blocks, rows of 20
     double* sG = reinterpret_cast<double*>(sD + 4 * 16 * 20);  // of four value heads: G (log2 units), beta
     float* sBeta = reinterpret_cast<float*>(sG + 4 * 64);
     float* sEnd = sBeta + 4 * 64;                              // of the head at work: e^(G_i - G at its row tile's end
@@ -304,8 +310,10 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
                 const int at = frag + ((row & 15) + 16 * dg) * 16, sw = frag + (((row & 15) ^ (4 * s + dg)) + 16 * dg) * 16;
                 *reinterpret_cast<u32x4*>(fk + sw) = kp[i];
                 *reinterpret_cast<u32x4*>(fq + sw) = qp[i];
-                *reinterpret_cast<u32x4*>(kq + at) = kp[i];
-                *reinterpret_cast<u32x4*>(kq + Unit::kOne + at) = qp[i];
+                if constexpr (NP == 3) {
+                    *reinterpret_cast<u32x4*>(kq + at) = kp[i];
+                    *reinterpret_cast<u32x4*>(kq + Unit::kQ + at) = qp[i];
+                }
             }
             auto row_sum = [](float x) {  // over the row's lanes
                 x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xB1, 0xF, 0xF, false));
@@ -339,7 +347,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
             for (int s = 0; s < KS; s++) {
                 const f32x4 z = {0.f, 0.f, 0.f, 0.f};
                 const f32x4 v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(fk, p, wave, s), unit, z, 0, 0, 0);
-                *reinterpret_cast<u32x2*>(kq + 2 * Unit::kOne + (((p * KS + s) * 2 + j) * 2 + (wave >> 1)) * 1024 + lane * 16 +
+                *reinterpret_cast<u32x2*>(kq + Unit::kKT + (((p * KS + s) * 2 + j) * 2 + (wave >> 1)) * 1024 + lane * 16 +
                                           (wave & 1) * 8) = u32x2{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
             }
     }
@@ -369,6 +377,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
         for (int i = 0; i < 4; i++) kk[m][i] = sum(ck, i), qk[m][i] = sum(cq, i);
     }
 
+    __syncthreads();  // the fragments' place is free
 #pragma unroll 1
     for (int hi = 0; hi < R; hi++) {
         const int slot = hi & 3;
@@ -433,8 +442,8 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
             }
         }
         __syncthreads();
-        uint8_t* tp = ws.tp + unit * kTpBytes;
-        auto write_frags = [&](uint8_t* to) {
+        uint8_t* tp = ws.tp + unit * tp_bytes(DT);
+        auto write_frags = [&](uint8_t* to, int parts) {
             for (int i = tid; i < kTriFrags * 64; i += 256) {
                 const int f = i >> 6, l = i & 63;
                 const int tile = f < 2 ? f : 1 + (f >> 1), step = f < 2 ? 0 : f & 1;
@@ -444,10 +453,11 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
                 u32x4 w[3];
                 split3(v, w);
 #pragma unroll
-                for (int p = 0; p < 3; p++) *reinterpret_cast<u32x4*>(to + (p * kTriFrags + f) * 1024 + l * 16) = w[p];
+                for (int p = 0; p < 3; p++)
+                    if (p < parts) *reinterpret_cast<u32x4*>(to + (p * kTriFrags + f) * 1024 + l * 16) = w[p];
             }
         };
-        write_frags(tp + kTpOne);  // P
+        write_frags(tp + kTpOne, out_parts(DT));  // P
         {  // the inverse of A's diagonal block `wave` (unit lower triangular): lane c its column c, row after row
             const float* blk = sA + (16 * wave) * LD + 16 * wave;
             float x[16];
@@ -495,14 +505,15 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
             });
         });
         __syncthreads();
-        write_frags(tp);
+        write_frags(tp, 3);
         __syncthreads();
     }
 }
 
 template <int DT, int DK>
 constexpr size_t prep_lds() {
-    return 2 * KqUnit<DK, DT ? 1 : 3>::kOne + (2 * 64 * 68 + 4 * 16 * 20 + (4 + 3 + 1 + 2) * 64) * 4 + 4 * 64 * 8;
+    constexpr int one = KqUnit<DK, DT ? 1 : 3>::kOne, first = 2 * one > 2 * 64 * 68 * 4 ? 2 * one : 2 * 64 * 68 * 4;
+    return first + (4 * 16 * 20 + (4 + 3 + 1 + 2) * 64) * 4 + 4 * 64 * 8;
 }
 
 // Waves 0 .. 3 carry the state: row tile w of X and U, dims 32 w .. of S. Waves 4 .. 7, beside them on the same SIMDs,
@@ -530,17 +541,26 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
     // that moves on by a chunk and a lane offset; no load is conditional (a wave without an operand loads one of
     // another's), so that no branch waits for loads.
     const uint32_t lane16 = lane * 16;
-    const size_t kq_step = (size_t)a.k_heads * Unit::kBytes, tp_step = (size_t)a.v_heads * kTpBytes, vec_step = (size_t)a.v_heads * kVec * 4;
+    const size_t kq_step = (size_t)a.k_heads * Unit::kBytes, tp_step = (size_t)a.v_heads * tp_bytes(DT), vec_step = (size_t)a.v_heads * kVec * 4;
     const uint8_t* kq = ws.kq + ((size_t)b * ncs * a.k_heads + kh) * Unit::kBytes;
-    const uint8_t* tp = ws.tp + ((size_t)b * ncs * a.v_heads + h) * kTpBytes;
+    const uint8_t* tp = ws.tp + ((size_t)b * ncs * a.v_heads + h) * tp_bytes(DT);
     const uint8_t* vec = reinterpret_cast<const uint8_t*>(ws.vec + ((size_t)b * ncs * a.v_heads + h) * kVec);
     auto frag = [&](const uint8_t* p) { return *reinterpret_cast<const bf16x8*>(p + lane16); };
     auto vec4 = [&](int which) { return *reinterpret_cast<const f32x4*>(vec + 256 * which + (uint32_t)tok * 4); };
+    constexpr int OP = out_parts(DT);
     bf16x8 fM[2][3];  // T or P
+    // bf16 K and Q: the fragment of row tile i and dim step s as the rows lie in memory, rows past the last as the last
+    // one (their results are multiplied by zero, or not stored)
+    auto raw = [&](const void* base, size_t stride, int ch, int i, int s) {
+        const int r = min(16 * i + c, left - 1 - ch * kChunk);
+        return *reinterpret_cast<const bf16x8*>(static_cast<const uint16_t*>(base) + (row0 + (size_t)ch * kChunk) * stride + kh * DK +
+                                                32 * s + ((size_t)r * stride + 8 * g));
+    };
     const int f0 = wave < 2 ? wave : 2 * (wave - 1), f1 = wave < 2 ? f0 : f0 + 1;  // this row tile's two steps
-    auto load_tri = [&](const uint8_t* p) {
+    auto load_tri = [&](const uint8_t* p, int parts) {
 #pragma unroll
         for (int i = 0; i < 3; i++) {
+            if (i >= parts) break;
             fM[0][i] = frag(p + (i * kTriFrags + f0) * 1024);
             fM[1][i] = frag(p + (i * kTriFrags + f1) * 1024);
         }
@@ -557,18 +577,19 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
     if (wave8 >= 4) {
         f32x4 vq, acc[3];
         bf16x8 fQ[KS][NP];
-        auto load_q = [&] {
-            const uint8_t* p = kq + Unit::kOne + wave * (KS * 1024);
+        auto load_q = [&](int ch) {
+            const uint8_t* p = kq + Unit::kQ + wave * (KS * 1024);
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int i = 0; i < NP; i++) fQ[s][i] = frag(p + (i * 4 * KS + s) * 1024);
+                for (int i = 0; i < NP; i++)
+                    fQ[s][i] = NP == 1 ? raw(a.q, a.q_stride, ch, wave, s) : frag(p + (i * 4 * KS + s) * 1024);
         };
         const size_t stride = O32 ? (size_t)a.v_heads * DV : a.out_stride;
         size_t first = row0 * stride + h * DV + 16 * slice, at[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) at[i] = (tok + i) * stride + c;
-        load_q(), load_tri(tp + kTpOne), vq = vec4(2);
+        load_q(0), load_tri(tp + kTpOne, OP), vq = vec4(2);
 #pragma unroll 1
         for (int ch = 0; ch < nc; ch++) {
             move_on(ch + 1 < nc);
@@ -577,10 +598,11 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 bf16x8 bs[3];
-                get(sS[s], bs);
-                mfma_parts<NP>(fQ[s], bs, acc);
+#pragma unroll
+                for (int p = 0; p < OP; p++) bs[p] = frag(sS[s][p]);
+                mfma_parts<NP, OP>(fQ[s], bs, acc);
             }
-            load_q();
+            load_q(min(ch + 1, nc - 1));
             f32x4 qs;
 #pragma unroll
             for (int i = 0; i < 4; i++) qs[i] = vq[i] * sum(acc, i);
@@ -599,9 +621,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
                 u32x4 w[3];
                 split3(v, w);
                 const bf16x8 bu[3] = {__builtin_bit_cast(bf16x8, w[0]), __builtin_bit_cast(bf16x8, w[1]), __builtin_bit_cast(bf16x8, w[2])};
-                mfma_parts<3>(fM[st], bu, acc);
+                mfma_parts<3, OP>(fM[st], bu, acc);
             }
-            load_tri(tp + kTpOne);
+            load_tri(tp + kTpOne, OP);
             const int more = left - ch * kChunk - tok;
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -628,15 +650,16 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
     size_t first = row0 * a.v_stride + h * DV + 16 * slice, at[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) at[i] = (tok + i) * a.v_stride + c;
-    auto load_k = [&] {
+    auto load_k = [&](int ch) {
         const uint8_t* p = kq + wave % KS * 1024;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int q = 0; q < NP; q++) fK[i][q] = frag(p + (q * 4 + i) * (KS * 1024));
+            for (int q = 0; q < NP; q++)
+                fK[i][q] = NP == 1 ? raw(a.k, a.k_stride, ch, i, wave % KS) : frag(p + (q * 4 + i) * (KS * 1024));
     };
     auto load_kt = [&] {
-        const uint8_t* p = kq + 2 * Unit::kOne + wave % KS * 4096;
+        const uint8_t* p = kq + Unit::kKT + wave % KS * 4096;
 #pragma unroll
         for (int f = 0; f < 4; f++)
 #pragma unroll
@@ -673,7 +696,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         for (int p = 0; p < 3; p++)
             *reinterpret_cast<u32x2*>(to[wave >> 1][p] + lane16 + (wave & 1) * 8) = u32x2{lo[p], hi[p]};
     };
-    load_k(), load_x(0), load_tri(tp);
+    load_k(0), load_x(0), load_tri(tp, 3);
     put_state();
     __builtin_amdgcn_s_setprio(2);  // ahead of the output waves
 #pragma unroll 1
@@ -711,7 +734,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         lds_barrier();  // X
         bf16x8 bx[2][3];
         get(sX[0], bx[0]), get(sX[1], bx[1]);
-        load_k(), load_x(min(ch + 1, nc - 1));
+        load_k(min(ch + 1, nc - 1)), load_x(min(ch + 1, nc - 1));
 #pragma unroll
         for (int p = 0; p < 3; p++) {
             u32x4 v = __builtin_bit_cast(u32x4, bx[1][p]);
@@ -729,7 +752,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         lds_barrier();  // U, and with the scales of K^T's columns
         bf16x8 bw[2][3];
         get(sW[0], bw[0]), get(sW[1], bw[1]);
-        load_tri(tp);
+        load_tri(tp, 3);
         if (KS == 4 || wave < KS) {
             f32x4 s[2][3];
 #pragma unroll
@@ -780,7 +803,7 @@ __global__ __launch_bounds__(256) void k_delta_norm(DeltaArgs a, const float* o3
 // Token by token up to this many, and where every state is kept.
 constexpr int kStepMost = 16;
 // Chunks of a call are worked off in segments of about this many (chunk, value head) pairs at a time, whose
-// workspace (60 KB a pair in bf16, 108 KB in fp32) stays in the last-level cache.
+// workspace (39 KB a pair of two a key head in bf16, 109 KB in fp32) stays in the last-level cache.
 constexpr int kSegmentPairs = 2048;
 
 static bool by_steps(const DeltaArgs& a) { return a.snap || a.n <= kStepMost; }
@@ -796,7 +819,7 @@ struct DeltaSizes {
 };
 static DeltaSizes delta_sizes(const DeltaArgs& a, bool bf16) {
     const size_t chunks = (size_t)a.n_seq * segment_chunks(a);
-    return {up256(chunks * a.k_heads * (bf16 ? 1 : 3) * 3 * kChunk * a.key_dim * 2), up256(chunks * a.v_heads * kTpBytes),
+    return {up256(chunks * a.k_heads * (bf16 ? 1 : 9) * kChunk * a.key_dim * 2), up256(chunks * a.v_heads * tp_bytes(bf16)),
             up256(chunks * a.v_heads * kVec * 4),
             a.z ? up256((size_t)a.n_seq * a.n * a.v_heads * a.val_dim * 4) : 0};
 }
