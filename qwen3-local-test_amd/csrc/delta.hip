@@ -800,13 +800,20 @@ __global__ __launch_bounds__(256) void k_delta_norm(DeltaArgs a, const float* o3
         store_out<DT>(a.out, r * a.out_stride + h * DV + d + e, o[e] * (rms * a.gamma[d + e] * (z[e] * sigmoid(z[e]))));
 }
 
-// Token by token up to this many, and where every state is kept.
-constexpr int kStepMost = 16;
+// Token by token where every state is kept, and while that takes less: a token takes 1 us (up to 256 (sequence, value
+// head) pairs, a workgroup each) to 5 us (1,536 pairs), a chunk of all pairs 20 us (32 pairs, bf16) to 250 (1,536), in fp32
+// up to twice as much. Measured with 32 heads of 128 x 128, by tokens and in chunks: one sequence of 19 tokens 24 and 20
+// us (bf16), 26 (fp32); 4 of 48 tokens 53 and 33, 55 and 48; 8 of 64 tokens in fp32 73 and 102; 48 of 64 tokens in bf16
+// 337 and 252.
+static int step_most(const DeltaArgs& a, bool bf16) {
+    const long long pairs = (long long)a.n_seq * a.v_heads;
+    return (int)(bf16 ? std::min(18 + pairs / 10, 48ll) : std::min(18 + pairs / 6, 100ll));
+}
 // Chunks of a call are worked off in segments of about this many (chunk, value head) pairs at a time, whose
 // workspace (39 KB a pair of two a key head in bf16, 109 KB in fp32) stays in the last-level cache.
 constexpr int kSegmentPairs = 2048;
 
-static bool by_steps(const DeltaArgs& a) { return a.snap || a.n <= kStepMost; }
+static bool by_steps(const DeltaArgs& a, bool bf16) { return a.snap || a.n <= step_most(a, bf16); }
 static int segment_chunks(const DeltaArgs& a) {
     const int nc = (a.n + kChunk - 1) / kChunk;
     const long long pairs = (long long)a.n_seq * a.v_heads;
@@ -824,7 +831,7 @@ static DeltaSizes delta_sizes(const DeltaArgs& a, bool bf16) {
             a.z ? up256((size_t)a.n_seq * a.n * a.v_heads * a.val_dim * 4) : 0};
 }
 size_t delta_workspace(const DeltaArgs& a, bool bf16) {
-    if (by_steps(a)) return 0;
+    if (by_steps(a, bf16)) return 0;
     const DeltaSizes s = delta_sizes(a, bf16);
     return s.kq + s.tp + s.vec + s.o;
 }
@@ -855,7 +862,7 @@ static hipError_t delta_chunks(const DeltaArgs& a, hipStream_t s) {
 
 template <int DT, int DK>
 static hipError_t delta_dims(const DeltaArgs& a, hipStream_t s) {
-    if (by_steps(a)) return delta_step<DT, DK>(a, s);
+    if (by_steps(a, DT == 1)) return delta_step<DT, DK>(a, s);
     return a.val_dim == 64 ? delta_chunks<DT, DK, 64>(a, s) : delta_chunks<DT, DK, 128>(a, s);
 }
 

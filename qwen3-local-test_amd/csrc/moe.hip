@@ -126,28 +126,26 @@ __global__ __launch_bounds__(256) void k_moe_pair_up(MoeArgs a) {
     }
 }
 
+// (a token's pairs one after the other make one row of top_k x ffn columns: ffn is often half a wave's 1,024. Decode of 8
+// experts of 512: 8.9 us with a pair at a time)
 template <int DT>
 __global__ __launch_bounds__(256) void k_moe_pair_down(MoeArgs a) {
     const int tok = blockIdx.x, lane = threadIdx.x & 63;
     const int r0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * kPairRows;
+    const int per = a.ffn >> 4, pieces = a.top_k * per;  // of 16 columns
     float y[kPairRows] = {};
-    for (int j = 0; j < a.top_k; j++) {
-        const int pair = tok * a.top_k + j, e = a.ids[pair];
+#pragma unroll 4
+    for (int p = lane; p < pieces; p += 64) {
+        const int j = p / per, c = (p - j * per) * 16, pair = tok * a.top_k + j, e = a.ids[pair];
         if (e < 0 || e >= a.n_experts) continue;
-        float acc[kPairRows] = {};
-        for (int c = lane * 16; c < a.ffn; c += 1024) {
-            float h[16];
-            load_vec<0, 16>(a.h, (size_t)pair * a.ffn + c, h);
-#pragma unroll
-            for (int i = 0; i < kPairRows; i++) {
-                if (r0 + i >= a.hidden) break;
-                const size_t at = ((size_t)e * a.hidden + r0 + i) * a.ffn + c;
-                acc[i] = fmaf(dot16(*reinterpret_cast<const u32x4*>(a.w_down + at), h), a.s_down[at >> 5], acc[i]);
-            }
-        }
         const float wt = a.weights[pair];
+        float h[16];
+        load_vec<0, 16>(a.h, (size_t)pair * a.ffn + c, h);
 #pragma unroll
-        for (int i = 0; i < kPairRows; i++) y[i] = fmaf(wt, acc[i], y[i]);
+        for (int i = 0; i < kPairRows; i++) {
+            const size_t at = ((size_t)e * a.hidden + min(r0 + i, a.hidden - 1)) * a.ffn + c;
+            y[i] = fmaf(wt * a.s_down[at >> 5], dot16(*reinterpret_cast<const u32x4*>(a.w_down + at), h), y[i]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < kPairRows; i++) {
@@ -546,8 +544,17 @@ __global__ __launch_bounds__(256) void k_moe_combine(MoeArgs a, MoeWs ws) {
 }
 
 // ---- which form -----------------------------------------------------------------------------------------------
-// Pair by pair while the experts' rows are few (each pair streams its expert's weights, repeated ones from the cache).
-static bool by_pairs(const MoeArgs& a) { return (long long)a.n * a.top_k <= std::max(16, a.n_experts); }
+// Pair by pair while the pairs are few: a pair streams its expert's weights (repeated ones from the cache), about 0.18 us
+// a million; the grouped form takes 26 us and 0.26 us a million weights of each expert that is hit. Measured: 8 of 128 experts
+// of 2,048 x 512: 16 tokens 88 us by pairs and 99 grouped, 32 tokens 154 and 122; 2 of 8 of 1,024 x 352: 32 tokens 22
+// and 30, 64 tokens 36 and 30.
+static bool by_pairs(const MoeArgs& a) {
+    const long long pairs = (long long)a.n * a.top_k, weights = 3ll * a.hidden * a.ffn;
+    return pairs <= 150000000ll / weights + std::min<long long>(pairs, a.n_experts) * 14 / 10;
+}
+// Rows of a tile: 64 where a mean expert has this many rows, else 32. Measured with 8 of 128 experts of 2,048 x 512, bf16:
+// 48 rows an expert 221 us in tiles of 64 and 208 of 32, 64 rows 237 and 243, 128 rows 363 and 387.
+constexpr int kTileRows64 = 56;
 
 constexpr int kMoeSegment = 1 << 16;  // pairs worked off at a time: bounds the workspace
 static int segment_tokens(const MoeArgs& a) { return std::max(1, std::min(a.n, kMoeSegment / a.top_k)); }
@@ -623,7 +630,7 @@ static hipError_t moe_grouped(MoeArgs a, uint8_t* workspace, hipStream_t s) {
         b.ids = a.ids + (size_t)t * a.top_k, b.weights = a.weights + (size_t)t * a.top_k;
         const long long rows = (long long)b.n * a.top_k / a.n_experts;  // a mean expert's
         hipError_t e;
-        if (rows >= 24) e = moe_tiles<2, DT>(b, w, s);
+        if (rows >= kTileRows64) e = moe_tiles<2, DT>(b, w, s);
         else e = moe_tiles<1, DT>(b, w, s);
         if (e) return e;
     }
