@@ -439,9 +439,11 @@ class Attention:
             return given.data_ptr(), given.numel() * given.element_size(), given
         if not size:
             return 0, 0, None
-        t = torch.empty(size, dtype=torch.uint8, device=self._torch_device)
-        if stream is not None:
-            t.record_stream(stream)
+        if stream is None:
+            t = torch.empty(size, dtype=torch.uint8, device=self._torch_device)
+        else:  # from that stream's memory: another stream's may still be in use there
+            with torch.cuda.stream(stream):
+                t = torch.empty(size, dtype=torch.uint8, device=self._torch_device)
         return t.data_ptr(), size, t
 
     def conv_silu(self, x, w, state, y, bias=None, lens=None, snap=None, stream=None):

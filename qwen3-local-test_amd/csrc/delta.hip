@@ -274,7 +274,9 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
     float* sRk = sSince + 64;
     float* sRq = sRk + 64;
 
-    const int cl = blockIdx.x, kh = blockIdx.y, b = blockIdx.z;
+    // a workgroup a key head, or (where those leave CUs idle) several, which share out its value heads
+    const int cl = blockIdx.x, kh = blockIdx.y % a.k_heads, b = blockIdx.z, share = blockIdx.y / a.k_heads;
+    const int shares = gridDim.y / a.k_heads;
     const int len = a.lens ? min(max(a.lens[b], 0), a.n) : a.n;
     const int t0 = (c0 + cl) * kChunk, nt = min(kChunk, len - t0);
     if (nt <= 0) return;
@@ -310,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
                 const int at = frag + ((row & 15) + 16 * dg) * 16, sw = frag + (((row & 15) ^ (4 * s + dg)) + 16 * dg) * 16;
                 *reinterpret_cast<u32x4*>(fk + sw) = kp[i];
                 *reinterpret_cast<u32x4*>(fq + sw) = qp[i];
-                if constexpr (NP == 3) {
+                if (NP == 3 && share == 0) {
                     *reinterpret_cast<u32x4*>(kq + at) = kp[i];
                     *reinterpret_cast<u32x4*>(kq + Unit::kQ + at) = qp[i];
                 }
@@ -329,8 +331,12 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
             }
         }
     }
-    const int R = a.v_heads / a.k_heads;
-    auto head = [&](int hi) { return a.tiled ? kh + hi * a.k_heads : kh * R + hi; };
+    // this workgroup's value heads
+    const int all = a.v_heads / a.k_heads, R = (all - share + shares - 1) / shares;
+    auto head = [&](int i) {
+        const int hi = share + i * shares;
+        return a.tiled ? kh + hi * a.k_heads : kh * all + hi;
+    };
     __syncthreads();
     auto frag = [&](const uint8_t* f, int part, int tile, int s) {
         return *reinterpret_cast<const bf16x8*>(f + ((part * 4 + tile) * KS + s) * 1024 + ((c ^ (4 * s + g)) + 16 * g) * 16);
@@ -338,6 +344,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
     // K^T of the row tile `wave`, by products with the unit matrix (exact): its accumulators hold four tokens of a dim
 #pragma unroll
     for (int j = 0; j < 2; j++) {
+        if (share) break;
         bf16x8 unit;
 #pragma unroll
         for (int e = 0; e < 8; e++) unit[e] = 8 * g + e == 8 * (c >> 2) + 4 * j + (c & 3) ? (__bf16)1.f : (__bf16)0.f;
@@ -848,7 +855,9 @@ static hipError_t delta_chunks(const DeltaArgs& a, hipStream_t s) {
     const int nc = (a.n + kChunk - 1) / kChunk, seg = segment_chunks(a);
     for (int c0 = 0; c0 < nc; c0 += seg) {
         const int ncs = std::min(seg, nc - c0);
-        k_delta_prep<DT, DK><<<dim3(ncs, a.k_heads, a.n_seq), 256, lds, s>>>(a, ws, c0, ncs);
+        // 333 tokens of 16 key heads and 32 value heads in fp32: 21 us with a workgroup a key head, 18 with one a value head
+        const int shares = (long long)ncs * a.v_heads * a.n_seq <= 256 ? a.v_heads / a.k_heads : 1;
+        k_delta_prep<DT, DK><<<dim3(ncs, a.k_heads * shares, a.n_seq), 256, lds, s>>>(a, ws, c0, ncs);
         const int grid = a.v_heads * a.n_seq * (DV / 16);
         if (a.z) k_delta_chunks<DT, DK, DV, true><<<grid, 512, 0, s>>>(a, ws, c0, ncs);
         else k_delta_chunks<DT, DK, DV, false><<<grid, 512, 0, s>>>(a, ws, c0, ncs);

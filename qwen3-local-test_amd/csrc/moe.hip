@@ -544,13 +544,14 @@ __global__ __launch_bounds__(256) void k_moe_combine(MoeArgs a, MoeWs ws) {
 }
 
 // ---- which form -----------------------------------------------------------------------------------------------
-// Pair by pair while the pairs are few: a pair streams its expert's weights (repeated ones from the cache), about 0.18 us
-// a million; the grouped form takes 26 us and 0.26 us a million weights of each expert that is hit. Measured: 8 of 128 experts
-// of 2,048 x 512: 16 tokens 88 us by pairs and 99 grouped, 32 tokens 154 and 122; 2 of 8 of 1,024 x 352: 32 tokens 22
-// and 30, 64 tokens 36 and 30.
+// Pair by pair while that takes less: a pair costs 0.09 us a million weights and 0.1 us a thousand weight rows (hidden and
+// ffn; 6 us beside them), the grouped form 20 us and 0.26 us a million weights of each expert that is hit. Measured, by
+// pairs and grouped: 8 of 128 experts of 2,048 x 512: 16 tokens 88 and 99 us, 32 tokens 154 and 122; 2 of 8 of 1,024 x
+// 352: 32 tokens 22 and 30, 64 tokens 36 and 30; 2 of 16 of 256 x 96: 250 tokens 26 and 21; 2 of 4 of 64 x 32: 500 tokens
+// 18 and 20, 1,000 tokens 28 and 21.
 static bool by_pairs(const MoeArgs& a) {
-    const long long pairs = (long long)a.n * a.top_k, weights = 3ll * a.hidden * a.ffn;
-    return pairs <= 150000000ll / weights + std::min<long long>(pairs, a.n_experts) * 14 / 10;
+    const double pairs = (double)a.n * a.top_k, weights = 3e-6 * a.hidden * a.ffn;
+    return 6 + pairs * (0.09 * weights + 1e-4 * (a.hidden + a.ffn)) <= 20 + 0.26 * weights * std::min(pairs, (double)a.n_experts);
 }
 // Rows of a tile: 64 where a mean expert has this many rows, else 32. Measured with 8 of 128 experts of 2,048 x 512, bf16:
 // 48 rows an expert 221 us in tiles of 64 and 208 of 32, 64 rows 237 and 243, 128 rows 363 and 387.

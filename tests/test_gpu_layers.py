@@ -243,6 +243,17 @@ def test_delta_chunks_join(att):
         close(state, S, 320 * 151 * EPS32 * scale[:, :, None, :], f"state of {cuts[:4]}")
 
 
+def test_delta_segments_join(att):
+    """More (chunk, head) pairs than are worked off at a time: the bits of the same sequences in calls of one segment."""
+    d = delta_inputs(85, 32, 200, 16, 32, 64, 64, BF16, True, True)
+    lens = [200 - 3 * i for i in range(32)]
+    out, state, _ = delta_run(att, d, lens=lens)
+    for s in range(0, 32, 8):
+        part = {k: v[s:s + 8].contiguous() if k not in ("a_coef", "dt_bias", "gamma") else v for k, v in d.items()}
+        o, st, _ = delta_run(att, part, lens=lens[s:s + 8])
+        assert torch.equal(o, out[s:s + 8]) and torch.equal(st, state[s:s + 8])
+
+
 def test_delta_same_bits_again(att):
     for n in (5, 300):
         d = delta_inputs(90 + n, 2, n, 2, 4, 128, 128, BF16, True, True)
@@ -321,7 +332,8 @@ def moe_check(att, x, ids, weights, q, what=""):
     (1, 4, 2, 64, 32, F32), (1, 16, 4, 256, 96, BF16), (1, 3, 3, 2048, 512, F32), (2, 8, 2, 96, 64, F32),
     (3, 5, 5, 32, 32, BF16), (7, 16, 4, 288, 160, F32), (13, 64, 8, 512, 128, BF16), (20, 2, 1, 128, 352, F32),
     (33, 4, 2, 160, 96, BF16), (64, 8, 3, 256, 64, F32), (100, 1, 1, 128, 128, BF16), (150, 6, 4, 320, 224, F32),
-    (257, 3, 2, 544, 96, BF16), (300, 40, 2, 128, 160, F32)])
+    (257, 3, 2, 544, 96, BF16), (300, 40, 2, 128, 160, F32), (400, 40, 2, 160, 96, BF16), (1000, 4, 2, 96, 32, F32),
+    (700, 5, 3, 288, 352, BF16), (513, 9, 2, 1056, 64, F32)])
 def test_moe(att, n, e, k, hidden, ffn, dtype):
     r, q = gen(n * 3 + e), experts(n, e, hidden, ffn)
     x = r(n, hidden).to(dtype)
@@ -362,7 +374,7 @@ def test_moe_rows_of_many_magnitudes(att, n):
 def test_moe_strides_offsets_and_neighbours(att):
     """x and y as column slices, and as rows behind 2^32 bytes; columns beside the slice stay as they were."""
     q, r = experts(5, 4, 64, 96), gen(11)
-    for n in (2, 40):
+    for n in (2, 40, 900):
         ids, w = torch.arange(n * 2, device=DEV, dtype=torch.int32).view(n, 2) % 4, r(n, 2)
         wide, out = r(n, 136), torch.full((n, 88), 7.0, device=DEV)
         x, y = wide[:, 8:72], out[:, 16:80]
@@ -383,13 +395,29 @@ def test_moe_weights_past_32_bits(att):
     for (w, s), (w2, s2) in zip(q, small):
         w[1023], s[1023], w[900], s[900] = w2[0], s2[0], w2[1], s2[1]
     r = gen(12)
-    for n in (1, 40):
+    for n in (1, 40, 1300):
         x, ids, wt = r(n, hidden), torch.tensor([[1023, 900]], dtype=torch.int32, device=DEV).repeat(n, 1), r(n, 2)
         y, y2 = torch.empty_like(x), torch.empty_like(x)
         att.moe(x, ids, wt, *q, y)
         att.moe(x, (ids == 900).int(), wt, *small, y2)
         # the same pairs in the same order, whatever the number of experts chose as the form
         close(y, y2, 1e-5 * float(y2.abs().max()), f"n = {n}")
+
+
+def test_moe_segments_join(att):
+    """More pairs than are worked off at a time: the bits of the same rows in calls of one segment."""
+    n, k, e = 20000, 4, 3
+    q, r = experts(7, e, 64, 32), gen(14)
+    g = torch.Generator(device=DEV).manual_seed(15)
+    x, w = r(n, 64), r(n, k)
+    ids = torch.randint(-1, e + 1, (n, k), generator=g, device=DEV, dtype=torch.int32)
+    y, parts = torch.empty_like(x), torch.empty_like(x)
+    att.moe(x, ids, w, *q, y)
+    for a, b in ((0, 9000), (9000, n)):  # (both grouped: the form by pairs sums in another order)
+        att.moe(x[a:b], ids[a:b], w[a:b], *q, parts[a:b])
+    assert torch.equal(y, parts)
+    want, mag = lo.moe(x[::499], ids[::499], w[::499], *q)
+    close(y[::499], want, (64 / 32 + 32 / 32 + 48) * EPS32 * mag + EPS32 * want.abs(), "y")
 
 
 def test_moe_same_bits_again(att):
