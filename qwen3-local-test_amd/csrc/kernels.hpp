@@ -328,8 +328,9 @@ struct RouteArgs {
     int stride, n, n_experts, top_k, renorm;
     int32_t* ids;
     float* weights;
+    bool whole;  // the lanes' shares of a row are whole and aligned (set by the launcher)
 };
-hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s);
+hipError_t launch_moe_route(RouteArgs a, hipStream_t s);
 
 // qwattn_moe's (include/qwattn.h)
 struct MoeArgs {

