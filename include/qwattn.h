@@ -432,7 +432,8 @@ int qwattn_conv_silu(qwattn_ctx* ctx, void* stream, const qwattn_conv* args);
  *   S <- decay S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q
  * with g = a and beta = b as given, or, with a_coef and dt_bias, g = a_coef[h] softplus(a + dt_bias[h]) and
  * beta = 1 / (1 + e^-b). With z and gamma the output is o rsqrt(mean o^2 + rms_eps) gamma silu(z), else o.
- * fp32 arithmetic (chunks of many tokens: products of fp32 accuracy on the matrix cores), one rounding to dtype.
+ * fp32 arithmetic (chunks of many tokens: products of fp32 accuracy on the matrix cores; of what only a bf16 output
+ * reads, 16 bits), one rounding to dtype.
  * Few tokens run token by token; more run in chunks of 64 tokens whose chunk-internal part is computed for all
  * chunks at once (that form needs the workspace). Results do not depend on timing. */
 typedef struct qwattn_delta {
@@ -481,8 +482,9 @@ typedef struct qwattn_moe_layer {
 /* y[t] = sum_j weights[t][j] W_down (silu(W_gate x[t]) * (W_up x[t])) of expert ids[t][j], j < top_k <= 64. An id
  * outside [0, n_experts) is skipped (a free place of a batch: its row of y is then zero); the same expert may
  * occur twice. x and y are dtype (QWATTN_F32 or QWATTN_BF16) rows at strides that are multiples of 8, x 16-byte
- * aligned; fp32 accuracy, one rounding to dtype. The result of a row does not depend on the other rows nor on
- * timing. workspace: qwattn_moe_workspace bytes, 256-byte aligned. */
+ * aligned; fp32 accuracy, one rounding to dtype. Results do not depend on timing; the same row in calls of other n
+ * or top_k may differ within that accuracy, since few pairs and many are computed in different orders.
+ * workspace: qwattn_moe_workspace bytes, 256-byte aligned. */
 int qwattn_moe(qwattn_ctx* ctx, void* stream, const qwattn_moe_layer* layer, const void* x, int dtype,
                int64_t x_stride, const int32_t* ids, const float* weights, int top_k, void* y, int64_t y_stride, int n,
                void* workspace, size_t workspace_bytes);

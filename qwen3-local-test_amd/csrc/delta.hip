@@ -181,7 +181,7 @@ static hipError_t delta_step(const DeltaArgs& a, hipStream_t s) {
 //                                      five vectors: beta, and the row scales of K S, Q S and K^T U; e^(G_end)
 // Where tokens are the summed index (K^T, T, P and the X and U beside them) lane group g of a 32-token step holds the
 // tokens 4 g .. 4 g + 3 of its first 16 and of its second 16: accumulator registers again.
-// What only the output takes part in (Q S and P U) has two parts where the output is bf16: within 2^-16 beside its 2^-9.
+// What only the output takes part in (Q S and P U) has two parts where the output is bf16: within 2^-16 beside its 2^-8.
 constexpr int kChunk = 64, kTriFrags = 6, kVec = 320;
 
 struct DeltaWs {
