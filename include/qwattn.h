@@ -437,8 +437,8 @@ int qwattn_conv_silu(qwattn_ctx* ctx, void* stream, const qwattn_conv* args);
  * Few tokens run token by token; more run in chunks of 64 tokens whose chunk-internal part is computed for all
  * chunks at once (that form needs the workspace). Results do not depend on timing. */
 typedef struct qwattn_delta {
-    int n_seq, n;
-    int k_heads, v_heads; /* v_heads a multiple of k_heads */
+    int n_seq, n;         /* n_seq <= 65535; n_seq * v_heads < 2^20, with z also n_seq * n * v_heads < 2^27 */
+    int k_heads, v_heads; /* v_heads a multiple of k_heads, <= 1024 */
     int key_dim, val_dim; /* 64 or 128 each */
     int tiled;            /* value head h uses key head h / (v_heads / k_heads) (0) or h % k_heads (1) */
     int dtype;            /* of q, k, v, z and out: QWATTN_F32 or QWATTN_BF16 */
@@ -466,7 +466,7 @@ int qwattn_delta_workspace(const qwattn_delta* args, size_t* bytes);
 /* The router: per row of logits[n][logits_stride] (n_experts used) the top_k largest, largest first, the lower
  * index first among equal ones, into ids[n][top_k], and their weights[n][top_k]: the softmax over all experts,
  * divided by the selected ones' sum when renorm != 0. A logit of -inf or NaN is no choice: a row with fewer
- * choices than top_k ends with ids of -1 and weights of 0. n_experts <= 1024, top_k <= 64. */
+ * choices than top_k ends with ids of -1 and weights of 0. n < 2^26 - 4, n_experts <= 1024, top_k <= 64. */
 int qwattn_moe_route(qwattn_ctx* ctx, void* stream, const float* logits, int logits_stride, int n, int n_experts,
                      int top_k, int renorm, int32_t* ids, float* weights);
 

@@ -66,6 +66,10 @@ inline int check_delta_shape(const qwattn_delta* a, CheckText& m) {
     if (a->k_heads <= 0 || a->v_heads <= 0 || a->v_heads > 1024 || a->v_heads % a->k_heads)
         return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: k_heads %d, v_heads %d (a multiple of k_heads, <= 1024)",
                       a->k_heads, a->v_heads);
+    // a launch has less than 2^32 threads in x: 4,096 a (sequence, value head), and 32 a row and head for the gated norm
+    if ((int64_t)a->n_seq * a->v_heads >= (1 << 20) || (a->z && (int64_t)a->n_seq * a->n * a->v_heads >= (1 << 27)))
+        return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: n_seq %d x v_heads %d (< 2^20), with z x n %d (< 2^27)", a->n_seq,
+                      a->v_heads, a->n);
     if ((a->key_dim != 64 && a->key_dim != 128) || (a->val_dim != 64 && a->val_dim != 128))
         return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: key_dim %d, val_dim %d (64 or 128)", a->key_dim, a->val_dim);
     if (bad_dtype(a->dtype) || a->tiled < 0 || a->tiled > 1)
@@ -105,10 +109,11 @@ inline int check_delta(const qwattn_delta* a, size_t workspace, CheckText& m) {
 inline int check_route(const float* logits, int stride, int n, int n_experts, int top_k, const int32_t* ids,
                        const float* weights, CheckText& m) {
     if (!logits || !ids || !weights) return refuse(m, QWATTN_EINVAL, "qwattn_moe_route: null pointer");
-    if (n <= 0 || n_experts <= 0 || n_experts > 1024 || top_k <= 0 || top_k > 64 || top_k > n_experts ||
+    // a wave a row, and less than 2^32 threads
+    if (n <= 0 || n >= (1 << 26) - 4 || n_experts <= 0 || n_experts > 1024 || top_k <= 0 || top_k > 64 || top_k > n_experts ||
         (int64_t)n * top_k > INT32_MAX)
-        return refuse(m, QWATTN_EINVAL, "qwattn_moe_route: n %d, n_experts %d (<= 1024), top_k %d (<= 64 and n_experts)", n,
-                      n_experts, top_k);
+        return refuse(m, QWATTN_EINVAL, "qwattn_moe_route: n %d (< 2^26 - 4), n_experts %d (<= 1024), top_k %d (<= 64 and "
+                      "n_experts)", n, n_experts, top_k);
     if (stride < n_experts) return refuse(m, QWATTN_EINVAL, "qwattn_moe_route: logits_stride %d (>= n_experts)", stride);
     return QWATTN_OK;
 }

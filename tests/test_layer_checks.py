@@ -169,3 +169,26 @@ def test_mirror_refuses(att):
                      (dict(ids=z(3, 2, dtype=torch.int64)), "ids must be"), ({}, "on cuda:0")):
         with pytest.raises(ValueError, match=text):
             att.moe(**{**call, **kw})
+
+
+def test_sizes_beyond_a_launch_are_refused(lib, qw):
+    """Fewer than 2^32 threads in a launch's x: 4,096 a (sequence, value head), 32 a row and head of the gated norm, 64 a
+    row of the router in workgroups of four rows."""
+    big = dict(k_heads=16, v_heads=32, q_stride=1024, k_stride=1024, v_stride=4096, out_stride=4096, n=1)
+    far = {name: (i + 1) << 44 for i, name in enumerate(("q", "k", "v", "z", "out"))}  # apart at any of these sizes
+    plain = {**big, **far, "z": 0}
+    gated = {**big, **far, "gamma": P, "z_stride": 4096}
+    assert 4096 * 32767 * 32 < 2**32 <= 4096 * 32768 * 32
+    assert lib.layer_delta(delta_args(qw, **{**plain, "n_seq": 32767}), 0) == 0
+    assert lib.layer_delta(delta_args(qw, **{**plain, "n_seq": 32768}), 0) == EINVAL
+    assert "2^20" in lib.layer_text().decode()
+    n = 2**27 // 32
+    assert lib.layer_delta(delta_args(qw, **{**gated, "n_seq": 1, "n": n - 1}), 0) == 0
+    assert lib.layer_delta(delta_args(qw, **{**gated, "n_seq": 1, "n": n}), 0) == EINVAL
+    assert "2^27" in lib.layer_text().decode()
+    assert lib.layer_delta(delta_args(qw, **{**plain, "n_seq": 1, "n": n}), 0) == 0
+    most = 2**26 - 5
+    assert (most + 3) // 4 * 256 < 2**32
+    assert lib.layer_route(P, 8, most, 8, 8, P, P) == 0
+    assert lib.layer_route(P, 8, most + 1, 8, 8, P, P) == EINVAL
+    assert "2^26" in lib.layer_text().decode()
