@@ -435,7 +435,8 @@ int qwattn_conv_silu(qwattn_ctx* ctx, void* stream, const qwattn_conv* args);
  * fp32 arithmetic (chunks of many tokens: products of fp32 accuracy on the matrix cores; of what only a bf16 output
  * reads, 16 bits), one rounding to dtype.
  * Few tokens run token by token; more run in chunks of 64 tokens whose chunk-internal part is computed for all
- * chunks at once (that form needs the workspace). Results do not depend on timing. */
+ * chunks at once (that form needs the workspace). Results do not depend on timing. An infinity or NaN in a token
+ * stays in its sequence and heads; in chunks it also reaches earlier tokens of its own chunk. */
 typedef struct qwattn_delta {
     int n_seq, n;         /* n_seq <= 65535; n_seq * v_heads < 2^20, with z also n_seq * n * v_heads < 2^27 */
     int k_heads, v_heads; /* v_heads a multiple of k_heads, <= 1024 */

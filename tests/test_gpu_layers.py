@@ -230,6 +230,23 @@ def test_delta_edges(att, case, n):
     delta_check(att, d)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [12, 200])
+def test_delta_token_that_is_not_finite(att, n, dtype):
+    """A NaN value reaches its own sequence and head alone, and no token before it (in chunks: before its chunk)."""
+    d = delta_inputs(90 + n, 2, n, 1, 2, 64, 64, dtype, True, True)
+    bad = {k: v.clone() for k, v in d.items()}
+    at = n - 3
+    bad["v"][1, at, 0] = float("nan")
+    out, state, _ = delta_run(att, d)
+    out2, state2, _ = delta_run(att, bad)
+    assert torch.equal(out[0], out2[0]) and torch.equal(state[0], state2[0])
+    assert torch.equal(out[1, :, 1], out2[1, :, 1]) and torch.equal(state[1, 1], state2[1, 1])
+    before = at if n < 64 else at // 64 * 64
+    assert torch.equal(out[1, :before, 0], out2[1, :before, 0])
+    assert torch.isnan(out2[1, at:, 0]).all() and torch.isnan(state2[1, 0]).all()
+
+
 def test_delta_chunks_join(att):
     """A prompt in one call, in ragged calls of both forms, and token by token: states and outputs agree."""
     d = delta_inputs(80, 1, 150, 2, 4, 128, 128, F32, True, True)
@@ -369,6 +386,25 @@ def test_moe_rows_of_many_magnitudes(att, n):
     ids = torch.arange(2 * n, device=DEV, dtype=torch.int32).view(n, 2) % 3
     y = moe_check(att, x, ids, r(n, 2), q)
     assert (y[n // 2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [5, 40, 300])
+def test_moe_rows_that_are_not_finite(att, n, dtype):
+    """Infinities and NaN in a token's row reach its own row of y alone; a NaN weight of a free place reaches nothing."""
+    q, r = experts(9, 3, 256, 64), gen(n + 5)
+    x, w = r(n, 256).to(dtype), r(n, 2)
+    ids = torch.arange(2 * n, device=DEV, dtype=torch.int32).view(n, 2) % 3
+    ids[3, 1], w[3, 1] = -1, float("nan")
+    bad = x.clone()
+    bad[0, 17], bad[2, 255], bad[n - 1] = float("nan"), float("inf"), float("-inf")
+    y, y2 = torch.empty_like(x), torch.empty_like(x)
+    att.moe(x, ids, w, *q, y)
+    att.moe(bad, ids, w, *q, y2)
+    rows = torch.ones(n, dtype=torch.bool, device=DEV)
+    rows[[0, 2, n - 1]] = False
+    assert torch.isfinite(y).all() and torch.equal(y[rows], y2[rows])
+    assert not torch.isfinite(y2[~rows]).any()
 
 
 def test_moe_strides_offsets_and_neighbours(att):
