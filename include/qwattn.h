@@ -432,8 +432,7 @@ int qwattn_conv_silu(qwattn_ctx* ctx, void* stream, const qwattn_conv* args);
  *   S <- decay S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q
  * with g = a and beta = b as given, or, with a_coef and dt_bias, g = a_coef[h] softplus(a + dt_bias[h]) and
  * beta = 1 / (1 + e^-b). With z and gamma the output is o rsqrt(mean o^2 + rms_eps) gamma silu(z), else o.
- * fp32 arithmetic (chunks of many tokens: products of fp32 accuracy on the matrix cores; of what only a bf16 output
- * reads, 16 bits), one rounding to dtype.
+ * fp32 arithmetic (chunks of many tokens: products of fp32 accuracy on the matrix cores), one rounding to dtype.
  * Few tokens run token by token; more run in chunks of 64 tokens whose chunk-internal part is computed for all
  * chunks at once (that form needs the workspace). Results do not depend on timing. An infinity or NaN in a token
  * stays in its sequence and heads; in chunks it also reaches earlier tokens of its own chunk. */

@@ -181,7 +181,9 @@ static hipError_t delta_step(const DeltaArgs& a, hipStream_t s) {
 //                                      five vectors: beta, and the row scales of K S, Q S and K^T U; e^(G_end)
 // Where tokens are the summed index (K^T, T, P and the X and U beside them) lane group g of a 32-token step holds the
 // tokens 4 g .. 4 g + 3 of its first 16 and of its second 16: accumulator registers again.
-// What only the output takes part in (Q S and P U) has two parts where the output is bf16: within 2^-16 beside its 2^-8.
+// That holds for a bf16 output too: where its terms cancel, 16 bits of them show in it. (Two parts of Q S and P U there:
+// 4,096 tokens of 32 heads of 128 x 128 in 177 us instead of 183, but a quarter of the outputs that are 2^-13 of their
+// terms beyond half a step of bf16.)
 constexpr int kChunk = 64, kTriFrags = 6, kVec = 320;
 
 struct DeltaWs {
@@ -196,22 +198,20 @@ struct KqUnit {
     static constexpr int kSteps = DK / 32, kOne = NP * 4 * kSteps * 1024;
     static constexpr int kQ = NP == 3 ? kOne : 0, kKT = NP == 3 ? 2 * kOne : 0, kBytes = kKT + kOne;  // (K at 0)
 };
-constexpr int kTpOne = 3 * kTriFrags * 1024;
-constexpr int out_parts(int dt) { return dt ? 2 : 3; }
-constexpr int tp_bytes(int dt) { return kTpOne + out_parts(dt) * kTriFrags * 1024; }
+constexpr int kTpOne = 3 * kTriFrags * 1024, kTpBytes = 2 * kTpOne;
 
 // The six (or, with one part on the left, three) part products. Those of one order of magnitude share an accumulator:
 // three short chains instead of one long one, whose steps would wait for each other (a wave has no other on its SIMD to
 // fill the gaps).
-template <int NP, int ORDERS = 3>  // ORDERS 2: without the smallest
+template <int NP>
 __device__ __forceinline__ void mfma_parts(const bf16x8 (&a)[NP], const bf16x8 (&b)[3], f32x4 (&c)[3]) {
-    if constexpr (ORDERS == 3) c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[2], c[2], 0, 0, 0);
+    c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[2], c[2], 0, 0, 0);
     c[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[1], c[1], 0, 0, 0);
     c[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[0], c[0], 0, 0, 0);
     if constexpr (NP == 3) {
-        if constexpr (ORDERS == 3) c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[1], c[2], 0, 0, 0);
+        c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[1], c[2], 0, 0, 0);
         c[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[0], c[1], 0, 0, 0);
-        if constexpr (ORDERS == 3) c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[2], b[0], c[2], 0, 0, 0);
+        c[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[2], b[0], c[2], 0, 0, 0);
     }
 }
 __device__ __forceinline__ void zero(f32x4 (&c)[3]) { c[0] = c[1] = c[2] = f32x4{0.f, 0.f, 0.f, 0.f}; }
@@ -449,8 +449,8 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
             }
         }
         __syncthreads();
-        uint8_t* tp = ws.tp + unit * tp_bytes(DT);
-        auto write_frags = [&](uint8_t* to, int parts) {
+        uint8_t* tp = ws.tp + unit * kTpBytes;
+        auto write_frags = [&](uint8_t* to) {
             for (int i = tid; i < kTriFrags * 64; i += 256) {
                 const int f = i >> 6, l = i & 63;
                 const int tile = f < 2 ? f : 1 + (f >> 1), step = f < 2 ? 0 : f & 1;
@@ -460,11 +460,10 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
                 u32x4 w[3];
                 split3(v, w);
 #pragma unroll
-                for (int p = 0; p < 3; p++)
-                    if (p < parts) *reinterpret_cast<u32x4*>(to + (p * kTriFrags + f) * 1024 + l * 16) = w[p];
+                for (int p = 0; p < 3; p++) *reinterpret_cast<u32x4*>(to + (p * kTriFrags + f) * 1024 + l * 16) = w[p];
             }
         };
-        write_frags(tp + kTpOne, out_parts(DT));  // P
+        write_frags(tp + kTpOne);  // P
         {  // the inverse of A's diagonal block `wave` (unit lower triangular): lane c its column c, row after row
             const float* blk = sA + (16 * wave) * LD + 16 * wave;
             float x[16];
@@ -512,7 +511,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
             });
         });
         __syncthreads();
-        write_frags(tp, 3);
+        write_frags(tp);
         __syncthreads();
     }
 }
@@ -548,13 +547,12 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
     // that moves on by a chunk and a lane offset; no load is conditional (a wave without an operand loads one of
     // another's), so that no branch waits for loads.
     const uint32_t lane16 = lane * 16;
-    const size_t kq_step = (size_t)a.k_heads * Unit::kBytes, tp_step = (size_t)a.v_heads * tp_bytes(DT), vec_step = (size_t)a.v_heads * kVec * 4;
+    const size_t kq_step = (size_t)a.k_heads * Unit::kBytes, tp_step = (size_t)a.v_heads * kTpBytes, vec_step = (size_t)a.v_heads * kVec * 4;
     const uint8_t* kq = ws.kq + ((size_t)b * ncs * a.k_heads + kh) * Unit::kBytes;
-    const uint8_t* tp = ws.tp + ((size_t)b * ncs * a.v_heads + h) * tp_bytes(DT);
+    const uint8_t* tp = ws.tp + ((size_t)b * ncs * a.v_heads + h) * kTpBytes;
     const uint8_t* vec = reinterpret_cast<const uint8_t*>(ws.vec + ((size_t)b * ncs * a.v_heads + h) * kVec);
     auto frag = [&](const uint8_t* p) { return *reinterpret_cast<const bf16x8*>(p + lane16); };
     auto vec4 = [&](int which) { return *reinterpret_cast<const f32x4*>(vec + 256 * which + (uint32_t)tok * 4); };
-    constexpr int OP = out_parts(DT);
     bf16x8 fM[2][3];  // T or P
     // bf16 K and Q: the fragment of row tile i and dim step s as the rows lie in memory, rows past the last as the last
     // one (their results are multiplied by zero, or not stored)
@@ -564,10 +562,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
                                                 32 * s + ((size_t)r * stride + 8 * g));
     };
     const int f0 = wave < 2 ? wave : 2 * (wave - 1), f1 = wave < 2 ? f0 : f0 + 1;  // this row tile's two steps
-    auto load_tri = [&](const uint8_t* p, int parts) {
+    auto load_tri = [&](const uint8_t* p) {
 #pragma unroll
         for (int i = 0; i < 3; i++) {
-            if (i >= parts) break;
             fM[0][i] = frag(p + (i * kTriFrags + f0) * 1024);
             fM[1][i] = frag(p + (i * kTriFrags + f1) * 1024);
         }
@@ -596,7 +593,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         size_t first = row0 * stride + h * DV + 16 * slice, at[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) at[i] = (tok + i) * stride + c;
-        load_q(0), load_tri(tp + kTpOne, OP), vq = vec4(2);
+        load_q(0), load_tri(tp + kTpOne), vq = vec4(2);
 #pragma unroll 1
         for (int ch = 0; ch < nc; ch++) {
             move_on(ch + 1 < nc);
@@ -606,8 +603,8 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
             for (int s = 0; s < KS; s++) {
                 bf16x8 bs[3];
 #pragma unroll
-                for (int p = 0; p < OP; p++) bs[p] = frag(sS[s][p]);
-                mfma_parts<NP, OP>(fQ[s], bs, acc);
+                for (int p = 0; p < 3; p++) bs[p] = frag(sS[s][p]);
+                mfma_parts<NP>(fQ[s], bs, acc);
             }
             load_q(min(ch + 1, nc - 1));
             f32x4 qs;
@@ -628,9 +625,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
                 u32x4 w[3];
                 split3(v, w);
                 const bf16x8 bu[3] = {__builtin_bit_cast(bf16x8, w[0]), __builtin_bit_cast(bf16x8, w[1]), __builtin_bit_cast(bf16x8, w[2])};
-                mfma_parts<3, OP>(fM[st], bu, acc);
+                mfma_parts<3>(fM[st], bu, acc);
             }
-            load_tri(tp + kTpOne, OP);
+            load_tri(tp + kTpOne);
             const int more = left - ch * kChunk - tok;
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -703,7 +700,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         for (int p = 0; p < 3; p++)
             *reinterpret_cast<u32x2*>(to[wave >> 1][p] + lane16 + (wave & 1) * 8) = u32x2{lo[p], hi[p]};
     };
-    load_k(0), load_x(0), load_tri(tp, 3);
+    load_k(0), load_x(0), load_tri(tp);
     put_state();
     __builtin_amdgcn_s_setprio(2);  // ahead of the output waves
 #pragma unroll 1
@@ -759,7 +756,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
         lds_barrier();  // U, and with the scales of K^T's columns
         bf16x8 bw[2][3];
         get(sW[0], bw[0]), get(sW[1], bw[1]);
-        load_tri(tp, 3);
+        load_tri(tp);
         if (KS == 4 || wave < KS) {
             f32x4 s[2][3];
 #pragma unroll
@@ -817,7 +814,7 @@ static int step_most(const DeltaArgs& a, bool bf16) {
     return (int)(bf16 ? std::min(18 + pairs / 10, 48ll) : std::min(18 + pairs / 6, 100ll));
 }
 // Chunks of a call are worked off in segments of about this many (chunk, value head) pairs at a time, whose
-// workspace (39 KB a pair of two a key head in bf16, 109 KB in fp32) stays in the last-level cache.
+// workspace (45 KB a pair of two a key head in bf16, 109 KB in fp32) stays in the last-level cache.
 constexpr int kSegmentPairs = 2048;
 
 static bool by_steps(const DeltaArgs& a, bool bf16) { return a.snap || a.n <= step_most(a, bf16); }
@@ -833,7 +830,7 @@ struct DeltaSizes {
 };
 static DeltaSizes delta_sizes(const DeltaArgs& a, bool bf16) {
     const size_t chunks = (size_t)a.n_seq * segment_chunks(a);
-    return {up256(chunks * a.k_heads * (bf16 ? 1 : 9) * kChunk * a.key_dim * 2), up256(chunks * a.v_heads * tp_bytes(bf16)),
+    return {up256(chunks * a.k_heads * (bf16 ? 1 : 9) * kChunk * a.key_dim * 2), up256(chunks * a.v_heads * kTpBytes),
             up256(chunks * a.v_heads * kVec * 4),
             a.z ? up256((size_t)a.n_seq * a.n * a.v_heads * a.val_dim * 4) : 0};
 }

@@ -247,6 +247,40 @@ def test_delta_token_that_is_not_finite(att, n, dtype):
     assert torch.isnan(out2[1, at:, 0]).all() and torch.isnan(state2[1, 0]).all()
 
 
+@pytest.mark.parametrize("gated", [False, True])
+def test_delta_bf16_chunks_where_terms_cancel(att, gated):
+    """bf16 outputs that are 2^-13 of their terms: q reads pairs of tokens whose keys are unit vectors and whose updates,
+    fp32 values of 24 bits, cancel but for that (within a chunk and, through the state, from the one before). A term takes
+    at most 24 roundings to fp32: beta v one, its key's and q's norms four each, the scales they enter four, decay,
+    products and sums of parts the rest. Operands cut to 16 bits would be off by up to 2^-16 of a term, 2^-3 of an output."""
+    n, dk, dv, hv = 100, 128, 64, 2
+    d = delta_inputs(77, 1, n, 1, hv, dk, dv, BF16, False, gated)
+    d["state"].zero_(), d["a"].zero_(), d["q"].zero_(), d["k"].zero_()
+    g = torch.Generator().manual_seed(78)
+    d["q"][0, 0, 0, 0] = 1
+    for t in range(n):
+        d["k"][0, t, 0, t] = 1
+        if t:
+            m = int(torch.randint((t + 1) // 2, (1,), generator=g))
+            d["q"][0, t, 0, 2 * m:2 * m + 2] = 1
+    d["v"][:] *= 512
+    d["v"][:, 1::2] = -d["v"][:, ::2]
+    d["b"][:] = 0.5 + 0.4 * torch.rand(1, n, hv, generator=g).to(DEV)
+    d["b"][:, 1::2] = d["b"][:, ::2] * (1 - 2.0 ** -13)
+    o, want, _, _, _ = lo.delta(**d)
+    # every token's sum of magnitudes: the same with all values positive
+    term = lo.delta(**{**d, "v": d["v"].abs()})[0]
+    E = 24 * EPS32 * term
+    if gated:
+        z, gamma = f64(d["z"]), f64(d["gamma"])
+        rms = 1 / torch.sqrt((o * o).mean(-1, keepdim=True) + 1e-6)
+        gate = rms * (gamma * z / (1 + torch.exp(-z))).abs()
+        E = 2 * gate * (E + o.abs() * rms * (E * E).mean(-1, keepdim=True).sqrt()) + (2 * z.abs() + 24) * EPS32 * want.abs()
+    out, _, _ = delta_run(att, d)
+    close(out, want, E + HALF[BF16] * want.abs() * 1.01, "out")
+    assert float((o[0, 1:].abs() / term[0, 1:]).max()) < 2.0 ** -13  # the case is the one meant
+
+
 def test_delta_chunks_join(att):
     """A prompt in one call, in ragged calls of both forms, and token by token: states and outputs agree."""
     d = delta_inputs(80, 1, 150, 2, 4, 128, 128, F32, True, True)
