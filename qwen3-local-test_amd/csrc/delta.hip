@@ -390,11 +390,12 @@ __global__ __launch_bounds__(256, 2) void k_delta_prep(DeltaArgs a, DeltaWs ws, 
         const int slot = hi & 3;
         const size_t unit = (size_t)(b * ncs + cl) * a.v_heads + head(hi);
         if (slot == 0) {  // the gates of the next four heads, a wave a head, a lane a token. G in 64 bits (its differences
-                          // are what counts), each g at least -2000 (e^g is 0 from -104 on; sums of -inf have none)
+                          // are what counts), each g at least -2000 (e^g is 0 from -104 on; sums of -inf have none); a
+                          // NaN stays one (fmaxf would make it -2000)
             if (hi + wave < R) {
                 const int h = head(hi + wave);
                 const size_t r = (size_t)b * a.n + t0 + min(lane, nt - 1);
-                const float lg = fmaxf(delta_log_decay(a, r, h), -2000.f), be = delta_beta(a, r, h);
+                const float given = delta_log_decay(a, r, h), lg = given < -2000.f ? -2000.f : given, be = delta_beta(a, r, h);
                 const double G = scan64(lane < nt ? (double)lg * 1.4426950408889634074 : 0.0);
                 const uint64_t u = __builtin_bit_cast(uint64_t, G);
                 const double end = __builtin_bit_cast(

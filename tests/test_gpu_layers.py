@@ -281,6 +281,45 @@ def test_delta_bf16_chunks_where_terms_cancel(att, gated):
     assert float((o[0, 1:].abs() / term[0, 1:]).max()) < 2.0 ** -13  # the case is the one meant
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [12, 200])
+@pytest.mark.parametrize("name", ["a", "b", "q", "k", "v", "a_coef", "dt_bias"])
+def test_delta_nan_in_any_operand(att, name, n, dtype):
+    """A NaN reaches every output and state that the definition computes from it: a gate's or value's its head from its
+    token on, a key's the key head's value heads, a query's its token's outputs alone, a parameter's its head in every
+    sequence; what it does not reach (in chunks: and earlier tokens of its chunk) has the bits of a clean call."""
+    d = delta_inputs(190 + n, 2, n, 2, 4, 64, 64, dtype, True, True)
+    bad, at = {k: v.clone() for k, v in d.items()}, n - 3
+    seqs, rows, heads = [1], slice(at, n), [0]
+    if name in ("a", "b"):
+        bad[name][1, at, 0] = float("nan")
+    elif name == "v":
+        bad[name][1, at, 0, 5] = float("nan")
+    elif name in ("q", "k"):
+        bad[name][1, at, 0, 5] = float("nan")
+        heads, rows = [0, 1], slice(at, at + 1) if name == "q" else rows
+    else:
+        bad[name][0] = float("nan")
+        seqs, rows = [0, 1], slice(0, n)
+    out, state, _ = delta_run(att, d)
+    out2, state2, _ = delta_run(att, bad)
+    reached = torch.zeros(2, n, 4, dtype=torch.bool, device=DEV)
+    free = torch.ones_like(reached)
+    first = rows.start if n < 64 else rows.start // 64 * 64
+    for s in seqs:
+        for h in heads:
+            reached[s, rows, h] = True
+            free[s, first if name != "q" else rows.start:rows.stop, h] = False
+            if name != "q":
+                # a value's NaN stays in its column of the state, and the gated norm spreads it over the output
+                where = state2[s, h, :, 5] if name == "v" else state2[s, h]
+                assert torch.isnan(where).all(), f"state of sequence {s}, head {h}"
+    assert torch.isnan(out2[reached]).all()
+    assert torch.equal(out2[free], out[free]) and torch.isfinite(out2[free]).all()
+    kept = [(s, h) for s in range(2) for h in range(4) if name == "q" or not (s in seqs and h in heads)]
+    assert all(torch.equal(state2[s, h], state[s, h]) for s, h in kept)
+
+
 def test_delta_chunks_join(att):
     """A prompt in one call, in ragged calls of both forms, and token by token: states and outputs agree."""
     d = delta_inputs(80, 1, 150, 2, 4, 128, 128, F32, True, True)
