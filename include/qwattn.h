@@ -410,8 +410,8 @@ int qwattn_layer_attention_qsa(qwattn_ctx* ctx, void* stream, int slot, const vo
  * rows before the first token from `state`, which then receives the last taps - 1 rows. fp32 sums, one rounding
  * to dtype. */
 typedef struct qwattn_conv {
-    int n_seq, n;
-    int channels;         /* a multiple of 8 */
+    int n_seq, n;         /* n_seq <= 65535, n_seq * n <= 2^31 - 2^16 */
+    int channels;         /* a multiple of 8, <= 2^24 */
     int taps;             /* 2, 3 or 4 */
     int dtype;            /* of x and y: QWATTN_F32 or QWATTN_BF16 */
     const int32_t* lens;  /* device [n_seq] or NULL */
@@ -437,7 +437,8 @@ int qwattn_conv_silu(qwattn_ctx* ctx, void* stream, const qwattn_conv* args);
  * chunks at once (that form needs the workspace). Results do not depend on timing. An infinity or NaN in a token
  * stays in its sequence and heads; in chunks it also reaches earlier tokens of its own chunk. */
 typedef struct qwattn_delta {
-    int n_seq, n;         /* n_seq <= 65535; n_seq * v_heads < 2^20, with z also n_seq * n * v_heads < 2^27 */
+    int n_seq, n;         /* n_seq <= 65535, n_seq * n <= 2^31 - 2^16; n_seq * v_heads < 2^20, with z also
+                             n_seq * n * v_heads < 2^27 */
     int k_heads, v_heads; /* v_heads a multiple of k_heads, <= 1024 */
     int key_dim, val_dim; /* 64 or 128 each */
     int tiled;            /* value head h uses key head h / (v_heads / k_heads) (0) or h % k_heads (1) */

@@ -39,10 +39,13 @@ inline bool rows_meet(const void* p, int64_t p_width, int64_t p_stride, const vo
     return d < p_width || d + q_width > p_stride;
 }
 
+// Rows of a call: tiles of up to 32,768 tokens and chunks of 64 are counted by 32-bit sums behind the last row
+constexpr int64_t kMostRows = (int64_t(1) << 31) - (1 << 16);
+
 inline int check_conv(const qwattn_conv* a, CheckText& m) {
     if (!a) return refuse(m, QWATTN_EINVAL, "qwattn_conv_silu: null arguments");
-    if (a->n_seq <= 0 || a->n <= 0 || (int64_t)a->n_seq * a->n > INT32_MAX || a->n_seq > 65535)
-        return refuse(m, QWATTN_EINVAL, "qwattn_conv_silu: n_seq %d (1..65535), n %d", a->n_seq, a->n);
+    if (a->n_seq <= 0 || a->n <= 0 || (int64_t)a->n_seq * a->n > kMostRows || a->n_seq > 65535)
+        return refuse(m, QWATTN_EINVAL, "qwattn_conv_silu: n_seq %d (1..65535), n %d (n_seq x n <= 2^31 - 2^16)", a->n_seq, a->n);
     if (a->channels <= 0 || a->channels % 8 || a->channels > (1 << 24) || a->taps < 2 || a->taps > 4 || bad_dtype(a->dtype))
         return refuse(m, QWATTN_EINVAL, "qwattn_conv_silu: channels %d (a multiple of 8), taps %d (2..4), dtype %d",
                       a->channels, a->taps, a->dtype);
@@ -61,8 +64,8 @@ inline int check_conv(const qwattn_conv* a, CheckText& m) {
 
 inline int check_delta_shape(const qwattn_delta* a, CheckText& m) {
     if (!a) return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: null arguments");
-    if (a->n_seq <= 0 || a->n <= 0 || (int64_t)a->n_seq * a->n > INT32_MAX || a->n_seq > 65535)
-        return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: n_seq %d (1..65535), n %d", a->n_seq, a->n);
+    if (a->n_seq <= 0 || a->n <= 0 || (int64_t)a->n_seq * a->n > kMostRows || a->n_seq > 65535)
+        return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: n_seq %d (1..65535), n %d (n_seq x n <= 2^31 - 2^16)", a->n_seq, a->n);
     if (a->k_heads <= 0 || a->v_heads <= 0 || a->v_heads > 1024 || a->v_heads % a->k_heads)
         return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: k_heads %d, v_heads %d (a multiple of k_heads, <= 1024)",
                       a->k_heads, a->v_heads);

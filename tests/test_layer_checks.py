@@ -192,3 +192,21 @@ def test_sizes_beyond_a_launch_are_refused(lib, qw):
     assert lib.layer_route(P, 8, most, 8, 8, P, P) == 0
     assert lib.layer_route(P, 8, most + 1, 8, 8, P, P) == EINVAL
     assert "2^26" in lib.layer_text().decode()
+
+
+def test_rows_beyond_32_bit_sums_are_refused(lib, qw):
+    """The launchers count tiles (of 16 tokens, doubled while there are more than a grid's y dimension takes) and chunks
+    by sums of n and less than a tile: up to the limit they stay below 2^31."""
+    most, tile = 2**31 - 2**16, 16
+    while (most + tile - 1) // tile > 65535:
+        tile *= 2
+    assert most + tile - 1 < 2**31
+    far = dict(channels=8, dtype=1, x=1 << 44, y=2 << 44, x_stride=8, y_stride=8, n_seq=1)
+    assert lib.layer_conv(conv_args(qw, **{**far, "n": most})) == 0
+    for n_seq, n in ((1, most + 1), (1, 2**31 - 20001), (1, 2**31 - 1), (2, 2**30 - 2**15 + 1), (65535, 32768)):
+        assert lib.layer_conv(conv_args(qw, **{**far, "n_seq": n_seq, "n": n})) == EINVAL
+        assert "2^31 - 2^16" in lib.layer_text().decode()
+    apart = {name: (i + 1) << 50 for i, name in enumerate(("q", "k", "v", "out"))}
+    assert lib.layer_delta(delta_args(qw, **{**apart, "n_seq": 1, "n": most}), 0) == 0
+    assert lib.layer_delta(delta_args(qw, **{**apart, "n_seq": 1, "n": most + 1}), 0) == EINVAL
+    assert "2^31 - 2^16" in lib.layer_text().decode()
