@@ -404,7 +404,7 @@ int qwattn_layer_attention_qsa(qwattn_ctx* ctx, void* stream, int slot, const vo
  *
  * Sequences: n_seq of them, n rows each (row b * n + t is token t of sequence b). `lens` (device int32 [n_seq],
  * NULL: n everywhere) shortens them: sequence b has min(max(lens[b], 0), n) tokens; rows past them are neither
- * used nor written, and the state is that after the last token. */
+ * used nor written, and the state is that after the last token. A row stride times the rows is at most 2^59. */
 
 /* Short causal depthwise convolution with SiLU: y[t][c] = silu(bias[c] + sum_j w[c][j] x[t - taps + 1 + j][c]),
  * rows before the first token from `state`, which then receives the last taps - 1 rows. fp32 sums, one rounding

@@ -24,11 +24,11 @@ __attribute__((format(printf, 3, 4))) inline int refuse(CheckText& m, int code, 
 
 inline bool bad_dtype(int d) { return d != QWATTN_F32 && d != QWATTN_BF16; }
 inline bool unaligned(const void* p, unsigned to = 16) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
-// A row stride of at least `width` elements, a multiple of 8; rows * stride stays far below 2^62 bytes
-inline bool bad_stride(int64_t s, int64_t width) { return s < width || s % 8 || s > (int64_t(1) << 40); }
+// A row stride of at least `width` elements, a multiple of 8, that spans at most 2^59 elements (2^61 bytes) over the rows
+inline bool bad_stride(int64_t s, int64_t width, int64_t rows) { return s < width || s % 8 || s > (int64_t(1) << 59) / rows; }
 
 // Whether the byte ranges of two row sets meet: `rows` rows of `width` bytes at `stride` bytes from p, and likewise
-// from q. Rows at one stride whose columns do not meet (two slices of one buffer's rows) count as apart.
+// from q (each within 2^61 bytes: bad_stride). Rows at one stride whose columns do not meet (two slices of one buffer's rows) count as apart.
 inline bool rows_meet(const void* p, int64_t p_width, int64_t p_stride, const void* q, int64_t q_width, int64_t q_stride,
                       int64_t rows) {
     const int64_t a = (int64_t)reinterpret_cast<uintptr_t>(p), b = (int64_t)reinterpret_cast<uintptr_t>(q);
@@ -50,14 +50,14 @@ inline int check_conv(const qwattn_conv* a, CheckText& m) {
         return refuse(m, QWATTN_EINVAL, "qwattn_conv_silu: channels %d (a multiple of 8), taps %d (2..4), dtype %d",
                       a->channels, a->taps, a->dtype);
     if (!a->x || !a->w || !a->state || !a->y) return refuse(m, QWATTN_EINVAL, "qwattn_conv_silu: null pointer");
-    if (bad_stride(a->x_stride, a->channels) || bad_stride(a->y_stride, a->channels))
-        return refuse(m, QWATTN_EINVAL, "qwattn_conv_silu: x_stride %lld, y_stride %lld (>= channels, multiples of 8)",
+    const int64_t rows = (int64_t)a->n_seq * a->n;
+    if (bad_stride(a->x_stride, a->channels, rows) || bad_stride(a->y_stride, a->channels, rows))
+        return refuse(m, QWATTN_EINVAL, "qwattn_conv_silu: x_stride %lld, y_stride %lld (>= channels, multiples of 8, x rows <= 2^59)",
                       (long long)a->x_stride, (long long)a->y_stride);
     if (unaligned(a->x) || unaligned(a->w) || unaligned(a->bias) || unaligned(a->state) || unaligned(a->snap) || unaligned(a->y))
         return refuse(m, QWATTN_EINVAL, "qwattn_conv_silu: pointers must be 16-byte aligned");
     const int64_t size = a->dtype == QWATTN_F32 ? 4 : 2;
-    if (rows_meet(a->x, a->channels * size, a->x_stride * size, a->y, a->channels * size, a->y_stride * size,
-                  (int64_t)a->n_seq * a->n))
+    if (rows_meet(a->x, a->channels * size, a->x_stride * size, a->y, a->channels * size, a->y_stride * size, rows))
         return refuse(m, QWATTN_EINVAL, "qwattn_conv_silu: x and y overlap");
     return QWATTN_OK;
 }
@@ -87,15 +87,16 @@ inline int check_delta(const qwattn_delta* a, size_t workspace, CheckText& m) {
     if (!a->a_coef != !a->dt_bias) return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: a_coef and dt_bias come together");
     if (!a->z != !a->gamma) return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: z and gamma come together");
     const int64_t kw = (int64_t)a->k_heads * a->key_dim, vw = (int64_t)a->v_heads * a->val_dim;
-    if (bad_stride(a->q_stride, kw) || bad_stride(a->k_stride, kw) || bad_stride(a->v_stride, vw) ||
-        bad_stride(a->out_stride, vw) || (a->z && bad_stride(a->z_stride, vw)))
+    const int64_t rows = (int64_t)a->n_seq * a->n;
+    if (bad_stride(a->q_stride, kw, rows) || bad_stride(a->k_stride, kw, rows) || bad_stride(a->v_stride, vw, rows) ||
+        bad_stride(a->out_stride, vw, rows) || (a->z && bad_stride(a->z_stride, vw, rows)))
         return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: strides q %lld, k %lld, v %lld, z %lld, out %lld (at least the "
-                      "heads' elements, multiples of 8)", (long long)a->q_stride, (long long)a->k_stride,
+                      "heads' elements, multiples of 8, x rows <= 2^59)", (long long)a->q_stride, (long long)a->k_stride,
                       (long long)a->v_stride, (long long)a->z_stride, (long long)a->out_stride);
     if (unaligned(a->q) || unaligned(a->k) || unaligned(a->v) || unaligned(a->z) || unaligned(a->out) || unaligned(a->state) ||
         unaligned(a->snap))
         return refuse(m, QWATTN_EINVAL, "qwattn_delta_rule: q, k, v, z, out, state and snap must be 16-byte aligned");
-    const int64_t size = a->dtype == QWATTN_F32 ? 4 : 2, rows = (int64_t)a->n_seq * a->n;
+    const int64_t size = a->dtype == QWATTN_F32 ? 4 : 2;
     struct {
         const void* p;
         int64_t width, stride;
@@ -139,8 +140,8 @@ inline int check_moe(const qwattn_moe_layer* l, const void* x, int dtype, int64_
     if (int rc = check_moe_layer(l, dtype, n, top_k, m)) return rc;
     if (!l->w_gate || !l->w_up || !l->w_down || !l->s_gate || !l->s_up || !l->s_down || !x || !ids || !weights || !y)
         return refuse(m, QWATTN_EINVAL, "qwattn_moe: null pointer");
-    if (bad_stride(x_stride, l->hidden) || bad_stride(y_stride, l->hidden))
-        return refuse(m, QWATTN_EINVAL, "qwattn_moe: x_stride %lld, y_stride %lld (>= hidden, multiples of 8)",
+    if (bad_stride(x_stride, l->hidden, n) || bad_stride(y_stride, l->hidden, n))
+        return refuse(m, QWATTN_EINVAL, "qwattn_moe: x_stride %lld, y_stride %lld (>= hidden, multiples of 8, x n <= 2^59)",
                       (long long)x_stride, (long long)y_stride);
     if (unaligned(l->w_gate) || unaligned(l->w_up) || unaligned(l->w_down) || unaligned(x) || unaligned(y))
         return refuse(m, QWATTN_EINVAL, "qwattn_moe: the int8 weights, x and y must be 16-byte aligned");

@@ -210,3 +210,24 @@ def test_rows_beyond_32_bit_sums_are_refused(lib, qw):
     assert lib.layer_delta(delta_args(qw, **{**apart, "n_seq": 1, "n": most}), 0) == 0
     assert lib.layer_delta(delta_args(qw, **{**apart, "n_seq": 1, "n": most + 1}), 0) == EINVAL
     assert "2^31 - 2^16" in lib.layer_text().decode()
+
+
+def test_strides_beyond_64_bit_addresses_are_refused(lib, qw):
+    """Rows that would span more than 2^59 elements: their byte addresses, and the check for overlaps, stay within 64 bits."""
+    rows = 2**31 - 2**16
+    most = 2**59 // rows // 8 * 8
+    assert rows * most * 4 + 2**57 < 2**63 <= rows * 2**40 * 4
+    far = dict(n_seq=1, n=rows, channels=8, x=1 << 44, y=(1 << 44) + 64)
+    assert lib.layer_conv(conv_args(qw, **{**CONV, **far, "x_stride": most, "y_stride": most})) == 0  # slices of one buffer
+    assert lib.layer_conv(conv_args(qw, **{**CONV, **far, "x_stride": most, "y_stride": most + 8})) == EINVAL
+    assert lib.layer_conv(conv_args(qw, **{**CONV, **far, "x_stride": 2**40, "y_stride": 2**40})) == EINVAL
+    assert "2^59" in lib.layer_text().decode()
+    one = dict(n_seq=1, n=rows, q=1 << 50, k=1 << 51, v=1 << 52, out=1 << 44)  # out ends below the others
+    assert lib.layer_delta(delta_args(qw, **{**one, "q_stride": most}), 0) == 0
+    for name in ("q", "k", "v", "out"):
+        assert lib.layer_delta(delta_args(qw, **{**one, name + "_stride": most + 8}), 0) == EINVAL
+        assert "2^59" in lib.layer_text().decode()
+    n, layer = 2**22, qw._MOE_LAYER.pack(*LAYER.values())
+    for stride, rc in ((2**37, 0), (2**37 + 8, EINVAL), (2**40, EINVAL)):
+        call = {**CALL, "n": n, "x": 1 << 50, "y": (1 << 50) + 256, "x_stride": stride, "y_stride": stride}
+        assert lib.layer_moe(layer, *call.values()) == rc
