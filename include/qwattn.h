@@ -457,11 +457,13 @@ typedef struct qwattn_delta {
     const float* gamma;   /* [val_dim], with z */
     void* out;            /* rows of v_heads * val_dim elements at out_stride (as v) */
     int64_t out_stride;
-    void* workspace;      /* qwattn_delta_workspace bytes, 256-byte aligned (NULL where that is 0) */
+    void* workspace;      /* qwattn_delta_workspace bytes (of this call's sizes or larger ones), 256-byte aligned (NULL
+                             where that is 0) */
     size_t workspace_bytes;
 } qwattn_delta;
 int qwattn_delta_rule(qwattn_ctx* ctx, void* stream, const qwattn_delta* args);
-/* The workspace of such a call (only sizes, dtype, snap and z of *args are looked at). */
+/* The workspace of such a call and of every one of fewer sequences or tokens, with z also of those without (only sizes,
+ * dtype, snap and z of *args are looked at; calls with snap need none). */
 int qwattn_delta_workspace(const qwattn_delta* args, size_t* bytes);
 
 /* The router: per row of logits[n][logits_stride] (n_experts used) the top_k largest, largest first, the lower
@@ -485,7 +487,7 @@ typedef struct qwattn_moe_layer {
  * occur twice. x and y are dtype (QWATTN_F32 or QWATTN_BF16) rows at strides that are multiples of 8, x 16-byte
  * aligned; fp32 accuracy, one rounding to dtype. Results do not depend on timing; the same row in calls of other n
  * or top_k may differ within that accuracy, since few pairs and many are computed in different orders.
- * workspace: qwattn_moe_workspace bytes, 256-byte aligned. */
+ * workspace: qwattn_moe_workspace bytes (of this n or a larger one), 256-byte aligned. */
 int qwattn_moe(qwattn_ctx* ctx, void* stream, const qwattn_moe_layer* layer, const void* x, int dtype,
                int64_t x_stride, const int32_t* ids, const float* weights, int top_k, void* y, int64_t y_stride, int n,
                void* workspace, size_t workspace_bytes);

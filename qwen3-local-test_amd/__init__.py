@@ -644,7 +644,8 @@ def decode_noalloc(cfg, qg, k, v, qn, kn, rope, kcache, vcache, kv_cap, out, pos
 
 @functools.lru_cache(maxsize=4096)
 def delta_workspace(n_seq, n, k_heads, v_heads, key_dim, val_dim, dtype, gated=False, snap=False):
-    """Bytes of workspace an Attention.delta_rule call of these sizes needs (gated: with z)."""
+    """Bytes of workspace that an Attention.delta_rule call of these sizes, or of fewer sequences or tokens, needs at most
+    (gated: with z, or without)."""
     lib, size = load_library(), ctypes.c_size_t()
     some = 256  # any address: only whether z and snap are set is looked at
     args = _DELTA.pack(n_seq, n, k_heads, v_heads, key_dim, val_dim, 0, _ROW_DT[dtype], 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
@@ -657,7 +658,7 @@ def delta_workspace(n_seq, n, k_heads, v_heads, key_dim, val_dim, dtype, gated=F
 
 @functools.lru_cache(maxsize=4096)
 def moe_workspace(n_experts, hidden, ffn, dtype, n, top_k):
-    """Bytes of workspace an Attention.moe call of these sizes needs."""
+    """Bytes of workspace that an Attention.moe call of these sizes, or of fewer rows, needs at most."""
     lib, size = load_library(), ctypes.c_size_t()
     rc = lib.qwattn_moe_workspace(_MOE_LAYER.pack(n_experts, hidden, ffn, 0, 0, 0, 0, 0, 0), _ROW_DT[dtype], n, top_k,
                                   ctypes.byref(size))

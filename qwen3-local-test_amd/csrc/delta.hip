@@ -835,10 +835,20 @@ static DeltaSizes delta_sizes(const DeltaArgs& a, bool bf16) {
             up256(chunks * a.v_heads * kVec * 4),
             a.z ? up256((size_t)a.n_seq * a.n * a.v_heads * a.val_dim * 4) : 0};
 }
-size_t delta_workspace(const DeltaArgs& a, bool bf16) {
+size_t delta_need(const DeltaArgs& a, bool bf16) {
     if (by_steps(a, bf16)) return 0;
     const DeltaSizes s = delta_sizes(a, bf16);
     return s.kq + s.tp + s.vec + s.o;
+}
+// Fewer tokens never need more. Fewer sequences can: a segment then has more whole chunks of each, and fewer tokens run
+// token by token. With more pairs than a segment's both are at their end, and the need grows with the sequences.
+size_t delta_workspace(DeltaArgs a, bool bf16) {
+    size_t most = delta_need(a, bf16);
+    for (int b = std::min(a.n_seq, kSegmentPairs / a.v_heads); b > 0; b--) {
+        a.n_seq = b;
+        most = std::max(most, delta_need(a, bf16));
+    }
+    return most;
 }
 
 template <int DT, int DK, int DV>

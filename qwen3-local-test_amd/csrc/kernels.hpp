@@ -319,8 +319,10 @@ struct DeltaArgs {
     void* out;
     void* ws;
 };
-// Bytes of workspace that launch_delta needs (0: none); only sizes, z and snap of `a` are looked at.
-size_t delta_workspace(const DeltaArgs& a, bool bf16);
+// Bytes of workspace that launch_delta needs (0: none), and that calls of up to as many sequences and tokens need; only
+// sizes, z and snap of `a` are looked at.
+size_t delta_need(const DeltaArgs& a, bool bf16);
+size_t delta_workspace(DeltaArgs a, bool bf16);
 hipError_t launch_delta(const DeltaArgs& a, bool bf16, hipStream_t s);
 
 struct RouteArgs {

@@ -1167,7 +1167,7 @@ int qwattn_delta_rule(qwattn_ctx* c, void* stream, const qwattn_delta* p) {
     if (int rc = qw::check_delta_shape(p, m)) return fail(c, rc, "%s", m.text);
     const qw::DeltaArgs a = delta_args(*p, c->cfg.rms_eps);
     const bool bf16 = p->dtype == QWATTN_BF16;
-    if (int rc = qw::check_delta(p, qw::delta_workspace(a, bf16), m)) return fail(c, rc, "%s", m.text);
+    if (int rc = qw::check_delta(p, qw::delta_need(a, bf16), m)) return fail(c, rc, "%s", m.text);
     DeviceGuard dg(c->device);
     HIP_TRY(c, qw::launch_delta(a, bf16, (hipStream_t)stream));
     return QWATTN_OK;

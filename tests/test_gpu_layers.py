@@ -676,6 +676,30 @@ def test_two_streams_at_once(att):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_workspace_for_smaller_calls(att, qw, dtype):
+    """A workspace for the largest call serves every smaller one (fewer sequences can need more than the largest): the
+    bits of calls with workspaces of their own, whatever bytes the last call left in it."""
+    hk, hv, d = 16, 32, 64
+    size = qw.delta_workspace(40, 130, hk, hv, d, d, dtype, True)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device=DEV)
+    for n_seq, n in ((40, 130), (33, 130), (32, 130), (3, 130), (1, 130), (1, 40), (40, 40), (7, 19)):
+        i = delta_inputs(300 + n_seq, n_seq, n, hk, hv, d, d, dtype, True, True)
+        out, state, _ = delta_run(att, i)
+        s2, o2 = i["state"].clone(), torch.empty_like(out)
+        att.delta_rule(**{**i, "state": s2}, out=o2, workspace=ws)
+        assert torch.equal(out, o2) and torch.equal(state, s2), (n_seq, n)
+    q, e, k = experts(10, 8, 128, 96), 8, 2
+    ws = torch.full((qw.moe_workspace(e, 128, 96, dtype, 700, k),), 255, dtype=torch.uint8, device=DEV)
+    for n in (700, 300, 31, 5, 1):
+        r = gen(n)
+        x, ids, w = r(n, 128).to(dtype), torch.arange(n * k, device=DEV, dtype=torch.int32).view(n, k) % e, r(n, k)
+        y, y2 = torch.empty_like(x), torch.empty_like(x)
+        att.moe(x, ids, w, *q, y)
+        att.moe(x, ids, w, *q, y2, workspace=ws)
+        assert torch.equal(y, y2), n
+
+
 def test_library_refuses_on_the_gpu(att, qw):
     """The library's own checks behind the mirror's: an error with its text, nothing launched."""
     z = lambda *s, dtype=F32: torch.zeros(s, device=DEV, dtype=dtype)

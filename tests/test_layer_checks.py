@@ -231,3 +231,22 @@ def test_strides_beyond_64_bit_addresses_are_refused(lib, qw):
     for stride, rc in ((2**37, 0), (2**37 + 8, EINVAL), (2**40, EINVAL)):
         call = {**CALL, "n": n, "x": 1 << 50, "y": (1 << 50) + 256, "x_stride": stride, "y_stride": stride}
         assert lib.layer_moe(layer, *call.values()) == rc
+
+
+def test_a_workspace_serves_every_smaller_call(qw):
+    """A program asks once, at its largest: the bytes for (n_seq, n) suffice for any fewer sequences and tokens, for the
+    delta rule with z also without, for the experts at any smaller n."""
+    lengths = [1, 17, 19, 22, 40, 49, 64, 65, 101, 128, 333, 4096]
+    for heads in ((16, 32, 128, 128), (1, 3, 64, 128), (8, 512, 64, 64)):
+        for dtype in (torch.float32, torch.bfloat16):
+            for gated in (False, True):
+                size = {(b, n): qw.delta_workspace(b, n, *heads, dtype, gated) for b in (*range(1, 70), 300) for n in lengths
+                        if b * n * heads[1] < 2**27}  # (larger ones are refused with z)
+                for (b, n), bytes_ in size.items():
+                    assert size[max(1, b - 1 if b < 300 else 69), n] <= bytes_, (heads, dtype, gated, b, n)
+                    assert all(size[b, m] <= bytes_ for m in lengths if m < n), (heads, dtype, gated, b, n)
+                    assert qw.delta_workspace(b, n, *heads, dtype, False) <= bytes_
+    for e, hidden, ffn, k in ((128, 2048, 512, 8), (4, 64, 32, 2), (8, 1024, 352, 2), (1024, 256, 96, 10), (1, 32, 32, 1)):
+        for dtype in (torch.float32, torch.bfloat16):
+            sizes = [qw.moe_workspace(e, hidden, ffn, dtype, n, k) for n in (*range(1, 600), 2048, 6553, 6554, 20000, 65536, 70000)]
+            assert sizes == sorted(sizes)
