@@ -66,6 +66,63 @@ def delta(q, k, v, a, b, state, a_coef=None, dt_bias=None, z=None, gamma=None, l
     return out, gated, S, snap, scale
 
 
+# How far fp32 results may be from 64 bits as a 2-norm, relative: errors of independent roundings, each 0.41 of half a step
+# in the mean square, add as squares. In the chunked delta rule at most 400 reach a value at its full size: the additions of
+# its four products (key_dim and three times a chunk's 64) and some tens in norms, gates and scales.
+CHUNK_LIMIT = 0.41 * math.sqrt(400) * EPS32
+
+
+def remembering(normal, n_seq, n, hk, hv, dk, dv, dtype):
+    """Inputs of the delta rule that keep most of their state (decays of 1% a token), so that every product of the chunked
+    form counts in its results; normal(*shape): standard normal values."""
+    q, k, v = (normal(n_seq, n, h, d).to(dtype) for h, d in ((hk, dk), (hk, dk), (hv, dv)))
+    return dict(q=q, k=k, v=v, a=-torch.exp(normal(n_seq, n, hv)) * 0.01, b=torch.sigmoid(1 + normal(n_seq, n, hv)),
+                state=normal(n_seq, hv, dk, dv))
+
+
+def cut(x, parts):
+    """x as the sum of that many bf16 parts, each what rounding leaves to the next."""
+    out, left = torch.zeros_like(x), x
+    for _ in range(parts):
+        part = left.float().bfloat16().double()
+        out, left = out + part, left - part
+    return out
+
+
+def delta_chunks(q, k, v, a, b, state, parts, eps=1e-6):
+    """The delta rule (direct gates) in chunks of 64 tokens in 64 bits, the products' operands cut to bf16 parts (three, or
+    parts[name]): (out, state). Names: kk and qk the rows in K K^T and Q K^T, k and s in K S, t and x in T X, q and qs in
+    Q S, p and u in P U, kt and w in K^T W."""
+    def op(x, name):
+        return cut(x, parts.get(name, 3))
+
+    q, k, v, a, b, S = f64(q), f64(k), f64(v), f64(a), f64(b), f64(state).clone()
+    hk, dk, hv = k.shape[2], k.shape[3], v.shape[2]
+    q = q / torch.sqrt((q * q).sum(-1, keepdim=True) + eps) / math.sqrt(dk)
+    k = k / torch.sqrt((k * k).sum(-1, keepdim=True) + eps)
+    head, out = torch.arange(hv) // (hv // hk), []
+    for t in range(0, v.shape[1], 64):
+        Q, K, V = (x[:, t:t + 64].transpose(1, 2) for x in (q[:, :, head], k[:, :, head], v))
+        G, B = a[:, t:t + 64].cumsum(1).transpose(1, 2), b[:, t:t + 64].transpose(1, 2)[..., None]
+        D, since, last = torch.exp(G[..., :, None] - G[..., None, :]).tril(), torch.exp(G)[..., None], G[..., -1:]
+        A = (B * D * (op(K, "kk") @ op(K, "kk").transpose(2, 3))).tril(-1)
+        T, P = torch.linalg.inv(torch.eye(A.shape[-1], dtype=A.dtype) + A), D * (op(Q, "qk") @ op(K, "qk").transpose(2, 3))
+        U = op(T, "t") @ op(B * (V - since * (op(K, "k") @ op(S, "s"))), "x")
+        out.append((since * (op(Q, "q") @ op(S, "qs")) + op(P, "p") @ op(U, "u")).transpose(1, 2))
+        S = torch.exp(last)[..., None] * S + op(K, "kt").transpose(2, 3) @ op(torch.exp(last - G)[..., None] * U, "w")
+    return torch.cat(out, 1), S
+
+
+def moe_limit(hidden, ffn):
+    """As CHUNK_LIMIT, for the experts: the additions of a gate and an up value, those of a result, and some tens beside."""
+    return 0.41 * math.sqrt(2 * hidden + ffn + 100) * EPS32
+
+
+def apart(got, want):
+    """The 2-norm of the difference, relative."""
+    return float((f64(got) - want).norm() / want.norm())
+
+
 def route(logits, top_k, renorm):
     """(ids, weights) by repeated maximum; -inf and NaN are no choice."""
     n, e = logits.shape

@@ -320,6 +320,19 @@ def test_delta_nan_in_any_operand(att, name, n, dtype):
     assert all(torch.equal(state2[s, h], state[s, h]) for s, h in kept)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n_seq,n,hk,hv,dk,dv", [(1, 333, 1, 2, 64, 64), (2, 65, 2, 2, 128, 128), (1, 200, 1, 1, 128, 64),
+                                                 (1, 1000, 2, 4, 64, 128)])
+def test_delta_chunks_of_fp32_accuracy(att, n_seq, n, hk, hv, dk, dv, dtype):
+    """Beside the worst case: the 2-norm of the errors, within what independent roundings to fp32 make of it (any operand
+    short of one of its three parts is beyond: test_layer_accuracy.py). A bf16 output is not looked at here."""
+    d = lo.remembering(gen(500 + n), n_seq, n, hk, hv, dk, dv, dtype)
+    want, _, S, _, _ = lo.delta(**d)
+    out, state, _ = delta_run(att, d)
+    errors = {"state": lo.apart(state, S), **({"out": lo.apart(out, want)} if dtype is F32 else {})}
+    assert max(errors.values()) <= lo.CHUNK_LIMIT, errors
+
+
 def test_delta_chunks_join(att):
     """A prompt in one call, in ragged calls of both forms, and token by token: states and outputs agree."""
     d = delta_inputs(80, 1, 150, 2, 4, 128, 128, F32, True, True)
@@ -429,6 +442,20 @@ def test_moe(att, n, e, k, hidden, ffn, dtype):
     x = r(n, hidden).to(dtype)
     top = torch.topk(r(n, e) + r(e), k, dim=1)
     moe_check(att, x, top.indices.to(torch.int32), torch.softmax(top.values, 1), q)
+
+
+@pytest.mark.parametrize("n,e,k,hidden,ffn", [(1, 4, 2, 1056, 352), (200, 3, 2, 1056, 352), (700, 5, 3, 288, 352),
+                                              (300, 40, 2, 128, 160)])
+def test_moe_of_fp32_accuracy(att, n, e, k, hidden, ffn):
+    """Beside the worst case: the 2-norm of the errors, in both forms and both heights of tiles (activations short of their
+    second part are beyond it: test_layer_accuracy.py)."""
+    r, q = gen(n * 5 + e), experts(n, e, hidden, ffn)
+    x, w = r(n, hidden), r(n, k)
+    ids = torch.topk(r(n, e), k, dim=1).indices.to(torch.int32)
+    y = torch.empty_like(x)
+    att.moe(x, ids, w, *q, y)
+    error = lo.apart(y, lo.moe(x, ids, w, *q)[0])
+    assert error <= lo.moe_limit(hidden, ffn)
 
 
 @pytest.mark.parametrize("n", [1, 6, 40, 200])
