@@ -432,7 +432,8 @@ int qwattn_conv_silu(qwattn_ctx* ctx, void* stream, const qwattn_conv* args);
  *   S <- decay S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q
  * with g = a and beta = b as given, or, with a_coef and dt_bias, g = a_coef[h] softplus(a + dt_bias[h]) and
  * beta = 1 / (1 + e^-b). With z and gamma the output is o rsqrt(mean o^2 + rms_eps) gamma silu(z), else o.
- * fp32 arithmetic (chunks of many tokens: products of fp32 accuracy on the matrix cores), one rounding to dtype.
+ * fp32 arithmetic (chunks of many tokens: products of fp32 accuracy on the matrix cores), one rounding to dtype. The
+ * sums of squares of q and k have to be finite in fp32; in chunks magnitudes stay below 2^127.
  * Few tokens run token by token; more run in chunks of 64 tokens whose chunk-internal part is computed for all
  * chunks at once (that form needs the workspace). Results do not depend on timing. An infinity or NaN in a token
  * stays in its sequence and heads; in chunks it also reaches earlier tokens of its own chunk. */
@@ -484,9 +485,11 @@ typedef struct qwattn_moe_layer {
 
 /* y[t] = sum_j weights[t][j] W_down (silu(W_gate x[t]) * (W_up x[t])) of expert ids[t][j], j < top_k <= 64. An id
  * outside [0, n_experts) is skipped (a free place of a batch: its row of y is then zero); the same expert may
- * occur twice. x and y are dtype (QWATTN_F32 or QWATTN_BF16) rows at strides that are multiples of 8, x 16-byte
- * aligned; fp32 accuracy, one rounding to dtype. Results do not depend on timing; the same row in calls of other n
- * or top_k may differ within that accuracy, since few pairs and many are computed in different orders.
+ * occur twice. x and y are dtype (QWATTN_F32 or QWATTN_BF16) rows at strides that are multiples of 8, both 16-byte
+ * aligned; fp32 sums, one rounding to dtype. Few pairs take x and the SwiGLU products h as they are. Many are grouped by
+ * expert, which keeps a value of x or h to 2^-23 of itself (bf16 x: exactly) but not below 2^-39 of its row's largest.
+ * Results do not depend on timing; the same row in calls of other n or top_k may differ within that accuracy, since few
+ * pairs and many are computed in different orders.
  * workspace: qwattn_moe_workspace bytes (of this n or a larger one), 256-byte aligned. */
 int qwattn_moe(qwattn_ctx* ctx, void* stream, const qwattn_moe_layer* layer, const void* x, int dtype,
                int64_t x_stride, const int32_t* ids, const float* weights, int top_k, void* y, int64_t y_stride, int n,

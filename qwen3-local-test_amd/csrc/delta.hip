@@ -169,7 +169,8 @@ static hipError_t delta_step(const DeltaArgs& a, hipStream_t s) {
 //
 // fp32 accuracy on the bf16 matrix cores: an fp32 value is three bf16 parts (24 bits), a product of two such values the
 // six part products down to 2^-24; bf16 q and k are one exact part, their norms and decays scale the results. Parts
-// keep fp32's range, so nothing is scaled beforehand.
+// have fp32's exponents, so nothing is scaled beforehand (the last parts of values below 2^-109 lose bits, a value from
+// 2^128 - 2^119 on rounds to an infinite part).
 //
 // Every operand that k_delta_chunks reads lies in the workspace as matrix-core fragments, a contiguous kilobyte each:
 //   per (sequence, chunk, key head):   K, Q  [part][16-token tile][32-dim step]   rows tokens, k dims (fp32; bf16 rows are

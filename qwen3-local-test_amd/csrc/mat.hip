@@ -222,6 +222,8 @@ __device__ __forceinline__ void split_bf16(const float (&v)[8], bf16x8& hi, bf16
 // fp32 sums), for the token counts below 16. bf16 ends at 2^-133, so the last part of an |x| below 2^-109 loses bits:
 // rows whose values are all that small keep 1.2e-6 at 2^-115 and 4e-5 at 2^-120 of their outputs, with two parts
 // 2.8e-6 and 4e-5.
+// (pk_bf16 and rest_bf16 in common.hpp take the parts.)
+
 // Eight int8 weights (two words) as bf16, exactly.
 __device__ __forceinline__ bf16x8 weights_bf16(uint32_t lo, uint32_t hi) {
     u32x4 w;

@@ -172,8 +172,10 @@ __global__ __launch_bounds__(256) void k_moe_pair_down(MoeArgs a) {
 // rows); k_moe_combine sums a token's pairs in their order.
 //
 // Operands: an int8 weight is exact in fp16. A row of activations is scaled by the power of two that puts its largest
-// magnitude into [2^14, 2^15) and becomes the sum of two fp16 (within 2^-22, small values within 2^-39 of the row's
-// largest; one is enough for a bf16 x). The block scales multiply each 32-column product in fp32.
+// magnitude into [2^14, 2^15) and becomes the sum of two fp16 (11 bits each: within 2^-23 of the value; below 2^-2, where
+// the second has steps of 2^-24, within 2^-25, 2^-39 of the row's largest). A bf16 x is exact in one from 2^-17 on, below
+// that within the same 2^-25. fp32 operands would take a third part and half as many matrix instructions again, for values
+// 2^-39 of their row's largest. The block scales multiply each 32-column product in fp32.
 
 struct MoeTile {
     int expert, row, rows;

@@ -489,6 +489,43 @@ def test_moe_rows_of_many_magnitudes(att, n):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [4, 300, 700])
+@pytest.mark.parametrize("power", [10, 28, 34])
+def test_moe_values_beside_one_far_larger(att, n, dtype, power):
+    """Rows with one value 2^power that no weight reads (its columns are zeros), so that only what the operands keep of the
+    others shows: all of them by pairs; grouped each to 2^-23 of itself or 2^-39 of the row's largest. The same for h, one
+    of whose values the down product does not read."""
+    e, hidden, ffn = 3, 128, 96
+    r, (gate, up, down) = gen(n + power), experts(12, e, hidden, ffn)
+    gate[0][:, :, 5], up[0][:, :, 5] = 0, 0
+    x, ids, w = r(n, hidden).to(dtype), torch.arange(2 * n, device=DEV, dtype=torch.int32).view(n, 2) % e, r(n, 2)
+    x[:, 5] = 2.0 ** power
+    gate[0][:, 7], up[0][:, 7], down[0][:, :, 7] = 127, 127, 0  # h's value 7 is large
+    gate[1][:, 7], up[1][:, 7] = 8.0, 8.0
+    y = torch.empty_like(x)
+    att.moe(x, ids, w, gate, up, down, y)
+    want, mag = lo.moe(x, ids, w, gate, up, down)
+    # what the split leaves of x and h, through the same products
+    G, U, D = (lo.widen(m) for m in (gate, up, down))
+    G[:, 7], U[:, 7] = 0, 0  # (not read by the down product)
+    kept = torch.zeros_like(want)
+    dx = 2.0 ** -39 * 2.0 ** power * torch.ones(hidden, dtype=torch.float64)
+    for t in range(n):
+        for j in range(2):
+            i, xt = int(ids[t, j]), f64(x[t])
+            g, u = G[i] @ xt, U[i] @ xt
+            s = 1 / (1 + torch.exp(-g))
+            full = (lo.widen(gate)[i][7] @ xt, lo.widen(up)[i][7] @ xt)
+            h7 = full[0] / (1 + torch.exp(-full[0])) * full[1]
+            dh = 1.1 * u.abs() * (G[i].abs() @ dx) + (g * s).abs() * (U[i].abs() @ dx) + 2.0 ** -39 * max(h7.abs(), (g * s * u).abs().max())
+            # (second order: the two errors of g and u meet)
+            kept[t] += f64(w[t, j]).abs() * (D[i].abs() @ (dh + 1.1 * (G[i].abs() @ dx) * (U[i].abs() @ dx)))
+    # (mag with |x|'s large value read by zeros, h's by zeros: neither counts)
+    factor = (hidden / 32 + ffn / 32 + 48) * EPS32
+    close(y, want, factor * mag + (0 if n == 4 else 1) * kept + HALF[dtype] * want.abs() * 1.01, "y")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("n", [5, 40, 300])
 def test_moe_rows_that_are_not_finite(att, n, dtype):
     """Infinities and NaN in a token's row reach its own row of y alone; a NaN weight of a free place reaches nothing."""
