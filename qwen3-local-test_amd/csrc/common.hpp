@@ -122,6 +122,18 @@ __device__ __forceinline__ float max32(float x) {
     return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
 }
 
+// Sum and maximum over the wave, in every lane: its halves, then a half swap (permlane32_swap).
+__device__ __forceinline__ float sum64(float x) {
+    x = sum32(x);
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+}
+__device__ __forceinline__ float max64(float x) {
+    x = max32(x);
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 1 / (1 + e^-x) with the hardware exponential and reciprocal (about 1 ulp each); saturates to 0 for

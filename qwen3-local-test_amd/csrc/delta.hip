@@ -10,12 +10,6 @@
 
 namespace qw {
 
-__device__ __forceinline__ float delta_wave_sum(float x) {
-    x = sum32(x);
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-}
-
 // Sum over the 16 lanes with this lane's l % 4 (row groups l / 4): within 16-lane rows by rotation, then across rows.
 __device__ __forceinline__ float sum_groups(float x) {
     x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x124, 0xF, 0xF, false));
@@ -86,15 +80,15 @@ __global__ __launch_bounds__(DV * 4) void k_delta_step(DeltaArgs a) {
 #pragma unroll
             for (int i = 0; i < DV / 64; i++)
                 sv[t][64 * i + lane] = load_in<DT>(a.v, r * a.v_stride + h * DV + 64 * i + lane);
-            const float qr = rsqrtf(delta_wave_sum(qq) + a.eps) * (DK == 128 ? 0.08838834764831845f : 0.125f);
-            const float kr = rsqrtf(delta_wave_sum(kk) + a.eps);
+            const float qr = rsqrtf(sum64(qq) + a.eps) * (DK == 128 ? 0.08838834764831845f : 0.125f);
+            const float kr = rsqrtf(sum64(kk) + a.eps);
 #pragma unroll
             for (int i = 0; i < DK / 64; i++) {
                 q[i] *= qr, k[i] *= kr;
                 sq[t][64 * i + lane] = q[i], sk[t][64 * i + lane] = k[i];
                 kq = fmaf(q[i], k[i], kq);
             }
-            kq = delta_wave_sum(kq);
+            kq = sum64(kq);
             if (lane == 0) gates[t][0] = expf(delta_log_decay(a, r, h)), gates[t][1] = delta_beta(a, r, h), gates[t][2] = kq;
         }
         __syncthreads();
@@ -137,7 +131,7 @@ __global__ __launch_bounds__(DV * 4) void k_delta_step(DeltaArgs a) {
 #pragma unroll
             for (int i = 0; i < DV / 64; i++) o[i] = so[t][64 * i + lane], ss = fmaf(o[i], o[i], ss);
             if (a.z) {
-                const float rms = rsqrtf(delta_wave_sum(ss) * (1.f / DV) + a.eps);
+                const float rms = rsqrtf(sum64(ss) * (1.f / DV) + a.eps);
 #pragma unroll
                 for (int i = 0; i < DV / 64; i++) {
                     const float z = load_in<DT>(a.z, r * a.z_stride + h * DV + 64 * i + lane);
@@ -549,7 +543,8 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
     // that moves on by a chunk and a lane offset; no load is conditional (a wave without an operand loads one of
     // another's), so that no branch waits for loads.
     const uint32_t lane16 = lane * 16;
-    const size_t kq_step = (size_t)a.k_heads * Unit::kBytes, tp_step = (size_t)a.v_heads * kTpBytes, vec_step = (size_t)a.v_heads * kVec * 4;
+    const size_t kq_step = (size_t)a.k_heads * Unit::kBytes, tp_step = (size_t)a.v_heads * kTpBytes;
+    const size_t vec_step = (size_t)a.v_heads * kVec * 4;
     const uint8_t* kq = ws.kq + ((size_t)b * ncs * a.k_heads + kh) * Unit::kBytes;
     const uint8_t* tp = ws.tp + ((size_t)b * ncs * a.v_heads + h) * kTpBytes;
     const uint8_t* vec = reinterpret_cast<const uint8_t*>(ws.vec + ((size_t)b * ncs * a.v_heads + h) * kVec);
@@ -626,7 +621,8 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaArgs a, DeltaWs ws, i
                     for (int e = 0; e < 8; e++) v[e] = __uint_as_float(__float_as_uint(v[e]) & later);
                 u32x4 w[3];
                 split3(v, w);
-                const bf16x8 bu[3] = {__builtin_bit_cast(bf16x8, w[0]), __builtin_bit_cast(bf16x8, w[1]), __builtin_bit_cast(bf16x8, w[2])};
+                const bf16x8 bu[3] = {__builtin_bit_cast(bf16x8, w[0]), __builtin_bit_cast(bf16x8, w[1]),
+                                      __builtin_bit_cast(bf16x8, w[2])};
                 mfma_parts<3>(fM[st], bu, acc);
             }
             load_tri(tp + kTpOne);
@@ -825,7 +821,6 @@ static int segment_chunks(const DeltaArgs& a) {
     const long long pairs = (long long)a.n_seq * a.v_heads;
     return (int)std::max(1ll, std::min<long long>(nc, kSegmentPairs / pairs));
 }
-static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct DeltaSizes {
     size_t kq, tp, vec, o;

@@ -290,6 +290,9 @@ __host__ __device__ constexpr unsigned gemm_s_off(int row, int j, int k, int nkb
 // Whether they stay below kFar, and below 2^32 with it added, over a tile's 256 rows and 128 tokens.
 constexpr bool gemm_offsets_fit(int cols, int x_stride) { return cols <= 1 << 22 && (127ll * x_stride + cols) * 4 < kFar; }
 
+// Parts of a workspace start at multiples of 256 bytes
+inline size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
 // qwattn_conv_silu's arguments (include/qwattn.h)
 struct ConvArgs {
     int n_seq, n, channels, taps;

@@ -27,13 +27,6 @@ namespace {
 
 constexpr int kMatNTP = 4;  // tokens a workgroup (f32 weights)
 
-// Sum over the 64 lanes, in every lane.
-__device__ __forceinline__ float mat_wave_sum(float x) {
-    x = sum32(x);
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-}
-
 // f32 weights: a wave's RW rows a 16-column group at a time (f32 projections are the small ones)
 template <int NTP, int RW>
 __device__ __forceinline__ void mat_f32_body(const MatArgs& a, int bx) {
@@ -77,7 +70,7 @@ __device__ __forceinline__ void mat_f32_body(const MatArgs& a, int bx) {
     for (int r = 0; r < RW; r++)
 #pragma unroll
         for (int t = 0; t < NTP; t++) {
-            float v = mat_wave_sum(acc[r][t]);
+            float v = sum64(acc[r][t]);
             if (a.post == 1) {
                 const float u = v * a.post_scale;
                 v = u / (1.0f + __expf(-u));
@@ -148,7 +141,7 @@ __device__ __forceinline__ void mat_q8_body(const MatArgs& a, int bx) {
     }
 #pragma unroll
     for (int r = 0; r < RW; r++) {
-        float v = mat_wave_sum(acc[r]);
+        float v = sum64(acc[r]);
         if (a.post == 1) {
             const float u = v * a.post_scale;
             v = u / (1.0f + __expf(-u));

@@ -9,21 +9,11 @@
 
 namespace qw {
 
-__device__ __forceinline__ float moe_wave_sum(float x) {
-    x = sum32(x);
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-}
-__device__ __forceinline__ float moe_wave_max(float x) {
-    x = max32(x);
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-}
-
 // ---- the router ----------------------------------------------------------------------------------------------
-// A wave a token (4,096 tokens, 10 of 512 experts: 8 us; bound by the rounds' dependent steps). Lane l holds the PER consecutive experts from l * PER, so among equal logits the first lane (and
-// in it the first value) has the lowest index: each of the top_k rounds is a wave maximum, a ballot and the removal
-// of one value. -inf and NaN are no choice. Equal to the maximum counts as e^0 also where both are +inf.
+// A wave a token (4,096 tokens, 10 of 512 experts: 8 us; bound by the rounds' dependent steps). Lane l holds the PER
+// consecutive experts from l * PER, so among equal logits the first lane (and in it the first value) has the lowest
+// index: each of the top_k rounds is a wave maximum, a ballot and the removal of one value. -inf and NaN are no choice.
+// Equal to the maximum counts as e^0 also where both are +inf.
 template <int PER>
 __global__ __launch_bounds__(256) void k_moe_route(RouteArgs a) {
     const int tok = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -46,17 +36,17 @@ __global__ __launch_bounds__(256) void k_moe_route(RouteArgs a) {
     float best = v[0];
 #pragma unroll
     for (int i = 1; i < PER; i++) best = fmaxf(best, v[i]);
-    const float top = moe_wave_max(best);
+    const float top = max64(best);
     float all = 0.f;
     if (!a.renorm) {
 #pragma unroll
         for (int i = 0; i < PER; i++) all += v[i] == kNegInf ? 0.f : v[i] == top ? 1.f : expf(v[i] - top);
-        all = moe_wave_sum(all);
+        all = sum64(all);
     }
     float mine = kNegInf;  // lane j: the j-th choice
     int id = -1;
     for (int j = 0; j < a.top_k; j++) {
-        const float m = moe_wave_max(best);
+        const float m = max64(best);
         if (m == kNegInf) break;
         const int src = __builtin_ctzll(__ballot(best == m));
         int at = 0;
@@ -73,7 +63,7 @@ __global__ __launch_bounds__(256) void k_moe_route(RouteArgs a) {
         if (lane == j) mine = m, id = at;
     }
     const float p = id < 0 ? 0.f : mine == top ? 1.f : expf(mine - top);
-    if (a.renorm) all = moe_wave_sum(p);
+    if (a.renorm) all = sum64(p);
     if (lane < a.top_k) {
         a.ids[(size_t)tok * a.top_k + lane] = id;
         a.weights[(size_t)tok * a.top_k + lane] = id < 0 ? 0.f : p / all;
@@ -129,7 +119,7 @@ __global__ __launch_bounds__(256) void k_moe_pair_up(MoeArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < kPairRows; i++) {
-        const float gs = moe_wave_sum(g[i]), us = moe_wave_sum(u[i]);
+        const float gs = sum64(g[i]), us = sum64(u[i]);
         if (lane == 0 && f0 + i < a.ffn) a.h[(size_t)pair * a.ffn + f0 + i] = gs * sigmoid(gs) * us;
     }
 }
@@ -157,7 +147,7 @@ __global__ __launch_bounds__(256) void k_moe_pair_down(MoeArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < kPairRows; i++) {
-        const float s = moe_wave_sum(y[i]);
+        const float s = sum64(y[i]);
         if (lane == 0 && r0 + i < a.hidden) {
             const size_t at = (size_t)tok * a.y_stride + r0 + i;
             if constexpr (DT == 0) static_cast<float*>(a.y)[at] = s;
@@ -259,7 +249,7 @@ __device__ __forceinline__ void moe_row(const void* x, size_t stride, int cols, 
 #pragma unroll
             for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
         }
-    m = moe_wave_max(m);
+    m = max64(m);
     if ((lane & 63) == 0) most[lane >> 6] = m;
     __syncthreads();
     if (!there) return;
@@ -395,7 +385,8 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(MoeArgs a, MoeWs ws) {
     }
     auto load_a = [&](int k, int stage) {
 #pragma unroll
-        for (int i = 0; i < T::AL; i++) load16_to_lds(ap[i] + min(k, steps - 1) * 64, smem + stage * T::kA + (wave * T::AL + i) * 1024);
+        for (int i = 0; i < T::AL; i++)
+            load16_to_lds(ap[i] + min(k, steps - 1) * 64, smem + stage * T::kA + (wave * T::AL + i) * 1024);
     };
     // (past the row: any weights and scales, on the operands' zeros or in steps that do not run)
     auto load_w = [&](int m, int buffer) {  // columns 128 m ..
@@ -468,7 +459,8 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(MoeArgs a, MoeWs ws) {
 #pragma unroll
                         for (int q = 0; q < 2; q++) {
                             const int r = m * 32 + c;
-                            x[j][m][p][q] = *reinterpret_cast<const f16x8*>(A + (p * BM + r) * 128 + (((4 * j + 2 * h + q) ^ turn(r)) << 4));
+                            x[j][m][p][q] =
+                                *reinterpret_cast<const f16x8*>(A + (p * BM + r) * 128 + (((4 * j + 2 * h + q) ^ turn(r)) << 4));
                         }
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
@@ -514,11 +506,13 @@ __global__ __launch_bounds__(256, 2) void k_moe_gemm(MoeArgs a, MoeWs ws) {
                 // the lane pair (c, c + 16) holds a gate and an up value: the first takes one row of two, the second the other
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
-                    const auto p0 = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[m][4 * e4 + e]), __float_as_uint(acc[m][4 * e4 + e]), false, false);
-                    const auto p1 = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[m][4 * e4 + e + 1]), __float_as_uint(acc[m][4 * e4 + e + 1]), false, false);
+                    const uint32_t a0 = __float_as_uint(acc[m][4 * e4 + e]), a1 = __float_as_uint(acc[m][4 * e4 + e + 1]);
+                    const auto p0 = __builtin_amdgcn_permlane16_swap(a0, a0, false, false);
+                    const auto p1 = __builtin_amdgcn_permlane16_swap(a1, a1, false, false);
                     const bool odd = c & 16;
                     const int sh = odd ? s[e + 1] : s[e];
-                    const float g = ldexpf(__uint_as_float(odd ? p1[0] : p0[0]), sh), u = ldexpf(__uint_as_float(odd ? p1[1] : p0[1]), sh);
+                    const float g = ldexpf(__uint_as_float(odd ? p1[0] : p0[0]), sh);
+                    const float u = ldexpf(__uint_as_float(odd ? p1[1] : p0[1]), sh);
                     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(g * sigmoid(g) * u), ro,
                                                           (int)((unsigned)(r0 + e + (odd ? 1 : 0)) * outs * 4u + col), 0, 0);
                 }
@@ -549,7 +543,8 @@ __global__ __launch_bounds__(256) void k_moe_combine(MoeArgs a, MoeWs ws) {
     if constexpr (DT == 0) {
         *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + tok * a.y_stride + o) = s;
     } else {
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.y) + tok * a.y_stride + o) = u32x2{pk_bf16(s[0], s[1]), pk_bf16(s[2], s[3])};
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.y) + tok * a.y_stride + o) =
+            u32x2{pk_bf16(s[0], s[1]), pk_bf16(s[2], s[3])};
     }
 }
 
@@ -570,7 +565,6 @@ constexpr int kTileRows64 = 56;
 constexpr int kMoeSegment = 1 << 16;  // pairs worked off at a time: bounds the workspace
 static int segment_tokens(const MoeArgs& a) { return std::max(1, std::min(a.n, kMoeSegment / a.top_k)); }
 
-static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 // Bytes of the grouped form's workspace; the pointers into it with `base`.
 static size_t lay_out(const MoeArgs& a, int parts, uint8_t* base, MoeWs& w) {
     const size_t n = segment_tokens(a), pairs = n * a.top_k, hp = (a.hidden + 63) & ~63, fp = (a.ffn + 63) & ~63;
@@ -580,7 +574,8 @@ static size_t lay_out(const MoeArgs& a, int parts, uint8_t* base, MoeWs& w) {
         at += up256(bytes);
     };
     take(w.tiles, (pairs / 32 + a.n_experts) * sizeof(MoeTile));
-    take(w.row_tok, pairs * 4), take(w.pair_row, pairs * 4), take(w.row_weight, pairs * 4), take(w.x_shift, n * 4), take(w.h_shift, pairs * 4);
+    take(w.row_tok, pairs * 4), take(w.pair_row, pairs * 4), take(w.row_weight, pairs * 4);
+    take(w.x_shift, n * 4), take(w.h_shift, pairs * 4);
     take(w.x16, parts * n * hp * 2), take(w.h16, 2 * pairs * fp * 2);
     w.x_part = n * hp, w.h_part = pairs * fp;
     take(w.y, pairs * std::max(a.hidden, a.ffn) * 4);

@@ -41,13 +41,6 @@ __device__ __forceinline__ float sum16(float x) {
     return x;
 }
 
-// Sum over the wave, in every lane: 32-lane halves (DPP + permlane16), then the halves (permlane32).
-__device__ __forceinline__ float wave_sum(float x) {
-    x = sum32(x);
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-}
-
 // Integer sum over the wave, in every lane (DPP within 16-lane rows, then permlane16 and permlane32 swaps).
 __device__ __forceinline__ unsigned wave_isum(unsigned x) {
     x += (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, false);
@@ -180,7 +173,7 @@ __global__ __launch_bounds__(64) void k_qsa_pool(QsaPoolArgs a) {
 #pragma unroll
     for (int k = 0; k < 8; k++)
         if (k < KD) ss += pk[k] * pk[k];
-    ss = wave_sum(ss);
+    ss = sum64(ss);
     const float r = 1.0f / sqrtf(ss / (float)ID + a.eps);
 #pragma unroll
     for (int k = 0; k < 8; k++)
@@ -789,7 +782,7 @@ __device__ __forceinline__ void score_chunk(const QsaSelectArgs& a, __amdgpu_buf
             x[k] = load_in<IN_DT>(a.iq, ((size_t)t * a.IH + h) * ID + lane + 64 * k);
             ss += x[k] * x[k];
         }
-        ss = wave_sum(ss);
+        ss = sum64(ss);
         const float r = 1.0f / sqrtf(ss / (float)ID + a.eps);
 #pragma unroll
         for (int k = 0; k < ID / 64; k++) s_t[h * ID + lane + 64 * k] = x[k] * r * a.gamma[lane + 64 * k];
