@@ -433,7 +433,8 @@ int qwattn_conv_silu(qwattn_ctx* ctx, void* stream, const qwattn_conv* args);
  * with g = a and beta = b as given, or, with a_coef and dt_bias, g = a_coef[h] softplus(a + dt_bias[h]) and
  * beta = 1 / (1 + e^-b). With z and gamma the output is o rsqrt(mean o^2 + rms_eps) gamma silu(z), else o.
  * fp32 arithmetic (chunks of many tokens: products of fp32 accuracy on the matrix cores), one rounding to dtype. The
- * sums of squares of q and k have to be finite in fp32; in chunks magnitudes stay below 2^127.
+ * sums of squares of q and k have to be finite in fp32; in chunks magnitudes stay below 2^127, and where log decays
+ * are positive (a growth) their sums over successive tokens of a chunk below 88.
  * Few tokens run token by token; more run in chunks of 64 tokens whose chunk-internal part is computed for all
  * chunks at once (that form needs the workspace). Results do not depend on timing. An infinity or NaN in a token
  * stays in its sequence and heads; in chunks it also reaches earlier tokens of its own chunk. */

@@ -803,10 +803,10 @@ __global__ __launch_bounds__(256) void k_delta_norm(DeltaArgs a, const float* o3
 }
 
 // Token by token where every state is kept, and while that takes less: a token takes 1 us (up to 256 (sequence, value
-// head) pairs, a workgroup each) to 5 us (1,536 pairs), a chunk of all pairs 20 us (32 pairs, bf16) to 250 (1,536), in fp32
-// up to twice as much. Measured with 32 heads of 128 x 128, by tokens and in chunks: one sequence of 19 tokens 24 and 20
-// us (bf16), 26 (fp32); 4 of 48 tokens 53 and 33, 55 and 48; 8 of 64 tokens in fp32 73 and 102; 48 of 64 tokens in bf16
-// 337 and 252.
+// head) pairs, a workgroup each) to 5 us (1,536 pairs), a chunk of all pairs 16 us (32 pairs, bf16) to 267 (1,536), in fp32
+// up to twice as much; the gated norm behind chunks 5 us and more. Measured with 32 heads of 128 x 128 without it, by
+// tokens and in chunks: one sequence of 19 tokens 25 and 16 us (bf16), 22 (fp32); 4 of 48 tokens 54 and 31, 54 and 45; 8 of
+// 64 tokens in fp32 74 and 99; 48 of 64 tokens in bf16 337 and 267.
 static int step_most(const DeltaArgs& a, bool bf16) {
     const long long pairs = (long long)a.n_seq * a.v_heads;
     return (int)(bf16 ? std::min(18 + pairs / 10, 48ll) : std::min(18 + pairs / 6, 100ll));

@@ -10,9 +10,10 @@
 namespace qw {
 
 // ---- the router ----------------------------------------------------------------------------------------------
-// A wave a token (4,096 tokens, 10 of 512 experts: 8 us; bound by the rounds' dependent steps). Lane l holds the PER
-// consecutive experts from l * PER, so among equal logits the first lane (and in it the first value) has the lowest
-// index: each of the top_k rounds is a wave maximum, a ballot and the removal of one value. -inf and NaN are no choice.
+// A wave a token (4,096 tokens, 10 of 512 experts: 8 us; bound by vector instructions, 837 a token, which issue in 74% of
+// a CU's busy cycles; one token: 2.9 us, its wave waiting 82% of its cycles). Lane l holds the PER consecutive experts
+// from l * PER, so among equal logits the first lane (and in it the first value) has the lowest index: each of the top_k
+// rounds is a wave maximum, a ballot and the removal of one value. -inf and NaN are no choice.
 // Equal to the maximum counts as e^0 also where both are +inf.
 template <int PER>
 __global__ __launch_bounds__(256) void k_moe_route(RouteArgs a) {
@@ -84,7 +85,10 @@ hipError_t launch_moe_route(RouteArgs a, hipStream_t s) {
 
 // ---- the experts, pair by pair -------------------------------------------------------------------------------
 // h[pair][f] = silu(W_gate x) (W_up x) of the pair's expert, then y[t] = sum over its pairs of weight W_down h:
-// a wave a row of the weights, 16 columns a lane at a time (half a Q8 block: one scale), fp32 products.
+// a wave a row of the weights, 16 columns a lane at a time (half a Q8 block: one scale), fp32 products. One token, 8 of 128
+// experts of 2,048 x 512: 7.4 + 5.9 us, waves waiting three quarters of their cycles for their few loads (vector
+// instructions 23% and 17% of the busy cycles); 10 of 13 tokens: 33 + 24 us, waiting 73% and 61% behind 3.8 TB/s, vector
+// instructions 52% and 53%.
 
 // sum over 16 int8 weights (a word each four) with their values
 __device__ __forceinline__ float dot16(const u32x4 w, const float (&x)[16]) {
@@ -314,7 +318,7 @@ constexpr int kMoeGroup = 4;  // M tiles whose column tiles follow each other on
 // rows, 32 each, so that each int8 weight is converted by one wave. The LDS takes operands as they come from memory, by
 // direct loads: ST stages of activations [part][BM][128 bytes], ST - 1 steps ahead; two of int8 weights [BN][128 columns];
 // two of scales [BN][8 blocks]; rows are read by whole lines where they can be, so that fewer requests go to L2. Bound by
-// no one unit: 2,048 tokens of 8 of 128 experts, gate and up, 183-199 us at 2.0 GHz, of a CU's busy cycles vector
+// no one unit: 2,048 tokens of 8 of 128 experts, gate and up, 181-208 us at 2.0 GHz, of a CU's busy cycles vector
 // instructions 54% (the conversion, the block scales), the matrix pipe 24%, the LDS 18%.
 template <int P, int MT, int ST>
 struct MoeTileShape {
