@@ -497,6 +497,77 @@ int qwattn_moe(qwattn_ctx* ctx, void* stream, const qwattn_moe_layer* layer, con
                void* workspace, size_t workspace_bytes);
 int qwattn_moe_workspace(const qwattn_moe_layer* layer, int dtype, int n, int top_k, size_t* bytes);
 
+/* ---- Batches of sequences over a paged K/V cache ---------------------------------------------------------
+ * The full-attention layer's body for a batch: qwattn_paged_append, then qwattn_paged_attend on the queries it wrote.
+ * The reference serves one sequence (its dispatches: shaders/qk_norm_rope.comp, shaders/attention.comp,
+ * shaders/attn_combine.comp); these do the same work with the keys and values of many in pages of one pool.
+ *
+ * Sequences as above (n_seq, n, lens). `pos` (device int32 [n_seq]) is the number of positions before a sequence's first
+ * row: its token t is at position pos[b] + t. Positions run over [0, pages * page); a row at any other position is not
+ * appended and its outputs are zero. A page number outside [0, n_pages) has no memory: nothing is written there,
+ * and its keys are hidden from every token (pages that a window has left behind can be given to others).
+ * Sequences may share pages that no call of the batch appends to.
+ *
+ * Like the operators above, the calls use no state of the context but its shape, device, rms_eps and (rope NULL) rope
+ * table, allocate nothing, read no device data on the host and can be captured; calls that may overlap need workspaces
+ * of their own. Outputs must not overlap inputs or each other. */
+typedef struct qwattn_paged_cache {
+    void *k, *v;           /* pools [n_pages][NKV][page / 32][32 * D] fp16, blocks as in the K and V caches above;
+                              16-byte aligned */
+    const int32_t* table;  /* device [n_seq][table_stride]: the page of positions [i * page, (i + 1) * page) */
+    int64_t table_stride;  /* >= pages */
+    int n_pages, pages;    /* pages of the pools, and of a sequence */
+    int page;              /* positions a page: a power of two from 32 to 65536; pages * page <= 2^26 */
+} qwattn_paged_cache;
+
+/* QK-RMSNorm + partial RoPE + append, as qwattn_qk_norm_rope_append for every sequence: y = x rsqrt(mean x^2 + rms_eps)
+ * (1 + w), rotate-half on the first R dims by the table's row of the token's position; keys to fp16 into their pages, values
+ * to fp16, queries to q_out. fp32 arithmetic, one rounding. A position at or past n_rope is like one past the pages. */
+typedef struct qwattn_paged_append_args {
+    qwattn_paged_cache cache;
+    int n_seq, n;           /* n_seq <= 65535, n_seq * n * (NH + 2 NKV) < 2^26 */
+    int dtype;              /* of q, k, v and q_out: QWATTN_F32 or QWATTN_BF16 */
+    int n_rope;             /* rows of rope, where it is given */
+    const int32_t* lens;    /* device [n_seq] or NULL */
+    const int32_t* pos;     /* device [n_seq] */
+    const void* q;          /* NULL (keys and values only), or rows of NH heads of D elements, q_head elements apart */
+    int64_t q_stride, q_head;
+    const void *k, *v;      /* rows of NKV * D elements */
+    int64_t k_stride, v_stride; /* strides: multiples of 8; rows: 16-byte aligned */
+    const float *qn, *kn;   /* [D] gamma - 1, 16-byte aligned; NULL: no norm (of the queries, of the keys) */
+    const float* rope;      /* [n_rope][R/2][2] (cos, sin), 16-byte aligned; NULL: the context's table */
+    void* q_out;            /* with q: rows of NH * D elements */
+    int64_t q_out_stride;
+} qwattn_paged_append_args;
+int qwattn_paged_append(qwattn_ctx* ctx, void* stream, const qwattn_paged_append_args* args);
+
+/* Attention of the rows over their sequences' pages: out[t][h] = sum_j softmax_j(scale q[t][h] . K[j][h / G]) V[j][h / G]
+ * sigmoid(gate[t][h]), G = NH / NKV, over the keys j that token t at position p sees: j <= p, and with a window only
+ * j > p - window or j < sinks. The rows' own keys must be in the cache. A row that sees no key (or all of whose scores are
+ * -inf) is zero. Sums, maxima and the output before its one rounding are fp32; f32 rows take products of fp32 accuracy
+ * (queries and weights in two fp16 parts), bf16 rows queries and weights in one fp16 part. Hidden keys and values, and
+ * cache memory past a sequence's last row, may hold anything, infinities and NaN among it. Results do not depend on timing. */
+typedef struct qwattn_paged_attend_args {
+    qwattn_paged_cache cache;
+    int n_seq, n;           /* as for qwattn_paged_append */
+    int dtype;              /* of q, gate and out */
+    int window, sinks;      /* window 0: none (sinks are then not looked at); both >= 0 */
+    float scale;            /* 0: 1 / sqrt(D); else positive and finite */
+    const int32_t* lens;
+    const int32_t* pos;
+    const void* q;          /* normalized, rotated queries (q_out), rows of heads as q above */
+    int64_t q_stride, q_head;
+    const void* gate;       /* NULL, or rows of heads */
+    int64_t gate_stride, gate_head;
+    void* out;              /* rows of NH * D elements */
+    int64_t out_stride;
+    void* workspace;        /* qwattn_paged_workspace bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} qwattn_paged_attend_args;
+int qwattn_paged_attend(qwattn_ctx* ctx, void* stream, const qwattn_paged_attend_args* args);
+/* The workspace of every qwattn_paged_attend call of this context. */
+int qwattn_paged_workspace(qwattn_ctx* ctx, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -136,6 +136,19 @@ public:
                                workspace_bytes), "qwattn_moe");
     }
 
+    // Batches of sequences over a paged K/V cache (arguments and formulas: qwattn.h).
+    void paged_append(void* stream, const qwattn_paged_append_args& a) {
+        check(ctx_, qwattn_paged_append(ctx_, stream, &a), "qwattn_paged_append");
+    }
+    size_t paged_workspace() const {
+        size_t bytes = 0;
+        check(ctx_, qwattn_paged_workspace(ctx_, &bytes), "qwattn_paged_workspace");
+        return bytes;
+    }
+    void paged_attend(void* stream, const qwattn_paged_attend_args& a) {
+        check(ctx_, qwattn_paged_attend(ctx_, stream, &a), "qwattn_paged_attend");
+    }
+
     // Waits for `stream` and throws if a bounded in-kernel wait of an earlier decode launch gave up.
     void sync(void* stream) { check(ctx_, qwattn_sync_status(ctx_, stream), "qwattn_sync_status"); }
 

@@ -48,10 +48,14 @@ _MAT_OUT = struct.Struct("@PPI4xPIif4x")  # MatOut's layout; packing it costs a 
 assert _MAT_OUT.size == ctypes.sizeof(MatOut)
 
 
-# qwattn_conv, qwattn_delta and qwattn_moe_layer as the C ABI lays them out
+# qwattn_conv, qwattn_delta, qwattn_moe_layer, qwattn_paged_append_args and qwattn_paged_attend_args as the C ABI lays
+# them out (a qwattn_paged_cache is the first part of the last two)
 _CONV = struct.Struct("@5i4xPPqPPPPPq")
 _DELTA = struct.Struct("@8iPPPPqqqPPPPPPPqPPqPN")
 _MOE_LAYER = struct.Struct("@3i4xPPPPPP")
+_PAGED_CACHE = "PPPqiii4x"
+_PAGED_APPEND = struct.Struct("@" + _PAGED_CACHE + "4iPPPqqPPqqPPPPq")
+_PAGED_ATTEND = struct.Struct("@" + _PAGED_CACHE + "5if" + "PPPqqPqqPqPN")
 
 
 _lib = None
@@ -106,6 +110,9 @@ def load_library():
         "qwattn_moe_route": [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P],
         "qwattn_moe": [_P, _P, _P, _P, _I, ctypes.c_int64, _P, _P, _I, _P, ctypes.c_int64, _I, _P, ctypes.c_size_t],
         "qwattn_moe_workspace": [_P, _I, _I, _I, _P],
+        "qwattn_paged_append": [_P, _P, _P],
+        "qwattn_paged_attend": [_P, _P, _P],
+        "qwattn_paged_workspace": [_P, _P],
         "qwattn_set_wait_limits": [_P, _I, _I],
         "qwattn_set_alloc_fault": [_P, _I],
     }
@@ -162,7 +169,7 @@ def _stream(stream):
     return torch.cuda.current_stream().cuda_stream
 
 
-_F32, _I8 = torch.float32, torch.int8
+_F32, _F16, _I8 = torch.float32, torch.float16, torch.int8
 _DT = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
 
@@ -218,6 +225,21 @@ def _check_seq_rows(t, name, shape, dtype):
     return row
 
 
+def _check_head_rows(t, name, shape, dtype):
+    """(row stride, head stride) of a [n_seq, n, heads, dim] operand of the paged operators: `shape`, dtype, contiguous
+    heads at one stride, row b * n + t at one stride."""
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    n_seq, n, heads, dim = shape
+    seq, row, head, one = t.stride()
+    head = head if heads > 1 else dim
+    row = row if n > 1 else seq if n_seq > 1 else heads * head
+    if one != 1 or (n_seq > 1 and n > 1 and seq != n * row):
+        raise ValueError(f"{name}: a head must be contiguous and row b * n + t at (b * n + t) times one stride, got strides "
+                         f"{t.stride()}")
+    return row, head
+
+
 def _check_matrix(t, name, shape, dtype):
     """Row stride of a [n, width] operand of exactly `shape` and dtype with contiguous rows."""
     stride = t.stride()
@@ -266,6 +288,8 @@ def v_rows(vcache, cap, nkv, d):
 
 class Attention:
     """One qwattn context: attention shape, rope table, split partials and (optionally) K/V caches."""
+
+    _paged_ws = None  # bytes of paged_attend's workspace, once asked for
 
     def __init__(self, n_heads, n_kv_heads, head_dim, rope_dim, rope_theta=1e7, rms_eps=1e-6, max_ctx=262144,
                  max_tokens=2048, max_splits=1024, device=0):
@@ -549,6 +573,84 @@ class Attention:
                                 gate[1].data_ptr(), up[1].data_ptr(), down[1].data_ptr())
         self._check(self.lib.qwattn_moe(self.h, s, layer, x.data_ptr(), _ROW_DT[dtype], x_stride, ids.data_ptr(),
                                         weights.data_ptr(), top_k, y.data_ptr(), y_stride, n, ws, ws_bytes))
+
+    # ---- batches over a paged cache ---------------------------------------------------------------------
+
+    def _paged_cache(self, kpool, vpool, table, pos, lens, n_seq):
+        """The cache's part of the packed arguments, its operands checked."""
+        nkv, shape = self.NKV, kpool.shape
+        if len(shape) != 3 or shape[1] != nkv or shape[2] % self.D:
+            raise ValueError(f"kpool must be [n_pages, {nkv}, page * {self.D}], got {tuple(shape)}")
+        _check_whole(kpool, "kpool", shape, _F16)
+        _check_whole(vpool, "vpool", shape, _F16)
+        if table.dtype is not torch.int32 or len(table.shape) != 2 or table.shape[0] != n_seq or table.stride(1) != 1:
+            raise ValueError(f"table must be int32 [{n_seq}, pages] with unit column stride, got {table.dtype} {tuple(table.shape)}")
+        _check_whole(pos, "pos", (n_seq,), torch.int32)
+        if lens is not None:
+            _check_whole(lens, "lens", (n_seq,), torch.int32)
+        pages = table.shape[1]
+        return (kpool.data_ptr(), vpool.data_ptr(), table.data_ptr(), table.stride(0) if n_seq > 1 else pages, shape[0], pages,
+                shape[2] // self.D)
+
+    def paged_append(self, k, v, kpool, vpool, table, pos, q=None, q_out=None, qn=None, kn=None, rope=None, lens=None,
+                     stream=None):
+        """Appends new tokens' keys and values k, v [n_seq, n, KV heads, head_dim] to the pages of their sequences, the
+        keys normalized (kn [head_dim] as gamma - 1, None: not) and rotated to positions pos[b] + t; q [n_seq, n, heads,
+        head_dim] likewise (qn) into q_out. Pools kpool, vpool float16 [n_pages, KV heads, page * head_dim] in the block
+        layout (k_block, v_block), table int32 [n_seq, pages], pos int32 [n_seq]; rope [rows, rope_dim / 2, 2] (None:
+        the context's); lens [n_seq] int32 shortens sequences."""
+        if k.dtype not in _ROW_DT or len(k.shape) != 4:
+            raise ValueError(f"k must be float32 or bfloat16 [n_seq, n, KV heads, head_dim], got {k.dtype} {tuple(k.shape)}")
+        dtype, (n_seq, n) = k.dtype, k.shape[:2]
+        kv, heads = (n_seq, n, self.NKV, self.D), (n_seq, n, self.NH, self.D)
+        k_stride, v_stride = _check_seq_rows(k, "k", kv, dtype), _check_seq_rows(v, "v", kv, dtype)
+        q_stride = q_head = out_stride = 0
+        if q is not None:
+            q_stride, q_head = _check_head_rows(q, "q", heads, dtype)
+        if q_out is not None:
+            out_stride = _check_seq_rows(q_out, "q_out", heads, dtype)
+        if qn is not None:
+            _check_whole(qn, "qn", (self.D,))
+        if kn is not None:
+            _check_whole(kn, "kn", (self.D,))
+        if rope is not None:
+            _check_whole(rope, "rope", (rope.shape[0], self.R // 2, 2))
+        cache = self._paged_cache(kpool, vpool, table, pos, lens, n_seq)
+        s = self._on_device((k, v, kpool, vpool, table, pos, q, q_out, qn, kn, rope, lens), stream)
+        args = _PAGED_APPEND.pack(*cache, n_seq, n, _ROW_DT[dtype], 0 if rope is None else rope.shape[0], _ptr(lens) or 0,
+                                  pos.data_ptr(), _ptr(q) or 0, q_stride, q_head, k.data_ptr(), v.data_ptr(), k_stride, v_stride,
+                                  _ptr(qn) or 0, _ptr(kn) or 0, _ptr(rope) or 0, _ptr(q_out) or 0, out_stride)
+        self._check(self.lib.qwattn_paged_append(self.h, s, args))
+
+    def paged_workspace(self):
+        """Bytes of workspace that every paged_attend call of this context needs."""
+        size = ctypes.c_size_t()
+        self._check(self.lib.qwattn_paged_workspace(self.h, ctypes.byref(size)))
+        return size.value
+
+    def paged_attend(self, q, kpool, vpool, table, pos, out, gate=None, lens=None, window=0, sinks=0, scale=0.0,
+                     workspace=None, stream=None):
+        """Causal attention of q [n_seq, n, heads, head_dim] (normalized, rotated: paged_append's q_out) over the pages of
+        their sequences (as in paged_append, which must have written the rows' own keys) into out, times sigmoid(gate):
+        one token a sequence, a few or a chunk. window: a token sees its last `window` positions and the first `sinks`
+        (0: all). scale 0: 1 / sqrt(head_dim). workspace: a tensor of paged_workspace() bytes (None: from torch's
+        allocator)."""
+        if q.dtype not in _ROW_DT or len(q.shape) != 4:
+            raise ValueError(f"q must be float32 or bfloat16 [n_seq, n, heads, head_dim], got {q.dtype} {tuple(q.shape)}")
+        dtype, (n_seq, n) = q.dtype, q.shape[:2]
+        heads = (n_seq, n, self.NH, self.D)
+        q_stride, q_head = _check_head_rows(q, "q", heads, dtype)
+        gate_stride, gate_head = _check_head_rows(gate, "gate", heads, dtype) if gate is not None else (0, 0)
+        out_stride = _check_seq_rows(out, "out", heads, dtype)
+        cache = self._paged_cache(kpool, vpool, table, pos, lens, n_seq)
+        s = self._on_device((q, kpool, vpool, table, pos, out, gate, lens, workspace), stream)
+        if self._paged_ws is None:
+            self._paged_ws = self.paged_workspace()
+        ws, ws_bytes, keep = self._workspace(self._paged_ws, workspace, stream)
+        args = _PAGED_ATTEND.pack(*cache, n_seq, n, _ROW_DT[dtype], window, sinks, scale, _ptr(lens) or 0, pos.data_ptr(),
+                                  q.data_ptr(), q_stride, q_head, _ptr(gate) or 0, gate_stride, gate_head, out.data_ptr(),
+                                  out_stride, ws, ws_bytes)
+        self._check(self.lib.qwattn_paged_attend(self.h, s, args))
 
     def qsa_key_bits(self, mask, cr, pos, n, key_bits, stream=None):
         """Per-key visibility bits [n, kb_words] from a block mask [n, mask_words] (shaders/attention.comp:35-43)."""

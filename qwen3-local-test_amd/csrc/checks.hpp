@@ -1,5 +1,5 @@
-// Host-side checks of the linear-attention and expert operators' arguments (declared in include/qwattn.h), apart
-// from any GPU call so that they run on a machine without one. Each returns QWATTN_OK, or a status with its text
+// Host-side checks of the linear-attention, expert and paged-attention operators' arguments (declared in
+// include/qwattn.h), apart from any GPU call so that they run on a machine without one. Each returns QWATTN_OK, or a status with its text
 // in `msg`.
 #pragma once
 #include <stdarg.h>
@@ -151,6 +151,104 @@ inline int check_moe(const qwattn_moe_layer* l, const void* x, int dtype, int64_
     if (need && (!ws || ws_bytes < need || unaligned(ws, 256)))
         return refuse(m, QWATTN_EINVAL, "qwattn_moe: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", need,
                       ws ? ws_bytes : (size_t)0);
+    return QWATTN_OK;
+}
+
+inline int check_paged_cache(const qwattn_paged_cache& c, const qwattn_config& g, int n_seq, int n, const char* who, CheckText& m) {
+    // 32 threads a row and head, less than 2^31 of them
+    if (n_seq <= 0 || n <= 0 || n_seq > 65535 || (int64_t)n_seq * n > kMostRows ||
+        (int64_t)n_seq * n * (g.n_heads + 2 * g.n_kv_heads) >= (1 << 26))
+        return refuse(m, QWATTN_EINVAL, "%s: n_seq %d (1..65535), n %d (n_seq x n x (heads + 2 KV heads) < 2^26)", who, n_seq, n);
+    if (c.page < 32 || c.page > 65536 || (c.page & (c.page - 1)) || c.n_pages <= 0 || c.pages <= 0 || c.pages > (1 << 26) / c.page)
+        return refuse(m, QWATTN_EINVAL, "%s: page %d (a power of two, 32..65536), n_pages %d, pages %d (x page <= 2^26)", who, c.page,
+                      c.n_pages, c.pages);
+    if (!c.k || !c.v || !c.table) return refuse(m, QWATTN_EINVAL, "%s: null pointer of the cache", who);
+    if (c.table_stride < c.pages || c.table_stride > (int64_t(1) << 40))
+        return refuse(m, QWATTN_EINVAL, "%s: table_stride %lld (>= pages)", who, (long long)c.table_stride);
+    if (unaligned(c.k) || unaligned(c.v) || unaligned(c.table, 4))
+        return refuse(m, QWATTN_EINVAL, "%s: the pools must be 16-byte aligned", who);
+    const int64_t pool = (int64_t)c.n_pages * c.page * g.n_kv_heads * g.head_dim * 2;
+    if (rows_meet(c.k, pool, pool, c.v, pool, pool, 1)) return refuse(m, QWATTN_EINVAL, "%s: the K and V pools overlap", who);
+    return QWATTN_OK;
+}
+
+// Rows of `heads` heads of D elements, `head` elements apart
+struct HeadRows {
+    const char* name;
+    const void* p;
+    int64_t stride, head;
+    int heads;
+    int64_t width(int D) const { return (heads - 1) * head + D; }
+};
+
+inline int check_head_rows(const HeadRows& r, int D, int64_t rows, const char* who, CheckText& m) {
+    if (!r.p) return refuse(m, QWATTN_EINVAL, "%s: %s is null", who, r.name);
+    if (r.head < D || r.head % 8 || r.head > (1 << 24) || bad_stride(r.stride, r.width(D), rows))
+        return refuse(m, QWATTN_EINVAL, "%s: %s's strides %lld and %lld (at least a row's and a head's elements, multiples of 8, "
+                      "x rows <= 2^59)", who, r.name, (long long)r.stride, (long long)r.head);
+    if (unaligned(r.p)) return refuse(m, QWATTN_EINVAL, "%s: %s must be 16-byte aligned", who, r.name);
+    return QWATTN_OK;
+}
+
+// Whether the output rows meet the input rows, head by head where both lie at one row stride
+inline bool head_rows_meet(const HeadRows& in, const HeadRows& out, int D, int64_t rows, int64_t size) {
+    return rows_meet(in.p, in.width(D) * size, in.stride * size, out.p, out.width(D) * size, out.stride * size, rows);
+}
+
+inline bool meets_pools(const qwattn_paged_cache& c, const qwattn_config& g, const HeadRows& r, int64_t rows, int64_t size) {
+    const int64_t pool = (int64_t)c.n_pages * c.page * g.n_kv_heads * g.head_dim * 2;
+    const int64_t span = ((rows - 1) * r.stride + r.width(g.head_dim)) * size;
+    return rows_meet(c.k, pool, pool, r.p, span, span, 1) || rows_meet(c.v, pool, pool, r.p, span, span, 1);
+}
+
+inline int check_paged_append(const qwattn_paged_append_args* a, const qwattn_config& g, CheckText& m) {
+    const char* who = "qwattn_paged_append";
+    if (!a) return refuse(m, QWATTN_EINVAL, "%s: null arguments", who);
+    if (int rc = check_paged_cache(a->cache, g, a->n_seq, a->n, who, m)) return rc;
+    if (bad_dtype(a->dtype)) return refuse(m, QWATTN_EINVAL, "%s: dtype %d", who, a->dtype);
+    if (!a->pos) return refuse(m, QWATTN_EINVAL, "%s: pos is null", who);
+    if (!a->q != !a->q_out) return refuse(m, QWATTN_EINVAL, "%s: q and q_out come together", who);
+    if (a->rope && a->n_rope <= 0) return refuse(m, QWATTN_EINVAL, "%s: n_rope %d", who, a->n_rope);
+    if (unaligned(a->qn) || unaligned(a->kn) || unaligned(a->rope))
+        return refuse(m, QWATTN_EINVAL, "%s: qn, kn and rope must be 16-byte aligned", who);
+    const int D = g.head_dim;
+    const int64_t rows = (int64_t)a->n_seq * a->n, size = a->dtype == QWATTN_F32 ? 4 : 2;
+    const HeadRows in[] = {{"k", a->k, a->k_stride, D, g.n_kv_heads}, {"v", a->v, a->v_stride, D, g.n_kv_heads},
+                           {"q", a->q, a->q_stride, a->q_head, g.n_heads}};
+    const HeadRows out{"q_out", a->q_out, a->q_out_stride, D, g.n_heads};
+    for (int i = 0; i < (a->q ? 3 : 2); i++) {
+        if (int rc = check_head_rows(in[i], D, rows, who, m)) return rc;
+        if (meets_pools(a->cache, g, in[i], rows, size)) return refuse(m, QWATTN_EINVAL, "%s: %s overlaps the pools", who, in[i].name);
+    }
+    if (!a->q) return QWATTN_OK;
+    if (int rc = check_head_rows(out, D, rows, who, m)) return rc;
+    if (meets_pools(a->cache, g, out, rows, size)) return refuse(m, QWATTN_EINVAL, "%s: q_out overlaps the pools", who);
+    for (const HeadRows& i : in)
+        if (head_rows_meet(i, out, D, rows, size)) return refuse(m, QWATTN_EINVAL, "%s: q_out overlaps %s", who, i.name);
+    return QWATTN_OK;
+}
+
+inline int check_paged_attend(const qwattn_paged_attend_args* a, const qwattn_config& g, size_t need, CheckText& m) {
+    const char* who = "qwattn_paged_attend";
+    if (!a) return refuse(m, QWATTN_EINVAL, "%s: null arguments", who);
+    if (int rc = check_paged_cache(a->cache, g, a->n_seq, a->n, who, m)) return rc;
+    if (bad_dtype(a->dtype) || a->window < 0 || a->sinks < 0)
+        return refuse(m, QWATTN_EINVAL, "%s: dtype %d, window %d, sinks %d (>= 0)", who, a->dtype, a->window, a->sinks);
+    if (!(a->scale >= 0.f) || a->scale > 3.4e38f) return refuse(m, QWATTN_EINVAL, "%s: scale %g", who, (double)a->scale);
+    if (!a->pos) return refuse(m, QWATTN_EINVAL, "%s: pos is null", who);
+    const int D = g.head_dim;
+    const int64_t rows = (int64_t)a->n_seq * a->n, size = a->dtype == QWATTN_F32 ? 4 : 2;
+    const HeadRows in[] = {{"q", a->q, a->q_stride, a->q_head, g.n_heads}, {"gate", a->gate, a->gate_stride, a->gate_head, g.n_heads}};
+    const HeadRows out{"out", a->out, a->out_stride, D, g.n_heads};
+    if (int rc = check_head_rows(out, D, rows, who, m)) return rc;
+    if (meets_pools(a->cache, g, out, rows, size)) return refuse(m, QWATTN_EINVAL, "%s: out overlaps the pools", who);
+    for (int i = 0; i < (a->gate ? 2 : 1); i++) {
+        if (int rc = check_head_rows(in[i], D, rows, who, m)) return rc;
+        if (head_rows_meet(in[i], out, D, rows, size)) return refuse(m, QWATTN_EINVAL, "%s: out overlaps %s", who, in[i].name);
+    }
+    if (need && (!a->workspace || a->workspace_bytes < need || unaligned(a->workspace, 256)))
+        return refuse(m, QWATTN_EINVAL, "%s: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", who, need,
+                      a->workspace ? a->workspace_bytes : (size_t)0);
     return QWATTN_OK;
 }
 

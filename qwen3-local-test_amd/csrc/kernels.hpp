@@ -353,4 +353,35 @@ struct MoeArgs {
 size_t moe_workspace(const MoeArgs& a, bool bf16);
 hipError_t launch_moe(MoeArgs a, bool bf16, void* workspace, hipStream_t s);
 
+// The paged caches of a batch (qwattn_paged_cache, include/qwattn.h)
+struct PagedCache {
+    uint16_t *k, *v;
+    const int32_t* table;
+    int64_t table_stride;
+    int n_pages, pages, lg_page;  // 2^lg_page positions a page
+};
+struct PagedAppendArgs {
+    PagedCache c;
+    int n_seq, n, NH, NKV, R, limit;  // limit: positions a sequence can have
+    float eps;
+    const int32_t *lens, *pos;
+    const void *q, *k, *v;
+    size_t q_stride, q_head, k_stride, v_stride, q_out_stride;
+    const float *qn, *kn, *rope;
+    void* q_out;
+};
+hipError_t launch_paged_append(const PagedAppendArgs& a, int D, bool bf16, hipStream_t s);
+
+struct PagedAttendArgs {
+    PagedCache c;
+    int n_seq, n, NH, NKV, limit, window, sinks;
+    float scale;  // times log2(e)
+    const int32_t *lens, *pos;
+    const void *q, *gate;
+    size_t q_stride, q_head, gate_stride, gate_head, out_stride;
+    void* out;
+};
+size_t paged_workspace(int NH, int NKV, int D, int n_cu);
+hipError_t launch_paged_attend(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* workspace, hipStream_t s);
+
 }  // namespace qw

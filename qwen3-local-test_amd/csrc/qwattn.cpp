@@ -239,6 +239,10 @@ qw::MoeArgs moe_args(const qwattn_moe_layer& l, int n, int top_k) {
     return a;
 }
 
+qw::PagedCache paged_cache(const qwattn_paged_cache& p) {
+    return {(uint16_t*)p.k, (uint16_t*)p.v, p.table, p.table_stride, p.n_pages, p.pages, __builtin_ctz((unsigned)p.page)};
+}
+
 }  // namespace
 
 extern "C" {
@@ -1205,6 +1209,51 @@ int qwattn_moe(qwattn_ctx* c, void* stream, const qwattn_moe_layer* l, const voi
     a.x = x, a.x_stride = (size_t)x_stride, a.ids = ids, a.weights = weights, a.y = y, a.y_stride = (size_t)y_stride;
     DeviceGuard dg(c->device);
     HIP_TRY(c, qw::launch_moe(a, bf16, workspace, (hipStream_t)stream));
+    return QWATTN_OK;
+}
+
+// ---- batches over a paged cache (checks: checks.hpp) ----------------------------------------------------
+
+int qwattn_paged_append(qwattn_ctx* c, void* stream, const qwattn_paged_append_args* p) {
+    if (!c) return QWATTN_EINVAL;
+    qw::CheckText m;
+    if (int rc = qw::check_paged_append(p, c->cfg, m)) return fail(c, rc, "%s", m.text);
+    qw::PagedAppendArgs a{};
+    a.c = paged_cache(p->cache), a.n_seq = p->n_seq, a.n = p->n, a.NH = c->cfg.n_heads, a.NKV = c->cfg.n_kv_heads;
+    a.R = c->cfg.rope_dim, a.eps = c->cfg.rms_eps, a.lens = p->lens, a.pos = p->pos;
+    a.limit = p->cache.pages * p->cache.page;
+    if (a.R) a.limit = std::min(a.limit, p->rope ? p->n_rope : c->cfg.max_ctx);
+    a.q = p->q, a.k = p->k, a.v = p->v, a.q_out = p->q_out;
+    a.q_stride = (size_t)p->q_stride, a.q_head = (size_t)p->q_head, a.k_stride = (size_t)p->k_stride;
+    a.v_stride = (size_t)p->v_stride, a.q_out_stride = (size_t)p->q_out_stride;
+    a.qn = p->qn, a.kn = p->kn, a.rope = p->rope ? p->rope : c->rope;
+    DeviceGuard dg(c->device);
+    HIP_TRY(c, qw::launch_paged_append(a, c->cfg.head_dim, p->dtype == QWATTN_BF16, (hipStream_t)stream));
+    return QWATTN_OK;
+}
+
+int qwattn_paged_workspace(qwattn_ctx* c, size_t* bytes) {
+    if (!c) return QWATTN_EINVAL;
+    if (!bytes) return fail(c, QWATTN_EINVAL, "qwattn_paged_workspace: null pointer");
+    *bytes = qw::paged_workspace(c->cfg.n_heads, c->cfg.n_kv_heads, c->cfg.head_dim, c->n_cu);
+    return QWATTN_OK;
+}
+
+int qwattn_paged_attend(qwattn_ctx* c, void* stream, const qwattn_paged_attend_args* p) {
+    if (!c) return QWATTN_EINVAL;
+    const qwattn_config& g = c->cfg;
+    qw::CheckText m;
+    if (int rc = qw::check_paged_attend(p, g, qw::paged_workspace(g.n_heads, g.n_kv_heads, g.head_dim, c->n_cu), m))
+        return fail(c, rc, "%s", m.text);
+    qw::PagedAttendArgs a{};
+    a.c = paged_cache(p->cache), a.n_seq = p->n_seq, a.n = p->n, a.NH = g.n_heads, a.NKV = g.n_kv_heads;
+    a.limit = p->cache.pages * p->cache.page, a.window = p->window, a.sinks = p->sinks;
+    a.scale = qw::kLog2eHost * (p->scale > 0.f ? p->scale : 1.f / std::sqrt((float)g.head_dim));
+    a.lens = p->lens, a.pos = p->pos, a.q = p->q, a.gate = p->gate, a.out = p->out;
+    a.q_stride = (size_t)p->q_stride, a.q_head = (size_t)p->q_head, a.gate_stride = (size_t)p->gate_stride;
+    a.gate_head = (size_t)p->gate_head, a.out_stride = (size_t)p->out_stride;
+    DeviceGuard dg(c->device);
+    HIP_TRY(c, qw::launch_paged_attend(a, g.head_dim, p->dtype == QWATTN_BF16, c->n_cu, p->workspace, (hipStream_t)stream));
     return QWATTN_OK;
 }
 
