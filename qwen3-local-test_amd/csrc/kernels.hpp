@@ -372,16 +372,21 @@ struct PagedAppendArgs {
 };
 hipError_t launch_paged_append(const PagedAppendArgs& a, int D, bool bf16, hipStream_t s);
 
+constexpr int kNoWindow = 1 << 30;
 struct PagedAttendArgs {
     PagedCache c;
-    int n_seq, n, NH, NKV, limit, window, sinks;
-    float scale;  // times log2(e)
+    int n_seq, n, NH, NKV, limit;
+    int window, sinks;  // at most `limit` each, kNoWindow without a window
+    float scale;        // times log2(e)
     const int32_t *lens, *pos;
     const void *q, *gate;
     size_t q_stride, q_head, gate_stride, gate_head, out_stride;
     void* out;
 };
-size_t paged_workspace(int NH, int NKV, int D, int n_cu);
+size_t paged_workspace(int D, int n_cu);
+// up to 32 query rows a KV head
+size_t paged_few_workspace(int D, int n_cu);
+hipError_t launch_paged_few(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* workspace, hipStream_t s);
 hipError_t launch_paged_attend(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* workspace, hipStream_t s);
 
 }  // namespace qw

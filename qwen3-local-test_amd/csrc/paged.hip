@@ -2,22 +2,16 @@
 //
 // A page holds 2^lg_page positions of every KV head, in the 32-position blocks of common.hpp; table[b] names the
 // pages of sequence b. The reference serves one sequence (src/qwen4_vk.cpp:937-996).
-#include "common.hpp"
-#include "kernels.hpp"
+#include "paged.hpp"
 
 namespace qw {
 
 namespace {
 
-// The sequence's new tokens: min(max(lens[b], 0), n)
-__device__ __forceinline__ int seq_len(const int32_t* lens, int b, int n) { return lens ? min(max(lens[b], 0), n) : n; }
-
-// Element offset of the block of KV head h that holds position p of sequence b, in either pool; -1 without a page.
-__device__ __forceinline__ int64_t paged_block(const PagedCache& c, int b, int p, int h, int nkv, int D) {
+// ... of position p of sequence b; -1 without a page
+__device__ __forceinline__ int64_t paged_block_at(const PagedCache& c, int b, int p, int h, int nkv, int D) {
     const int32_t page = c.table[(size_t)b * c.table_stride + (p >> c.lg_page)];
-    if ((uint32_t)page >= (uint32_t)c.n_pages) return -1;
-    const int in_page = p & ((1 << c.lg_page) - 1);
-    return (((int64_t)page * nkv + h) * (1 << (c.lg_page - 5)) + (in_page >> 5)) * (int64_t)(kBlk * D);
+    return (uint32_t)page < (uint32_t)c.n_pages ? paged_block(c, page, p, h, nkv, D) : -1;
 }
 
 // ---- append --------------------------------------------------------------------------------------------------
@@ -39,7 +33,7 @@ __device__ __forceinline__ void paged_v_copy(const PagedAppendArgs& a, int64_t v
     // tokens [t0, t1) of the sequence lie in this group at valid positions
     const int64_t lo = max(max(p0, pos), (int64_t)0), hi = min(min(p0 + 8, pos + len), (int64_t)a.limit);
     if (lo >= hi) return;
-    const int64_t blk = paged_block(a.c, b, (int)p0, h, a.NKV, D);  // (p0 >= 0: lo < p0 + 8 and lo >= 0, p0 a multiple of 8)
+    const int64_t blk = paged_block_at(a.c, b, (int)p0, h, a.NKV, D);  // (p0 >= 0: lo < p0 + 8 and lo >= 0, p0 a multiple of 8)
     if (blk < 0) return;
     float x[8][8];
 #pragma unroll
@@ -136,7 +130,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs a) {
         return;
     }
     if (!there) return;
-    const int64_t blk = paged_block(a.c, b, (int)p, h, a.NKV, D);
+    const int64_t blk = paged_block_at(a.c, b, (int)p, h, a.NKV, D);
     if (blk < 0) return;
     typedef f16 f16v __attribute__((ext_vector_type(DPL)));
     f16v o;
@@ -170,10 +164,10 @@ __global__ __launch_bounds__(256) void k_paged_simple(PagedAttendArgs a) {
     if (tid < 32) sm[tid] = kNegInf, sl[tid] = 0.f;
     __syncthreads();
     const int end = p >= 0 && p < a.limit ? (int)p + 1 : 0;
-    const int first = a.window && end > a.window ? end - a.window : 0;
+    const int first = end > a.window ? end - a.window : 0;
     for (int k0 = 0; k0 < end; k0 += 32) {
-        if (a.window && k0 + 32 <= first && k0 >= a.sinks) continue;
-        const int64_t blk = paged_block(a.c, b, k0, h, a.NKV, D);
+        if (k0 + 32 <= first && k0 >= a.sinks) continue;
+        const int64_t blk = paged_block_at(a.c, b, k0, h, a.NKV, D);
         if (blk < 0) continue;
         const f16 *K = reinterpret_cast<const f16*>(a.c.k) + blk, *V = reinterpret_cast<const f16*>(a.c.v) + blk;
         for (int i = tid; i < G * 32; i += 256) {
@@ -246,9 +240,10 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, int D, bool bf16, hipSt
     return append_d<64>(a, bf16, s);
 }
 
-size_t paged_workspace(int, int, int, int) { return 256; }
+size_t paged_workspace(int D, int n_cu) { return paged_few_workspace(D, n_cu); }
 
-hipError_t launch_paged_attend(const PagedAttendArgs& a, int D, bool bf16, int, void*, hipStream_t s) {
+hipError_t launch_paged_attend(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* workspace, hipStream_t s) {
+    if (a.n * (a.NH / a.NKV) <= 32) return launch_paged_few(a, D, bf16, n_cu, workspace, s);
     if (D == 256) return attend_d<256>(a, bf16, s);
     if (D == 128) return attend_d<128>(a, bf16, s);
     return attend_d<64>(a, bf16, s);

@@ -1235,7 +1235,7 @@ int qwattn_paged_append(qwattn_ctx* c, void* stream, const qwattn_paged_append_a
 int qwattn_paged_workspace(qwattn_ctx* c, size_t* bytes) {
     if (!c) return QWATTN_EINVAL;
     if (!bytes) return fail(c, QWATTN_EINVAL, "qwattn_paged_workspace: null pointer");
-    *bytes = qw::paged_workspace(c->cfg.n_heads, c->cfg.n_kv_heads, c->cfg.head_dim, c->n_cu);
+    *bytes = qw::paged_workspace(c->cfg.head_dim, c->n_cu);
     return QWATTN_OK;
 }
 
@@ -1243,11 +1243,12 @@ int qwattn_paged_attend(qwattn_ctx* c, void* stream, const qwattn_paged_attend_a
     if (!c) return QWATTN_EINVAL;
     const qwattn_config& g = c->cfg;
     qw::CheckText m;
-    if (int rc = qw::check_paged_attend(p, g, qw::paged_workspace(g.n_heads, g.n_kv_heads, g.head_dim, c->n_cu), m))
+    if (int rc = qw::check_paged_attend(p, g, qw::paged_workspace(g.head_dim, c->n_cu), m))
         return fail(c, rc, "%s", m.text);
     qw::PagedAttendArgs a{};
     a.c = paged_cache(p->cache), a.n_seq = p->n_seq, a.n = p->n, a.NH = g.n_heads, a.NKV = g.n_kv_heads;
-    a.limit = p->cache.pages * p->cache.page, a.window = p->window, a.sinks = p->sinks;
+    a.limit = p->cache.pages * p->cache.page;
+    a.window = p->window > 0 && p->window < a.limit ? p->window : qw::kNoWindow, a.sinks = std::min(p->sinks, a.limit);
     a.scale = qw::kLog2eHost * (p->scale > 0.f ? p->scale : 1.f / std::sqrt((float)g.head_dim));
     a.lens = p->lens, a.pos = p->pos, a.q = p->q, a.gate = p->gate, a.out = p->out;
     a.q_stride = (size_t)p->q_stride, a.q_head = (size_t)p->q_head, a.gate_stride = (size_t)p->gate_stride;
