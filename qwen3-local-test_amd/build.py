@@ -13,7 +13,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "lib", "libqwattn.so")
 BUILD = os.path.join(HERE, "_build")
 SOURCES = ["norm_rope.hip", "decode.hip", "prefill.hip", "qsa.hip", "mat.hip", "conv.hip", "delta.hip", "moe.hip",
-           "paged.hip", "paged_few.hip", "qwattn.cpp"]
+           "paged.hip", "paged_few.hip", "paged_chunk.hip", "qwattn.cpp"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-result",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 

@@ -387,6 +387,9 @@ size_t paged_workspace(int D, int n_cu);
 // up to 32 query rows a KV head
 size_t paged_few_workspace(int D, int n_cu);
 hipError_t launch_paged_few(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* workspace, hipStream_t s);
+// any number of rows
+size_t paged_chunk_workspace(int D, int n_cu);
+hipError_t launch_paged_chunk(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* workspace, hipStream_t s);
 hipError_t launch_paged_attend(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* workspace, hipStream_t s);
 
 }  // namespace qw

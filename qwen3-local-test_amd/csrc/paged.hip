@@ -4,6 +4,8 @@
 // pages of sequence b. The reference serves one sequence (src/qwen4_vk.cpp:937-996).
 #include "paged.hpp"
 
+#include <algorithm>
+
 namespace qw {
 
 namespace {
@@ -139,81 +141,6 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs a) {
     *reinterpret_cast<f16v*>(reinterpret_cast<f16*>(a.c.k) + blk + k_off((int)p & (kBlk - 1), d0)) = o;
 }
 
-// ---- attention -----------------------------------------------------------------------------------------------
-
-__device__ __forceinline__ void store_row(void* out, size_t at, float x, bool bf16) {
-    if (bf16) static_cast<uint16_t*>(out)[at] = (uint16_t)pk_bf16(x, x);
-    else static_cast<float*>(out)[at] = x;
-}
-
-// A workgroup a (token, KV head): scores of a block of 32 keys for the G heads, running maximum and sum, weighted values.
-template <int D, int DT>
-__global__ __launch_bounds__(256) void k_paged_simple(PagedAttendArgs a) {
-    __shared__ float sq[32 * D];
-    __shared__ float ss[32][33];
-    __shared__ float sm[32], sl[32], sc[32];
-    const int G = a.NH / a.NKV, tid = threadIdx.x;
-    const int h = blockIdx.x % a.NKV, row = blockIdx.x / a.NKV, b = row / a.n, t = row - b * a.n;
-    if (t >= seq_len(a.lens, b, a.n)) return;
-    const int64_t p = (int64_t)a.pos[b] + t;
-    constexpr int ACC = 32 * D / 256;  // outputs a thread of 32 heads
-    float acc[ACC];
-#pragma unroll
-    for (int i = 0; i < ACC; i++) acc[i] = 0.f;
-    for (int i = tid; i < G * D; i += 256) sq[i] = load_in<DT>(a.q, (size_t)row * a.q_stride + (size_t)(h * G + i / D) * a.q_head + i % D);
-    if (tid < 32) sm[tid] = kNegInf, sl[tid] = 0.f;
-    __syncthreads();
-    const int end = p >= 0 && p < a.limit ? (int)p + 1 : 0;
-    const int first = end > a.window ? end - a.window : 0;
-    for (int k0 = 0; k0 < end; k0 += 32) {
-        if (k0 + 32 <= first && k0 >= a.sinks) continue;
-        const int64_t blk = paged_block_at(a.c, b, k0, h, a.NKV, D);
-        if (blk < 0) continue;
-        const f16 *K = reinterpret_cast<const f16*>(a.c.k) + blk, *V = reinterpret_cast<const f16*>(a.c.v) + blk;
-        for (int i = tid; i < G * 32; i += 256) {
-            const int kb = i & 31, g = i >> 5, j = k0 + kb;
-            float s = kNegInf;
-            if (j < end && (j >= first || j < a.sinks)) {
-                s = 0.f;
-                for (int d = 0; d < D; d++) s = __builtin_fmaf(sq[g * D + d], (float)K[k_off(kb, d)], s);
-                s *= a.scale;
-            }
-            ss[g][kb] = s;
-        }
-        __syncthreads();
-        if (tid < G) {
-            float m = sm[tid];
-            for (int kb = 0; kb < 32; kb++) m = fmaxf(m, ss[tid][kb]);
-            const float corr = m == kNegInf ? 1.f : exp2_fast(sm[tid] - m);
-            float l = sl[tid] * corr;
-            for (int kb = 0; kb < 32; kb++) {
-                const float w = ss[tid][kb] == kNegInf ? 0.f : exp2_fast(ss[tid][kb] - m);
-                ss[tid][kb] = w, l += w;
-            }
-            sm[tid] = m, sl[tid] = l, sc[tid] = corr;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < ACC; i++) {
-            const int e = tid + 256 * i, g = e / D, d = e % D;
-            if (g >= G) break;
-            float o = acc[i] * sc[g];
-            for (int kb = 0; kb < 32; kb++)
-                if (ss[g][kb] != 0.f) o = __builtin_fmaf(ss[g][kb], (float)V[v_off(kb, d)], o);
-            acc[i] = o;
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < ACC; i++) {
-        const int e = tid + 256 * i, g = e / D, d = e % D;
-        if (g >= G) break;
-        float o = sl[g] > 0.f || sl[g] != sl[g] ? acc[i] / sl[g] : 0.f;
-        if (a.gate) o *= sigmoid(load_in<DT>(a.gate, (size_t)row * a.gate_stride + (size_t)(h * G + g) * a.gate_head + d));
-        store_row(a.out, (size_t)row * a.out_stride + (size_t)(h * G + g) * D + d, o, DT == 1);
-    }
-}
-
 template <int D>
 hipError_t append_d(const PagedAppendArgs& a, bool bf16, hipStream_t s) {
     const int64_t items = (int64_t)a.n_seq * a.n * ((a.q ? a.NH : 0) + a.NKV);
@@ -221,14 +148,6 @@ hipError_t append_d(const PagedAppendArgs& a, bool bf16, hipStream_t s) {
     const dim3 grid((unsigned)((items + 7) / 8 + (v_lanes + 255) / 256)), block(256);
     if (bf16) hipLaunchKernelGGL((k_paged_append<D, 1>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((k_paged_append<D, 0>), grid, block, 0, s, a);
-    return hipGetLastError();
-}
-
-template <int D>
-hipError_t attend_d(const PagedAttendArgs& a, bool bf16, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)a.n_seq * a.n * a.NKV)), block(256);
-    if (bf16) hipLaunchKernelGGL((k_paged_simple<D, 1>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_paged_simple<D, 0>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 
@@ -240,13 +159,11 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, int D, bool bf16, hipSt
     return append_d<64>(a, bf16, s);
 }
 
-size_t paged_workspace(int D, int n_cu) { return paged_few_workspace(D, n_cu); }
+size_t paged_workspace(int D, int n_cu) { return std::max(paged_few_workspace(D, n_cu), paged_chunk_workspace(D, n_cu)); }
 
 hipError_t launch_paged_attend(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* workspace, hipStream_t s) {
     if (a.n * (a.NH / a.NKV) <= 32) return launch_paged_few(a, D, bf16, n_cu, workspace, s);
-    if (D == 256) return attend_d<256>(a, bf16, s);
-    if (D == 128) return attend_d<128>(a, bf16, s);
-    return attend_d<64>(a, bf16, s);
+    return launch_paged_chunk(a, D, bf16, n_cu, workspace, s);
 }
 
 }  // namespace qw
