@@ -5,13 +5,14 @@ namespace qw {
 
 namespace {
 
-constexpr int kChWaves = 8;
+constexpr int kChWaves = 8, kChRing = 4;
 
 template <int D, int DT, int NT>
 struct ChCfg {
     static constexpr int PARTS = DT == 0 ? 2 : 1, NKS = D / 32, NDT = D / 16, ROWS = kChWaves * 16 * NT;
-    static constexpr int BLKE = kBlk * D, TILEE = 2 * BLKE;  // elements of a block, of a tile of 64 keys
-    static constexpr int LDS = 2 * 2 * TILEE * 2;            // two buffers of keys, two of values
+    static constexpr int BLKE = kBlk * D;              // elements of a block
+    static constexpr int LDS = 2 * kChRing * BLKE * 2;  // rings of blocks of keys and of values
+    static constexpr int COPIES = D / 64;              // kilobytes a wave copies a step (a block of keys and one of values)
     static constexpr int PART = 16 * NT * D + 64 * NT * 2;   // floats of a wave's partial
 };
 // Tiles of 16 rows a wave: what fits the 256 registers of a wave beside the queries' operands
@@ -81,20 +82,36 @@ __global__ __launch_bounds__(1024) void k_paged_plan(PagedAttendArgs a, void* ws
     }
 }
 
-__device__ __forceinline__ void chunk_barrier() {  // every wave's loads to the LDS are there, its LDS reads done
+// The lane, worked out where it stands: kept in a register through the loop of 32-row waves it would be spilled, and a
+// reload waits for every copy in flight.
+__device__ __forceinline__ int lane_here() {
+    int l;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+    return l;
+}
+// A barrier that waits for nothing else; nothing moves across it
+__device__ __forceinline__ void phase() {
+    __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);
     __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// Waits until at most N (< 16) vector loads of the wave are in flight
+template <int N>
+__device__ __forceinline__ void landed() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | N);
     asm volatile("" ::: "memory");
 }
 
 template <int D, int DT, int NT>
 __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArgs a, void* ws, bool joined) {
     using C = ChCfg<D, DT, NT>;
-    constexpr int PARTS = C::PARTS, NKS = C::NKS, NDT = C::NDT, BLKE = C::BLKE, TILEE = C::TILEE;
+    constexpr int PARTS = C::PARTS, NKS = C::NKS, NDT = C::NDT, BLKE = C::BLKE;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    f16* sk = reinterpret_cast<f16*>(smem);  // two tiles of keys
-    f16* sv = sk + 2 * TILEE;                // two of values
+    f16* sk = reinterpret_cast<f16*>(smem);  // blocks of keys
+    f16* sv = sk + kChRing * BLKE;           // and of values
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int G = a.NH / a.NKV, tok = C::ROWS / G, groups = gridDim.x;
@@ -125,109 +142,153 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
         }
         const int lo = off, hi = (int)min((int64_t)kt.count, off + (stop - at));
 
-        // ---- staging: a wave copies a quarter of one of the tile's two blocks, of the keys and of the values ----
-        const int32_t* table = a.c.table + (size_t)b * a.c.table_stride;
-        int pages = -1, it0 = lo;
-        const int half = wave >> 2;
-        auto fetch_pages = [&](int i) {  // lane l: the page of block l % 2 of entry i + l / 2
-            it0 = i;
-            const int p = kt.tile(min(i + (lane >> 1), kt.count - 1)) * 2 + (lane & 1);
-            pages = p * kBlk < a.limit ? table[p >> (a.c.lg_page - 5)] : -1;
-        };
-        auto page_of = [&](int i, int hb) { return __builtin_amdgcn_readlane(pages, ((i - it0) * 2 + hb) & 63); };
-        auto is_page = [&](int page) { return (uint32_t)page < (uint32_t)a.c.n_pages; };
-        auto copy = [&](int i, uint16_t* pool, f16* dst) __attribute__((always_inline)) {
-            const int page = page_of(i, half);
-            const bool there = is_page(page);
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-                pool + paged_block(a.c, there ? page : 0, (kt.tile(i) * 2 + half) * kBlk, h, a.NKV, D), (short)0, there ? BLKE * 2 : 0, 0x00020000);
-#pragma unroll
-            for (int j = 0; j < NDT / 4; j++) {
-                const int piece = (wave & 3) * (NDT / 4) + j;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + half * BLKE + piece * 512), 16,
-                                                         piece * 1024 + lane * 16, 0, 0, 0);
-            }
-        };
-        auto blocks_there = [&](int i) { return (is_page(page_of(i, 0)) ? 1 : 0) | (is_page(page_of(i, 1)) ? 2 : 0); };
-        fetch_pages(lo);
-        __syncthreads();  // the last segment's readers of the buffers are done
-        copy(lo, a.c.k, sk), copy(lo, a.c.v, sv);
+        const int n = 2 * (hi - lo);  // blocks of 32 keys, block i of the segment in ring place i % 4
+        auto key_of = [&](int i) { return kt.tile(lo + (i >> 1)) * 64 + (i & 1) * kBlk; };
 
-        // ---- the wave's rows: row r of the tile is token t0 + r / G, head h G + r % G ----
-        f16x8 q[NT][PARTS][NKS];
-        float fac[NT], m_run[NT], l_run[NT];
-        Sight see[NT];
-        f32x4 acc[NT][NDT];
+        // ---- the wave's rows as they lie in memory: row r of the tile is token t0 + r / G, head h G + r % G ----
+        typedef typename std::conditional<DT == 0, f32x4, u32x4>::type raw_t;
+        constexpr int RAW = DT == 0 ? 2 : 1;
+        raw_t raw[NT][NKS][RAW];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int r = (wave * NT + nt) * 16 + col, t = t0 + r / G;
-            const bool ok = r < tok * G && t < t1;
-            see[nt] = ok ? sight(a, pos + t) : Sight{0, 0};
-            const size_t base = ((size_t)b * a.n + (ok ? t : t0)) * a.q_stride + (size_t)(h * G + r % G) * a.q_head + 8 * g;
-            float x[NKS][8], largest = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < NKS; kk++) load_vec<DT, 8>(a.q, base + 32 * kk, x[kk]);
+            const int r = (wave * NT + nt) * 16 + col, t = min(t0 + r / G, t1 - 1);
+            const size_t base = ((size_t)b * a.n + t) * a.q_stride + (size_t)(h * G + r % G) * a.q_head + 8 * g;
 #pragma unroll
             for (int kk = 0; kk < NKS; kk++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) largest = fmaxf(largest, fabsf(x[kk][j]));
+                for (int k = 0; k < RAW; k++) {
+                    if constexpr (DT == 0) raw[nt][kk][k] = *reinterpret_cast<const raw_t*>(static_cast<const float*>(a.q) + base + 32 * kk + 4 * k);
+                    else raw[nt][kk][k] = *reinterpret_cast<const raw_t*>(static_cast<const uint16_t*>(a.q) + base + 32 * kk);
+                }
+        }
+
+        // positions of the wave's tokens, the keys that all of them see, that some of them see, and that some of the item's do
+        const int w0 = pos + t0 + wave * 16 * NT / G, w1 = min(pos + t0 + (wave * 16 * NT + 16 * NT - 1) / G, pos + t1 - 1);
+        const Sight all_see = sight_of_all(a, w0, w1), some_see = sight_of_some(a, w0, w1);
+        const Sight item_see = sight_of_some(a, pos + t0, pos + t1 - 1);
+
+        // ---- staging. What a step needs to know of its blocks is worked out for 64 of them at a time, a lane each: scalar
+        // arithmetic in every step (page, offset, masks: some 150 instructions) took as long as its matrix instructions ----
+        const int32_t* table = a.c.table + (size_t)b * a.c.table_stride;
+        int base = 0;
+        int64_t offset = -1;   // lane l: byte offset of block base + l in a pool, -1 without a page or past the last block
+        int first_key = 0;     // its first position
+        uint64_t paged, whole, stale;  // bit l: it has a page; all rows of the wave see all of it; it has keys that no row of the item sees
+        auto survey = [&](int i) __attribute__((always_inline)) {
+            base = i;
+            const int l = lane_here();
+            const bool in = i + l < n;
+            first_key = key_of(min(i + l, n - 1));
+            const int page = in && first_key < a.limit ? table[first_key >> a.c.lg_page] : -1;
+            const bool there = (uint32_t)page < (uint32_t)a.c.n_pages;
+            offset = there ? 2 * paged_block(a.c, page, first_key, h, a.NKV, D) : -1;
+            paged = __builtin_amdgcn_ballot_w64(there);
+            whole = __builtin_amdgcn_ballot_w64(there && sees_whole(all_see, first_key, first_key + kBlk, a.sinks));
+            stale = __builtin_amdgcn_ballot_w64(in && !sees_whole(item_see, first_key, first_key + kBlk, a.sinks));
+        };
+        auto key_at = [&](int i) { return __builtin_amdgcn_readlane(first_key, i - base); };
+        // this wave's share of block i of `pool` into ring place i % 4 (zeros without a page): pieces from `first` on
+        auto copy = [&](int i, uint16_t* pool, f16* ring, int first, auto count) __attribute__((always_inline)) {
+            const uint32_t lo32 = (uint32_t)__builtin_amdgcn_readlane((int)offset, i - base);
+            const int hi32 = __builtin_amdgcn_readlane((int)(offset >> 32), i - base);
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+                reinterpret_cast<char*>(pool) + (((int64_t)(hi32 < 0 ? 0 : hi32) << 32) | lo32), (short)0, hi32 < 0 ? 0 : BLKE * 2, 0x00020000);
+            f16* dst = ring + (i & (kChRing - 1)) * BLKE;
+            const int l16 = lane_here() * 16;
+#pragma unroll
+            for (int j = 0; j < decltype(count)::value; j++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (first + j) * 512), 16,
+                                                         (first + j) * 1024 + l16, 0, 0, 0);
+        };
+        auto stage = [&](bool keys, int i) __attribute__((always_inline)) {
+            if constexpr (D >= 128) {
+                constexpr int P = D / 128;
+                copy(i, keys ? a.c.k : a.c.v, keys ? sk : sv, wave * P, std::integral_constant<int, P>{});
+            } else {  // the first four waves copy keys and the others values
+                if (keys == (wave < 4)) copy(i, keys ? a.c.k : a.c.v, keys ? sk : sv, wave & 3, std::integral_constant<int, 1>{});
+            }
+        };
+        survey(0);
+        __syncthreads();  // the last segment's readers of the rings are done
+        stage(true, 0), stage(true, 1), stage(false, 0);
+
+        // ---- the rows' operands ----
+        f16x8 q[NT][PARTS][NKS];
+        float fac[NT], m_run[NT], l_run[NT];
+        f32x4 acc[NT][NDT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            auto at_raw = [&](int kk, int j) {
+                if constexpr (DT == 0) return raw[nt][kk][j >> 2][j & 3];
+                else return __uint_as_float((j & 1) ? raw[nt][kk][0][j >> 1] & 0xffff0000u : raw[nt][kk][0][j >> 1] << 16);
+            };
+            float largest = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < NKS; kk++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) largest = fmaxf(largest, fabsf(at_raw(kk, j)));
             const int sh = query_shift(max_rows(largest));
             fac[nt] = __builtin_ldexpf(a.scale, -sh);
 #pragma unroll
             for (int kk = 0; kk < NKS; kk++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float y = ok ? __builtin_ldexpf(x[kk][j], sh) : 0.f;
+                    const float y = __builtin_ldexpf(at_raw(kk, j), sh);
                     q[nt][0][kk][j] = (f16)y;
                     if constexpr (PARTS == 2) q[nt][1][kk][j] = (f16)(y - (float)q[nt][0][kk][j]);
                 }
             m_run[nt] = kNegInf, l_run[nt] = 0.f;
 #pragma unroll
             for (int dt = 0; dt < NDT; dt++) acc[nt][dt] = f32x4{};
-            __builtin_amdgcn_sched_barrier(0);
         }
-        // positions of the wave's tokens
-        const int w0 = pos + t0 + wave * 16 * NT / G, w1 = min(pos + t0 + (wave * 16 * NT + 16 * NT - 1) / G, pos + t1 - 1);
-        const Sight all_see = sight_of_all(a, w0, w1), some_see = sight_of_some(a, w0, w1);
+        auto unseen = [&](int k0) { return k0 >= some_see.end || (k0 + kBlk <= some_see.from && k0 >= a.sinks); };
+        auto row_sight = [&](int nt, int l) {
+            const int r = (wave * NT + nt) * 16 + (l & 15), t = t0 + r / G;
+            return r < tok * G && t < t1 ? sight(a, pos + t) : Sight{0, 0};
+        };
 
-        // ---- a block of 32 keys ----
-        // (EACH: the weighted values token by token, those hidden from it zeroed, for blocks some of whose values are not
-        // finite: a weight of zero does not hide these. It runs on its own, after the loop)
-        bool odd_values = false;
-        auto block = [&](auto each, auto&& kfrag, auto&& vfrag, int k0) __attribute__((always_inline)) {
-            constexpr bool EACH = decltype(each)::value;
-            if (k0 >= some_see.end || (k0 + kBlk <= some_see.from && k0 >= a.sinks)) return;  // no row sees any of it
-            f32x4 s[NT][2];
+        f32x4 s[NT][2];        // scores of a block: value i of key set s of lane (col, g) is key 8 g + 4 s + i
+        f16x8 w[NT][PARTS];    // its weights: keys 8 g .. 8 g + 7
+        // Matrix instructions of a phase: the scores of one block and (VALUES) the weighted values of the block before, a fragment of
+        // each in turn, read AHEAD of its use
+        constexpr int AHEAD = NT == 2 && D == 256 ? 3 : 5;
+        auto products = [&](auto values, auto&& kfrag, auto&& vfrag) __attribute__((always_inline)) {
+            constexpr bool VALUES = decltype(values)::value;
+            constexpr int STEP = VALUES ? 2 : 1, SLOTS = STEP * NDT;
+            f16x8 fr[AHEAD + 1];
+            auto read = [&](auto ic) __attribute__((always_inline)) {
+                constexpr int i = decltype(ic)::value;
+                if constexpr (VALUES && i % STEP == 0) fr[i % (AHEAD + 1)] = vfrag(i / STEP);
+                else fr[i % (AHEAD + 1)] = kfrag(i / STEP);
+            };
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) s[nt][0] = f32x4{}, s[nt][1] = f32x4{};
-            {
-                constexpr int PF = 2;  // fragment pairs ahead
-                f16x8 fr[PF + 1][2];
-                auto read = [&](int kk) __attribute__((always_inline)) {
-                    fr[kk % (PF + 1)][0] = kfrag(2 * kk), fr[kk % (PF + 1)][1] = kfrag(2 * kk + 1);
-                };
-                static_for<0, PF>([&](auto ic) __attribute__((always_inline)) { read(ic.value); });
-                static_for<0, NKS>([&](auto ic) __attribute__((always_inline)) {
-                    constexpr int kk = decltype(ic)::value;
-                    if constexpr (kk + PF < NKS) read(kk + PF);
+            static_for<0, AHEAD>(read);
+            static_for<0, SLOTS>([&](auto ic) __attribute__((always_inline)) {
+                constexpr int i = decltype(ic)::value, f = i / STEP;
+                if constexpr (i + AHEAD < SLOTS) read(std::integral_constant<int, i + AHEAD>{});
 #pragma unroll
-                    for (int part = 0; part < PARTS; part++)
+                for (int part = 0; part < PARTS; part++)
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
+                    for (int nt = 0; nt < NT; nt++) {
+                        if constexpr (VALUES && i % STEP == 0) acc[nt][f] = mfma16(fr[i % (AHEAD + 1)], w[nt][part], acc[nt][f]);
+                        else s[nt][f & 1] = mfma16(fr[i % (AHEAD + 1)], q[nt][part][f >> 1], s[nt][f & 1]);
+                    }
+                __builtin_amdgcn_sched_barrier(0);  // keep the reads ahead
+            });
+        };
+        // Weights of a block from its scores; the running maximum moves only where a row's passes it by more than kTau
+        auto softmax = [&](int k0, bool there, bool all) __attribute__((always_inline)) {
+            if (!all) {
+                const int l = lane_here(), key = k0 + 8 * (l >> 4);
 #pragma unroll
-                            for (int set = 0; set < 2; set++) s[nt][set] = mfma16(fr[kk % (PF + 1)][set], q[nt][part][kk], s[nt][set]);
-                    __builtin_amdgcn_sched_barrier(0);  // keep the reads ahead
-                });
-            }
-            const bool whole = sees_whole(all_see, k0, k0 + kBlk, a.sinks);
-            if (!whole) {  // value i of key set s of lane (col, g) is key 8 g + 4 s + i
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int nt = 0; nt < NT; nt++) {
+                    const Sight see = row_sight(nt, l);
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        s[nt][i >> 2][i & 3] = see[nt].sees(k0 + 8 * g + i, a.sinks) ? s[nt][i >> 2][i & 3] : kNegInf;
+                        s[nt][i >> 2][i & 3] = there && see.sees(key + i, a.sinks) ? s[nt][i >> 2][i & 3] : kNegInf;
+                }
             }
-            f16x8 w[NT][PARTS];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 float mx = fmaxf(fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3])),
@@ -244,81 +305,101 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
                 const float o = m_run[nt] == kNegInf ? 0.f : kShift - m_run[nt];
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
-                    const float w0 = exp2_fast(__builtin_fmaf(s[nt][i >> 2][i & 3], fac[nt], o));
-                    const float w1 = exp2_fast(__builtin_fmaf(s[nt][i >> 2][(i & 3) + 1], fac[nt], o));
-                    f16x2 hi, lo;
-                    weight_parts<PARTS>(w0, w1, hi, lo);
-                    w[nt][0][i] = hi[0], w[nt][0][i + 1] = hi[1];
-                    if constexpr (PARTS == 2) w[nt][1][i] = lo[0], w[nt][1][i + 1] = lo[1], l_run[nt] += w0 + w1;
-                    else l_run[nt] = __builtin_amdgcn_fdot2(hi, f16x2{(f16)1.f, (f16)1.f}, l_run[nt], false);
+                    const float x0 = exp2_fast(__builtin_fmaf(s[nt][i >> 2][i & 3], fac[nt], o));
+                    const float x1 = exp2_fast(__builtin_fmaf(s[nt][i >> 2][(i & 3) + 1], fac[nt], o));
+                    f16x2 hi16, lo16;
+                    weight_parts<PARTS>(x0, x1, hi16, lo16);
+                    w[nt][0][i] = hi16[0], w[nt][0][i + 1] = hi16[1];
+                    if constexpr (PARTS == 2) w[nt][1][i] = lo16[0], w[nt][1][i + 1] = lo16[1], l_run[nt] += x0 + x1;
+                    else l_run[nt] = __builtin_amdgcn_fdot2(hi16, f16x2{(f16)1.f, (f16)1.f}, l_run[nt], false);
                 }
-            }
-            if constexpr (EACH) {
-#pragma unroll 1
-                for (int p = w0; p <= w1; p++) {
-                    const Sight sp = sight(a, p);
-#pragma unroll
-                    for (int dt = 0; dt < NDT; dt++) {
-                        const f16x8 v = keep_keys(vfrag(dt), [&](int i) { return sp.sees(k0 + 8 * g + i, a.sinks); });
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            f32x4 o = acc[nt][dt];
-#pragma unroll
-                            for (int part = 0; part < PARTS; part++) o = mfma16(v, w[nt][part], o);
-                            const bool own = pos + t0 + ((wave * NT + nt) * 16 + col) / G == p;
-#pragma unroll
-                            for (int i = 0; i < 4; i++) acc[nt][dt][i] = own ? o[i] : acc[nt][dt][i];
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    }
-                }
-                return;
-            }
-            if (!whole) {
-                uint32_t odd = 0;
-#pragma unroll 4
-                for (int dt = 0; dt < NDT; dt++) odd |= not_finite(vfrag(dt));
-                if (__builtin_amdgcn_ballot_w64(odd != 0)) odd_values = true;
-            }
-            {
-                constexpr int PF = 4;
-                f16x8 fr[PF + 2];
-                auto read = [&](int dt) __attribute__((always_inline)) { fr[dt % (PF + 2)] = vfrag(dt); };
-                static_for<0, PF>([&](auto ic) __attribute__((always_inline)) { read(ic.value); });
-                static_for<0, NDT / 2>([&](auto ic) __attribute__((always_inline)) {
-                    constexpr int dt = 2 * decltype(ic)::value;
-                    if constexpr (dt + PF < NDT) read(dt + PF), read(dt + PF + 1);
-#pragma unroll
-                    for (int part = 0; part < PARTS; part++)
-#pragma unroll
-                        for (int d2 = dt; d2 < dt + 2; d2++)
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) acc[nt][d2] = mfma16(fr[d2 % (PF + 2)], w[nt][part], acc[nt][d2]);
-                    __builtin_amdgcn_sched_barrier(0);
-                });
             }
         };
 
-        // ---- the segment's tiles, the next one on its way while one is used ----
-#pragma unroll 1
-        for (int i = lo; i < hi; i++) {
-            const int buf = (i - lo) & 1;
-            chunk_barrier();
-            const int there = blocks_there(i);
-            if (i + 1 < hi) {
-                if (i + 1 - it0 >= 32) fetch_pages(i + 1);
-                copy(i + 1, a.c.k, sk + (buf ^ 1) * TILEE), copy(i + 1, a.c.v, sv + (buf ^ 1) * TILEE);
+        // ---- two groups of four waves, one of each on every SIMD, take turns: in a phase one runs the matrix instructions
+        // of a block (and the weighted values of the block before) while the other takes its softmax. Copies run two blocks
+        // ahead of the keys' use; both groups issue them in the even phases (of the first group's matrix instructions)
+        // and wait for the last ones at their end. ----
+        bool odd_values = false;
+        const bool second = wave >= 4;
+        auto kfrag_of = [&](int i) {
+            const f16* p = sk + (i & (kChRing - 1)) * BLKE + lane_here() * 8;
+            return [=](int f) { return *reinterpret_cast<const f16x8*>(p + f * 512); };
+        };
+        auto vfrag_of = [&](int i) {
+            const f16* p = sv + (i & (kChRing - 1)) * BLKE + lane_here() * 8;
+            return [=](int f) { return *reinterpret_cast<const f16x8*>(p + f * 512); };
+        };
+        // Values that no row of the item sees are zeroed in the ring (stale memory may hold anything) by the wave that copied
+        // them, once they have landed.
+        auto clean = [&](int i) __attribute__((always_inline)) {
+            const int l = lane_here(), k0 = key_at(i) + 8 * (l >> 4);
+            u32x4 keep;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                keep[k] = (item_see.sees(k0 + 2 * k, a.sinks) ? 0x0000ffffu : 0u) | (item_see.sees(k0 + 2 * k + 1, a.sinks) ? 0xffff0000u : 0u);
+            if (D >= 128 || wave >= 4) {
+#pragma unroll
+                for (int j = 0; j < (D >= 128 ? D / 128 : 1); j++) {
+                    const int piece = D >= 128 ? wave * (D / 128) + j : wave & 3;
+                    u32x4* at = reinterpret_cast<u32x4*>(sv + (i & (kChRing - 1)) * BLKE + piece * 512 + l * 8);
+                    *at = *at & keep;
+                }
             }
-            const int k0 = kt.tile(i) * 64;
-#pragma unroll 1
-            for (int hb = 0; hb < 2; hb++) {
-                if (!(there >> hb & 1)) continue;  // keys without a page are hidden
-                const f16 *K = sk + buf * TILEE + hb * BLKE + lane * 8, *V = sv + buf * TILEE + hb * BLKE + lane * 8;
-                block(std::false_type{}, [&](int f) { return *reinterpret_cast<const f16x8*>(K + f * 512); },
-                      [&](int f) { return *reinterpret_cast<const f16x8*>(V + f * 512); }, k0 + hb * kBlk);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        };
+        // Step i: the copies of keys of block i + 2 and values of block i + 1; those of the step before have landed at its end
+        auto step = [&](int i) __attribute__((always_inline)) {
+            if (i + 2 - base >= 64) survey(i);
+            stage(true, i + 2), stage(false, i + 1);
+            landed<C::COPIES>();
+            if (stale >> (i - base) & 1) clean(i);
+        };
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int part = 0; part < PARTS; part++) w[nt][part] = f16x8{};
+        auto matrix_phase = [&](int i) __attribute__((always_inline)) {  // scores of block i, values of block i - 1
+            products(std::true_type{}, kfrag_of(i), vfrag_of(i - 1));
+        };
+        auto softmax_phase = [&](int i) __attribute__((always_inline)) {
+            const bool all = whole >> (i - base) & 1;
+            softmax(key_at(i), paged >> (i - base) & 1, all);
+            if (!all) {
+                const auto read = vfrag_of(i);
+                uint32_t odd = 0;
+#pragma unroll 4
+                for (int dt = 0; dt < NDT; dt++) odd |= not_finite(read(dt));
+                if (__builtin_amdgcn_ballot_w64(odd != 0)) odd_values = true;
             }
+        };
+        // (the values of the block before the first)
+        for (int k = tid; k < BLKE / 8; k += 64 * kChWaves) *reinterpret_cast<u32x4*>(sv + (kChRing - 1) * BLKE + k * 8) = u32x4{};
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        landed<C::COPIES>();
+        phase();
+        if (second) {
+            step(0);
+            phase();
         }
-        if (odd_values) {  // the segment again, from memory
+#pragma unroll 1
+        for (int i = 0; i < n; i++) {
+            matrix_phase(i);
+            if (!second) step(i);
+            phase();
+            softmax_phase(i);
+            if (second) step(i + 1);
+            phase();
+        }
+        matrix_phase(n);  // (its scores are of no block)
+        if (!second) phase();
+        landed<0>();  // (copies past the last block write zeros)
+
+        if (odd_values) {
+            // a value that only some of the wave's rows see is not finite, and a weight of zero does not hide it: the segment again,
+            // from memory, its weighted values token by token with those hidden from it zeroed
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 m_run[nt] = kNegInf, l_run[nt] = 0.f;
@@ -326,17 +407,36 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
                 for (int dt = 0; dt < NDT; dt++) acc[nt][dt] = f32x4{};
             }
 #pragma unroll 1
-            for (int i = 2 * lo; i < 2 * hi; i++) {
-                const int k0 = kt.tile(i >> 1) * 64 + (i & 1) * kBlk;
+            for (int i = 0; i < n; i++) {
+                const int k0 = key_of(i);
                 const int page = k0 < a.limit ? __builtin_amdgcn_readfirstlane(table[k0 >> a.c.lg_page]) : -1;
-                if (!is_page(page)) continue;
+                if ((uint32_t)page >= (uint32_t)a.c.n_pages || unseen(k0)) continue;
                 const int64_t from = paged_block(a.c, page, k0, h, a.NKV, D);
                 const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(a.c.k + from, (short)0, BLKE * 2, 0x00020000);
                 const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(a.c.v + from, (short)0, BLKE * 2, 0x00020000);
                 auto get = [&](const __amdgpu_buffer_rsrc_t& r, int f) __attribute__((always_inline)) {
                     return __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(r, f * 1024 + lane * 16, 0, 0));
                 };
-                block(std::true_type{}, [&](int f) { return get(rk, f); }, [&](int f) { return get(rv, f); }, k0);
+                products(std::false_type{}, [&](int f) { return get(rk, f); }, [&](int f) { return get(rv, f); });
+                softmax(k0, true, false);
+#pragma unroll 1
+                for (int p = w0; p <= w1; p++) {
+                    const Sight sp = sight(a, p);
+#pragma unroll
+                    for (int dt = 0; dt < NDT; dt++) {
+                        const f16x8 v = keep_keys(get(rv, dt), [&](int j) { return sp.sees(k0 + 8 * g + j, a.sinks); });
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            f32x4 o = acc[nt][dt];
+#pragma unroll
+                            for (int part = 0; part < PARTS; part++) o = mfma16(v, w[nt][part], o);
+                            const bool own = pos + t0 + ((wave * NT + nt) * 16 + col) / G == p;
+#pragma unroll
+                            for (int j = 0; j < 4; j++) acc[nt][dt][j] = own ? o[j] : acc[nt][dt][j];
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                }
             }
         }
 
@@ -488,7 +588,7 @@ hipError_t go(const PagedAttendArgs& a, int n_cu, void* ws, hipStream_t s) {
     using C = ChCfg<D, DT, NT>;
     const int groups = n_cu & ~7, tok = C::ROWS / (a.NH / a.NKV);
     const int64_t pairs = (int64_t)a.n_seq * ((a.n + tok - 1) / tok), items = pairs * a.NKV;
-    const bool joined = items * 2 <= groups && pairs <= kJoinItems;
+    const bool joined = items * 8 <= groups && pairs <= kJoinItems;
     hipLaunchKernelGGL(k_paged_plan, dim3(1), dim3(1024), 0, s, a, ws, groups, C::PART, tok, joined);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
