@@ -516,7 +516,7 @@ typedef struct qwattn_paged_cache {
                               16-byte aligned */
     const int32_t* table;  /* device [n_seq][table_stride]: the page of positions [i * page, (i + 1) * page) */
     int64_t table_stride;  /* >= pages */
-    int n_pages, pages;    /* pages of the pools, and of a sequence */
+    int n_pages, pages;    /* pages of the pools (x NKV x page / 32 < 2^31), and of a sequence */
     int page;              /* positions a page: a power of two from 32 to 65536; pages * page <= 2^26 */
 } qwattn_paged_cache;
 

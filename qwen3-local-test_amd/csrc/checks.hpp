@@ -162,6 +162,8 @@ inline int check_paged_cache(const qwattn_paged_cache& c, const qwattn_config& g
     if (c.page < 32 || c.page > 65536 || (c.page & (c.page - 1)) || c.n_pages <= 0 || c.pages <= 0 || c.pages > (1 << 26) / c.page)
         return refuse(m, QWATTN_EINVAL, "%s: page %d (a power of two, 32..65536), n_pages %d, pages %d (x page <= 2^26)", who, c.page,
                       c.n_pages, c.pages);
+    if ((int64_t)c.n_pages * g.n_kv_heads > INT32_MAX / (c.page / 32))  // blocks have 32-bit numbers
+        return refuse(m, QWATTN_EINVAL, "%s: pools of %d pages of %d positions (pages x KV heads x page / 32 < 2^31)", who, c.n_pages, c.page);
     if (!c.k || !c.v || !c.table) return refuse(m, QWATTN_EINVAL, "%s: null pointer of the cache", who);
     if (c.table_stride < c.pages || c.table_stride > (int64_t(1) << 40))
         return refuse(m, QWATTN_EINVAL, "%s: table_stride %lld (>= pages)", who, (long long)c.table_stride);

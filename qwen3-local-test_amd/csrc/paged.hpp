@@ -8,10 +8,14 @@ namespace qw {
 // The sequence's new tokens: min(max(lens[b], 0), n)
 __device__ __forceinline__ int seq_len(const int32_t* lens, int b, int n) { return lens ? min(max(lens[b], 0), n) : n; }
 
-// Element offset, in either pool, of the block of KV head h that holds position p of a sequence, on page `page`.
-__device__ __forceinline__ int64_t paged_block(const PagedCache& c, int page, int p, int h, int nkv, int D) {
+// Number, in either pool, of the block of KV head h that holds position p of a sequence, on page `page` (a pool has less
+// than 2^31 blocks), and the elements before it.
+__device__ __forceinline__ int paged_number(const PagedCache& c, int page, int p, int h, int nkv) {
     const int in_page = p & ((1 << c.lg_page) - 1);
-    return (((int64_t)page * nkv + h) * (1 << (c.lg_page - 5)) + (in_page >> 5)) * (int64_t)(kBlk * D);
+    return (page * nkv + h) * (1 << (c.lg_page - 5)) + (in_page >> 5);
+}
+__device__ __forceinline__ int64_t paged_block(const PagedCache& c, int page, int p, int h, int nkv, int D) {
+    return (int64_t)paged_number(c, page, p, h, nkv) * (kBlk * D);
 }
 
 // A sequence's first position, within +-2^28 (what lies further out is outside every table, as a position of 2^28 is), so
@@ -40,7 +44,7 @@ __device__ __forceinline__ KeyTiles key_tiles(const PagedAttendArgs& a, int pos,
 // What a token at position p sees: keys [from, end) and [0, sinks) below end
 struct Sight {
     int from, end;
-    __device__ __forceinline__ bool sees(int j, int sinks) const { return j < end && (j >= from || j < sinks); }
+    __device__ __forceinline__ bool sees(int j, int sinks) const { return (j < end) & ((j >= from) | (j < sinks)); }
 };
 __device__ __forceinline__ Sight sight(const PagedAttendArgs& a, int p) {
     return {p - a.window + 1, p >= 0 && p < a.limit ? p + 1 : 0};
@@ -62,8 +66,10 @@ __device__ __forceinline__ bool sees_whole(const Sight& s, int k0, int k1, int s
 // 8 bits of bf16 rows whole. The scores' factor takes the power back. Keys and values are fp16 themselves, so a score
 // is exact but for that and the fp32 sums.
 __device__ __forceinline__ int query_shift(float largest) {
-    return largest > 0.f && largest < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(largest) : 0;
+    return largest > 0.f && largest < __builtin_inff() ? min(max(15 - __builtin_amdgcn_frexp_expf(largest), -126), 126) : 0;
 }
+// 2^sh, |sh| <= 126
+__device__ __forceinline__ float power_of_two(int sh) { return __uint_as_float((uint32_t)(127 + sh) << 23); }
 
 // Weights are taken as 2^(score - maximum + kShift): with the lazy maximum (a weight may pass it by 2^kTau) they stay
 // below fp16's largest, and the smallest are kept to 2^-24 of 2^kShift.
@@ -77,22 +83,29 @@ __device__ __forceinline__ void weight_parts(float w0, float w1, f16x2& hi, f16x
 }
 
 // ---- output rows -----------------------------------------------------------------------------------------------
-// Four outputs of one row and head: o * inv, times sigmoid(gate), rounded once
+// Four outputs of one row and head at dim d: o * inv, times sigmoid(gate), rounded once. The gates are loaded apart, so that
+// many loads are in flight.
 template <int DT>
-__device__ __forceinline__ void store_out4(const PagedAttendArgs& a, size_t row, int h, int D, int d, f32x4 o, float inv) {
-    o *= inv;
-    if (a.gate) {
-        float g[4];
-        if constexpr (DT == 0) {
-            load_vec<0, 4>(a.gate, row * a.gate_stride + (size_t)h * a.gate_head + d, g);
-        } else {
-            const u32x2 v = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.gate) + row * a.gate_stride + (size_t)h * a.gate_head + d);
-            g[0] = __uint_as_float(v[0] << 16), g[1] = __uint_as_float(v[0] & 0xffff0000u);
-            g[2] = __uint_as_float(v[1] << 16), g[3] = __uint_as_float(v[1] & 0xffff0000u);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] *= sigmoid(g[i]);
+struct Gate4 {
+    typename std::conditional<DT == 0, f32x4, u32x2>::type v;
+    __device__ __forceinline__ void none() {  // sigmoid(inf) is 1
+        if constexpr (DT == 0) v = f32x4{1, 1, 1, 1} * __builtin_inff();
+        else v = u32x2{0x7f807f80u, 0x7f807f80u};
     }
+    __device__ __forceinline__ void load(const PagedAttendArgs& a, size_t row, int h, int d) {
+        const size_t at = row * a.gate_stride + (size_t)h * a.gate_head + d;
+        if constexpr (DT == 0) v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.gate) + at);
+        else v = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.gate) + at);
+    }
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (DT == 0) return v[i];
+        else return __uint_as_float((i & 1) ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16);
+    }
+};
+template <int DT>
+__device__ __forceinline__ void store_out4(const PagedAttendArgs& a, size_t row, int h, int D, int d, f32x4 o, float inv, const Gate4<DT>& g) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] *= inv * sigmoid(g.at(i));
     const size_t at = row * a.out_stride + (size_t)h * D + d;
     if constexpr (DT == 0) *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = o;
     else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at) = u32x2{pk_bf16(o[0], o[1]), pk_bf16(o[2], o[3])};

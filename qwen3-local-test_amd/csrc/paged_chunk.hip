@@ -22,8 +22,9 @@ constexpr int ch_nt(int D, bool bf16) { return D == 256 && !bf16 ? 1 : 2; }
 struct ChPlan {
     float* part;    // [2 * groups][waves][PART]
     int4* start;    // [groups]: KV head (-1: nothing to do), sequence, query tile, first key tile
-    int* cnt;       // [groups][waves] arrivals at the item that is the workgroup's last
-    int64_t* head;  // key tiles a KV head, key tiles a workgroup
+    int* cnt;       // [groups][waves][2] arrivals at the 16-row tiles of the item that is the workgroup's last
+    int64_t* head;  // key tiles a KV head
+    int64_t* unit;  // [groups + 1]: the workgroups' first units
     int64_t* first; // joined calls: first key tile of each (sequence, query tile)
 };
 constexpr int kJoinItems = 1024;  // most (sequence, query tile) pairs of a joined call
@@ -32,16 +33,34 @@ __host__ __device__ inline ChPlan ch_plan(void* ws, int groups, int part_floats)
     p.part = static_cast<float*>(ws);
     p.start = reinterpret_cast<int4*>(p.part + (size_t)2 * groups * kChWaves * part_floats);
     p.cnt = reinterpret_cast<int*>(p.start + groups);
-    p.head = reinterpret_cast<int64_t*>(p.cnt + groups * kChWaves);
-    p.first = p.head + 2;
+    p.head = reinterpret_cast<int64_t*>(p.cnt + groups * kChWaves * 2);
+    p.unit = p.head + 2;
+    p.first = p.unit + groups + 1;
     return p;
 }
+// The workgroup whose run holds unit u
+__device__ __forceinline__ int group_of(const ChPlan& plan, int64_t u, int groups) {
+    int lo = 0, hi = groups;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (plan.unit[mid] <= u) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
 
-// Items are (KV head, sequence, query tile) in this order, each of as many units as it has key tiles; every workgroup of
-// the chunk kernel takes an equal run of units. One workgroup: a thread sums a run of (sequence, query tile) pairs, a
-// scan places the runs, and the threads write the starts that fall into theirs.
+// Items are (KV head, sequence, query tile) in this order, each of as many units as it has key tiles. Every workgroup of
+// the chunk kernel takes a run of units, in one of two ways (a segment, what a workgroup takes of an item, costs some three to
+// four units beside its own: the rows, the first copies, the partial and its joining):
+//  - items in equal parts of at most `run` units, a workgroup a part, for the least run whose parts fit the workgroups;
+//  - equal runs over all items, their ends moved by up to a twelfth to an item's edge where one is that near: where there are more
+//    items than workgroups, or where the first way's run is more than kSegment units longer.
+// One workgroup: a thread sums a run of (sequence, query tile) pairs, a scan places the runs, and the threads write the starts
+// that fall into theirs.
+constexpr int kSegment = 3, kPartPairs = 1024;  // (pairs whose tiles the first way holds in LDS)
 __global__ __launch_bounds__(1024) void k_paged_plan(PagedAttendArgs a, void* ws, int groups, int part_floats, int tok, bool joined) {
     __shared__ int64_t sums[16];
+    __shared__ int most[16], count[kPartPairs], fits[16];
     const ChPlan plan = ch_plan(ws, groups, part_floats);
     const int nqt = (a.n + tok - 1) / tok, pairs = a.n_seq * nqt;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -50,24 +69,77 @@ __global__ __launch_bounds__(1024) void k_paged_plan(PagedAttendArgs a, void* ws
         const int b = pair / nqt, t0 = (pair - b * nqt) * tok;
         return key_tiles<6>(a, seq_pos(a.pos, b), t0, min(t0 + tok, seq_len(a.lens, b, a.n))).count;
     };
-    int64_t mine = 0;
-    for (int i = 0; i < per; i++)
-        if (tid * per + i < pairs) mine += tiles(tid * per + i);
-    int64_t incl = mine;
+    // the sum of x over the threads before this one; `total` over all
+    auto scan = [&](int64_t x, int64_t& total) {
+        int64_t incl = x;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const int64_t o = __shfl_up((long long)incl, m, 64);
-        if (lane >= m) incl += o;
+        for (int m = 1; m < 64; m <<= 1) {
+            const int64_t o = __shfl_up((long long)incl, m, 64);
+            if (lane >= m) incl += o;
+        }
+        __syncthreads();
+        if (lane == 63) sums[wave] = incl;
+        __syncthreads();
+        int64_t before = incl - x;
+        total = 0;
+        for (int w = 0; w < 16; w++) before += w < wave ? sums[w] : 0, total += sums[w];
+        return before;
+    };
+    int64_t mine = 0;
+    int top = 0;
+    for (int i = 0; i < per; i++) {
+        const int pair = tid * per + i, c = pair < pairs ? tiles(pair) : 0;
+        mine += c, top = max(top, c);
+        if (per == 1) count[tid] = c;
     }
-    if (lane == 63) sums[wave] = incl;
-    for (int i = tid; i < groups * kChWaves; i += 1024) plan.cnt[i] = 0;
-    __syncthreads();
-    int64_t x = incl - mine, total = 0;
-    for (int w = 0; w < 16; w++) x += w < wave ? sums[w] : 0, total += sums[w];
+    for (int i = tid; i < groups * kChWaves * 2; i += 1024) plan.cnt[i] = 0;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) top = max(top, __shfl_xor(top, m, 64));
+    if (lane == 0) most[wave] = top;
+    int64_t total;
+    int64_t x = scan(mine, total);
+    for (int w = 0; w < 16; w++) top = max(top, most[w]);
     const int64_t all = total * a.NKV, run = max((int64_t)1, (all + groups - 1) / groups);
+    if (tid == 0) plan.head[0] = total, plan.unit[groups] = all;
+
+    // (an item has at most 2^20 key tiles, so that a run of 2^20 and more is never better than whole items)
+    int lo = (int)min(run, (int64_t)1 << 20), hi = max(top, lo);  // the first way's run lies in [lo, hi], if whole items fit
+    if ((int64_t)pairs * a.NKV <= groups && per == 1) {
+        while (lo < hi) {  // sixteen runs at a time, a wave each
+            const int step = (hi - lo + 15) / 16, r = min(hi, lo + step * wave);
+            int parts = 0;
+            for (int i = lane; i < pairs; i += 64) parts += (int)((unsigned)(count[i] + r - 1) / (unsigned)r);
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) parts += __shfl_xor(parts, m, 64);
+            __syncthreads();
+            if (lane == 0) fits[wave] = parts * a.NKV <= groups;
+            __syncthreads();
+            int w = 0;
+            while (w < 16 && !fits[w]) w++;
+            const int was = lo;
+            if (w == 0) break;
+            lo = min(hi, was + step * (w - 1) + 1);
+            if (w < 16) hi = min(hi, was + step * w);
+        }
+        const int part = lo;
+        if (part <= run + kSegment) {
+            const int c = tid < pairs ? count[tid] : 0, k = (int)((unsigned)(c + part - 1) / (unsigned)part);
+            int64_t all_parts;
+            const int64_t at = scan(k, all_parts);
+            if (joined && tid < pairs) plan.first[tid] = x;
+            for (int h = 0; h < a.NKV; h++)
+                for (int j = 0; j < k; j++) {
+                    const int w = h * (int)all_parts + (int)at + j, off = (int)((unsigned)c * (unsigned)j / (unsigned)k);  // (c j < 2^28)
+                    plan.start[w] = int4{h, tid / nqt, tid % nqt, off}, plan.unit[w] = h * total + x + off;
+                }
+            for (int w = tid; w < groups; w += 1024)
+                if (w >= all_parts * a.NKV) plan.start[w].x = -1, plan.unit[w] = all;
+            return;
+        }
+    }
     for (int w = tid; w < groups; w += 1024)
-        if (w * run >= all) plan.start[w].x = -1;
-    if (tid == 0) plan.head[0] = total, plan.head[1] = run;
+        if (w * run >= all) plan.start[w].x = -1, plan.unit[w] = all;
+    const int near = (int)min(run / 12, (int64_t)1 << 20);
     for (int i = 0; i < per; i++) {
         const int pair = tid * per + i;
         if (pair >= pairs) break;
@@ -75,8 +147,12 @@ __global__ __launch_bounds__(1024) void k_paged_plan(PagedAttendArgs a, void* ws
         if (joined) plan.first[pair] = x;
         for (int h = 0; h < a.NKV && c; h++) {
             const int64_t g0 = h * total + x;
-            for (int64_t w = (g0 + run - 1) / run; w * run < g0 + c; w++)
-                plan.start[w] = int4{h, pair / nqt, pair % nqt, (int)(w * run - g0)};
+            for (int64_t w = (g0 + run - 1) / run; w * run < g0 + c; w++) {
+                int off = (int)(w * run - g0);
+                if (off <= near) off = 0;
+                else if (c - off <= near) off = c;  // the item after this
+                plan.start[w] = int4{h, pair / nqt, pair % nqt, off}, plan.unit[w] = g0 + off;
+            }
         }
         x += c;
     }
@@ -112,9 +188,8 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     f16* sk = reinterpret_cast<f16*>(smem);  // blocks of keys
     f16* sv = sk + kChRing * BLKE;           // and of values
-    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int G = a.NH / a.NKV, tok = C::ROWS / G, groups = gridDim.x;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int lgG = __builtin_ctz(a.NH / a.NKV), G = 1 << lgG, tok = C::ROWS >> lgG, groups = gridDim.x;
     const ChPlan plan = ch_plan(ws, groups, C::PART);
     // neighbouring runs on one XCD: they read the same keys
     const int wg = (blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);
@@ -122,9 +197,8 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
     int h = __builtin_amdgcn_readfirstlane(st.x), b = __builtin_amdgcn_readfirstlane(st.y);
     int qt = __builtin_amdgcn_readfirstlane(st.z), off = __builtin_amdgcn_readfirstlane(st.w);
     if (h < 0) return;
-    const int64_t total = plan.head[0], run = plan.head[1], all = total * a.NKV;
-    int64_t at = wg * run;  // unit of the segment at hand
-    const int64_t stop = min(at + run, all);
+    const int64_t stop = plan.unit[wg + 1];
+    int64_t at = plan.unit[wg];  // unit of the segment at hand
 
     while (at < stop) {
         const int pos = seq_pos(a.pos, b), len = seq_len(a.lens, b, a.n);
@@ -145,25 +219,8 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
         const int n = 2 * (hi - lo);  // blocks of 32 keys, block i of the segment in ring place i % 4
         auto key_of = [&](int i) { return kt.tile(lo + (i >> 1)) * 64 + (i & 1) * kBlk; };
 
-        // ---- the wave's rows as they lie in memory: row r of the tile is token t0 + r / G, head h G + r % G ----
-        typedef typename std::conditional<DT == 0, f32x4, u32x4>::type raw_t;
-        constexpr int RAW = DT == 0 ? 2 : 1;
-        raw_t raw[NT][NKS][RAW];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const int r = (wave * NT + nt) * 16 + col, t = min(t0 + r / G, t1 - 1);
-            const size_t base = ((size_t)b * a.n + t) * a.q_stride + (size_t)(h * G + r % G) * a.q_head + 8 * g;
-#pragma unroll
-            for (int kk = 0; kk < NKS; kk++)
-#pragma unroll
-                for (int k = 0; k < RAW; k++) {
-                    if constexpr (DT == 0) raw[nt][kk][k] = *reinterpret_cast<const raw_t*>(static_cast<const float*>(a.q) + base + 32 * kk + 4 * k);
-                    else raw[nt][kk][k] = *reinterpret_cast<const raw_t*>(static_cast<const uint16_t*>(a.q) + base + 32 * kk);
-                }
-        }
-
         // positions of the wave's tokens, the keys that all of them see, that some of them see, and that some of the item's do
-        const int w0 = pos + t0 + wave * 16 * NT / G, w1 = min(pos + t0 + (wave * 16 * NT + 16 * NT - 1) / G, pos + t1 - 1);
+        const int w0 = pos + t0 + (wave * 16 * NT >> lgG), w1 = min(pos + t0 + ((wave * 16 * NT + 16 * NT - 1) >> lgG), pos + t1 - 1);
         const Sight all_see = sight_of_all(a, w0, w1), some_see = sight_of_some(a, w0, w1);
         const Sight item_see = sight_of_some(a, pos + t0, pos + t1 - 1);
 
@@ -171,7 +228,7 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
         // arithmetic in every step (page, offset, masks: some 150 instructions) took as long as its matrix instructions ----
         const int32_t* table = a.c.table + (size_t)b * a.c.table_stride;
         int base = 0;
-        int64_t offset = -1;   // lane l: byte offset of block base + l in a pool, -1 without a page or past the last block
+        int number = -1;       // lane l: number of block base + l in a pool, -1 without a page or past the last block
         int first_key = 0;     // its first position
         uint64_t paged, whole, stale;  // bit l: it has a page; all rows of the wave see all of it; it has keys that no row of the item sees
         auto survey = [&](int i) __attribute__((always_inline)) {
@@ -181,36 +238,51 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
             first_key = key_of(min(i + l, n - 1));
             const int page = in && first_key < a.limit ? table[first_key >> a.c.lg_page] : -1;
             const bool there = (uint32_t)page < (uint32_t)a.c.n_pages;
-            offset = there ? 2 * paged_block(a.c, page, first_key, h, a.NKV, D) : -1;
+            number = there ? paged_number(a.c, page, first_key, h, a.NKV) : -1;
             paged = __builtin_amdgcn_ballot_w64(there);
             whole = __builtin_amdgcn_ballot_w64(there && sees_whole(all_see, first_key, first_key + kBlk, a.sinks));
             stale = __builtin_amdgcn_ballot_w64(in && !sees_whole(item_see, first_key, first_key + kBlk, a.sinks));
         };
         auto key_at = [&](int i) { return __builtin_amdgcn_readlane(first_key, i - base); };
-        // this wave's share of block i of `pool` into ring place i % 4 (zeros without a page): pieces from `first` on
-        auto copy = [&](int i, uint16_t* pool, f16* ring, int first, auto count) __attribute__((always_inline)) {
-            const uint32_t lo32 = (uint32_t)__builtin_amdgcn_readlane((int)offset, i - base);
-            const int hi32 = __builtin_amdgcn_readlane((int)(offset >> 32), i - base);
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-                reinterpret_cast<char*>(pool) + (((int64_t)(hi32 < 0 ? 0 : hi32) << 32) | lo32), (short)0, hi32 < 0 ? 0 : BLKE * 2, 0x00020000);
-            f16* dst = ring + (i & (kChRing - 1)) * BLKE;
+        // This wave's share of the copies of keys of block i + 1 (zeros without a page) into ring place (i + 1) % 4 and of values of block i
+        // into place i % 4, a kilobyte a piece (at 64 dims four waves copy keys and the others values)
+        constexpr int PIECES = D >= 128 ? D / 128 : 1;
+        auto copy = [&](bool keys, int of) __attribute__((always_inline)) {
+            if (D < 128 && keys != (wave < 4)) return;
+            const int blk = __builtin_amdgcn_readlane(number, of - base), at = D >= 128 ? wave * PIECES : wave & 3;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((keys ? a.c.k : a.c.v) + (int64_t)max(blk, 0) * BLKE, (short)0,
+                                                                               blk < 0 ? 0 : BLKE * 2, 0x00020000);
+            f16* to = (keys ? sk : sv) + (of & (kChRing - 1)) * BLKE + at * 512;
             const int l16 = lane_here() * 16;
 #pragma unroll
-            for (int j = 0; j < decltype(count)::value; j++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (first + j) * 512), 16,
-                                                         (first + j) * 1024 + l16, 0, 0, 0);
-        };
-        auto stage = [&](bool keys, int i) __attribute__((always_inline)) {
-            if constexpr (D >= 128) {
-                constexpr int P = D / 128;
-                copy(i, keys ? a.c.k : a.c.v, keys ? sk : sv, wave * P, std::integral_constant<int, P>{});
-            } else {  // the first four waves copy keys and the others values
-                if (keys == (wave < 4)) copy(i, keys ? a.c.k : a.c.v, keys ? sk : sv, wave & 3, std::integral_constant<int, 1>{});
-            }
+            for (int k = 0; k < PIECES; k++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + k * 512), 16, l16 + (at + k) * 1024, 0, 0, 0);
         };
         survey(0);
-        __syncthreads();  // the last segment's readers of the rings are done
-        stage(true, 0), stage(true, 1), stage(false, 0);
+
+        // ---- the wave's rows as they lie in memory: row r of the tile is token t0 + (r >> lgG), head h G + (r & (G - 1)) ----
+        typedef typename std::conditional<DT == 0, f32x4, u32x4>::type raw_t;
+        constexpr int RAW = DT == 0 ? 2 : 1;
+        raw_t raw[NT][NKS][RAW];
+        {
+            const int lane = lane_here(), col = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int r = (wave * NT + nt) * 16 + col, t = min(t0 + (r >> lgG), t1 - 1);
+            const size_t base = ((size_t)b * a.n + t) * a.q_stride + (size_t)(h * G + (r & (G - 1))) * a.q_head + 8 * g;
+#pragma unroll
+            for (int kk = 0; kk < NKS; kk++)
+#pragma unroll
+                for (int k = 0; k < RAW; k++) {
+                    if constexpr (DT == 0) raw[nt][kk][k] = *reinterpret_cast<const raw_t*>(static_cast<const float*>(a.q) + base + 32 * kk + 4 * k);
+                    else raw[nt][kk][k] = *reinterpret_cast<const raw_t*>(static_cast<const uint16_t*>(a.q) + base + 32 * kk);
+                }
+        }
+        }
+
+        // (their loads and the pages' are on their way) the last segment's readers of the rings are done
+        phase();
+        copy(true, 0), copy(true, 1), copy(false, 0);
 
         // ---- the rows' operands ----
         f16x8 q[NT][PARTS][NKS];
@@ -226,14 +298,16 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
 #pragma unroll
             for (int kk = 0; kk < NKS; kk++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) largest = fmaxf(largest, fabsf(at_raw(kk, j)));
+                for (int j = 0; j < 8; j += 2)  // (in assembly: without the compiler's canonical operands)
+                    asm("v_max3_f32 %0, |%1|, |%2|, %0" : "+v"(largest) : "v"(at_raw(kk, j)), "v"(at_raw(kk, j + 1)));
             const int sh = query_shift(max_rows(largest));
-            fac[nt] = __builtin_ldexpf(a.scale, -sh);
+            const float up = power_of_two(sh);
+            fac[nt] = a.scale * power_of_two(-sh);
 #pragma unroll
             for (int kk = 0; kk < NKS; kk++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float y = __builtin_ldexpf(at_raw(kk, j), sh);
+                    const float y = at_raw(kk, j) * up;
                     q[nt][0][kk][j] = (f16)y;
                     if constexpr (PARTS == 2) q[nt][1][kk][j] = (f16)(y - (float)q[nt][0][kk][j]);
                 }
@@ -243,83 +317,217 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
         }
         auto unseen = [&](int k0) { return k0 >= some_see.end || (k0 + kBlk <= some_see.from && k0 >= a.sinks); };
         auto row_sight = [&](int nt, int l) {
-            const int r = (wave * NT + nt) * 16 + (l & 15), t = t0 + r / G;
-            return r < tok * G && t < t1 ? sight(a, pos + t) : Sight{0, 0};
+            const int r = (wave * NT + nt) * 16 + (l & 15), t = t0 + (r >> lgG);
+            return t < t1 ? sight(a, pos + t) : Sight{0, 0};
         };
 
         f32x4 s[NT][2];        // scores of a block: value i of key set s of lane (col, g) is key 8 g + 4 s + i
         f16x8 w[NT][PARTS];    // its weights: keys 8 g .. 8 g + 7
-        // Matrix instructions of a phase: the scores of one block and (VALUES) the weighted values of the block before, a fragment of
-        // each in turn, read AHEAD of its use
-        constexpr int AHEAD = NT == 2 && D == 256 ? 3 : 5;
-        auto products = [&](auto values, auto&& kfrag, auto&& vfrag) __attribute__((always_inline)) {
-            constexpr bool VALUES = decltype(values)::value;
-            constexpr int STEP = VALUES ? 2 : 1, SLOTS = STEP * NDT;
+        // Matrix instructions of a phase: the weighted values of one block, then the scores of the next, their fragments read AHEAD of
+        // their use (one after the other: scores and weights are then not live together, which leaves registers for fragments)
+        constexpr int AHEAD = 5;
+        auto products = [&](auto&& kfrag, auto&& vfrag) __attribute__((always_inline)) {
             f16x8 fr[AHEAD + 1];
             auto read = [&](auto ic) __attribute__((always_inline)) {
                 constexpr int i = decltype(ic)::value;
-                if constexpr (VALUES && i % STEP == 0) fr[i % (AHEAD + 1)] = vfrag(i / STEP);
-                else fr[i % (AHEAD + 1)] = kfrag(i / STEP);
+                fr[i % (AHEAD + 1)] = i < NDT ? vfrag(i) : kfrag(i - NDT);
             };
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) s[nt][0] = f32x4{}, s[nt][1] = f32x4{};
             static_for<0, AHEAD>(read);
-            static_for<0, SLOTS>([&](auto ic) __attribute__((always_inline)) {
-                constexpr int i = decltype(ic)::value, f = i / STEP;
-                if constexpr (i + AHEAD < SLOTS) read(std::integral_constant<int, i + AHEAD>{});
+            static_for<0, 2 * NDT>([&](auto ic) __attribute__((always_inline)) {
+                constexpr int i = decltype(ic)::value, f = i % NDT;
+                if constexpr (i + AHEAD < 2 * NDT) read(std::integral_constant<int, i + AHEAD>{});
 #pragma unroll
                 for (int part = 0; part < PARTS; part++)
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        if constexpr (VALUES && i % STEP == 0) acc[nt][f] = mfma16(fr[i % (AHEAD + 1)], w[nt][part], acc[nt][f]);
-                        else s[nt][f & 1] = mfma16(fr[i % (AHEAD + 1)], q[nt][part][f >> 1], s[nt][f & 1]);
+                        if constexpr (i < NDT) acc[nt][f] = mfma16(fr[i % (AHEAD + 1)], w[nt][part], acc[nt][f]);
+                        else s[nt][f & 1] = mfma16(fr[i % (AHEAD + 1)], q[nt][part][f >> 1], f < 2 && part == 0 ? f32x4{} : s[nt][f & 1]);
                     }
                 __builtin_amdgcn_sched_barrier(0);  // keep the reads ahead
             });
+            asm volatile("s_nop 15\n\ts_nop 3");  // the last scores are out before assembly reads them
         };
-        // Weights of a block from its scores; the running maximum moves only where a row's passes it by more than kTau
-        auto softmax = [&](int k0, bool there, bool all) __attribute__((always_inline)) {
-            if (!all) {
-                const int l = lane_here(), key = k0 + 8 * (l >> 4);
+        // Scores that the rows of 16-row tile nt do not see, of the block at key k0
+        auto hide = [&](f32x4 (&x)[2], int nt, int k0, bool there) __attribute__((always_inline)) {
+            const int l = lane_here(), key = k0 + 8 * (l >> 4);
+            const Sight see = row_sight(nt, l);
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const Sight see = row_sight(nt, l);
+            for (int i = 0; i < 8; i++) x[i >> 2][i & 3] = there && see.sees(key + i, a.sinks) ? x[i >> 2][i & 3] : kNegInf;
+        };
+        // (the maxima in assembly: the compiler would make every operand canonical first, which doubles them. The scores are those of
+        // an earlier phase, or of products() behind its own wait)
+        auto max3 = [](float x, float y, float z) __attribute__((always_inline)) {
+            float r;
+            asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+            return r;
+        };
+        auto largest = [&](const f32x4 (&x)[2]) __attribute__((always_inline)) {
+            float r = max3(max3(x[0][0], x[0][1], x[0][2]), max3(x[0][3], x[1][0], x[1][1]), max3(x[1][2], x[1][3], x[1][3]));
+            const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(r), __float_as_uint(r), false, false);
+            r = max3(__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[1]));
+            const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(r), __float_as_uint(r), false, false);
+            return max3(__uint_as_float(z[0]), __uint_as_float(z[1]), __uint_as_float(z[1]));
+        };
+        // The running maximum moves only where a row's passes it by more than kTau (at first from -inf); the factor of what was
+        // summed before
+        auto raise = [&](float mx, float& m, float& l) __attribute__((always_inline)) {
+            const float to = mx > m + kTau ? mx : m, corr = to == kNegInf ? 1.f : exp2_fast(m - to);
+            m = to, l *= corr;
+            return corr;
+        };
+        auto weigh = [&](const f32x4 (&x)[2], float f, float m, float& l, f16x8 (&wt)[PARTS]) __attribute__((always_inline)) {
+            const float o = m == kNegInf ? 0.f : kShift - m;
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        s[nt][i >> 2][i & 3] = there && see.sees(key + i, a.sinks) ? s[nt][i >> 2][i & 3] : kNegInf;
-                }
+            for (int i = 0; i < 8; i += 2) {
+                const float x0 = exp2_fast(__builtin_fmaf(x[i >> 2][i & 3], f, o)), x1 = exp2_fast(__builtin_fmaf(x[i >> 2][(i & 3) + 1], f, o));
+                f16x2 hi16, lo16;
+                weight_parts<PARTS>(x0, x1, hi16, lo16);
+                wt[0][i] = hi16[0], wt[0][i + 1] = hi16[1];
+                if constexpr (PARTS == 2) wt[1][i] = lo16[0], wt[1][i + 1] = lo16[1], l += x0 + x1;
+                else l = __builtin_amdgcn_fdot2(hi16, f16x2{(f16)1.f, (f16)1.f}, l, false);
             }
+        };
+        // Weights of a block from its scores, the copies of step `step` between: a piece takes the memory path 16 cycles, and one behind
+        // the other they would hold the wave up
+        auto softmax = [&](int k0, bool there, bool all, int step) __attribute__((always_inline)) {
+            copy(true, step + 1);
+            if (!all) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) hide(s[nt], nt, k0, there);
+            }
+            float mx[NT];
+            uint64_t grow = 0;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                float mx = fmaxf(fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3])),
-                                 fmaxf(fmaxf(s[nt][1][0], s[nt][1][1]), fmaxf(s[nt][1][2], s[nt][1][3])));
-                mx = max_rows(mx) * fac[nt];
-                const bool grow = m_run[nt] == kNegInf ? mx != kNegInf : mx > m_run[nt] + kTau;
-                if (__builtin_amdgcn_ballot_w64(grow)) {
-                    const float to = grow ? mx : m_run[nt];
-                    const float corr = to == kNegInf ? 1.f : exp2_fast(m_run[nt] - to);
-                    m_run[nt] = to, l_run[nt] *= corr;
+                mx[nt] = largest(s[nt]) * fac[nt];
+                grow |= __builtin_amdgcn_ballot_w64(mx[nt] > m_run[nt] + kTau);
+            }
+            if (grow) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const float corr = raise(mx[nt], m_run[nt], l_run[nt]);
 #pragma unroll
                     for (int dt = 0; dt < NDT; dt++) acc[nt][dt] *= corr;
                 }
-                const float o = m_run[nt] == kNegInf ? 0.f : kShift - m_run[nt];
+            }
+            copy(false, step);
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float x0 = exp2_fast(__builtin_fmaf(s[nt][i >> 2][i & 3], fac[nt], o));
-                    const float x1 = exp2_fast(__builtin_fmaf(s[nt][i >> 2][(i & 3) + 1], fac[nt], o));
-                    f16x2 hi16, lo16;
-                    weight_parts<PARTS>(x0, x1, hi16, lo16);
-                    w[nt][0][i] = hi16[0], w[nt][0][i + 1] = hi16[1];
-                    if constexpr (PARTS == 2) w[nt][1][i] = lo16[0], w[nt][1][i + 1] = lo16[1], l_run[nt] += x0 + x1;
-                    else l_run[nt] = __builtin_amdgcn_fdot2(hi16, f16x2{(f16)1.f, (f16)1.f}, l_run[nt], false);
+            for (int nt = 0; nt < NT; nt++) weigh(s[nt], fac[nt], m_run[nt], l_run[nt], w[nt]);
+        };
+        // Rows of 16-row tile nt whose unnormalized outputs lie in `mine`: an item of one part to the output, parts to the workspace,
+        // where the wave that arrives last joins them, from the first to the last whichever it is. Loads go out together: their
+        // latency, not their bytes, is what this takes.
+        auto write_rows = [&](int nt, const f32x4* mine, auto&& region, int parts, int own) __attribute__((always_inline)) {
+            const int lane = lane_here(), col = lane & 15, g = lane >> 4;
+            const int r = (wave * NT + nt) * 16 + col, t = t0 + (r >> lgG);
+            const bool ok = t < t1;
+            const size_t row = (size_t)b * a.n + (ok ? t : t0);
+            const int head = h * G + (r & (G - 1));
+            Gate4<DT> gate[NDT];
+            auto load_gates = [&]() __attribute__((always_inline)) {
+                if (a.gate) {
+#pragma unroll
+                    for (int dt = 0; dt < NDT; dt++) gate[dt].load(a, row, head, 16 * dt + 4 * g);
+                } else {
+#pragma unroll
+                    for (int dt = 0; dt < NDT; dt++) gate[dt].none();
                 }
+            };
+            const auto xs = __builtin_amdgcn_permlane16_swap(__float_as_uint(l_run[nt]), __float_as_uint(l_run[nt]), false, false);
+            float l = __uint_as_float(xs[0]) + __uint_as_float(xs[1]);
+            const auto ys = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+            l = __uint_as_float(ys[0]) + __uint_as_float(ys[1]);
+            const float m = m_run[nt];
+            if (parts == 1) {
+                load_gates();
+                if (ok) {
+                    const float inv = inverse_sum(l);
+#pragma unroll
+                    for (int dt = 0; dt < NDT; dt++) store_out4<DT>(a, row, head, D, 16 * dt + 4 * g, mine[dt * 64], inv, gate[dt]);
+                }
+                return;
+            }
+            int* arrived = plan.cnt + ((wg - own) * kChWaves + wave) * 2 + nt;
+            // (the last to arrive need not store its own part)
+            if (joined || __builtin_amdgcn_readfirstlane(__hip_atomic_load(arrived, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) < parts - 1) {
+                const __amdgpu_buffer_rsrc_t rp = region(own);
+#pragma unroll
+                for (int dt = 0; dt < NDT; dt++)
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, mine[dt * 64]), rp, ((nt * NDT + dt) * 64 + lane) * 16, 0, kScDevice);
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{m, l}), rp, NT * NDT * 1024 + (nt * 64 + lane) * 8, 0, kScDevice);
+                if (joined) return;
+                __builtin_amdgcn_s_waitcnt(0x0F70);  // the partial is out before it is counted
+                int old = 0;
+                if (lane == 0) old = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (__builtin_amdgcn_readfirstlane(old) < parts - 1) return;
+            }
+            asm volatile("" ::: "memory");
+            load_gates();
+            auto sums = [&](const __amdgpu_buffer_rsrc_t& rq) __attribute__((always_inline)) {
+                return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rq, NT * NDT * 1024 + (nt * 64 + lane) * 8, 0, kScDevice));
+            };
+            auto values = [&](const __amdgpu_buffer_rsrc_t& rq, int dt) __attribute__((always_inline)) {
+                return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rq, ((nt * NDT + dt) * 64 + lane) * 16, 0, kScDevice));
+            };
+            f32x4 o[NDT];
+            if (parts == 2) {  // x cx + y cy, x the first part's
+                const __amdgpu_buffer_rsrc_t rq = region(1 - own);
+                const f32x2 ml = sums(rq);
+#pragma unroll
+                for (int dt = 0; dt < NDT; dt++) o[dt] = values(rq, dt);
+                const float to = fmaxf(m, ml[0]);
+                const float cm = m == kNegInf ? 0.f : exp2_fast(m - to), co = ml[0] == kNegInf ? 0.f : exp2_fast(ml[0] - to);
+                const float cx = own ? co : cm, cy = own ? cm : co;
+                const float inv = inverse_sum(__builtin_fmaf(own ? l : ml[1], cy, (own ? ml[1] : l) * cx));
+                if (ok) {
+#pragma unroll
+                    for (int dt = 0; dt < NDT; dt++) {
+                        const f32x4 me = mine[dt * 64];
+                        f32x4 v;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) v[i] = __builtin_fmaf(own ? me[i] : o[dt][i], cy, (own ? o[dt][i] : me[i]) * cx);
+                        store_out4<DT>(a, row, head, D, 16 * dt + 4 * g, v, inv, gate[dt]);
+                    }
+                }
+                return;
+            }
+            float rm = kNegInf, rl = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < NDT; dt++) o[dt] = f32x4{};
+#pragma unroll 1
+            for (int part = 0; part < parts; part++) {
+                f32x2 ml = f32x2{m, l};
+                f32x4 v[NDT];
+                if (part == own) {
+#pragma unroll
+                    for (int dt = 0; dt < NDT; dt++) v[dt] = mine[dt * 64];
+                } else {
+                    const __amdgpu_buffer_rsrc_t rq = region(part);
+                    ml = sums(rq);
+#pragma unroll
+                    for (int dt = 0; dt < NDT; dt++) v[dt] = values(rq, dt);
+                }
+                const float to = fmaxf(rm, ml[0]);
+                const float cx = rm == kNegInf ? 0.f : exp2_fast(rm - to), cy = ml[0] == kNegInf ? 0.f : exp2_fast(ml[0] - to);
+                rm = to, rl = __builtin_fmaf(ml[1], cy, rl * cx);
+#pragma unroll
+                for (int dt = 0; dt < NDT; dt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[dt][i] = __builtin_fmaf(v[dt][i], cy, o[dt][i] * cx);
+            }
+            if (ok) {
+                const float inv = inverse_sum(rl);
+#pragma unroll
+                for (int dt = 0; dt < NDT; dt++) store_out4<DT>(a, row, head, D, 16 * dt + 4 * g, o[dt], inv, gate[dt]);
             }
         };
 
         // ---- two groups of four waves, one of each on every SIMD, take turns: in a phase one runs the matrix instructions
-        // of a block (and the weighted values of the block before) while the other takes its softmax. Copies run two blocks
-        // ahead of the keys' use; both groups issue them in the even phases (of the first group's matrix instructions)
-        // and wait for the last ones at their end. ----
+        // of a block (and the weighted values of the block before) while the other takes its softmax and copies. In the first
+        // group's phases 2 i (matrix) and 2 i + 1 (softmax of block i) the second group's are one later. Keys of block j are read in
+        // phases 2 j and 2 j + 1, values of block j in 2 j + 2 and 2 j + 3; the first group copies its share of keys of block i + 2 and
+        // values of block i + 1 in phase 2 i + 1 and the second its in phase 2 i, behind the last reads of the places (keys of block i - 2
+        // in phase 2 i - 3, values of block i - 3 in 2 i - 3), and each waits for them two phases later, before phase 2 i + 4. ----
         bool odd_values = false;
         const bool second = wave >= 4;
         auto kfrag_of = [&](int i) {
@@ -349,173 +557,131 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
         };
-        // Step i: the copies of keys of block i + 2 and values of block i + 1; those of the step before have landed at its end
-        auto step = [&](int i) __attribute__((always_inline)) {
-            if (i + 2 - base >= 64) survey(i);
-            stage(true, i + 2), stage(false, i + 1);
-            landed<C::COPIES>();
+        // The copies of the step before have landed (keys of block i + 1, values of block i); step i copies keys of block i + 2 and values
+        // of block i + 1.
+        auto arrive = [&](int i) __attribute__((always_inline)) {
+            if (i + 2 - base >= 64) survey(i - 1);
+            landed<0>();
             if (stale >> (i - base) & 1) clean(i);
         };
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int part = 0; part < PARTS; part++) w[nt][part] = f16x8{};
+        bool check = false;  // the block before is not whole: its values may be some that only some rows see
         auto matrix_phase = [&](int i) __attribute__((always_inline)) {  // scores of block i, values of block i - 1
-            products(std::true_type{}, kfrag_of(i), vfrag_of(i - 1));
-        };
-        auto softmax_phase = [&](int i) __attribute__((always_inline)) {
-            const bool all = whole >> (i - base) & 1;
-            softmax(key_at(i), paged >> (i - base) & 1, all);
-            if (!all) {
-                const auto read = vfrag_of(i);
+            if (check) {
+                const auto read = vfrag_of(i - 1);
                 uint32_t odd = 0;
 #pragma unroll 4
                 for (int dt = 0; dt < NDT; dt++) odd |= not_finite(read(dt));
                 if (__builtin_amdgcn_ballot_w64(odd != 0)) odd_values = true;
             }
+            products(kfrag_of(i), vfrag_of(i - 1));
+        };
+        auto softmax_phase = [&](int i) __attribute__((always_inline)) {
+            const bool all = whole >> (i - base) & 1;
+            softmax(key_at(i), paged >> (i - base) & 1, all, i + second + 1);
+            check = !all;
         };
         // (the values of the block before the first)
-        for (int k = tid; k < BLKE / 8; k += 64 * kChWaves) *reinterpret_cast<u32x4*>(sv + (kChRing - 1) * BLKE + k * 8) = u32x4{};
+        for (int k = wave * 64 + lane_here(); k < BLKE / 8; k += 64 * kChWaves) *reinterpret_cast<u32x4*>(sv + (kChRing - 1) * BLKE + k * 8) = u32x4{};
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0xC07F);
         landed<C::COPIES>();
         phase();
         if (second) {
-            step(0);
+            arrive(0);
+            copy(true, 2), copy(false, 1);
             phase();
         }
 #pragma unroll 1
         for (int i = 0; i < n; i++) {
             matrix_phase(i);
-            if (!second) step(i);
             phase();
+            arrive(i + second);
             softmax_phase(i);
-            if (second) step(i + 1);
             phase();
         }
         matrix_phase(n);  // (its scores are of no block)
         if (!second) phase();
         landed<0>();  // (copies past the last block write zeros)
+        phase();      // the rings are free
 
-        if (odd_values) {
-            // a value that only some of the wave's rows see is not finite, and a weight of zero does not hide it: the segment again,
-            // from memory, its weighted values token by token with those hidden from it zeroed
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                m_run[nt] = kNegInf, l_run[nt] = 0.f;
-#pragma unroll
-                for (int dt = 0; dt < NDT; dt++) acc[nt][dt] = f32x4{};
-            }
-#pragma unroll 1
-            for (int i = 0; i < n; i++) {
-                const int k0 = key_of(i);
-                const int page = k0 < a.limit ? __builtin_amdgcn_readfirstlane(table[k0 >> a.c.lg_page]) : -1;
-                if ((uint32_t)page >= (uint32_t)a.c.n_pages || unseen(k0)) continue;
-                const int64_t from = paged_block(a.c, page, k0, h, a.NKV, D);
-                const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(a.c.k + from, (short)0, BLKE * 2, 0x00020000);
-                const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(a.c.v + from, (short)0, BLKE * 2, 0x00020000);
-                auto get = [&](const __amdgpu_buffer_rsrc_t& r, int f) __attribute__((always_inline)) {
-                    return __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(r, f * 1024 + lane * 16, 0, 0));
-                };
-                products(std::false_type{}, [&](int f) { return get(rk, f); }, [&](int f) { return get(rv, f); });
-                softmax(k0, true, false);
-#pragma unroll 1
-                for (int p = w0; p <= w1; p++) {
-                    const Sight sp = sight(a, p);
-#pragma unroll
-                    for (int dt = 0; dt < NDT; dt++) {
-                        const f16x8 v = keep_keys(get(rv, dt), [&](int j) { return sp.sees(k0 + 8 * g + j, a.sinks); });
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            f32x4 o = acc[nt][dt];
-#pragma unroll
-                            for (int part = 0; part < PARTS; part++) o = mfma16(v, w[nt][part], o);
-                            const bool own = pos + t0 + ((wave * NT + nt) * 16 + col) / G == p;
-#pragma unroll
-                            for (int j = 0; j < 4; j++) acc[nt][dt][j] = own ? o[j] : acc[nt][dt][j];
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    }
-                }
-            }
+        // ---- 16 rows at a time through the wave's part of the rings' room: the loop's registers hold the outputs only in the
+        // loop (with what follows working on them there, 32-row waves spill inside it) ----
+        const int lane = lane_here(), col = lane & 15, g = lane >> 4;
+        f32x4* mine = reinterpret_cast<f32x4*>(smem) + wave * NDT * 64 + lane;  // [dim tile][lane]
+        const int64_t item = at - off;
+        const bool split = lo > 0 || hi < kt.count;
+        int first = wg, parts = 1;
+        if (split && joined) {
+            first -= lo > 0, parts = 2;  // (only whether this is the first part matters here)
+        } else if (split) {
+            while (plan.unit[first] > item) first--;
+            int last = wg;
+            while (plan.unit[last + 1] < item + kt.count) last++;
+            parts = last - first + 1;
         }
-
-        // ---- sums across the row's lanes; whole items to the output, parts to the workspace ----
+        const int own = wg - first;
+        auto region = [&](int part) {
+            const size_t slot = part == 0 ? 2 * first + 1 : 2 * (first + part);
+            return __builtin_amdgcn_make_buffer_rsrc(plan.part + (slot * kChWaves + wave) * C::PART, (short)0, C::PART * 4, 0x00020000);
+        };
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(l_run[nt]), __float_as_uint(l_run[nt]), false, false);
-            const float l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-            const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-            l_run[nt] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
-        }
-        const int64_t item = at - off;
-        const int first = (int)(item / run), parts = (int)((item + kt.count - 1) / run) - first + 1, own = wg - first;
-        bool write = parts == 1;
-        if (parts > 1) {
-            auto region = [&](int part) {
-                const size_t slot = part == 0 ? 2 * first + 1 : 2 * (first + part);
-                return __builtin_amdgcn_make_buffer_rsrc(plan.part + (slot * kChWaves + wave) * C::PART, (short)0, C::PART * 4, 0x00020000);
-            };
-            const __amdgpu_buffer_rsrc_t rp = region(own);
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                for (int dt = 0; dt < NDT; dt++)
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[nt][dt]), rp, ((nt * NDT + dt) * 64 + lane) * 16, 0, kScDevice);
-                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{m_run[nt], l_run[nt]}), rp,
-                                                      NT * NDT * 1024 + (nt * 64 + lane) * 8, 0, kScDevice);
-            }
-            if (!joined) {
-                // the wave that arrives last joins the parts, from the first to the last whichever it is
-                __builtin_amdgcn_s_waitcnt(0x0F70);  // the partial is out before it is counted
-                int old = 0;
-                if (lane == 0) old = __hip_atomic_fetch_add(plan.cnt + first * kChWaves + wave, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                write = __builtin_amdgcn_readfirstlane(old) == parts - 1;
-                asm volatile("" ::: "memory");
-                if (write) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        float m = kNegInf, l = 0.f;
-#pragma unroll
-                        for (int dt = 0; dt < NDT; dt++) acc[nt][dt] = f32x4{};
+            if (odd_values) {
+                // a value that only some of the wave's rows see is not finite, and a weight of zero does not hide it: the segment
+                // again, from memory, its weighted values token by token with those hidden from it zeroed
+                float m = kNegInf, l = 0.f;
 #pragma unroll 1
-                        for (int part = 0; part < parts; part++) {
-                            const __amdgpu_buffer_rsrc_t rq = region(part);
-                            const f32x2 ml = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rq, NT * NDT * 1024 + (nt * 64 + lane) * 8, 0, kScDevice));
-                            const float to = fmaxf(m, ml[0]);
-                            const float cf = m == kNegInf ? 0.f : exp2_fast(m - to), cs = ml[0] == kNegInf ? 0.f : exp2_fast(ml[0] - to);
-                            m = to, l = __builtin_fmaf(ml[1], cs, l * cf);
-                            constexpr int NB = 4;
-                            static_for<0, NDT / NB>([&](auto ic) __attribute__((always_inline)) {
-                                constexpr int d0 = NB * decltype(ic)::value;
-                                f32x4 o[NB];
+                for (int dt = 0; dt < NDT; dt++) mine[dt * 64] = f32x4{};
+#pragma unroll 1
+                for (int i = 0; i < n; i++) {
+                    const int k0 = key_of(i);
+                    const int page = k0 < a.limit ? __builtin_amdgcn_readfirstlane(table[k0 >> a.c.lg_page]) : -1;
+                    if ((uint32_t)page >= (uint32_t)a.c.n_pages || unseen(k0)) continue;
+                    const int64_t from = paged_block(a.c, page, k0, h, a.NKV, D);
+                    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(a.c.k + from, (short)0, BLKE * 2, 0x00020000);
+                    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(a.c.v + from, (short)0, BLKE * 2, 0x00020000);
+                    auto get = [&](const __amdgpu_buffer_rsrc_t& r, int f) __attribute__((always_inline)) {
+                        return __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(r, f * 1024 + lane * 16, 0, 0));
+                    };
+                    f32x4 x[2] = {f32x4{}, f32x4{}};
 #pragma unroll
-                                for (int j = 0; j < NB; j++)
-                                    o[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rq, ((nt * NDT + d0 + j) * 64 + lane) * 16, 0, kScDevice));
+                    for (int f = 0; f < NDT; f++)
 #pragma unroll
-                                for (int j = 0; j < NB; j++)
+                        for (int part = 0; part < PARTS; part++) x[f & 1] = mfma16(get(rk, f), q[nt][part][f >> 1], x[f & 1]);
+                    asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x[0]), "+v"(x[1]));  // (as in products())
+                    hide(x, nt, k0, true);
+                    const float corr = raise(largest(x) * fac[nt], m, l);
+                    f16x8 wt[PARTS];
+                    weigh(x, fac[nt], m, l, wt);
+#pragma unroll 1
+                    for (int dt = 0; dt < NDT; dt++) {
+                        const f16x8 v = get(rv, dt);
+                        const f32x4 old = mine[dt * 64] * corr;
+                        f32x4 sum = old;
+#pragma unroll 1
+                        for (int p = w0; p <= w1; p++) {
+                            const Sight sp = sight(a, p);
+                            const f16x8 vp = keep_keys(v, [&](int j) { return sp.sees(k0 + 8 * g + j, a.sinks); });
+                            f32x4 o = old;
 #pragma unroll
-                                    for (int i = 0; i < 4; i++) acc[nt][d0 + j][i] = __builtin_fmaf(o[j][i], cs, acc[nt][d0 + j][i] * cf);
-                                __builtin_amdgcn_sched_barrier(0);
-                            });
+                            for (int part = 0; part < PARTS; part++) o = mfma16(vp, wt[part], o);
+                            const bool its = pos + t0 + (((wave * NT + nt) * 16 + col) >> lgG) == p;
+#pragma unroll
+                            for (int j = 0; j < 4; j++) sum[j] = its ? o[j] : sum[j];
                         }
-                        l_run[nt] = l;
+                        mine[dt * 64] = sum;
                     }
                 }
-            }
-        }
-        if (write) {
+                m_run[nt] = m, l_run[nt] = l;
+            } else {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const int r = (wave * NT + nt) * 16 + col, t = t0 + r / G;
-                if (r >= tok * G || t >= t1) continue;
-                const float inv = inverse_sum(l_run[nt]);
-#pragma unroll
-                for (int dt = 0; dt < NDT; dt++) {
-                    store_out4<DT>(a, (size_t)b * a.n + t, h * G + r % G, D, 16 * dt + 4 * g, acc[nt][dt], inv);
-                    if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                }
+                for (int dt = 0; dt < NDT; dt++) mine[dt * 64] = acc[nt][dt];
             }
+            write_rows(nt, mine, region, parts, own);
         }
         at += hi - lo;
         off = hi;
@@ -530,7 +696,7 @@ __global__ __launch_bounds__(256) void k_paged_join_chunk(PagedAttendArgs a, voi
     constexpr int NQ = C::NDT / 4;  // dim tiles of a quarter
     __shared__ f32x4 red[3][NQ][64];
     const ChPlan plan = ch_plan(ws, groups, C::PART);
-    const int G = a.NH / a.NKV, tok = C::ROWS / G, nqt = (a.n + tok - 1) / tok;
+    const int lgG = __builtin_ctz(a.NH / a.NKV), G = 1 << lgG, tok = C::ROWS >> lgG, nqt = (a.n + tok - 1) / tok;
     int x = blockIdx.x;
     const int quarter = x % 4, sub = x / 4 % (kChWaves * NT);
     x /= 4 * kChWaves * NT;
@@ -538,16 +704,24 @@ __global__ __launch_bounds__(256) void k_paged_join_chunk(PagedAttendArgs a, voi
     const int t1 = min(t0 + tok, seq_len(a.lens, b, a.n));
     const int count = key_tiles<6>(a, seq_pos(a.pos, b), t0, t1).count;
     if (count == 0) return;
-    const int64_t run = plan.head[1], item = h * plan.head[0] + plan.first[pair];
-    const int first = (int)(item / run), parts = (int)((item + count - 1) / run) - first + 1;
+    const int64_t item = h * plan.head[0] + plan.first[pair];
+    const int first = group_of(plan, item, groups), parts = group_of(plan, item + count - 1, groups) - first + 1;
     if (parts == 1) return;
     const int lane = threadIdx.x & 63, set = threadIdx.x >> 6, col = lane & 15, g = lane >> 4, wave = sub / NT, nt = sub % NT;
-    const int r = sub * 16 + col, t = t0 + r / G;
+    const int r = sub * 16 + col, t = t0 + (r >> lgG);
     auto region = [&](int part) {
         const size_t slot = part == 0 ? 2 * first + 1 : 2 * (first + part);
         return plan.part + (slot * kChWaves + wave) * C::PART;
     };
     auto sums = [&](int part) { return *reinterpret_cast<const f32x2*>(region(part) + NT * C::NDT * 256 + (nt * 64 + lane) * 2); };
+    const bool ok = t < t1;
+    Gate4<DT> gate[NQ];
+#pragma unroll
+    for (int j = 0; j < NQ; j++) gate[j].none();
+    if (a.gate) {
+#pragma unroll
+        for (int j = 0; j < NQ; j++) gate[j].load(a, (size_t)b * a.n + (ok ? t : t0), h * G + (r & (G - 1)), 16 * (quarter * NQ + j) + 4 * g);
+    }
     float m = kNegInf, l = 0.f;
 #pragma unroll 8
     for (int p = 0; p < parts; p++) m = fmaxf(m, sums(p)[0]);
@@ -573,12 +747,12 @@ __global__ __launch_bounds__(256) void k_paged_join_chunk(PagedAttendArgs a, voi
         for (int j = 0; j < NQ; j++) red[set - 1][j][lane] = o[j];
     }
     __syncthreads();
-    if (set > 0 || r >= tok * G || t >= t1) return;
+    if (set > 0 || !ok) return;
     const float inv = inverse_sum(l);
 #pragma unroll
     for (int j = 0; j < NQ; j++) {
         o[j] += (red[0][j][lane] + red[1][j][lane]) + red[2][j][lane];
-        store_out4<DT>(a, (size_t)b * a.n + t, h * G + r % G, D, 16 * (quarter * NQ + j) + 4 * g, o[j], inv);
+        store_out4<DT>(a, (size_t)b * a.n + t, h * G + (r & (G - 1)), D, 16 * (quarter * NQ + j) + 4 * g, o[j], inv, gate[j]);
     }
 }
 
@@ -604,7 +778,7 @@ hipError_t go(const PagedAttendArgs& a, int n_cu, void* ws, hipStream_t s) {
 
 size_t paged_chunk_workspace(int D, int n_cu) {
     const size_t part = (size_t)kChWaves * (32 * D + 256) * sizeof(float);
-    return up256(2 * n_cu * part + n_cu * (sizeof(int4) + kChWaves * sizeof(int)) + (2 + kJoinItems) * sizeof(int64_t));
+    return up256(2 * n_cu * part + n_cu * (sizeof(int4) + kChWaves * 2 * sizeof(int)) + (3 + n_cu + kJoinItems) * sizeof(int64_t));
 }
 
 hipError_t launch_paged_chunk(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* ws, hipStream_t s) {

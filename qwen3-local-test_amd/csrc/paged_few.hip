@@ -36,6 +36,7 @@ struct FewCfg {
     static constexpr int EXTRA = ROWS * 4 + 32;
     static constexpr bool TIGHT = Q_BYTES + KV_BYTES + EXTRA > 160 * 1024;
     static constexpr int LDS = Q_BYTES + KV_BYTES + (TIGHT ? 0 : EXTRA);
+    static_assert(NDT % kFewWaves == 0, "every wave writes as many dim tiles");
     static_assert(2 * kFewWaves * ROWS * 4 <= Q_BYTES, "the waves' maxima and sums fit the queries' room");
     static_assert(kFewWaves * ROWS * D * 4 <= KV_BYTES, "the waves' accumulators fit the blocks' room");
 };
@@ -178,7 +179,8 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
 #pragma unroll
             for (int m = 1; m < TPR; m <<= 1) largest = fmaxf(largest, __shfl_xor(largest, m, 64));
             const int sh = query_shift(largest);
-            if (tl == 0) sc[r] = __builtin_ldexpf(a.scale, -sh);
+            const float up = power_of_two(sh);
+            if (tl == 0) sc[r] = a.scale * power_of_two(-sh);
 #pragma unroll
             for (int i = 0; i < PPT; i++) {
                 const int pc = tl + i * TPR;
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
                 f16x8 hi, lo;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float y = __builtin_ldexpf(x[i][j], sh);
+                    const float y = x[i][j] * up;
                     hi[j] = (f16)y;
                     if constexpr (PARTS == 2) lo[j] = (f16)(y - (float)hi[j]);
                 }
@@ -371,14 +373,24 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
             for (int w = 0; w < kFewWaves; w++)
                 l += sl[w * ROWS + r] * (sm[w * ROWS + r] == kNegInf ? 0.f : exp2_fast(sm[w * ROWS + r] - m));
             const float inv = inverse_sum(l);
+            constexpr int PER = (NDT + kFewWaves - 1) / kFewWaves;  // dim tiles a wave
+            Gate4<DT> gate[PER];
+#pragma unroll
+            for (int k = 0; k < PER; k++) gate[k].none();
+            if (!split && a.gate) {
+#pragma unroll
+                for (int k = 0; k < PER; k++)
+                    gate[k].load(a, (size_t)b * a.n + t, h * G + r % G, 16 * (wave + k * kFewWaves) + 4 * g);
+            }
             if (split && wave == 0 && g == 0) *reinterpret_cast<f32x2*>(plan.ml + ((size_t)slot * ROWS + r) * 2) = f32x2{m, l};
 #pragma unroll
-            for (int dt = wave; dt < NDT; dt += kFewWaves) {
+            for (int k = 0; k < PER; k++) {
+                const int dt = wave + k * kFewWaves;
                 f32x4 o{};
 #pragma unroll
                 for (int w = 0; w < kFewWaves; w++) o += *reinterpret_cast<const f32x4*>(red + (((w * NT + nt) * NDT + dt) * 64 + lane) * 4);
                 if (split) *reinterpret_cast<f32x4*>(plan.o + ((size_t)slot * ROWS + r) * D + 16 * dt + 4 * g) = o;
-                else store_out4<DT>(a, (size_t)b * a.n + t, h * G + r % G, D, 16 * dt + 4 * g, o, inv);
+                else store_out4<DT>(a, (size_t)b * a.n + t, h * G + r % G, D, 16 * dt + 4 * g, o, inv, gate[k]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -405,6 +417,9 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttendArgs a, void* ws,
     const int first = (int)(at / run), last = (int)((at + nu - 1) / run), parts = last - first + 1;
     if (parts == 1) return;
     const int tid = threadIdx.x;
+    Gate4<DT> gate;
+    gate.none();
+    if (a.gate) gate.load(a, (size_t)row, head, 4 * (tid % LANES));
     auto slot = [&](int part) { return (size_t)(part == 0 ? 2 * first + 1 : 2 * (first + part)) * ROWS + r; };
     // maximum, then sums and outputs of 64 parts at a time against it
     float m = kNegInf;
@@ -440,7 +455,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttendArgs a, void* ws,
     if (tid < LANES) {
 #pragma unroll
         for (int s = 1; s < SETS; s++) o += *reinterpret_cast<const f32x4*>(&red[s][4 * tid]);
-        store_out4<DT>(a, (size_t)row, head, D, 4 * tid, o, inverse_sum(sr[4]));
+        store_out4<DT>(a, (size_t)row, head, D, 4 * tid, o, inverse_sum(sr[4]), gate);
     }
 }
 
