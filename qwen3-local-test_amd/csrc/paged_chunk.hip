@@ -23,67 +23,62 @@ struct ChPlan {
     float* part;    // [2 * groups][waves][PART]
     int4* start;    // [groups]: KV head (-1: nothing to do), sequence, query tile, first key tile
     int* cnt;       // [groups][waves][2] arrivals at the 16-row tiles of the item that is the workgroup's last
-    int64_t* head;  // key tiles a KV head
     int64_t* unit;  // [groups + 1]: the workgroups' first units
-    int64_t* first; // joined calls: first key tile of each (sequence, query tile)
+    // joined calls, instead: [0] parts a KV head, then of each (sequence, query tile) its first part and its parts
+    int* joined;
 };
-constexpr int kJoinItems = 1024;  // most (sequence, query tile) pairs of a joined call
+constexpr int kJoinPairs = 32;  // most (sequence, query tile) pairs of a joined call
 __host__ __device__ inline ChPlan ch_plan(void* ws, int groups, int part_floats) {
     ChPlan p;
     p.part = static_cast<float*>(ws);
     p.start = reinterpret_cast<int4*>(p.part + (size_t)2 * groups * kChWaves * part_floats);
     p.cnt = reinterpret_cast<int*>(p.start + groups);
-    p.head = reinterpret_cast<int64_t*>(p.cnt + groups * kChWaves * 2);
-    p.unit = p.head + 2;
-    p.first = p.unit + groups + 1;
+    p.unit = reinterpret_cast<int64_t*>(p.cnt + groups * kChWaves * 2);
+    p.joined = reinterpret_cast<int*>(p.unit + groups + 1);
     return p;
 }
-// The workgroup whose run holds unit u
-__device__ __forceinline__ int group_of(const ChPlan& plan, int64_t u, int groups) {
-    int lo = 0, hi = groups;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (plan.unit[mid] <= u) lo = mid;
-        else hi = mid;
+// Items are (KV head, sequence, query tile) in this order, each of as many units as it has key tiles (at most 2^20). Every
+// workgroup of the chunk kernel takes a run of units, in one of two ways (a segment, what a workgroup takes of an item, costs some
+// three to four units beside its own: the rows, the first copies, the partial and its joining):
+//  - items in equal parts of at most `run` units, a workgroup a part, for the least run whose parts fit the workgroups;
+//  - equal runs over all items, their ends moved by up to a twelfth to an item's edge where one is that near: where there are more
+//    items than workgroups, or where the first way's run is more than kSegment units longer.
+constexpr int kSegment = 3;
+
+// ceil(c / r) of 0 <= c <= 2^20, 1 <= r <= 2^20 (the quotient's error is below its distance from the next whole number, 1 / 2r)
+__device__ __forceinline__ int parts_of(int c, float r) { return (int)(((float)c + r - 0.5f) * __builtin_amdgcn_rcpf(r)); }
+
+// The least run in [lo, hi] whose parts fit the workgroups, hi's known to: 64 runs at a time, a lane each. count(i): tiles of pair i.
+template <typename F>
+__device__ __forceinline__ int least_run(F&& count, int pairs, int nkv, int groups, int lo, int hi, int lane) {
+    while (lo < hi) {
+        const int step = (hi - lo + 63) / 64;
+        const float r = (float)min(hi, lo + step * lane);
+        int parts = 0;
+        for (int i = 0; i < pairs; i++) parts += parts_of(count(i), r);
+        const uint64_t fits = __builtin_amdgcn_ballot_w64(parts * nkv <= groups);
+        const int f = fits ? (int)__builtin_ctzll(fits) : 64, was = lo;
+        if (f == 0) break;
+        lo = min(hi, was + step * (f - 1) + 1);
+        if (f < 64) hi = min(hi, was + step * f);
     }
     return lo;
 }
 
-// Items are (KV head, sequence, query tile) in this order, each of as many units as it has key tiles. Every workgroup of
-// the chunk kernel takes a run of units, in one of two ways (a segment, what a workgroup takes of an item, costs some three to
-// four units beside its own: the rows, the first copies, the partial and its joining):
-//  - items in equal parts of at most `run` units, a workgroup a part, for the least run whose parts fit the workgroups;
-//  - equal runs over all items, their ends moved by up to a twelfth to an item's edge where one is that near: where there are more
-//    items than workgroups, or where the first way's run is more than kSegment units longer.
-// One workgroup: a thread sums a run of (sequence, query tile) pairs, a scan places the runs, and the threads write the starts
-// that fall into theirs.
-constexpr int kSegment = 3, kPartPairs = 1024;  // (pairs whose tiles the first way holds in LDS)
-__global__ __launch_bounds__(1024) void k_paged_plan(PagedAttendArgs a, void* ws, int groups, int part_floats, int tok, bool joined) {
-    __shared__ int64_t sums[16];
-    __shared__ int most[16], count[kPartPairs], fits[16];
+// One workgroup: a thread a run of (sequence, query tile) pairs (one pair, where the first way is tried), a scan places the runs,
+// and the threads write the starts that fall into theirs.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void k_paged_plan(PagedAttendArgs a, void* ws, int groups, int part_floats, int tok) {
+    constexpr int WAVES = THREADS / 64;
+    __shared__ int64_t sums[WAVES];
+    __shared__ int tops[WAVES], ksums[WAVES], count[THREADS];
     const ChPlan plan = ch_plan(ws, groups, part_floats);
     const int nqt = (a.n + tok - 1) / tok, pairs = a.n_seq * nqt;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (pairs + 1023) / 1024;
+    const int per = (pairs + THREADS - 1) / THREADS;
     auto tiles = [&](int pair) {
         const int b = pair / nqt, t0 = (pair - b * nqt) * tok;
         return key_tiles<6>(a, seq_pos(a.pos, b), t0, min(t0 + tok, seq_len(a.lens, b, a.n))).count;
-    };
-    // the sum of x over the threads before this one; `total` over all
-    auto scan = [&](int64_t x, int64_t& total) {
-        int64_t incl = x;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int64_t o = __shfl_up((long long)incl, m, 64);
-            if (lane >= m) incl += o;
-        }
-        __syncthreads();
-        if (lane == 63) sums[wave] = incl;
-        __syncthreads();
-        int64_t before = incl - x;
-        total = 0;
-        for (int w = 0; w < 16; w++) before += w < wave ? sums[w] : 0, total += sums[w];
-        return before;
     };
     int64_t mine = 0;
     int top = 0;
@@ -92,59 +87,53 @@ __global__ __launch_bounds__(1024) void k_paged_plan(PagedAttendArgs a, void* ws
         mine += c, top = max(top, c);
         if (per == 1) count[tid] = c;
     }
-    for (int i = tid; i < groups * kChWaves * 2; i += 1024) plan.cnt[i] = 0;
+    for (int i = tid; i < groups * kChWaves * 2; i += THREADS) plan.cnt[i] = 0;
+    int64_t incl = mine;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) top = max(top, __shfl_xor(top, m, 64));
-    if (lane == 0) most[wave] = top;
-    int64_t total;
-    int64_t x = scan(mine, total);
-    for (int w = 0; w < 16; w++) top = max(top, most[w]);
+    for (int m = 1; m < 64; m <<= 1) {
+        const int64_t o = __shfl_up((long long)incl, m, 64);
+        if (lane >= m) incl += o;
+        top = max(top, __shfl_xor(top, m, 64));
+    }
+    if (lane == 63) sums[wave] = incl, tops[wave] = top;
+    __syncthreads();
+    int64_t x = incl - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) x += w < wave ? sums[w] : 0, total += sums[w], top = max(top, tops[w]);
     const int64_t all = total * a.NKV, run = max((int64_t)1, (all + groups - 1) / groups);
-    if (tid == 0) plan.head[0] = total, plan.unit[groups] = all;
+    if (tid == 0) plan.unit[groups] = all;
 
-    // (an item has at most 2^20 key tiles, so that a run of 2^20 and more is never better than whole items)
-    int lo = (int)min(run, (int64_t)1 << 20), hi = max(top, lo);  // the first way's run lies in [lo, hi], if whole items fit
-    if ((int64_t)pairs * a.NKV <= groups && per == 1) {
-        while (lo < hi) {  // sixteen runs at a time, a wave each
-            const int step = (hi - lo + 15) / 16, r = min(hi, lo + step * wave);
-            int parts = 0;
-            for (int i = lane; i < pairs; i += 64) parts += (int)((unsigned)(count[i] + r - 1) / (unsigned)r);
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) parts += __shfl_xor(parts, m, 64);
-            __syncthreads();
-            if (lane == 0) fits[wave] = parts * a.NKV <= groups;
-            __syncthreads();
-            int w = 0;
-            while (w < 16 && !fits[w]) w++;
-            const int was = lo;
-            if (w == 0) break;
-            lo = min(hi, was + step * (w - 1) + 1);
-            if (w < 16) hi = min(hi, was + step * w);
-        }
-        const int part = lo;
+    if (per == 1 && pairs * a.NKV <= groups && run <= top) {
+        const int part = least_run([&](int i) { return count[i]; }, pairs, a.NKV, groups, (int)run, top, lane);
         if (part <= run + kSegment) {
-            const int c = tid < pairs ? count[tid] : 0, k = (int)((unsigned)(c + part - 1) / (unsigned)part);
-            int64_t all_parts;
-            const int64_t at = scan(k, all_parts);
-            if (joined && tid < pairs) plan.first[tid] = x;
+            const int c = count[tid], k = parts_of(c, (float)part);
+            int kincl = k;
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) {
+                const int o = __shfl_up(kincl, m, 64);
+                if (lane >= m) kincl += o;
+            }
+            if (lane == 63) ksums[wave] = kincl;
+            __syncthreads();
+            int at = kincl - k, parts = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) at += w < wave ? ksums[w] : 0, parts += ksums[w];
             for (int h = 0; h < a.NKV; h++)
                 for (int j = 0; j < k; j++) {
-                    const int w = h * (int)all_parts + (int)at + j, off = (int)((unsigned)c * (unsigned)j / (unsigned)k);  // (c j < 2^28)
+                    const int w = h * parts + at + j, off = (int)((unsigned)c * (unsigned)j / (unsigned)k);  // (c j < 2^28)
                     plan.start[w] = int4{h, tid / nqt, tid % nqt, off}, plan.unit[w] = h * total + x + off;
                 }
-            for (int w = tid; w < groups; w += 1024)
-                if (w >= all_parts * a.NKV) plan.start[w].x = -1, plan.unit[w] = all;
+            for (int w = parts * a.NKV + tid; w < groups; w += THREADS) plan.start[w].x = -1, plan.unit[w] = all;
             return;
         }
     }
-    for (int w = tid; w < groups; w += 1024)
+    for (int w = tid; w < groups; w += THREADS)
         if (w * run >= all) plan.start[w].x = -1, plan.unit[w] = all;
     const int near = (int)min(run / 12, (int64_t)1 << 20);
     for (int i = 0; i < per; i++) {
         const int pair = tid * per + i;
         if (pair >= pairs) break;
         const int c = tiles(pair);
-        if (joined) plan.first[pair] = x;
         for (int h = 0; h < a.NKV && c; h++) {
             const int64_t g0 = h * total + x;
             for (int64_t w = (g0 + run - 1) / run; w * run < g0 + c; w++) {
@@ -155,6 +144,43 @@ __global__ __launch_bounds__(1024) void k_paged_plan(PagedAttendArgs a, void* ws
             }
         }
         x += c;
+    }
+}
+
+// The first way by every wave for itself, for calls of so few items that a second launch joins them: a lane a pair, then a lane a
+// run. What part w of all is: `first_key` tile of `count` and the next part's; false behind the last part.
+struct Part {
+    int h, pair, lo, hi;
+};
+template <typename F>
+__device__ __forceinline__ bool joined_part(F&& tiles, int pairs, int nkv, int groups, int w, int lane, int* out, Part& p) {
+    const int mine = lane < pairs ? tiles(lane) : 0;
+    int total = 0, hi = 1;
+    for (int i = 0; i < pairs; i++) {
+        const int c = __builtin_amdgcn_readlane(mine, i);
+        total += c, hi = max(hi, c);  // (at most 2^20 each)
+    }
+    const int lo = least_run([&](int i) { return __builtin_amdgcn_readlane(mine, i); }, pairs, nkv, groups,
+                             max(1, (int)(((int64_t)total * nkv + groups - 1) / groups)), hi, lane);
+    const int parts = parts_of(mine, (float)lo);
+    int all = 0;
+    for (int i = 0; i < pairs; i++) {
+        const int k = __builtin_amdgcn_readlane(parts, i);
+        if (out && lane == 0) out[1 + 2 * i] = all, out[2 + 2 * i] = k;
+        all += k;
+    }
+    if (out && lane == 0) out[0] = all;
+    if (w >= all * nkv) return false;
+    p.h = w / all;
+    int at = w - p.h * all;
+    for (p.pair = 0;; p.pair++) {
+        const int k = __builtin_amdgcn_readlane(parts, p.pair);
+        if (at < k) {
+            const unsigned c = __builtin_amdgcn_readlane(mine, p.pair);
+            p.lo = (int)(c * (unsigned)at / (unsigned)k), p.hi = (int)(c * (unsigned)(at + 1) / (unsigned)k);
+            return true;
+        }
+        at -= k;
     }
 }
 
@@ -193,12 +219,24 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
     const ChPlan plan = ch_plan(ws, groups, C::PART);
     // neighbouring runs on one XCD: they read the same keys
     const int wg = (blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);
-    const int4 st = plan.start[wg];
-    int h = __builtin_amdgcn_readfirstlane(st.x), b = __builtin_amdgcn_readfirstlane(st.y);
-    int qt = __builtin_amdgcn_readfirstlane(st.z), off = __builtin_amdgcn_readfirstlane(st.w);
-    if (h < 0) return;
-    const int64_t stop = plan.unit[wg + 1];
-    int64_t at = plan.unit[wg];  // unit of the segment at hand
+    int h, b, qt, off;
+    int64_t at, stop;  // units of the segment at hand and of the run's end
+    if (joined) {
+        const int nqt = (a.n + tok - 1) / tok;
+        auto tiles = [&](int pair) {
+            const int sb = pair / nqt, st0 = (pair - sb * nqt) * tok;
+            return key_tiles<6>(a, seq_pos(a.pos, sb), st0, min(st0 + tok, seq_len(a.lens, sb, a.n))).count;
+        };
+        Part p;
+        if (!joined_part(tiles, a.n_seq * nqt, a.NKV, groups, wg, lane_here(), wg == 0 && wave == 0 ? plan.joined : nullptr, p)) return;
+        h = p.h, b = p.pair / nqt, qt = p.pair - b * nqt, off = p.lo, at = 0, stop = p.hi - p.lo;
+    } else {
+        const int4 st = plan.start[wg];
+        h = __builtin_amdgcn_readfirstlane(st.x), b = __builtin_amdgcn_readfirstlane(st.y);
+        qt = __builtin_amdgcn_readfirstlane(st.z), off = __builtin_amdgcn_readfirstlane(st.w);
+        if (h < 0) return;
+        at = plan.unit[wg], stop = plan.unit[wg + 1];
+    }
 
     while (at < stop) {
         const int pos = seq_pos(a.pos, b), len = seq_len(a.lens, b, a.n);
@@ -688,71 +726,84 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
     }
 }
 
-// Joins the parts of split items where there are few items: a workgroup 16 rows of an item and a quarter of its dims, four
-// sets of threads a part each at a time, in a fixed order.
+// Joins the parts of split items where there are few items: a workgroup 16 rows of an item and a quarter of its dims; its four
+// waves take the parts in turn, four of them at a time, and are joined through the LDS, all in a fixed order.
 template <int D, int DT, int NT>
 __global__ __launch_bounds__(256) void k_paged_join_chunk(PagedAttendArgs a, void* ws, int groups) {
     using C = ChCfg<D, DT, NT>;
     constexpr int NQ = C::NDT / 4;  // dim tiles of a quarter
-    __shared__ f32x4 red[3][NQ][64];
+    __shared__ f32x4 red[4][NQ][64];
+    __shared__ f32x2 red_ml[4][64];
     const ChPlan plan = ch_plan(ws, groups, C::PART);
     const int lgG = __builtin_ctz(a.NH / a.NKV), G = 1 << lgG, tok = C::ROWS >> lgG, nqt = (a.n + tok - 1) / tok;
     int x = blockIdx.x;
     const int quarter = x % 4, sub = x / 4 % (kChWaves * NT);
     x /= 4 * kChWaves * NT;
     const int h = x % a.NKV, pair = x / a.NKV, b = pair / nqt, t0 = (pair - b * nqt) * tok;
+    const int first = h * plan.joined[0] + plan.joined[1 + 2 * pair], parts = plan.joined[2 + 2 * pair];
     const int t1 = min(t0 + tok, seq_len(a.lens, b, a.n));
-    const int count = key_tiles<6>(a, seq_pos(a.pos, b), t0, t1).count;
-    if (count == 0) return;
-    const int64_t item = h * plan.head[0] + plan.first[pair];
-    const int first = group_of(plan, item, groups), parts = group_of(plan, item + count - 1, groups) - first + 1;
-    if (parts == 1) return;
+    if (parts <= 1 || t0 >= t1) return;
     const int lane = threadIdx.x & 63, set = threadIdx.x >> 6, col = lane & 15, g = lane >> 4, wave = sub / NT, nt = sub % NT;
     const int r = sub * 16 + col, t = t0 + (r >> lgG);
-    auto region = [&](int part) {
-        const size_t slot = part == 0 ? 2 * first + 1 : 2 * (first + part);
-        return plan.part + (slot * kChWaves + wave) * C::PART;
-    };
-    auto sums = [&](int part) { return *reinterpret_cast<const f32x2*>(region(part) + NT * C::NDT * 256 + (nt * 64 + lane) * 2); };
     const bool ok = t < t1;
     Gate4<DT> gate[NQ];
 #pragma unroll
     for (int j = 0; j < NQ; j++) gate[j].none();
-    if (a.gate) {
+    if (a.gate && set == 0) {
 #pragma unroll
         for (int j = 0; j < NQ; j++) gate[j].load(a, (size_t)b * a.n + (ok ? t : t0), h * G + (r & (G - 1)), 16 * (quarter * NQ + j) + 4 * g);
     }
     float m = kNegInf, l = 0.f;
-#pragma unroll 8
-    for (int p = 0; p < parts; p++) m = fmaxf(m, sums(p)[0]);
     f32x4 o[NQ];
 #pragma unroll
     for (int j = 0; j < NQ; j++) o[j] = f32x4{};
-#pragma unroll 4
-    for (int p = 0; p < parts; p++) {
-        const f32x2 ml = sums(p);
-        const float w = ml[0] == kNegInf ? 0.f : exp2_fast(ml[0] - m);
-        l = __builtin_fmaf(ml[1], w, l);
-        if (p % 4 == set) {
+    constexpr int AT = 4;  // parts in flight
+    for (int p0 = set; p0 < parts; p0 += 4 * AT) {
+        f32x2 ml[AT];
+        f32x4 v[AT][NQ];
 #pragma unroll
-            for (int j = 0; j < NQ; j++) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(region(p) + ((nt * C::NDT + quarter * NQ + j) * 64 + lane) * 4);
+        for (int k = 0; k < AT; k++) {
+            const int p = min(p0 + 4 * k, parts - 1);  // (past the last one: not used)
+            const float* at = plan.part + ((size_t)(p == 0 ? 2 * first + 1 : 2 * (first + p)) * kChWaves + wave) * C::PART;
+            ml[k] = *reinterpret_cast<const f32x2*>(at + NT * C::NDT * 256 + (nt * 64 + lane) * 2);
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[j][i] = __builtin_fmaf(v[i], w, o[j][i]);
-            }
+            for (int j = 0; j < NQ; j++) v[k][j] = *reinterpret_cast<const f32x4*>(at + ((nt * C::NDT + quarter * NQ + j) * 64 + lane) * 4);
+        }
+#pragma unroll
+        for (int k = 0; k < AT; k++) {
+            if (p0 + 4 * k >= parts) break;
+            const float to = fmaxf(m, ml[k][0]);
+            const float cx = m == kNegInf ? 0.f : exp2_fast(m - to), cy = ml[k][0] == kNegInf ? 0.f : exp2_fast(ml[k][0] - to);
+            m = to, l = __builtin_fmaf(ml[k][1], cy, l * cx);
+#pragma unroll
+            for (int j = 0; j < NQ; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[j][i] = __builtin_fmaf(v[k][j][i], cy, o[j][i] * cx);
         }
     }
-    if (set > 0) {
+    red_ml[set][lane] = f32x2{m, l};
 #pragma unroll
-        for (int j = 0; j < NQ; j++) red[set - 1][j][lane] = o[j];
-    }
+    for (int j = 0; j < NQ; j++) red[set][j][lane] = o[j];
     __syncthreads();
     if (set > 0 || !ok) return;
+    float c[4], top = kNegInf;
+#pragma unroll
+    for (int k = 0; k < 4; k++) top = fmaxf(top, red_ml[k][lane][0]);
+    l = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        c[k] = red_ml[k][lane][0] == kNegInf ? 0.f : exp2_fast(red_ml[k][lane][0] - top);
+        l = __builtin_fmaf(red_ml[k][lane][1], c[k], l);
+    }
     const float inv = inverse_sum(l);
 #pragma unroll
     for (int j = 0; j < NQ; j++) {
-        o[j] += (red[0][j][lane] + red[1][j][lane]) + red[2][j][lane];
-        store_out4<DT>(a, (size_t)b * a.n + t, h * G + (r & (G - 1)), D, 16 * (quarter * NQ + j) + 4 * g, o[j], inv, gate[j]);
+        f32x4 v{};
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = __builtin_fmaf(red[k][j][lane][i], c[k], v[i]);
+        store_out4<DT>(a, (size_t)b * a.n + t, h * G + (r & (G - 1)), D, 16 * (quarter * NQ + j) + 4 * g, v, inv, gate[j]);
     }
 }
 
@@ -762,10 +813,13 @@ hipError_t go(const PagedAttendArgs& a, int n_cu, void* ws, hipStream_t s) {
     using C = ChCfg<D, DT, NT>;
     const int groups = n_cu & ~7, tok = C::ROWS / (a.NH / a.NKV);
     const int64_t pairs = (int64_t)a.n_seq * ((a.n + tok - 1) / tok), items = pairs * a.NKV;
-    const bool joined = items * 8 <= groups && pairs <= kJoinItems;
-    hipLaunchKernelGGL(k_paged_plan, dim3(1), dim3(1024), 0, s, a, ws, groups, C::PART, tok, joined);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    const bool joined = items * 8 <= groups && pairs <= kJoinPairs;
+    hipError_t e = hipSuccess;
+    if (!joined) {
+        if (pairs <= 256) hipLaunchKernelGGL((k_paged_plan<256>), dim3(1), dim3(256), 0, s, a, ws, groups, C::PART, tok);
+        else hipLaunchKernelGGL((k_paged_plan<1024>), dim3(1), dim3(1024), 0, s, a, ws, groups, C::PART, tok);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     auto kern = k_paged_chunk<D, DT, NT>;
     if ((e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS)) != hipSuccess) return e;
     hipLaunchKernelGGL(kern, dim3(groups), dim3(64 * kChWaves), C::LDS, s, a, ws, joined);
@@ -778,7 +832,7 @@ hipError_t go(const PagedAttendArgs& a, int n_cu, void* ws, hipStream_t s) {
 
 size_t paged_chunk_workspace(int D, int n_cu) {
     const size_t part = (size_t)kChWaves * (32 * D + 256) * sizeof(float);
-    return up256(2 * n_cu * part + n_cu * (sizeof(int4) + kChWaves * 2 * sizeof(int)) + (3 + n_cu + kJoinItems) * sizeof(int64_t));
+    return up256(2 * n_cu * part + n_cu * (sizeof(int4) + kChWaves * 2 * sizeof(int)) + (1 + n_cu) * sizeof(int64_t) + (1 + 2 * kJoinPairs) * sizeof(int));
 }
 
 hipError_t launch_paged_chunk(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* ws, hipStream_t s) {
