@@ -9,16 +9,18 @@ constexpr int kFewWaves = 4;                     // waves of a workgroup; each t
 constexpr int kFewUnit = kFewWaves;              // blocks of a unit of the schedule
 constexpr int few_occ(int D) { return D == 256 ? 1 : 2; }  // workgroups a CU
 
-// Workspace: [0] units a KV head, [1] units a workgroup, then every sequence's first unit; then the partial rows of
-// two segments a workgroup (its first and its last), [slot][row][D] and [slot][row] (maximum, sum).
-constexpr int kFewHead = 4;  // ints before the sequences' first units
+constexpr int kFewSpare = 3;  // units of extra length that whole parts may cost a workgroup: about what a second segment's start does
+
+// Workspace: the partial rows of two segments a workgroup (its first and its last), [slot][row][D] and [slot][row]
+// (maximum, sum), then [0] units a KV head and [1] units a workgroup (or parts a KV head, and 0), and every sequence's
+// first unit (part) and their number.
+constexpr int kFewHead = 4;  // ints before the sequences'
 
 struct FewPlan {
     int* head;
     float *o, *ml;
 };
-__host__ __device__ inline FewPlan few_plan(void* ws, int n_seq, int groups, int rows, int D) {
-    (void)n_seq;
+__host__ __device__ inline FewPlan few_plan(void* ws, int groups, int rows, int D) {
     char* p = static_cast<char*>(ws);
     FewPlan f;
     f.o = reinterpret_cast<float*>(p);
@@ -27,13 +29,33 @@ __host__ __device__ inline FewPlan few_plan(void* ws, int n_seq, int groups, int
     return f;
 }
 
+// Sums of the lanes up to each one
+__device__ __forceinline__ int scan64(int x) {
+#define QW_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false)
+    QW_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8
+    QW_STEP(0x112, 0xf);
+    QW_STEP(0x114, 0xf);
+    QW_STEP(0x118, 0xf);
+    QW_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+    QW_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef QW_STEP
+    return x;
+}
+
+// r / G for r < 32: by = 2^16 / G + 1 is off by at most 1, r by / 2^16 by at most 2^-11, and r / G is at least 2^-5 below
+// the next whole number
+struct FewHeads {
+    int G, by;
+    __device__ __forceinline__ int token(int r) const { return r * by >> 16; }
+};
+
 template <int D, int DT, int NT>
 struct FewCfg {
     static constexpr int PARTS = DT == 0 ? 2 : 1, NKS = D / 32, NDT = D / 16, ROWS = 16 * NT, BLKE = kBlk * D;
     static constexpr int Q_BYTES = PARTS * NT * NKS * 1024, KV_BYTES = kFewWaves * 2 * BLKE * 2;
-    // score factors [ROWS] and eight words of the schedule. Where queries and blocks fill the LDS, the first wave's values
-    // make room for them until the rows are laid out.
-    static constexpr int EXTRA = ROWS * 4 + 32;
+    // score factors [ROWS]. Where queries and blocks fill the LDS, the first wave's values make room for them until the
+    // rows are laid out.
+    static constexpr int EXTRA = ROWS * 4;
     static constexpr bool TIGHT = Q_BYTES + KV_BYTES + EXTRA > 160 * 1024;
     static constexpr int LDS = Q_BYTES + KV_BYTES + (TIGHT ? 0 : EXTRA);
     static_assert(NDT % kFewWaves == 0, "every wave writes as many dim tiles");
@@ -56,7 +78,7 @@ __device__ __forceinline__ void wait_lds() {
 }
 
 template <int D, int DT, int NT>
-__global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedAttendArgs a, void* ws) {
+__global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedAttendArgs a, FewHeads heads, void* ws) {
     using C = FewCfg<D, DT, NT>;
     constexpr int PARTS = C::PARTS, NKS = C::NKS, NDT = C::NDT, ROWS = C::ROWS, BLKE = C::BLKE;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -66,57 +88,69 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
     float* sm = reinterpret_cast<float*>(sq);                            // afterwards [waves][ROWS] maxima
     float* sl = sm + kFewWaves * ROWS;                                   // and sums
     float* sc = reinterpret_cast<float*>(C::TIGHT ? reinterpret_cast<unsigned char*>(kv + BLKE) : smem + C::Q_BYTES + C::KV_BYTES);
-    int* si = reinterpret_cast<int*>(sc + ROWS);                         // scan and schedule
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int G = a.NH / a.NKV, groups = gridDim.x;
-    const FewPlan plan = few_plan(ws, a.n_seq, groups, ROWS, D);
+    const int G = heads.G, groups = gridDim.x;
+    const FewPlan plan = few_plan(ws, groups, ROWS, D);
 
-    // ---- schedule: a sequence is ceil(blocks / 4) units a KV head, the units of KV head 0's sequences come first, and
-    // every workgroup takes an equal run of them. A thread sums a run of sequences, a scan places the runs.
-    const int per = (a.n_seq + 64 * kFewWaves - 1) / (64 * kFewWaves);
-    auto units = [&](int b) { return (key_tiles<5>(a, seq_pos(a.pos, b), 0, seq_len(a.lens, b, a.n)).count + kFewUnit - 1) / kFewUnit; };
-    int mine = 0;
-    for (int i = 0; i < per; i++)
-        if (tid * per + i < a.n_seq) mine += units(tid * per + i);
-    int incl = mine;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const int o = __shfl_up(incl, m, 64);
-        if (lane >= m) incl += o;
-    }
-    if (lane == 63) si[wave] = incl;
-    __syncthreads();
-    int before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kFewWaves; w++) before += w < wave ? si[w] : 0, total += si[w];
-    const int64_t all = (int64_t)total * a.NKV;
-    const int run = max(1, (int)((all + groups - 1) / groups));
-    const int64_t my0 = (int64_t)blockIdx.x * run;
-    if (blockIdx.x == 0) {  // for the kernel that joins split sequences
-        int at = before + incl - mine;
+    // ---- schedule, by every wave for itself: a sequence is ceil(blocks / 4) units a KV head, the units of KV head 0's
+    // sequences come first. Where they can be cut into no more parts than there are workgroups, none of them more than
+    // kFewSpare units longer than an equal share, a workgroup takes one part; else an equal run of units, which may end in
+    // one sequence and begin in the next. A lane holds one sequence, or a run of them. ----
+    const int per = (a.n_seq + 63) >> 6;
+    auto units = [&](int pos, int len) { return (key_tiles<5>(a, pos, 0, len).count + kFewUnit - 1) / kFewUnit; };
+    auto units_of = [&](int b) { return units(seq_pos(a.pos, b), seq_len(a.lens, b, a.n)); };
+    int lane_pos = 0, lane_len = 0, mine = 0;
+    if (per == 1) {
+        if (lane < a.n_seq) lane_pos = seq_pos(a.pos, lane), lane_len = seq_len(a.lens, lane, a.n);
+        mine = units(lane_pos, lane_len);
+    } else {
         for (int i = 0; i < per; i++)
-            if (tid * per + i < a.n_seq) plan.head[kFewHead + tid * per + i] = at, at += units(tid * per + i);
-        if (tid == 0) plan.head[0] = total, plan.head[1] = run;
+            if (lane * per + i < a.n_seq) mine += units_of(lane * per + i);
     }
-    if (my0 >= all) return;
-    int h = (int)(my0 / total), rest = (int)(my0 - (int64_t)h * total);
-    if (rest >= before + incl - mine && rest < before + incl) {  // one thread's
-        int at = before + incl - mine, i = 0;
-        for (;; i++) {
-            const int u = units(tid * per + i);
-            if (rest < at + u) break;
-            at += u;
+    int upto = scan64(mine), total = __builtin_amdgcn_readlane(upto, 63);
+    auto ratio = [](int64_t x, int y) { return x >> 31 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y); };
+    const int64_t all = (int64_t)total * a.NKV;
+    int run = max(1, (int)ratio(all + groups - 1, groups)), parts = 0;
+    if (per == 1) {
+        for (int k = 0; k <= kFewSpare; k++) {
+            const int p = (uint32_t)(mine + run + k - 1) / (uint32_t)(run + k), scan = scan64(p), sum = __builtin_amdgcn_readlane(scan, 63);
+            if (sum * a.NKV <= groups) {
+                parts = p, upto = scan, total = sum, run = 0;
+                break;
+            }
         }
-        si[kFewWaves] = tid * per + i, si[kFewWaves + 1] = rest - at;
     }
-    __syncthreads();
-    int b = __builtin_amdgcn_readfirstlane(si[kFewWaves]), u0 = __builtin_amdgcn_readfirstlane(si[kFewWaves + 1]);
-    h = __builtin_amdgcn_readfirstlane(h);
-    int left = (int)min((int64_t)run, all - my0);
+    if (blockIdx.x == 0 && wave == 0) {  // for the kernel that joins split sequences
+        int at = upto - (run ? mine : parts);
+        for (int i = 0; i < per; i++)
+            if (lane * per + i < a.n_seq) plan.head[kFewHead + lane * per + i] = at, at += per == 1 ? 0 : units_of(lane * per + i);
+        if (lane == 0) plan.head[0] = total, plan.head[1] = run, plan.head[kFewHead + a.n_seq] = total;
+    }
+    const int64_t my0 = (int64_t)blockIdx.x * max(run, 1);
+    if (my0 >= (int64_t)total * a.NKV) return;
+    int h = (int)ratio(my0, total), left = (int)min((int64_t)run, all - my0), b, u0;
+    {
+        const int rest = (int)(my0 - (int64_t)h * total), owner = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= rest));
+        const int whole = __builtin_amdgcn_readlane(mine, owner);
+        b = owner * per;
+        if (run) {
+            u0 = rest - (__builtin_amdgcn_readlane(upto, owner) - whole);
+            for (; per > 1; b++) {
+                const int u = units_of(b);
+                if (u0 < u) break;
+                u0 -= u;
+            }
+        } else {  // part `part` of `of`, the first ones a unit longer
+            const int of = __builtin_amdgcn_readlane(parts, owner), part = rest - (__builtin_amdgcn_readlane(upto, owner) - of);
+            const int each = (uint32_t)whole / (uint32_t)of, more = whole - each * of;
+            u0 = part * each + min(part, more), left = each + (part < more);
+        }
+    }
 
     for (bool first_seg = true; left > 0; first_seg = false) {
-        const int pos = seq_pos(a.pos, b), len = seq_len(a.lens, b, a.n);
+        const int pos = per == 1 ? __builtin_amdgcn_readlane(lane_pos, b) : seq_pos(a.pos, b);
+        const int len = per == 1 ? __builtin_amdgcn_readlane(lane_len, b) : seq_len(a.lens, b, a.n);
         const KeyTiles kt = key_tiles<5>(a, pos, 0, len);
         const int nu = (kt.count + kFewUnit - 1) / kFewUnit;
         if (u0 >= nu) {  // the next sequence (or KV head)
@@ -152,35 +186,32 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
                                                          i * 1024, 0, 0);
         };
         fetch_pages(0);
+
+        // ---- the rows, 256 / ROWS threads a row, pieces of 8 dims: asked for before the blocks, and laid out as operands ----
+        constexpr int TPR = 64 * kFewWaves / ROWS, PIECES = D / 8, PPT = (PIECES + TPR - 1) / TPR;
+        const int qr = tid / TPR, tl = tid % TPR;
+        float x[PPT][8];
+        {
+            const int t = heads.token(qr);
+            const size_t off = ((size_t)b * a.n + min(t, len - 1)) * a.q_stride + (size_t)(h * G + qr - t * G) * a.q_head;
+#pragma unroll
+            for (int i = 0; i < PPT; i++) load_vec<DT, 8>(a.q, off + 8 * ((tl + i * TPR) % PIECES), x[i]);
+        }
         if (!first_seg) __syncthreads();  // the last segment's readers of the LDS are done
         load(0, a.c.k, sk);
         if constexpr (!C::TIGHT) load(0, a.c.v, sv);
-
-        // ---- the rows' operands: 256 / ROWS threads a row, pieces of 8 dims ----
         {
-            constexpr int TPR = 64 * kFewWaves / ROWS, PIECES = D / 8;
-            constexpr int PPT = (PIECES + TPR - 1) / TPR;
-            const int r = tid / TPR, tl = tid % TPR, t = r / G;
-            const bool ok = t < len;
-            const size_t off = ((size_t)b * a.n + (ok ? t : 0)) * a.q_stride + (size_t)(h * G + r % G) * a.q_head;
-            float x[PPT][8], largest = 0.f;
+            const bool ok = heads.token(qr) < len;
+            float largest = 0.f;
 #pragma unroll
-            for (int i = 0; i < PPT; i++) {
-                const int pc = tl + i * TPR;
-                if (pc < PIECES && ok) {
-                    load_vec<DT, 8>(a.q, off + 8 * pc, x[i]);
-                } else {
+            for (int i = 0; i < PPT; i++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) x[i][j] = 0.f;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j++) largest = fmaxf(largest, fabsf(x[i][j]));
-            }
+                for (int j = 0; j < 8; j++) x[i][j] = ok ? x[i][j] : 0.f, largest = fmaxf(largest, fabsf(x[i][j]));
 #pragma unroll
             for (int m = 1; m < TPR; m <<= 1) largest = fmaxf(largest, __shfl_xor(largest, m, 64));
             const int sh = query_shift(largest);
             const float up = power_of_two(sh);
-            if (tl == 0) sc[r] = a.scale * power_of_two(-sh);
+            if (tl == 0) sc[qr] = a.scale * power_of_two(-sh);
 #pragma unroll
             for (int i = 0; i < PPT; i++) {
                 const int pc = tl + i * TPR;
@@ -192,7 +223,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
                     hi[j] = (f16)y;
                     if constexpr (PARTS == 2) lo[j] = (f16)(y - (float)hi[j]);
                 }
-                f16* dst = sq + (((r >> 4) * NKS + (pc >> 2)) * 64 + (pc & 3) * 16 + (r & 15)) * 8;
+                f16* dst = sq + (((qr >> 4) * NKS + (pc >> 2)) * 64 + (pc & 3) * 16 + (qr & 15)) * 8;
                 *reinterpret_cast<f16x8*>(dst) = hi;
                 if constexpr (PARTS == 2) *reinterpret_cast<f16x8*>(dst + NT * NKS * 512) = lo;
             }
@@ -209,7 +240,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
         Sight see[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int t = (nt * 16 + col) / G;
+            const int t = heads.token(nt * 16 + col);
             see[nt] = t < len ? sight(a, pos + t) : Sight{0, 0};
             m_run[nt] = kNegInf, l_run[nt] = 0.f, fac[nt] = sc[nt * 16 + col];
             asm volatile("" : "+v"(fac[nt]));
@@ -322,7 +353,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
                                 f32x4 o = acc[nt][dt];
 #pragma unroll
                                 for (int part = 0; part < PARTS; part++) o = mfma16(v, w[nt][part], o);
-                                const bool own = (nt * 16 + col) / G == t;
+                                const bool own = heads.token(nt * 16 + col) == t;
 #pragma unroll
                                 for (int i = 0; i < 4; i++) acc[nt][dt][i] = own ? o[i] : acc[nt][dt][i];
                                 __builtin_amdgcn_sched_barrier(0);
@@ -335,7 +366,19 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
             load(it + 1, a.c.v, sv);
         }
 
-        // ---- the waves' outputs against their common maximum, added through the blocks' room ----
+        // ---- the waves' outputs, through the blocks' room, added against their common maximum: a wave every fourth dim tile ----
+        constexpr int PER = NDT / kFewWaves;
+        Gate4<DT> gate[NT][PER];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int t = heads.token(nt * 16 + col);
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                gate[nt][k].none();
+                if (!split && a.gate && t < len)
+                    gate[nt][k].load(a, (size_t)b * a.n + t, h * G + nt * 16 + col - t * G, 16 * (wave + k * kFewWaves) + 4 * g);
+            }
+        }
         wait_loads<0>();  // (loads past the last block write zeros)
         __syncthreads();
 #pragma unroll
@@ -346,51 +389,34 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
             const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
             l_run[nt] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
             if (g == 0) sm[wave * ROWS + nt * 16 + col] = m_run[nt], sl[wave * ROWS + nt * 16 + col] = l_run[nt];
-        }
-        __syncthreads();
-        auto row_max = [&](int r) {
-            float m = sm[r];
 #pragma unroll
-            for (int w = 1; w < kFewWaves; w++) m = fmaxf(m, sm[w * ROWS + r]);
-            return m;
-        };
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const float corr = m_run[nt] == kNegInf ? 0.f : exp2_fast(m_run[nt] - row_max(nt * 16 + col));
-#pragma unroll
-            for (int dt = 0; dt < NDT; dt++)
-                *reinterpret_cast<f32x4*>(red + (((wave * NT + nt) * NDT + dt) * 64 + lane) * 4) = acc[nt][dt] * corr;
+            for (int dt = 0; dt < NDT; dt++) *reinterpret_cast<f32x4*>(red + (((wave * NT + nt) * NDT + dt) * 64 + lane) * 4) = acc[nt][dt];
         }
         __syncthreads();
         const int slot = 2 * blockIdx.x + (u0 == 0 ? 1 : 0);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int r = nt * 16 + col, t = r / G;
+            const int r = nt * 16 + col, t = heads.token(r);
             if (t >= len) continue;
-            const float m = row_max(r);
-            float l = 0.f;
+            float f[kFewWaves], m = kNegInf, l = 0.f;
 #pragma unroll
-            for (int w = 0; w < kFewWaves; w++)
-                l += sl[w * ROWS + r] * (sm[w * ROWS + r] == kNegInf ? 0.f : exp2_fast(sm[w * ROWS + r] - m));
+            for (int w = 0; w < kFewWaves; w++) f[w] = sm[w * ROWS + r], m = fmaxf(m, f[w]);
+#pragma unroll
+            for (int w = 0; w < kFewWaves; w++) f[w] = f[w] == kNegInf ? 0.f : exp2_fast(f[w] - m), l += sl[w * ROWS + r] * f[w];
             const float inv = inverse_sum(l);
-            constexpr int PER = (NDT + kFewWaves - 1) / kFewWaves;  // dim tiles a wave
-            Gate4<DT> gate[PER];
-#pragma unroll
-            for (int k = 0; k < PER; k++) gate[k].none();
-            if (!split && a.gate) {
-#pragma unroll
-                for (int k = 0; k < PER; k++)
-                    gate[k].load(a, (size_t)b * a.n + t, h * G + r % G, 16 * (wave + k * kFewWaves) + 4 * g);
-            }
             if (split && wave == 0 && g == 0) *reinterpret_cast<f32x2*>(plan.ml + ((size_t)slot * ROWS + r) * 2) = f32x2{m, l};
 #pragma unroll
             for (int k = 0; k < PER; k++) {
                 const int dt = wave + k * kFewWaves;
                 f32x4 o{};
 #pragma unroll
-                for (int w = 0; w < kFewWaves; w++) o += *reinterpret_cast<const f32x4*>(red + (((w * NT + nt) * NDT + dt) * 64 + lane) * 4);
+                for (int w = 0; w < kFewWaves; w++) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(red + (((w * NT + nt) * NDT + dt) * 64 + lane) * 4);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf(x[i], f[w], o[i]);
+                }
                 if (split) *reinterpret_cast<f32x4*>(plan.o + ((size_t)slot * ROWS + r) * D + 16 * dt + 4 * g) = o;
-                else store_out4<DT>(a, (size_t)b * a.n + t, h * G + r % G, D, 16 * dt + 4 * g, o, inv, gate[k]);
+                else store_out4<DT>(a, (size_t)b * a.n + t, h * G + r - t * G, D, 16 * dt + 4 * g, o, inv, gate[nt][k]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -399,63 +425,66 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
     }
 }
 
-// Joins the parts of split sequences: a workgroup a (sequence, token, head). Its first part is the last segment of one
-// workgroup of k_paged_few, the others the first segments of those after it. Fixed order.
+// Joins the parts of split sequences: a workgroup 64 dims of a (sequence, token, head), 16 lanes a part, 16 parts at a time.
+// Its first part is the last segment of one workgroup of k_paged_few, the others the first segments of those after it.
+// Every wave takes the parts' maxima and sums for itself, a lane each, so that their loads and the parts' are in flight
+// together. Fixed order.
 template <int D, int DT, int ROWS>
-__global__ __launch_bounds__(256) void k_paged_join(PagedAttendArgs a, void* ws, int groups) {
-    constexpr int LANES = D / 4, SETS = 256 / LANES;  // LANES threads x 4 dims a part, SETS parts at a time
-    __shared__ float red[SETS][D];
-    __shared__ float sw[64], sr[8];
-    const FewPlan plan = few_plan(ws, a.n_seq, groups, ROWS, D);
-    const int head = blockIdx.x % a.NH, row = blockIdx.x / a.NH, b = row / a.n, t = row - b * a.n;
-    const int len = seq_len(a.lens, b, a.n);
+__global__ __launch_bounds__(256) void k_paged_join(PagedAttendArgs a, FewHeads heads, void* ws, int groups) {
+    constexpr int SETS = 16, SLICES = D / 64;
+    __shared__ f32x4 red[4][16];
+    const FewPlan plan = few_plan(ws, groups, ROWS, D);
+    const int head = blockIdx.x / SLICES, slice = blockIdx.x % SLICES, t = blockIdx.y, b = blockIdx.z;
+    const size_t row = (size_t)b * a.n + t;
+    const int total = plan.head[0], run = plan.head[1], at0 = plan.head[kFewHead + b], at1 = plan.head[kFewHead + b + 1];
+    const int pos = seq_pos(a.pos, b), len = seq_len(a.lens, b, a.n);
     if (t >= len) return;
-    const int G = a.NH / a.NKV, h = head / G, r = t * G + head % G;
-    const int total = plan.head[0], run = plan.head[1];
-    const int nu = (key_tiles<5>(a, seq_pos(a.pos, b), 0, len).count + kFewUnit - 1) / kFewUnit;
-    const int64_t at = (int64_t)h * total + plan.head[kFewHead + b];
-    const int first = (int)(at / run), last = (int)((at + nu - 1) / run), parts = last - first + 1;
+    const int h = head / heads.G, r = t * heads.G + head - h * heads.G;
+    int64_t first = (int64_t)h * total + at0;
+    int parts = at1 - at0;
+    if (run) {
+        const int nu = (key_tiles<5>(a, pos, 0, len).count + kFewUnit - 1) / kFewUnit;
+        const int64_t last = (first + nu - 1) / run;
+        first /= run, parts = (int)(last - first) + 1;
+    }
     if (parts == 1) return;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, set = tid >> 4, d = 64 * slice + 4 * (tid & 15);
+    auto slot = [&](int part) { return (size_t)(part == 0 ? 2 * first + 1 : 2 * (first + part)) * ROWS + r; };
     Gate4<DT> gate;
     gate.none();
-    if (a.gate) gate.load(a, (size_t)row, head, 4 * (tid % LANES));
-    auto slot = [&](int part) { return (size_t)(part == 0 ? 2 * first + 1 : 2 * (first + part)) * ROWS + r; };
-    // maximum, then sums and outputs of 64 parts at a time against it
-    float m = kNegInf;
-    for (int p = tid; p < parts; p += 256) m = fmaxf(m, plan.ml[slot(p) * 2]);
-    m = max64(m);
-    if ((tid & 63) == 0) sr[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(sr[0], sr[1]), fmaxf(sr[2], sr[3]));
+    if (a.gate) gate.load(a, row, head, d);
+    float m = kNegInf, l = 0.f;
     f32x4 o{};
-    float l = 0.f;
     for (int p0 = 0; p0 < parts; p0 += 64) {
-        if (tid < 64) {
-            float w = 0.f, lw = 0.f;
-            if (p0 + tid < parts) {
-                const f32x2 v = *reinterpret_cast<const f32x2*>(plan.ml + slot(p0 + tid) * 2);
-                w = v[0] == kNegInf ? 0.f : exp2_fast(v[0] - m), lw = v[1] * w;
-            }
-            sw[tid] = w;
-            l += sum64(lw);
-        }
-        __syncthreads();
-#pragma unroll 8
-        for (int p = p0 + tid / LANES; p < min(parts, p0 + 64); p += SETS) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(plan.o + slot(p) * D + 4 * (tid % LANES));
+        const f32x2 ml = *reinterpret_cast<const f32x2*>(plan.ml + slot(min(p0 + lane, parts - 1)) * 2);
+        f32x4 x[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf(x[i], sw[p - p0], o[i]);
+        for (int k = 0; k < 4; k++) {
+            const int p = p0 + set + SETS * k;
+            x[k] = p < parts ? *reinterpret_cast<const f32x4*>(plan.o + slot(p) * D + d) : f32x4{};
         }
-        __syncthreads();
+        const float mine = p0 + lane < parts ? ml[0] : kNegInf, to = fmaxf(m, max64(mine));
+        const float w = mine == kNegInf ? 0.f : exp2_fast(mine - to), corr = m == kNegInf ? 0.f : exp2_fast(m - to);
+        m = to, l = l * corr + sum64(ml[1] * w), o *= corr;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float wk = __shfl(w, set + SETS * k, 64);
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf(x[k][i], wk, o[i]);
+        }
     }
-    if (tid == 0) sr[4] = l;
-    *reinterpret_cast<f32x4*>(&red[tid / LANES][4 * (tid % LANES)]) = o;
-    __syncthreads();
-    if (tid < LANES) {
 #pragma unroll
-        for (int s = 1; s < SETS; s++) o += *reinterpret_cast<const f32x4*>(&red[s][4 * tid]);
-        store_out4<DT>(a, (size_t)row, head, D, 4 * tid, o, inverse_sum(sr[4]), gate);
+    for (int i = 0; i < 4; i++) {  // the wave's four sets
+        const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(o[i]), __float_as_uint(o[i]), false, false);
+        const float y = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+        const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+        o[i] = __uint_as_float(z[0]) + __uint_as_float(z[1]);
+    }
+    if (lane < 16) red[tid >> 6][lane] = o;
+    __syncthreads();
+    if (tid < 16) {
+        o = red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid];
+        store_out4<DT>(a, row, head, D, d, o, inverse_sum(l), gate);
     }
 }
 
@@ -463,14 +492,15 @@ template <int D, int DT, int NT>
 hipError_t go(const PagedAttendArgs& a, int n_cu, void* ws, hipStream_t s) {
     using C = FewCfg<D, DT, NT>;
     constexpr int ROWS = C::ROWS;
-    const int groups = n_cu * few_occ(D);
+    const int groups = n_cu * few_occ(D), G = a.NH / a.NKV;
+    const FewHeads heads{G, 65536 / G + 1};
     constexpr int shm = C::LDS;
     auto kern = k_paged_few<D, DT, NT>;
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, shm);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kern, dim3(groups), dim3(64 * kFewWaves), shm, s, a, ws);
+    hipLaunchKernelGGL(kern, dim3(groups), dim3(64 * kFewWaves), shm, s, a, heads, ws);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL((k_paged_join<D, DT, ROWS>), dim3((unsigned)(a.n_seq * a.n * a.NH)), dim3(256), 0, s, a, ws, groups);
+    hipLaunchKernelGGL((k_paged_join<D, DT, ROWS>), dim3(a.NH * (D / 64), a.n, a.n_seq), dim3(256), 0, s, a, heads, ws, groups);
     return hipGetLastError();
 }
 
@@ -485,7 +515,7 @@ hipError_t go_d(const PagedAttendArgs& a, bool bf16, int n_cu, void* ws, hipStre
 
 size_t paged_few_workspace(int D, int n_cu) {
     const size_t rows = (size_t)2 * n_cu * few_occ(D) * 32;
-    return up256(rows * (D + 2) * sizeof(float) + (kFewHead + 65536) * sizeof(int));
+    return up256(rows * (D + 2) * sizeof(float) + (kFewHead + 65536 + 1) * sizeof(int));
 }
 
 hipError_t launch_paged_few(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* ws, hipStream_t s) {
