@@ -41,6 +41,9 @@ __device__ __forceinline__ KeyTiles key_tiles(const PagedAttendArgs& a, int pos,
     return k;
 }
 
+// ceil(c / r) of 0 <= c <= 2^20, 1 <= r <= 2^20 (the quotient's error is below its distance from the next whole number, 1 / 2r)
+__device__ __forceinline__ int parts_of(int c, float r) { return (int)(((float)c + r - 0.5f) * __builtin_amdgcn_rcpf(r)); }
+
 // What a token at position p sees: keys [from, end) and [0, sinks) below end
 struct Sight {
     int from, end;

@@ -45,9 +45,6 @@ __host__ __device__ inline ChPlan ch_plan(void* ws, int groups, int part_floats)
 //    items than workgroups, or where the first way's run is more than kSegment units longer.
 constexpr int kSegment = 3;
 
-// ceil(c / r) of 0 <= c <= 2^20, 1 <= r <= 2^20 (the quotient's error is below its distance from the next whole number, 1 / 2r)
-__device__ __forceinline__ int parts_of(int c, float r) { return (int)(((float)c + r - 0.5f) * __builtin_amdgcn_rcpf(r)); }
-
 // The least run in [lo, hi] whose parts fit the workgroups, hi's known to: 64 runs at a time, a lane each. count(i): tiles of pair i.
 template <typename F>
 __device__ __forceinline__ int least_run(F&& count, int pairs, int nkv, int groups, int lo, int hi, int lane) {

@@ -98,23 +98,29 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
     // kFewSpare units longer than an equal share, a workgroup takes one part; else an equal run of units, which may end in
     // one sequence and begin in the next. A lane holds one sequence, or a run of them. ----
     const int per = (a.n_seq + 63) >> 6;
+    const bool one = __builtin_expect(per == 1, true);
     auto units = [&](int pos, int len) { return (key_tiles<5>(a, pos, 0, len).count + kFewUnit - 1) / kFewUnit; };
     auto units_of = [&](int b) { return units(seq_pos(a.pos, b), seq_len(a.lens, b, a.n)); };
     int lane_pos = 0, lane_len = 0, mine = 0;
-    if (per == 1) {
-        if (lane < a.n_seq) lane_pos = seq_pos(a.pos, lane), lane_len = seq_len(a.lens, lane, a.n);
-        mine = units(lane_pos, lane_len);
+    if (one) {
+        const int at = min(lane, a.n_seq - 1);
+        lane_pos = seq_pos(a.pos, at), lane_len = seq_len(a.lens, at, a.n);
+        mine = lane < a.n_seq ? units(lane_pos, lane_len) : 0;
     } else {
+#pragma unroll 1
         for (int i = 0; i < per; i++)
             if (lane * per + i < a.n_seq) mine += units_of(lane * per + i);
     }
     int upto = scan64(mine), total = __builtin_amdgcn_readlane(upto, 63);
-    auto ratio = [](int64_t x, int y) { return x >> 31 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y); };
     const int64_t all = (int64_t)total * a.NKV;
-    int run = max(1, (int)ratio(all + groups - 1, groups)), parts = 0;
-    if (per == 1) {
+    int run, parts = 0, b, u0, left, h;
+    if (all == 0) return;  // (no sequence has new tokens: nothing is joined)
+    if (__builtin_expect(all <= 1 << 20, true)) run = max(1, parts_of((int)all, (float)groups));
+    else run = (int)((all + groups - 1) / groups);
+    if (one && run < 1 << 20) {
+#pragma unroll 1
         for (int k = 0; k <= kFewSpare; k++) {
-            const int p = (uint32_t)(mine + run + k - 1) / (uint32_t)(run + k), scan = scan64(p), sum = __builtin_amdgcn_readlane(scan, 63);
+            const int p = parts_of(mine, (float)(run + k)), scan = scan64(p), sum = __builtin_amdgcn_readlane(scan, 63);
             if (sum * a.NKV <= groups) {
                 parts = p, upto = scan, total = sum, run = 0;
                 break;
@@ -123,34 +129,38 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
     }
     if (blockIdx.x == 0 && wave == 0) {  // for the kernel that joins split sequences
         int at = upto - (run ? mine : parts);
+#pragma unroll 1
         for (int i = 0; i < per; i++)
-            if (lane * per + i < a.n_seq) plan.head[kFewHead + lane * per + i] = at, at += per == 1 ? 0 : units_of(lane * per + i);
+            if (lane * per + i < a.n_seq) plan.head[kFewHead + lane * per + i] = at, at += one ? 0 : units_of(lane * per + i);
         if (lane == 0) plan.head[0] = total, plan.head[1] = run, plan.head[kFewHead + a.n_seq] = total;
     }
-    const int64_t my0 = (int64_t)blockIdx.x * max(run, 1);
-    if (my0 >= (int64_t)total * a.NKV) return;
-    int h = (int)ratio(my0, total), left = (int)min((int64_t)run, all - my0), b, u0;
-    {
+    if (__builtin_expect(!run, true)) {  // part `part` of `of`, the first ones a unit longer
+        h = parts_of((int)blockIdx.x + 1, (float)total) - 1;
+        if (h >= a.NKV) return;
+        const int rest = (int)blockIdx.x - h * total;
+        b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= rest));
+        const int whole = __builtin_amdgcn_readlane(mine, b), of = __builtin_amdgcn_readlane(parts, b);
+        const int part = rest - (__builtin_amdgcn_readlane(upto, b) - of);
+        const int each = parts_of(whole + 1, (float)of) - 1, more = whole - each * of;
+        u0 = part * each + min(part, more), left = each + (part < more);
+    } else {
+        const int64_t my0 = (int64_t)blockIdx.x * run;
+        if (my0 >= all) return;
+        h = (int)(my0 / total), left = (int)min((int64_t)run, all - my0);
         const int rest = (int)(my0 - (int64_t)h * total), owner = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= rest));
-        const int whole = __builtin_amdgcn_readlane(mine, owner);
-        b = owner * per;
-        if (run) {
-            u0 = rest - (__builtin_amdgcn_readlane(upto, owner) - whole);
-            for (; per > 1; b++) {
-                const int u = units_of(b);
-                if (u0 < u) break;
-                u0 -= u;
-            }
-        } else {  // part `part` of `of`, the first ones a unit longer
-            const int of = __builtin_amdgcn_readlane(parts, owner), part = rest - (__builtin_amdgcn_readlane(upto, owner) - of);
-            const int each = (uint32_t)whole / (uint32_t)of, more = whole - each * of;
-            u0 = part * each + min(part, more), left = each + (part < more);
+        b = owner * per, u0 = rest - (__builtin_amdgcn_readlane(upto, owner) - __builtin_amdgcn_readlane(mine, owner));
+        for (; !one; b++) {
+            const int u = units_of(b);
+            if (u0 < u) break;
+            u0 -= u;
         }
     }
+    h = __builtin_amdgcn_readfirstlane(h), run = __builtin_amdgcn_readfirstlane(run);
+    left = __builtin_amdgcn_readfirstlane(left), u0 = __builtin_amdgcn_readfirstlane(u0);
 
     for (bool first_seg = true; left > 0; first_seg = false) {
-        const int pos = per == 1 ? __builtin_amdgcn_readlane(lane_pos, b) : seq_pos(a.pos, b);
-        const int len = per == 1 ? __builtin_amdgcn_readlane(lane_len, b) : seq_len(a.lens, b, a.n);
+        const int pos = one ? __builtin_amdgcn_readlane(lane_pos, b) : seq_pos(a.pos, b);
+        const int len = one ? __builtin_amdgcn_readlane(lane_len, b) : seq_len(a.lens, b, a.n);
         const KeyTiles kt = key_tiles<5>(a, pos, 0, len);
         const int nu = (kt.count + kFewUnit - 1) / kFewUnit;
         if (u0 >= nu) {  // the next sequence (or KV head)
