@@ -42,6 +42,20 @@ __device__ __forceinline__ int scan64(int x) {
     return x;
 }
 
+// Maximum over 8 or 16 neighbouring lanes, in each of them
+template <int N>
+__device__ __forceinline__ float max_lanes(float x) {
+    static_assert(N == 8 || N == 16, "");
+    auto with = [&](auto ctrl) {
+        x = fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), decltype(ctrl)::value, 0xF, 0xF, false)));
+    };
+    with(std::integral_constant<int, 0xB1>{});   // quad_perm 1 0 3 2
+    with(std::integral_constant<int, 0x4E>{});   // quad_perm 2 3 0 1
+    with(std::integral_constant<int, 0x141>{});  // row_half_mirror
+    if constexpr (N == 16) with(std::integral_constant<int, 0x140>{});  // row_mirror
+    return x;
+}
+
 // r / G for r < 32: by = 2^16 / G + 1 is off by at most 1, r by / 2^16 by at most 2^-11, and r / G is at least 2^-5 below
 // the next whole number
 struct FewHeads {
@@ -217,8 +231,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
             for (int i = 0; i < PPT; i++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[i][j] = ok ? x[i][j] : 0.f, largest = fmaxf(largest, fabsf(x[i][j]));
-#pragma unroll
-            for (int m = 1; m < TPR; m <<= 1) largest = fmaxf(largest, __shfl_xor(largest, m, 64));
+            largest = max_lanes<TPR>(largest);
             const int sh = query_shift(largest);
             const float up = power_of_two(sh);
             if (tl == 0) sc[qr] = a.scale * power_of_two(-sh);
