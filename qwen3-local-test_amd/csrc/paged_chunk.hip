@@ -41,9 +41,14 @@ __host__ __device__ inline ChPlan ch_plan(void* ws, int groups, int part_floats)
 // workgroup of the chunk kernel takes a run of units, in one of two ways (a segment, what a workgroup takes of an item, costs some
 // three to four units beside its own: the rows, the first copies, the partial and its joining):
 //  - items in equal parts of at most `run` units, a workgroup a part, for the least run whose parts fit the workgroups;
-//  - equal runs over all items, their ends moved by up to a twelfth to an item's edge where one is that near: where there are more
-//    items than workgroups, or where the first way's run is more than kSegment units longer.
-constexpr int kSegment = 3;
+//  - equal runs over all items, every item's first unit preceded by kSegment that stand for a segment's cost, their ends moved by up
+//    to a twelfth to an item's edge where one is that near: where there are more items than workgroups, or where the first way's run
+//    is longer by more than kUneven units. Measured on 2048 bf16 tokens behind 2048 (16 heads of 256, 128 items of 33 to 64 tiles):
+//    equal runs 131 us, with nothing for the segments 137; on 1024 fp32 tokens behind 7168 equal parts 224 us, equal runs 234.
+constexpr int kSegment = 4, kUneven = 2;
+constexpr int64_t kItem = (int64_t)1 << 42;  // sums of units (2^20 of an item) count the items (less than 2^21) from this bit on
+__device__ __forceinline__ int64_t units_of(int64_t sum) { return sum & (kItem - 1); }
+__device__ __forceinline__ int64_t costs_of(int64_t sum) { return units_of(sum) + (sum / kItem) * kSegment; }
 
 // The least run in [lo, hi] whose parts fit the workgroups, hi's known to: 64 runs at a time, a lane each. count(i): tiles of pair i.
 template <typename F>
@@ -81,7 +86,7 @@ __global__ __launch_bounds__(THREADS) void k_paged_plan(PagedAttendArgs a, void*
     int top = 0;
     for (int i = 0; i < per; i++) {
         const int pair = tid * per + i, c = pair < pairs ? tiles(pair) : 0;
-        mine += c, top = max(top, c);
+        mine += c + (c ? kItem : 0), top = max(top, c);
         if (per == 1) count[tid] = c;
     }
     for (int i = tid; i < groups * kChWaves * 2; i += THREADS) plan.cnt[i] = 0;
@@ -94,15 +99,16 @@ __global__ __launch_bounds__(THREADS) void k_paged_plan(PagedAttendArgs a, void*
     }
     if (lane == 63) sums[wave] = incl, tops[wave] = top;
     __syncthreads();
-    int64_t x = incl - mine, total = 0;
+    int64_t before = incl - mine, sum = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) x += w < wave ? sums[w] : 0, total += sums[w], top = max(top, tops[w]);
-    const int64_t all = total * a.NKV, run = max((int64_t)1, (all + groups - 1) / groups);
+    for (int w = 0; w < WAVES; w++) before += w < wave ? sums[w] : 0, sum += sums[w], top = max(top, tops[w]);
+    const int64_t total = units_of(sum), all = total * a.NKV, cost = costs_of(sum);
+    const int64_t run = max((int64_t)1, (cost * a.NKV + groups - 1) / groups);
     if (tid == 0) plan.unit[groups] = all;
 
-    if (per == 1 && pairs * a.NKV <= groups && run <= top) {
-        const int part = least_run([&](int i) { return count[i]; }, pairs, a.NKV, groups, (int)run, top, lane);
-        if (part <= run + kSegment) {
+    if (per == 1 && pairs * a.NKV <= groups && top > 0) {
+        const int part = least_run([&](int i) { return count[i]; }, pairs, a.NKV, groups, max(1, (int)((all + groups - 1) / groups)), top, lane);
+        if (part <= run + kUneven) {
             const int c = count[tid], k = parts_of(c, (float)part);
             int kincl = k;
 #pragma unroll
@@ -118,29 +124,29 @@ __global__ __launch_bounds__(THREADS) void k_paged_plan(PagedAttendArgs a, void*
             for (int h = 0; h < a.NKV; h++)
                 for (int j = 0; j < k; j++) {
                     const int w = h * parts + at + j, off = (int)((unsigned)c * (unsigned)j / (unsigned)k);  // (c j < 2^28)
-                    plan.start[w] = int4{h, tid / nqt, tid % nqt, off}, plan.unit[w] = h * total + x + off;
+                    plan.start[w] = int4{h, tid / nqt, tid % nqt, off}, plan.unit[w] = h * total + units_of(before) + off;
                 }
             for (int w = parts * a.NKV + tid; w < groups; w += THREADS) plan.start[w].x = -1, plan.unit[w] = all;
             return;
         }
     }
     for (int w = tid; w < groups; w += THREADS)
-        if (w * run >= all) plan.start[w].x = -1, plan.unit[w] = all;
+        if (w * run >= cost * a.NKV) plan.start[w].x = -1, plan.unit[w] = all;
     const int near = (int)min(run / 12, (int64_t)1 << 20);
     for (int i = 0; i < per; i++) {
         const int pair = tid * per + i;
         if (pair >= pairs) break;
         const int c = tiles(pair);
         for (int h = 0; h < a.NKV && c; h++) {
-            const int64_t g0 = h * total + x;
-            for (int64_t w = (g0 + run - 1) / run; w * run < g0 + c; w++) {
-                int off = (int)(w * run - g0);
+            const int64_t g0 = h * cost + costs_of(before);
+            for (int64_t w = (g0 + run - 1) / run; w * run < g0 + kSegment + c; w++) {
+                int off = max((int)(w * run - g0) - kSegment, 0);
                 if (off <= near) off = 0;
                 else if (c - off <= near) off = c;  // the item after this
-                plan.start[w] = int4{h, pair / nqt, pair % nqt, off}, plan.unit[w] = g0 + off;
+                plan.start[w] = int4{h, pair / nqt, pair % nqt, off}, plan.unit[w] = h * total + units_of(before) + off;
             }
         }
-        x += c;
+        before += c + (c ? kItem : 0);
     }
 }
 
