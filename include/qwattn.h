@@ -525,7 +525,7 @@ typedef struct qwattn_paged_cache {
  * to fp16, queries to q_out. fp32 arithmetic, one rounding. A position at or past n_rope is like one past the pages. */
 typedef struct qwattn_paged_append_args {
     qwattn_paged_cache cache;
-    int n_seq, n;           /* n_seq <= 65535, n_seq * n * (NH + 2 NKV) < 2^26 */
+    int n_seq, n;           /* n_seq <= 65535, n_seq * n * (NH + 2 NKV) < 2^26, n_seq * pages * page <= 2^36 */
     int dtype;              /* of q, k, v and q_out: QWATTN_F32 or QWATTN_BF16 */
     int n_rope;             /* rows of rope, where it is given */
     const int32_t* lens;    /* device [n_seq] or NULL */

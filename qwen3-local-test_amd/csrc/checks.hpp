@@ -162,6 +162,8 @@ inline int check_paged_cache(const qwattn_paged_cache& c, const qwattn_config& g
     if (c.page < 32 || c.page > 65536 || (c.page & (c.page - 1)) || c.n_pages <= 0 || c.pages <= 0 || c.pages > (1 << 26) / c.page)
         return refuse(m, QWATTN_EINVAL, "%s: page %d (a power of two, 32..65536), n_pages %d, pages %d (x page <= 2^26)", who, c.page,
                       c.n_pages, c.pages);
+    if ((int64_t)n_seq * c.pages * c.page > int64_t(1) << 36)  // the schedules' sums of key tiles fit 32 bits
+        return refuse(m, QWATTN_EINVAL, "%s: tables of %d x %d positions (n_seq x pages x page <= 2^36)", who, n_seq, c.pages * c.page);
     if ((int64_t)c.n_pages * g.n_kv_heads > INT32_MAX / (c.page / 32))  // blocks have 32-bit numbers
         return refuse(m, QWATTN_EINVAL, "%s: pools of %d pages of %d positions (pages x KV heads x page / 32 < 2^31)", who, c.n_pages, c.page);
     if (!c.k || !c.v || !c.table) return refuse(m, QWATTN_EINVAL, "%s: null pointer of the cache", who);

@@ -44,7 +44,7 @@ POOL = 10 * 32 * 2 * 64 * 2  # bytes of a pool
 BAD_CACHE = [(dict(n_seq=0), "n_seq 0"), (dict(n=0), "n 0"), (dict(n=-1), "n -1"), (dict(n_seq=70000), "65535"),
              (dict(n_seq=65535, n=1000), "2^26"), (dict(page=16), "page 16"), (dict(page=96), "page 96"), (dict(page=1 << 17), "page"),
              (dict(n_pages=0), "n_pages 0"), (dict(n_pages=(1 << 30) + 1), "2^31"), (dict(pages=0), "pages 0"), (dict(pages=1 << 22, table_stride=1 << 22), "2^26"),
-             (dict(kpool=0), "null"), (dict(vpool=0), "null"), (dict(table=0), "null"), (dict(table_stride=3), "table_stride 3"),
+             (dict(n_seq=65535, n=1, pages=1 << 16, table_stride=1 << 16), "2^36"), (dict(kpool=0), "null"), (dict(vpool=0), "null"), (dict(table=0), "null"), (dict(table_stride=3), "table_stride 3"),
              (dict(kpool=P + 8), "aligned"), (dict(table=3 * P + 2), "aligned"), (dict(vpool=P + POOL - 16), "pools overlap"),
              (dict(pos=0), "pos"), (dict(dtype=2), "dtype 2")]
 
