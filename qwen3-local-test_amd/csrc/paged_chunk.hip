@@ -27,7 +27,7 @@ struct ChPlan {
     // joined calls, instead: [0] parts a KV head, then of each (sequence, query tile) its first part and its parts
     int* joined;
 };
-constexpr int kJoinPairs = 32;  // most (sequence, query tile) pairs of a joined call
+constexpr int kJoinPairs = 64;  // most (sequence, query tile) pairs of a joined call
 __host__ __device__ inline ChPlan ch_plan(void* ws, int groups, int part_floats) {
     ChPlan p;
     p.part = static_cast<float*>(ws);
@@ -816,7 +816,10 @@ hipError_t go(const PagedAttendArgs& a, int n_cu, void* ws, hipStream_t s) {
     using C = ChCfg<D, DT, NT>;
     const int groups = n_cu & ~7, tok = C::ROWS / (a.NH / a.NKV);
     const int64_t pairs = (int64_t)a.n_seq * ((a.n + tok - 1) / tok), items = pairs * a.NKV;
-    const bool joined = items * 8 <= groups && pairs <= kJoinPairs;
+    // Few items: every workgroup finds its part by itself, and a second launch joins them many workgroups at a time. Measured on 61 fp32
+    // tokens behind 16384 (16 heads of 256, 8 items) 53 us, with the plan and the last wave to arrive as the joiner 95; 1000 bf16 tokens
+    // from the first on (64 items) 55 and 61. With more items equal parts are too uneven: 2048 behind 2048 (128 items) 142 and 129.
+    const bool joined = items * 4 <= groups && pairs <= kJoinPairs;
     hipError_t e = hipSuccess;
     if (!joined) {
         if (pairs <= 256) hipLaunchKernelGGL((k_paged_plan<256>), dim3(1), dim3(256), 0, s, a, ws, groups, C::PART, tok);
