@@ -1,4 +1,16 @@
 // Attention of chunks of new tokens (more than 32 query rows a KV head) over a paged cache, on the matrix cores.
+//
+// The one-pass softmax of paged_few.hip for items of 128 or 256 query rows (KV head x sequence x tokens), eight waves of 16 or 32 rows
+// each: scores are K Q^T, so that a lane's scores are of one row and its weights are already the second product's operand
+// (O^T = V^T W^T); rows stay in registers, blocks of keys and values pass through rings in the LDS, each read by all waves.
+//
+// Bound by the matrix cores and, as near, by the LDS: a block of 32 keys is 2048 clocks of 16x16x32 products on every SIMD
+// (256 dims; fp32 rows: two parts, half the rows) and 256 KB of the LDS for eight waves, at 128 bytes a clock 2048 as well. It
+// takes 2990 clocks (fp32) or 3250 (bf16, 32 rows a wave); with half the LDS reads an fp32 chunk took 181 us in place of 224, with half
+// the products the bf16 one 115 in place of 138, without weights 130. Measured with 16 heads over 2 KV heads of 256: 2048 bf16
+// tokens behind 2048 128 us (103 GFLOP: 0.81 PFLOP/s), 1024 fp32 behind 7168 213 us (129 GFLOP: 0.61, twice that in parts),
+// 4096 bf16 in a window of 1024 93 us (73 GFLOP: 0.78), 61 fp32 behind 16384 49 us, at a clock of 1.9 GHz.
+// An item's rows cost some 13000 clocks to begin and 10000 to 25000 to write, where all workgroups do so at once.
 #include "paged.hpp"
 
 namespace qw {
@@ -285,8 +297,8 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
             stale = __builtin_amdgcn_ballot_w64(in && !sees_whole(item_see, first_key, first_key + kBlk, a.sinks));
         };
         auto key_at = [&](int i) { return __builtin_amdgcn_readlane(first_key, i - base); };
-        // This wave's share of the copies of keys of block i + 1 (zeros without a page) into ring place (i + 1) % 4 and of values of block i
-        // into place i % 4, a kilobyte a piece (at 64 dims four waves copy keys and the others values)
+        // This wave's share of the copy of block `of`'s keys or values (zeros without a page) into ring place of % 4, a kilobyte a piece
+        // (at 64 dims four waves copy keys and the others values)
         constexpr int PIECES = D >= 128 ? D / 128 : 1;
         auto copy = [&](bool keys, int of) __attribute__((always_inline)) {
             if (D < 128 && keys != (wave < 4)) return;
