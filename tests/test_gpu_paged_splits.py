@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import paged_oracle as po
-from common import TINY, QWEN3_NEXT, D128
+from common import TINY, QWEN3_NEXT, D128, Shape
 from test_gpu_paged import BF16, DEV, EVEN, F32, MANY, NAN, Batch, attend, contexts  # noqa: F401 (contexts: a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -33,6 +33,19 @@ def test_row_counts_at_the_border_of_the_forms(contexts, s, n, dtype):  # noqa: 
     b.check(attend(contexts(s), b), left=7)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 2, 3, 20])
+@pytest.mark.parametrize("nh,nkv,d", [(32, 1, 64), (32, 2, 256), (16, 8, 128), (32, 32, 64)])
+def test_head_groups(qw, nh, nkv, d, n, dtype):
+    """Groups of 32, 16, 2 and 1 query heads to a KV head: a token's rows fill a tile, several or a part of one."""
+    s = Shape(nh, nkv, d, 0)
+    att = qw.Attention(nh, nkv, d, 0, max_ctx=64, max_tokens=8)
+    b = Batch(nh + n, s, [70, 0, 33], n, 32, dtype, lens=[n, 1, n - 1])
+    b.check(attend(att, b), left=7)
+    b.check(attend(att, b, 20, 2), 20, 2, left=7)
+    att.close()
+
+
 @pytest.mark.parametrize("s,pos,n,page,dtype,window,sinks", [
     (TINY, [20000], 1, 64, F32, 0, 0), (TINY, [20000, 40, 9000], 3, 32, BF16, 0, 0), (QWEN3_NEXT, [9000], 4, 256, F32, 0, 0),
     (D128, [12000, 31], 1, 64, BF16, 8000, 200),
@@ -47,7 +60,7 @@ def test_long_sequences(contexts, s, pos, n, page, dtype, window, sinks):  # noq
     check_tokens(b, out, {0, 1, n // 3, n // 2, n - 2, n - 1} | set(range(0, n, max(1, n // 24))), window, sinks)
 
 
-@pytest.mark.parametrize("count,n,dtype", [(64, 1, F32), (65, 1, BF16), (300, 2, F32), (300, 40, BF16), (1100, 33, F32)])
+@pytest.mark.parametrize("count,n,dtype", [(64, 1, F32), (65, 1, BF16), (300, 2, F32), (300, 40, BF16), (1100, 33, F32), (1500, 1, BF16)])
 def test_batches_of_many_sequences(contexts, count, n, dtype):  # noqa: F811
     pos = [(37 * i) % 97 for i in range(count)]
     lens = [n if i % 3 == 0 else i % (n + 1) for i in range(count)]  # none among them
@@ -112,3 +125,33 @@ def test_one_workspace_for_both_forms(contexts):  # noqa: F811
         check_all()
         run_all()
         check_all()
+
+
+@pytest.mark.parametrize("n", [1, 4, 30, 400])
+def test_a_captured_call_follows_lengths_and_tables(contexts, n):  # noqa: F811
+    """A captured call replayed as positions, lengths and the order of sequences change on the device: as the eager call."""
+    s = QWEN3_NEXT
+    att = contexts(s)
+    b = Batch(n, s, [2000, 1500, 900], n, 64, BF16, lens=[n, n, n])
+    kpool, vpool, table, pos = b.dev()
+    qg = b.qg.to(DEV)
+    ws = torch.empty(att.paged_workspace(), dtype=torch.uint8, device=DEV)
+    out = torch.full((3, n, s.NH, s.D), 7.0, dtype=BF16, device=DEV)
+    call = lambda o, w: att.paged_attend(qg[..., :s.D], kpool, vpool, table, pos, o, gate=qg[..., s.D:], lens=b.lens, workspace=w)  # noqa: E731
+    call(out, ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(out, ws)
+    for at, new, order in (([2000, 1500, 900], [n] * 3, [0, 1, 2]), ([3, 1500, 0], [n, 1, n], [0, 1, 2]), ([900, 2000, 33], [0, n, 1], [2, 0, 1]),
+                           ([1999, 70, 899], [1, n, 0], [0, 1, 2])):
+        pos.copy_(torch.tensor(at)), b.lens.copy_(torch.tensor(new)), table.copy_(b.table[order])
+        out.fill_(7.0)
+        want = out.clone()
+        g.replay()
+        call(want, None)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        b2 = Batch(n, s, [2000, 1500, 900], n, 64, BF16, lens=[n, n, n])
+        b2.pos, b2.new, b2.table = at, new, b.table[order]
+        check_tokens(b2, out, {0, n - 1})
