@@ -17,9 +17,10 @@ __device__ __forceinline__ int64_t paged_block_at(const PagedCache& c, int b, in
 }
 
 // ---- append --------------------------------------------------------------------------------------------------
-// The arithmetic and lane layout of k_qk_norm_rope (norm_rope.hip): a half-wave a (token, head) row, D / 32 dims a
-// lane; values by lanes of their own that turn 8 positions x 8 dims into the blocks' 16-byte pieces. Bound by memory where there
-// are many tokens: 2250 bf16 tokens of 16 heads of 256 (46.7 MB) 16.5 us, 2.8 TB/s; one token 4.2 us, a launch and its first loads.
+// y = x rsqrt(mean x^2 + eps) (1 + w), rotated, in the lane layout of k_qk_norm_rope (norm_rope.hip): a half-wave a (token, head) row,
+// D / 32 dims a lane, some heads one after the other; values by lanes of their own that turn 8 positions x 8 dims into the blocks'
+// 16-byte pieces. Bound by memory where there are many tokens (2250 bf16 tokens of 16 + 2 heads of 256, 46.7 MB: 13.8 us, 3.4 TB/s; 8192
+// fp32 at 4.7), by a launch and its chain of loads (position, page) where there are few: one token 3.9 us.
 
 // 8-position groups that a sequence's new tokens can touch, whatever its first position
 __host__ __device__ constexpr int paged_groups(int n) { return (n + 6) / 8 + 1; }
@@ -63,12 +64,13 @@ __device__ __forceinline__ void paged_v_copy(const PagedAppendArgs& a, int64_t v
     }
 }
 
-template <int D, int DT>
+// PER heads of a token a half-wave: their rows are on their way together, and position, page and rotation are looked up once
+template <int D, int DT, int PER>
 __global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs a) {
     constexpr int DPL = D / 32;
     const int hl = threadIdx.x & 31;
-    const int q_heads = a.q ? a.NH : 0, heads = q_heads + a.NKV;
-    const int n_items = a.n_seq * a.n * heads;
+    const int q_heads = a.q ? a.NH : 0, heads = q_heads + a.NKV, sets = (heads + PER - 1) / PER;
+    const int n_items = a.n_seq * a.n * sets;
     const int norm_blocks = (n_items + 7) / 8;
     if ((int)blockIdx.x >= norm_blocks) {
         paged_v_copy<D, DT>(a, (int64_t)((int)blockIdx.x - norm_blocks) * 256 + threadIdx.x);
@@ -76,80 +78,96 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs a) {
     }
     const int item = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (item >= n_items) return;  // (whole half-waves leave, as below)
-    const int row = item / heads, hh = item - row * heads;
+    const int row = item / sets, h0 = (item - row * sets) * PER;
     const int b = row / a.n, t = row - b * a.n;
     if (t >= seq_len(a.lens, b, a.n)) return;
-    const bool is_q = hh < q_heads;
-    const int h = is_q ? hh : hh - q_heads;
     const int d0 = hl * DPL;
-    float x[DPL], w[DPL], cs[2 * DPL];
-    load_vec<DT, DPL>(is_q ? a.q : a.k, is_q ? (size_t)row * a.q_stride + (size_t)h * a.q_head + d0 : (size_t)row * a.k_stride + (size_t)h * D + d0, x);
-    const float* gamma = is_q ? a.qn : a.kn;
-    if (gamma) load_vec<0, DPL>(gamma, d0, w);
+    float x[PER][DPL], cs[2 * DPL];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int hh = min(h0 + i, heads - 1);
+        const bool is_q = hh < q_heads;
+        load_vec<DT, DPL>(is_q ? a.q : a.k, is_q ? (size_t)row * a.q_stride + (size_t)hh * a.q_head + d0
+                                                 : (size_t)row * a.k_stride + (size_t)(hh - q_heads) * D + d0, x[i]);
+    }
     const int64_t p = (int64_t)a.pos[b] + t;
     const bool there = p >= 0 && p < a.limit;
     const int half_r = a.R >> 1;
     const bool rot = d0 < a.R && there;  // DPL divides R / 2: a lane's dims are all rotated or all not
     const bool low = d0 < half_r;
     if (rot) load_vec<0, 2 * DPL>(a.rope, (size_t)p * a.R + 2 * (low ? d0 : d0 - half_r), cs);
-    if (gamma) {
-        float ss = 0.f;
-#pragma unroll
-        for (int j = 0; j < DPL; j++) ss += x[j] * x[j];
-#pragma unroll
-        for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 32);
-        const float rn = 1.0f / sqrtf(ss / (float)D + a.eps);
-#pragma unroll
-        for (int j = 0; j < DPL; j++) x[j] = x[j] * rn * (1.0f + w[j]);
-    }
     // rotate-half: the partner dim d +- R / 2 sits (R / 2) / DPL lanes away in the same half-wave
     const int offl = half_r / DPL;
     const int src = (threadIdx.x & 32) + (rot ? (low ? hl + offl : hl - offl) : hl);
 #pragma unroll
-    for (int j = 0; j < DPL; j++) {
-        const float partner = __shfl(x[j], src, 64);
-        if (rot) x[j] = low ? x[j] * cs[2 * j] - partner * cs[2 * j + 1] : x[j] * cs[2 * j] + partner * cs[2 * j + 1];
-    }
-    if (is_q) {
-        const size_t at = (size_t)row * a.q_out_stride + (size_t)h * D + d0;
+    for (int i = 0; i < PER; i++) {
+        const int hh = h0 + i;
+        if (hh >= heads) return;
+        const bool is_q = hh < q_heads;
+        const float* gamma = is_q ? a.qn : a.kn;
+        if (gamma) {
+            float w[DPL], ss = 0.f;
+            load_vec<0, DPL>(gamma, d0, w);
 #pragma unroll
-        for (int j = 0; j < DPL; j++) x[j] = there ? x[j] : 0.f;
-        if constexpr (DT == 0) {
-            typedef float vec __attribute__((ext_vector_type(DPL)));
-            vec o;
+            for (int j = 0; j < DPL; j++) ss += x[i][j] * x[i][j];
+            const float rn = 1.0f / sqrtf(sum32(ss) / (float)D + a.eps);
 #pragma unroll
-            for (int j = 0; j < DPL; j++) o[j] = x[j];
-            *reinterpret_cast<vec*>(static_cast<float*>(a.q_out) + at) = o;
-        } else {
-            typedef uint32_t vec __attribute__((ext_vector_type(DPL / 2)));
-            vec o;
-#pragma unroll
-            for (int j = 0; j < DPL; j += 2) {
-                if constexpr (DPL == 2) o = vec{pk_bf16(x[0], x[1])};
-                else o[j / 2] = pk_bf16(x[j], x[j + 1]);
-            }
-            *reinterpret_cast<vec*>(static_cast<uint16_t*>(a.q_out) + at) = o;
+            for (int j = 0; j < DPL; j++) x[i][j] = x[i][j] * rn * (1.0f + w[j]);
         }
-        return;
-    }
-    if (!there) return;
-    const int64_t blk = paged_block_at(a.c, b, (int)p, h, a.NKV, D);
-    if (blk < 0) return;
-    typedef f16 f16v __attribute__((ext_vector_type(DPL)));
-    f16v o;
 #pragma unroll
-    for (int j = 0; j < DPL; j++) o[j] = (f16)x[j];
-    *reinterpret_cast<f16v*>(reinterpret_cast<f16*>(a.c.k) + blk + k_off((int)p & (kBlk - 1), d0)) = o;
+        for (int j = 0; j < DPL; j++) {
+            const float partner = __shfl(x[i][j], src, 64);
+            if (rot) x[i][j] = low ? x[i][j] * cs[2 * j] - partner * cs[2 * j + 1] : x[i][j] * cs[2 * j] + partner * cs[2 * j + 1];
+        }
+        if (is_q) {
+            const size_t at = (size_t)row * a.q_out_stride + (size_t)hh * D + d0;
+#pragma unroll
+            for (int j = 0; j < DPL; j++) x[i][j] = there ? x[i][j] : 0.f;
+            if constexpr (DT == 0) {
+                typedef float vec __attribute__((ext_vector_type(DPL)));
+                vec o;
+#pragma unroll
+                for (int j = 0; j < DPL; j++) o[j] = x[i][j];
+                *reinterpret_cast<vec*>(static_cast<float*>(a.q_out) + at) = o;
+            } else {
+                typedef uint32_t vec __attribute__((ext_vector_type(DPL / 2)));
+                vec o;
+#pragma unroll
+                for (int j = 0; j < DPL; j += 2) {
+                    if constexpr (DPL == 2) o = vec{pk_bf16(x[i][0], x[i][1])};
+                    else o[j / 2] = pk_bf16(x[i][j], x[i][j + 1]);
+                }
+                *reinterpret_cast<vec*>(static_cast<uint16_t*>(a.q_out) + at) = o;
+            }
+            continue;
+        }
+        if (!there) return;
+        const int64_t blk = paged_block_at(a.c, b, (int)p, hh - q_heads, a.NKV, D);
+        if (blk < 0) return;
+        typedef f16 f16v __attribute__((ext_vector_type(DPL)));
+        f16v o;
+#pragma unroll
+        for (int j = 0; j < DPL; j++) o[j] = (f16)x[i][j];
+        *reinterpret_cast<f16v*>(reinterpret_cast<f16*>(a.c.k) + blk + k_off((int)p & (kBlk - 1), d0)) = o;
+    }
 }
 
+template <int D, int DT, int PER>
+hipError_t append(const PagedAppendArgs& a, hipStream_t s) {
+    const int heads = (a.q ? a.NH : 0) + a.NKV;
+    const int64_t items = (int64_t)a.n_seq * a.n * ((heads + PER - 1) / PER);
+    const int64_t v_lanes = (int64_t)a.n_seq * a.NKV * paged_groups(a.n) * (D / 8);
+    hipLaunchKernelGGL((k_paged_append<D, DT, PER>), dim3((unsigned)((items + 7) / 8 + (v_lanes + 255) / 256)), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
 template <int D>
 hipError_t append_d(const PagedAppendArgs& a, bool bf16, hipStream_t s) {
-    const int64_t items = (int64_t)a.n_seq * a.n * ((a.q ? a.NH : 0) + a.NKV);
-    const int64_t v_lanes = (int64_t)a.n_seq * a.NKV * paged_groups(a.n) * (D / 8);
-    const dim3 grid((unsigned)((items + 7) / 8 + (v_lanes + 255) / 256)), block(256);
-    if (bf16) hipLaunchKernelGGL((k_paged_append<D, 1>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_paged_append<D, 0>), grid, block, 0, s, a);
-    return hipGetLastError();
+    // Two or four heads a half-wave, kernel time in us: one fp32 token of 16 + 2 heads of 256 3.9 and 4.6, 1024 bf16 8.4 and 8.9, 2250
+    // 14.2 and 13.8, 4096 fp32 of 8 + 8 heads of 64 15.7 and 13.0, 2048 bf16 of 32 + 8 of 128 16.8 and 15.6 (with one head 3.8,
+    // 9.4, 16.6, 18.9 and 19.6)
+    const bool many = (int64_t)a.n_seq * a.n * ((a.q ? a.NH : 0) + a.NKV) > 32768;
+    if (bf16) return many ? append<D, 1, 4>(a, s) : append<D, 1, 2>(a, s);
+    return many ? append<D, 0, 4>(a, s) : append<D, 0, 2>(a, s);
 }
 
 }  // namespace

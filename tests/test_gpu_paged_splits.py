@@ -6,7 +6,8 @@ import torch
 
 import paged_oracle as po
 from common import TINY, QWEN3_NEXT, D128, Shape
-from test_gpu_paged import BF16, DEV, EVEN, F32, MANY, NAN, Batch, attend, contexts  # noqa: F401 (contexts: a fixture)
+from test_gpu_paged import (BF16, DEV, EVEN, F32, MANY, NAN, Batch, attend, check_append, contexts,  # noqa: F401 (a fixture)
+                            rope_table)
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +156,14 @@ def test_a_captured_call_follows_lengths_and_tables(contexts, n):  # noqa: F811
         b2 = Batch(n, s, [2000, 1500, 900], n, 64, BF16, lens=[n, n, n])
         b2.pos, b2.new, b2.table = at, new, b.table[order]
         check_tokens(b2, out, {0, n - 1})
+
+
+@pytest.mark.parametrize("s,n,lens,dtype", [(EVEN, 1100, [1100, 987, 0], F32), (QWEN3_NEXT, 650, [650, 1, 649], BF16), (MANY, 420, None, F32),
+                                            (Shape(4, 4, 128, 64), 1400, [1400, 1399, 5], BF16)], ids=str)
+def test_append_many_rows(contexts, s, n, lens, dtype):  # noqa: F811
+    """Chunks of so many rows that a half-wave takes several heads, head counts that do not divide among them too."""
+    b = Batch(n, s, [31, 0, 77], n, 64, dtype, lens=lens)
+    k, v, qn, kn = b.r(3, n, s.NKV, s.D).to(dtype), b.r(3, n, s.NKV, s.D).to(dtype), b.r(s.D, sd=0.2), b.r(s.D, sd=0.2)
+    rope = rope_table(s, 2048)
+    check_append(contexts(s), b, k, v, qn, kn, rope)
+    check_append(contexts(s), b, k, v, None, kn, rope, with_q=False)
