@@ -8,8 +8,8 @@
 // (256 dims; fp32 rows: two parts, half the rows) and 256 KB of the LDS for eight waves, at 128 bytes a clock 2048 as well. It
 // takes 2990 clocks (fp32) or 3250 (bf16, 32 rows a wave); with half the LDS reads an fp32 chunk took 181 us in place of 224, with half
 // the products the bf16 one 115 in place of 138, without weights 130. Measured with 16 heads over 2 KV heads of 256: 2048 bf16
-// tokens behind 2048 128 us (103 GFLOP: 0.81 PFLOP/s), 1024 fp32 behind 7168 213 us (129 GFLOP: 0.61, twice that in parts),
-// 4096 bf16 in a window of 1024 93 us (73 GFLOP: 0.78), 61 fp32 behind 16384 49 us, at a clock of 1.9 GHz.
+// tokens behind 2048 128 to 130 us (103 GFLOP: 0.8 PFLOP/s), 1024 fp32 behind 7168 213 to 227 us (129 GFLOP: 0.6, twice that
+// in parts), 4096 bf16 in a window of 1024 93 to 97 us (73 GFLOP: 0.77), 61 fp32 behind 16384 49 to 51 us, at a clock of 1.9 GHz.
 // An item's rows cost some 13000 clocks to begin and 10000 to 25000 to write, where all workgroups do so at once.
 #include "paged.hpp"
 

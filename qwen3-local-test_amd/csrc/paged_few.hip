@@ -7,7 +7,7 @@
 // Bound by memory: every page is read once, 4 D bytes a key and KV head. A wave holds one block of 32 keys and its values in
 // flight, copied straight to the LDS (128 KB a CU at 256 dims), and takes the next keys where the scores are done, the next
 // values where the weighted sums are. Measured with 16 heads over 2 KV heads of 256: 32 bf16 sequences of up to 16000 positions
-// 107 us (578 MB: 5.4 TB/s, a large copy's 5.1), 8 sequences of 4 fp32 tokens at up to 8190 28 us (2.7 TB/s), one token at 32767
+// 107 to 112 us (578 MB: 5.2 to 5.4 TB/s, a large copy's 5.1), 8 sequences of 4 fp32 tokens at up to 8190 27 us (2.8 TB/s), one token at 32767
 // 19.5 us (67 MB: 3.4 TB/s; kernel 16.7, joining 3.9), at 500 13.2 us: there the first workgroups' chain of loads (positions,
 // pages, blocks: 10000 clocks) and code that is not in the instruction cache yet. A workgroup's compute of 4 blocks takes
 // 5300 clocks, their bytes at the copy's rate 15000.
