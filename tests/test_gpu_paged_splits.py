@@ -167,3 +167,11 @@ def test_append_many_rows(contexts, s, n, lens, dtype):  # noqa: F811
     rope = rope_table(s, 2048)
     check_append(contexts(s), b, k, v, qn, kn, rope)
     check_append(contexts(s), b, k, v, None, kn, rope, with_q=False)
+
+
+@pytest.mark.parametrize("n", [1, 4, 90])
+def test_sequences_share_a_prompts_pages(contexts, n):  # noqa: F811
+    """Three sequences whose first pages are one and the same, two of them all but their last page."""
+    b = Batch(n, QWEN3_NEXT, [500, 500, 300], n, 32, F32)
+    b.table[1, :15], b.table[2, :9] = b.table[0, :15], b.table[0, :9]
+    b.check(attend(contexts(QWEN3_NEXT), b))
