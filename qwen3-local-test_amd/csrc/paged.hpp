@@ -78,11 +78,11 @@ __device__ __forceinline__ float power_of_two(int sh) { return __uint_as_float((
 // below fp16's largest, and the smallest are kept to 2^-24 of 2^kShift.
 constexpr float kShift = 8.f, kTau = 7.f;
 
-// fp16 parts of two weights: the nearest fp16, and what it leaves
-template <int PARTS>
+// fp16 parts of two weights: the nearest fp16, and what it leaves, 22 bits together. bf16 rows take both too: the values are
+// fp16 whatever the rows are, and where their weighted sum cancels, an error of 2^-12 of a term is more than a step of the output.
+constexpr int kWeightParts = 2;
 __device__ __forceinline__ void weight_parts(float w0, float w1, f16x2& hi, f16x2& lo) {
-    hi = f16x2{(f16)w0, (f16)w1};
-    if constexpr (PARTS == 2) lo = f16x2{(f16)(w0 - (float)hi[0]), (f16)(w1 - (float)hi[1])};
+    hi = f16x2{(f16)w0, (f16)w1}, lo = f16x2{(f16)(w0 - (float)hi[0]), (f16)(w1 - (float)hi[1])};
 }
 
 // ---- output rows -----------------------------------------------------------------------------------------------

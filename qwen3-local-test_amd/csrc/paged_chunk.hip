@@ -375,7 +375,7 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
         };
 
         f32x4 s[NT][2];        // scores of a block: value i of key set s of lane (col, g) is key 8 g + 4 s + i
-        f16x8 w[NT][PARTS];    // its weights: keys 8 g .. 8 g + 7
+        f16x8 w[NT][kWeightParts];  // its weights: keys 8 g .. 8 g + 7
         // Matrix instructions of a phase: the weighted values of one block, then the scores of the next, their fragments read AHEAD of
         // their use (one after the other: scores and weights are then not live together, which leaves registers for fragments)
         constexpr int AHEAD = 5;
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
                 constexpr int i = decltype(ic)::value, f = i % NDT;
                 if constexpr (i + AHEAD < 2 * NDT) read(std::integral_constant<int, i + AHEAD>{});
 #pragma unroll
-                for (int part = 0; part < PARTS; part++)
+                for (int part = 0; part < (i < NDT ? kWeightParts : PARTS); part++)
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
                         if constexpr (i < NDT) acc[nt][f] = mfma16(fr[i % (AHEAD + 1)], w[nt][part], acc[nt][f]);
@@ -428,16 +428,15 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
             m = to, l *= corr;
             return corr;
         };
-        auto weigh = [&](const f32x4 (&x)[2], float f, float m, float& l, f16x8 (&wt)[PARTS]) __attribute__((always_inline)) {
+        auto weigh = [&](const f32x4 (&x)[2], float f, float m, float& l, f16x8 (&wt)[kWeightParts]) __attribute__((always_inline)) {
             const float o = m == kNegInf ? 0.f : kShift - m;
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
                 const float x0 = exp2_fast(__builtin_fmaf(x[i >> 2][i & 3], f, o)), x1 = exp2_fast(__builtin_fmaf(x[i >> 2][(i & 3) + 1], f, o));
                 f16x2 hi16, lo16;
-                weight_parts<PARTS>(x0, x1, hi16, lo16);
-                wt[0][i] = hi16[0], wt[0][i + 1] = hi16[1];
-                if constexpr (PARTS == 2) wt[1][i] = lo16[0], wt[1][i + 1] = lo16[1], l += x0 + x1;
-                else l = __builtin_amdgcn_fdot2(hi16, f16x2{(f16)1.f, (f16)1.f}, l, false);
+                weight_parts(x0, x1, hi16, lo16);
+                wt[0][i] = hi16[0], wt[0][i + 1] = hi16[1], wt[1][i] = lo16[0], wt[1][i + 1] = lo16[1];
+                l += x0 + x1;
             }
         };
         // Weights of a block from its scores, the copies of step `step` between: a piece takes the memory path 16 cycles, and one behind
@@ -620,7 +619,7 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int part = 0; part < PARTS; part++) w[nt][part] = f16x8{};
+            for (int part = 0; part < kWeightParts; part++) w[nt][part] = f16x8{};
         bool check = false;  // the block before is not whole: its values may be some that only some rows see
         auto matrix_phase = [&](int i) __attribute__((always_inline)) {  // scores of block i, values of block i - 1
             if (check) {
@@ -708,7 +707,7 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
                     asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x[0]), "+v"(x[1]));  // (as in products())
                     hide(x, nt, k0, true);
                     const float corr = raise(largest(x) * fac[nt], m, l);
-                    f16x8 wt[PARTS];
+                    f16x8 wt[kWeightParts];
                     weigh(x, fac[nt], m, l, wt);
 #pragma unroll 1
                     for (int dt = 0; dt < NDT; dt++) {
@@ -721,7 +720,7 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
                             const f16x8 vp = keep_keys(v, [&](int j) { return sp.sees(k0 + 8 * g + j, a.sinks); });
                             f32x4 o = old;
 #pragma unroll
-                            for (int part = 0; part < PARTS; part++) o = mfma16(vp, wt[part], o);
+                            for (int part = 0; part < kWeightParts; part++) o = mfma16(vp, wt[part], o);
                             const bool its = pos + t0 + (((wave * NT + nt) * 16 + col) >> lgG) == p;
 #pragma unroll
                             for (int j = 0; j < 4; j++) sum[j] = its ? o[j] : sum[j];

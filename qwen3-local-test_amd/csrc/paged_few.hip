@@ -324,7 +324,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
                     for (int i = 0; i < 8; i++)
                         s[nt][i >> 2][i & 3] = there && see[nt].sees(k0 + 8 * g + i, a.sinks) ? s[nt][i >> 2][i & 3] : kNegInf;
             }
-            f16x8 w[NT][PARTS];
+            f16x8 w[NT][kWeightParts];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 float mx = fmaxf(fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3])),
@@ -344,10 +344,9 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
                     const float w0 = exp2_fast(__builtin_fmaf(s[nt][i >> 2][i & 3], fac[nt], off));
                     const float w1 = exp2_fast(__builtin_fmaf(s[nt][i >> 2][(i & 3) + 1], fac[nt], off));
                     f16x2 hi, lo;
-                    weight_parts<PARTS>(w0, w1, hi, lo);
-                    w[nt][0][i] = hi[0], w[nt][0][i + 1] = hi[1];
-                    if constexpr (PARTS == 2) w[nt][1][i] = lo[0], w[nt][1][i + 1] = lo[1], l_run[nt] += w0 + w1;
-                    else l_run[nt] = __builtin_amdgcn_fdot2(hi, f16x2{(f16)1.f, (f16)1.f}, l_run[nt], false);
+                    weight_parts(w0, w1, hi, lo);
+                    w[nt][0][i] = hi[0], w[nt][0][i + 1] = hi[1], w[nt][1][i] = lo[0], w[nt][1][i + 1] = lo[1];
+                    l_run[nt] += w0 + w1;
                 }
             }
             wait_loads<NDT>();  // the values are there, the next keys may be on their way
@@ -359,7 +358,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int part = 0; part < PARTS; part++) acc[nt][dt] = mfma16(v, w[nt][part], acc[nt][dt]);
+                        for (int part = 0; part < kWeightParts; part++) acc[nt][dt] = mfma16(v, w[nt][part], acc[nt][dt]);
                     if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
@@ -376,7 +375,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                            for (int part = 0; part < PARTS; part++) acc[nt][dt] = mfma16(v, w[nt][part], acc[nt][dt]);
+                            for (int part = 0; part < kWeightParts; part++) acc[nt][dt] = mfma16(v, w[nt][part], acc[nt][dt]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 } else {
@@ -390,7 +389,7 @@ __global__ __launch_bounds__(64 * kFewWaves, few_occ(D)) void k_paged_few(PagedA
                             for (int nt = 0; nt < NT; nt++) {
                                 f32x4 o = acc[nt][dt];
 #pragma unroll
-                                for (int part = 0; part < PARTS; part++) o = mfma16(v, w[nt][part], o);
+                                for (int part = 0; part < kWeightParts; part++) o = mfma16(v, w[nt][part], o);
                                 const bool own = heads.token(nt * 16 + col) == t;
 #pragma unroll
                                 for (int i = 0; i < 4; i++) acc[nt][dt][i] = own ? o[i] : acc[nt][dt][i];
