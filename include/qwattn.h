@@ -544,7 +544,7 @@ int qwattn_paged_append(qwattn_ctx* ctx, void* stream, const qwattn_paged_append
 /* Attention of the rows over their sequences' pages: out[t][h] = sum_j softmax_j(scale q[t][h] . K[j][h / G]) V[j][h / G]
  * sigmoid(gate[t][h]), G = NH / NKV, over the keys j that token t at position p sees: j <= p, and with a window only
  * j > p - window or j < sinks. The rows' own keys must be in the cache. A row that sees no key (or all of whose scores are
- * -inf) is zero. Sums, maxima and the output before its one rounding are fp32, products of fp32 accuracy for rows of
+ * -inf) is zero, whatever its gate. Sums, maxima and the output before its one rounding are fp32, products of fp32 accuracy for rows of
  * either type (weights and f32 queries in two fp16 parts, bf16 queries whole in one). Hidden keys and values, and cache memory
  * past a sequence's last row, may hold anything, infinities and NaN among it. Results do not depend on timing. */
 typedef struct qwattn_paged_attend_args {

@@ -86,8 +86,8 @@ __device__ __forceinline__ void weight_parts(float w0, float w1, f16x2& hi, f16x
 }
 
 // ---- output rows -----------------------------------------------------------------------------------------------
-// Four outputs of one row and head at dim d: o * inv, times sigmoid(gate), rounded once. The gates are loaded apart, so that
-// many loads are in flight.
+// Four outputs of one row and head at dim d: o * inv, times sigmoid(gate), rounded once; zero for a row that saw nothing (inv 0),
+// whatever its gate. The gates are loaded apart, so that many loads are in flight.
 template <int DT>
 struct Gate4 {
     typename std::conditional<DT == 0, f32x4, u32x2>::type v;
@@ -108,7 +108,7 @@ struct Gate4 {
 template <int DT>
 __device__ __forceinline__ void store_out4(const PagedAttendArgs& a, size_t row, int h, int D, int d, f32x4 o, float inv, const Gate4<DT>& g) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) o[i] *= inv * sigmoid(g.at(i));
+    for (int i = 0; i < 4; i++) o[i] = inv == 0.f ? 0.f : o[i] * (inv * sigmoid(g.at(i)));
     const size_t at = row * a.out_stride + (size_t)h * D + d;
     if constexpr (DT == 0) *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = o;
     else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at) = u32x2{pk_bf16(o[0], o[1]), pk_bf16(o[2], o[3])};
