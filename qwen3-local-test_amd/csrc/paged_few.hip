@@ -19,7 +19,8 @@ namespace {
 
 constexpr int kFewWaves = 4;                     // waves of a workgroup; each takes every fourth block of 32 keys
 constexpr int kFewUnit = kFewWaves;              // blocks of a unit of the schedule
-constexpr int few_occ(int D) { return D == 256 ? 1 : 2; }  // workgroups a CU: what the LDS holds
+constexpr int few_occ(int D) { return D == 256 ? 1 : 2; }  // workgroups a CU, at most what its LDS holds
+constexpr int kLdsBytes = 160 * 1024;                      // of a CU
 
 // Units of extra length that whole parts may cost a workgroup: about what a second segment's start does (8 us, of 3 a unit).
 // Measured with whole parts and with equal runs alone: 8 sequences of 4 fp32 tokens at up to 8190 26 and 33 us, 16 of one bf16
@@ -82,11 +83,12 @@ template <int D, int DT, int NT>
 struct FewCfg {
     static constexpr int PARTS = DT == 0 ? 2 : 1, NKS = D / 32, NDT = D / 16, ROWS = 16 * NT, BLKE = kBlk * D;
     static constexpr int Q_BYTES = PARTS * NT * NKS * 1024, KV_BYTES = kFewWaves * 2 * BLKE * 2;
-    // score factors [ROWS]. Where queries and blocks fill the LDS, the first wave's values make room for them until the
-    // rows are laid out.
+    // score factors [ROWS]. Where queries and blocks of the CU's workgroups fill the LDS, the first wave's values make room for
+    // them until the rows are laid out.
     static constexpr int EXTRA = ROWS * 4;
-    static constexpr bool TIGHT = Q_BYTES + KV_BYTES + EXTRA > 160 * 1024;
+    static constexpr bool TIGHT = few_occ(D) * (Q_BYTES + KV_BYTES + EXTRA) > kLdsBytes;
     static constexpr int LDS = Q_BYTES + KV_BYTES + (TIGHT ? 0 : EXTRA);
+    static_assert(few_occ(D) * LDS <= kLdsBytes, "the schedule's workgroups are all resident");
     static_assert(NDT % kFewWaves == 0, "every wave writes as many dim tiles");
     static_assert(2 * kFewWaves * ROWS * 4 <= Q_BYTES, "the waves' maxima and sums fit the queries' room");
     static_assert(kFewWaves * ROWS * D * 4 <= KV_BYTES, "the waves' accumulators fit the blocks' room");
