@@ -3,8 +3,9 @@ one part, parts joined by a second launch, parts joined by the wave that arrives
 import pytest
 import torch
 
+import paged_oracle as po
 from common import TINY, QWEN3_NEXT, D128
-from test_gpu_paged import BF16, F32, NAN, Batch, attend, contexts  # noqa: F401 (a fixture)
+from test_gpu_paged import BF16, EVEN, F32, NAN, Batch, attend, contexts  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +34,51 @@ def test_rows_that_see_nothing_are_zero_whatever_their_gate(contexts, s, n, pos,
         out = attend(contexts(s), c)
         assert (out[0, 0] == 0).all()
         c.check(out)
+
+
+# few tokens in one part and in several, chunks joined by a second launch and by the last wave (64 dims: copies and cleaning by half the
+# waves each)
+@pytest.mark.parametrize("bad", [NAN, float("inf"), -float("inf")], ids=["nan", "inf", "-inf"])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("s,n,pos", [(TINY, 1, 30), (TINY, 6, 3000), (TINY, 8, 40), (D128, 4, 2000), (D128, 8, 70), (TINY, 9, 70), (TINY, 90, 1000),
+                                     (D128, 70, 500), (D128, 9, 3000), (TINY, 4200, 0), (D128, 1100, 1000), (EVEN, 1100, 500)], ids=str)
+def test_values_not_finite(contexts, s, n, pos, dtype, bad):  # noqa: F811
+    """A value that is not finite, of a token of the chunk or of one before: what sees it is not finite in its dim and keeps its
+    other dims; earlier tokens keep their bits. Before a window it changes nothing at all."""
+    b = Batch(n, s, [pos, pos // 2], n, 32, dtype, lens=[n, n - n // 3])
+    clean = attend(contexts(s), b)
+    dim, rest = 3, [i for i in range(s.D) if i != 3]
+    pages = b.table[0].tolist()
+    for at in {pos + n // 2, pos + n - 1, pos // 2}:
+        was = po.rows_of(b.vpool, pages, s.D, b.vi)[at].clone()
+        row = was.clone()
+        row[:, dim] = bad
+        po.put_rows(b.vpool, pages, s.D, b.vi, [at], [row])
+        got = attend(contexts(s), b)
+        first = max(at - pos, 0)
+        assert torch.equal(got[0, :first], clean[0, :first]) and torch.equal(got[1], clean[1])
+        assert not got[0, first:, :, dim].isfinite().any()
+        # (the other dims' terms are the same, added in the same order or tile by tile)
+        err = (got[0, first:, :, rest].double() - clean[0, first:, :, rest].double()).abs()
+        assert (err <= 2 * po.HALF[dtype] * clean[0, first:, :, rest].double().abs() + (pos + n) * 2.0 ** -23 * 8).all()
+        if at < pos:
+            hidden = attend(contexts(s), b, pos - at, 0)
+            po.put_rows(b.vpool, pages, s.D, b.vi, [at], [was])
+            assert torch.equal(hidden, attend(contexts(s), b, pos - at, 0))
+        po.put_rows(b.vpool, pages, s.D, b.vi, [at], [was])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("s,n,pos", [(TINY, 1, 400), (TINY, 3, 400), (D128, 4, 400), (TINY, 70, 400), (D128, 60, 400), (EVEN, 700, 400), (D128, 1100, 200)], ids=str)
+def test_hidden_memory_may_hold_anything(contexts, s, n, pos, dtype):  # noqa: F811
+    """Keys and values that are not finite before the window and behind the last row, at every head size."""
+    window, sinks = 80, 3
+    b = Batch(n, s, [pos], n, 32, dtype)
+    clean = attend(contexts(s), b, window, sinks)
+    assert not clean.isnan().any()
+    junk = torch.tensor([NAN, float("inf"), -float("inf"), 65504.0]).repeat(s.D // 4).expand(s.NKV, s.D)
+    pages = b.table[0].tolist()
+    hidden = list(range(sinks, pos - window + 1)) + list(range(pos + n, len(pages) * 32))
+    for pool, place in ((b.kpool, b.ki), (b.vpool, b.vi)):
+        po.put_rows(pool, pages, s.D, place, hidden, [junk] * len(hidden))
+    assert torch.equal(attend(contexts(s), b, window, sinks), clean)
