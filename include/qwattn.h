@@ -552,7 +552,7 @@ typedef struct qwattn_paged_attend_args {
     int n_seq, n;           /* as for qwattn_paged_append */
     int dtype;              /* of q, gate and out */
     int window, sinks;      /* window 0: none (sinks are then not looked at); both >= 0 */
-    float scale;            /* 0: 1 / sqrt(D); else positive and finite */
+    float scale;            /* 0: 1 / sqrt(D); else positive, at most 2^126 */
     const int32_t* lens;
     const int32_t* pos;
     const void* q;          /* normalized, rotated queries (q_out), rows of heads as q above */

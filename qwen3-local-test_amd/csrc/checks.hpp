@@ -238,7 +238,9 @@ inline int check_paged_attend(const qwattn_paged_attend_args* a, const qwattn_co
     if (int rc = check_paged_cache(a->cache, g, a->n_seq, a->n, who, m)) return rc;
     if (bad_dtype(a->dtype) || a->window < 0 || a->sinks < 0)
         return refuse(m, QWATTN_EINVAL, "%s: dtype %d, window %d, sinks %d (>= 0)", who, a->dtype, a->window, a->sinks);
-    if (!(a->scale >= 0.f) || a->scale > 3.4e38f) return refuse(m, QWATTN_EINVAL, "%s: scale %g", who, (double)a->scale);
+    // (the kernels take it times log2(e))
+    if (!(a->scale >= 0.f) || a->scale > 0x1p126f)
+        return refuse(m, QWATTN_EINVAL, "%s: scale %g (0, or positive and at most 2^126)", who, (double)a->scale);
     if (!a->pos) return refuse(m, QWATTN_EINVAL, "%s: pos is null", who);
     const int D = g.head_dim;
     const int64_t rows = (int64_t)a->n_seq * a->n, size = a->dtype == QWATTN_F32 ? 4 : 2;

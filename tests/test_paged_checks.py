@@ -125,3 +125,11 @@ def test_entry_points_need_a_context(qw):
     assert lib.qwattn_paged_append(None, None, None) == EINVAL
     assert lib.qwattn_paged_attend(None, None, None) == EINVAL
     assert lib.qwattn_paged_workspace(None, None) == EINVAL
+
+
+def test_attend_refuses_scales_that_pass_fp32_in_base_2(lib, qw, shape):
+    """The kernels take the scale times log2(e): 2^126 is the largest power of two that stays finite."""
+    pack = lambda x: qw._PAGED_ATTEND.pack(*{**ATTEND, "scale": x}.values())  # noqa: E731
+    assert lib.paged_attend(pack(2.0 ** 126), ctypes.byref(shape), 4096) == 0
+    for x in (2.0 ** 126 * (1 + 2.0 ** -23), 2.5e38, 3.3e38):
+        assert lib.paged_attend(pack(x), ctypes.byref(shape), 4096) == EINVAL and "scale" in lib.paged_text().decode()
