@@ -583,7 +583,8 @@ class Attention:
             raise ValueError(f"kpool must be [n_pages, {nkv}, page * {self.D}], got {tuple(shape)}")
         _check_whole(kpool, "kpool", shape, _F16)
         _check_whole(vpool, "vpool", shape, _F16)
-        if table.dtype is not torch.int32 or len(table.shape) != 2 or table.shape[0] != n_seq or table.stride(1) != 1:
+        if (table.dtype is not torch.int32 or len(table.shape) != 2 or table.shape[0] != n_seq or
+                (table.shape[1] != 1 and table.stride(1) != 1)):
             raise ValueError(f"table must be int32 [{n_seq}, pages] with unit column stride, got {table.dtype} {tuple(table.shape)}")
         _check_whole(pos, "pos", (n_seq,), torch.int32)
         if lens is not None:

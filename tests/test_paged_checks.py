@@ -133,3 +133,12 @@ def test_attend_refuses_scales_that_pass_fp32_in_base_2(lib, qw, shape):
     assert lib.paged_attend(pack(2.0 ** 126), ctypes.byref(shape), 4096) == 0
     for x in (2.0 ** 126 * (1 + 2.0 ** -23), 2.5e38, 3.3e38):
         assert lib.paged_attend(pack(x), ctypes.byref(shape), 4096) == EINVAL and "scale" in lib.paged_text().decode()
+
+
+def test_mirror_takes_a_table_of_one_page_at_any_stride(att):
+    """(refused only for being on the CPU)"""
+    pools = dict(kpool=z(9, 2, 64 * 64, dtype=torch.float16), vpool=z(9, 2, 64 * 64, dtype=torch.float16), pos=z(2, dtype=torch.int32))
+    for table in (z(1, 2, dtype=torch.int32).t(), z(2, 6, dtype=torch.int32)[:, ::7], z(2, 1, dtype=torch.int32)):
+        assert table.shape == (2, 1)
+        with pytest.raises(ValueError, match="must be on cuda:0"):
+            att.paged_attend(z(2, 5, 8, 64), table=table, out=z(2, 5, 8, 64), **pools)
