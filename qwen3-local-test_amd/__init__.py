@@ -599,7 +599,8 @@ class Attention:
         keys normalized (kn [head_dim] as gamma - 1, None: not) and rotated to positions pos[b] + t; q [n_seq, n, heads,
         head_dim] likewise (qn) into q_out. Pools kpool, vpool float16 [n_pages, KV heads, page * head_dim] in the block
         layout (k_block, v_block), table int32 [n_seq, pages], pos int32 [n_seq]; rope [rows, rope_dim / 2, 2] (None:
-        the context's); lens [n_seq] int32 shortens sequences."""
+        the context's); lens [n_seq] int32 shortens sequences. A token at a position past the table's pages or the rope
+        rows is not appended and its query is zero."""
         if k.dtype not in _ROW_DT or len(k.shape) != 4:
             raise ValueError(f"k must be float32 or bfloat16 [n_seq, n, KV heads, head_dim], got {k.dtype} {tuple(k.shape)}")
         dtype, (n_seq, n) = k.dtype, k.shape[:2]
@@ -634,7 +635,8 @@ class Attention:
         """Causal attention of q [n_seq, n, heads, head_dim] (normalized, rotated: paged_append's q_out) over the pages of
         their sequences (as in paged_append, which must have written the rows' own keys) into out, times sigmoid(gate):
         one token a sequence, a few or a chunk. window: a token sees its last `window` positions and the first `sinks`
-        (0: all). scale 0: 1 / sqrt(head_dim). workspace: a tensor of paged_workspace() bytes (None: from torch's
+        (0: all). scale 0: 1 / sqrt(head_dim). Tokens that paged_append left out for lying past the rope rows are to be kept
+        out by `lens` or a table of no more pages than those rows have positions. workspace: a tensor of paged_workspace() bytes (None: from torch's
         allocator)."""
         if q.dtype not in _ROW_DT or len(q.shape) != 4:
             raise ValueError(f"q must be float32 or bfloat16 [n_seq, n, heads, head_dim], got {q.dtype} {tuple(q.shape)}")

@@ -5,7 +5,7 @@ import torch
 
 import paged_oracle as po
 from common import TINY, QWEN3_NEXT, D128
-from test_gpu_paged import BF16, EVEN, F32, NAN, Batch, attend, contexts  # noqa: F401 (a fixture)
+from test_gpu_paged import BF16, DEV, EVEN, F32, NAN, Batch, attend, contexts  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,36 @@ def test_hidden_memory_may_hold_anything(contexts, s, n, pos, dtype):  # noqa: F
     for pool, place in ((b.kpool, b.ki), (b.vpool, b.vi)):
         po.put_rows(pool, pages, s.D, place, hidden, [junk] * len(hidden))
     assert torch.equal(attend(contexts(s), b, window, sinks), clean)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 4, 60])
+def test_tokens_past_the_rope_table(qw, n, dtype):
+    """A sequence that reaches the end of the context's rope table, in a table whose columns are held to its positions: appended
+    and attended up to the end, zeros from there on, the memory of the wider table's pages as it was; the same by `lens`."""
+    s, end, page = TINY, 96, 32
+    att = qw.Attention(s.NH, s.NKV, s.D, s.R, s.theta, s.eps, max_ctx=end, max_tokens=64)
+    b = Batch(n, s, [end - n // 2, 17], n, page, dtype)  # (of one token the first is past the end)
+    wide = torch.cat([b.table, torch.full((2, 3), -1, dtype=torch.int32)], 1)[:, :5]
+    kpool, vpool, _, pos = b.dev()
+    table = wide.to(DEV)
+    k, v = (b.r(2, n, s.NKV, s.D).to(dtype).to(DEV) for _ in "kv")
+    qg = b.qg.to(DEV)
+    q_out, out = (torch.full((2, n, s.NH, s.D), 7.0, dtype=dtype, device=DEV) for _ in range(2))
+    before = kpool.clone(), vpool.clone()
+    att.paged_append(k, v, kpool, vpool, table, pos, q=qg[..., :s.D], q_out=q_out)
+    att.paged_attend(q_out, kpool, vpool, table[:, :end // page], pos, out, gate=qg[..., s.D:])
+    short = torch.full_like(out, 7.0)
+    lens = torch.tensor([n // 2, n], dtype=torch.int32, device=DEV)
+    att.paged_attend(q_out, kpool, vpool, table, pos, short, gate=qg[..., s.D:], lens=lens)
+    torch.cuda.synchronize()
+    assert (q_out[0, n // 2:] == 0).all() and (out[0, n // 2:] == 0).all() and (short[0, n // 2:] == 7).all()
+    for pool, was in zip((kpool, vpool), before):
+        rows, old = (po.rows_of(x.cpu(), b.table[0].tolist(), s.D, b.ki if pool is kpool else b.vi) for x in (pool, was))
+        assert torch.equal(rows[end:].view(torch.int16), old[end:].view(torch.int16))
+    b.kpool, b.vpool = kpool.cpu(), vpool.cpu()
+    b.qg[..., :s.D] = q_out.cpu()
+    b.new[0] = n // 2
+    b.check(out)
+    b.check(short, left=7)
+    att.close()
