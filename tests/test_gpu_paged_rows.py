@@ -115,3 +115,24 @@ def test_tokens_past_the_rope_table(qw, n, dtype):
     b.check(out)
     b.check(short, left=7)
     att.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("s,n,pos", [(QWEN3_NEXT, 1, 700), (D128, 5, 900), (TINY, 60, 300), (QWEN3_NEXT, 700, 100)], ids=str)
+def test_a_query_that_is_not_finite_stays_in_its_row(contexts, s, n, pos, dtype):  # noqa: F811
+    """A NaN or an infinity in one head's query of one token, and in one element of a gate: the other rows keep their bits."""
+    b = Batch(n, s, [pos], n, 32, dtype)
+    clean = attend(contexts(s), b)
+    t, h = n // 2, s.NH - 1
+    for x in (NAN, float("inf")):
+        b.qg[0, t, h, 5] = x
+        got = attend(contexts(s), b)
+        assert got[0, t, h].isnan().all()
+        got[0, t, h] = clean[0, t, h]
+        assert torch.equal(got, clean)
+    b = Batch(n, s, [pos], n, 32, dtype)
+    b.qg[0, t, h, s.D + 5] = NAN
+    got = attend(contexts(s), b)
+    assert got[0, t, h, 5].isnan()
+    got[0, t, h, 5] = clean[0, t, h, 5]
+    assert torch.equal(got, clean)
