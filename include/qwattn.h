@@ -544,13 +544,14 @@ int qwattn_paged_append(qwattn_ctx* ctx, void* stream, const qwattn_paged_append
 
 /* Attention of the rows over their sequences' pages: out[t][h] = sum_j softmax_j(scale q[t][h] . K[j][h / G]) V[j][h / G]
  * sigmoid(gate[t][h]), G = NH / NKV, over the keys j that token t at position p sees: j <= p, and with a window only
- * j > p - window or j < sinks. The rows' own keys must be in the cache: this call does not know the rope table's rows, and a token
- * that qwattn_paged_append left out for lying past them would attend to memory that nothing wrote. Such tokens are kept out by
- * `lens`, or by `pages` of no more positions than rope rows (the table's columns may be a part of wider ones): then both
- * calls write zeros. Keys that a row sees must be finite, else the rows that see them may be NaN. A row that sees no key (or all of whose scores are
- * -inf) is zero, whatever its gate. Sums, maxima and the output before its one rounding are fp32, products of fp32 accuracy for rows of
- * either type (weights and f32 queries in two fp16 parts, bf16 queries whole in one). Hidden keys and values, and cache memory
- * past a sequence's last row, may hold anything, infinities and NaN among it. Results do not depend on timing. */
+ * j > p - window or j < sinks. The rows' own keys must be in the cache: this call does not know the rope table's rows, and a
+ * token that qwattn_paged_append left out for lying past them would attend to memory that nothing wrote. Such tokens are kept
+ * out by `lens`, or by `pages` of no more positions than rope rows (the table's columns may be the first of wider ones): then
+ * both calls write zeros. Keys that a row sees must be finite, else the rows that see them may be NaN. A row that sees no key
+ * (or all of whose scores are -inf) is zero, whatever its gate. Sums, maxima and the output before its one rounding are fp32,
+ * products of fp32 accuracy for rows of either type (weights and f32 queries in two fp16 parts, bf16 queries whole in one).
+ * Hidden keys and values, and cache memory past a sequence's last row, may hold anything, infinities and NaN among it.
+ * Results do not depend on timing. */
 typedef struct qwattn_paged_attend_args {
     qwattn_paged_cache cache;
     int n_seq, n;           /* as for qwattn_paged_append */

@@ -1,6 +1,5 @@
-// Host-side checks of the linear-attention, expert and paged-attention operators' arguments (declared in
-// include/qwattn.h), apart from any GPU call so that they run on a machine without one. Each returns QWATTN_OK, or a status with its text
-// in `msg`.
+// Host-side checks of the linear-attention, expert and paged-attention operators' arguments (declared in include/qwattn.h),
+// apart from any GPU call so that they run on a machine without one. Each returns QWATTN_OK, or a status with its text in `m`.
 #pragma once
 #include <stdarg.h>
 #include <stdint.h>
@@ -165,7 +164,8 @@ inline int check_paged_cache(const qwattn_paged_cache& c, const qwattn_config& g
     if ((int64_t)n_seq * c.pages * c.page > int64_t(1) << 36)  // the schedules' sums of key tiles fit 32 bits
         return refuse(m, QWATTN_EINVAL, "%s: tables of %d x %d positions (n_seq x pages x page <= 2^36)", who, n_seq, c.pages * c.page);
     if ((int64_t)c.n_pages * g.n_kv_heads > INT32_MAX / (c.page / 32))  // blocks have 32-bit numbers
-        return refuse(m, QWATTN_EINVAL, "%s: pools of %d pages of %d positions (pages x KV heads x page / 32 < 2^31)", who, c.n_pages, c.page);
+        return refuse(m, QWATTN_EINVAL, "%s: pools of %d pages of %d positions (pages x KV heads x page / 32 < 2^31)", who, c.n_pages,
+                      c.page);
     if (!c.k || !c.v || !c.table) return refuse(m, QWATTN_EINVAL, "%s: null pointer of the cache", who);
     if (c.table_stride < c.pages || c.table_stride > (int64_t(1) << 40))
         return refuse(m, QWATTN_EINVAL, "%s: table_stride %lld (>= pages)", who, (long long)c.table_stride);
@@ -194,7 +194,7 @@ inline int check_head_rows(const HeadRows& r, int D, int64_t rows, const char* w
     return QWATTN_OK;
 }
 
-// Whether the output rows meet the input rows, head by head where both lie at one row stride
+// Whether the output rows meet the input rows, from each row's first head to its last: heads between the other's are refused too
 inline bool head_rows_meet(const HeadRows& in, const HeadRows& out, int D, int64_t rows, int64_t size) {
     return rows_meet(in.p, in.width(D) * size, in.stride * size, out.p, out.width(D) * size, out.stride * size, rows);
 }

@@ -10,7 +10,7 @@ namespace qw {
 
 namespace {
 
-// ... of position p of sequence b; -1 without a page
+// Elements before the block of KV head h that holds position p of sequence b; -1 without a page
 __device__ __forceinline__ int64_t paged_block_at(const PagedCache& c, int b, int p, int h, int nkv, int D) {
     const int32_t page = c.table[(size_t)b * c.table_stride + (p >> c.lg_page)];
     return (uint32_t)page < (uint32_t)c.n_pages ? paged_block(c, page, p, h, nkv, D) : -1;
@@ -181,8 +181,9 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, int D, bool bf16, hipSt
 size_t paged_workspace(int D, int n_cu) { return std::max(paged_few_workspace(D, n_cu), paged_chunk_workspace(D, n_cu)); }
 
 // Up to 32 query rows a KV head (two matrix tiles) keep memory busier in k_paged_few; k_paged_chunk's 128 or 256 rows of an item
-// would mostly be padding. Measured, few and chunk: one fp32 token at 32767 20 and 44 us, 8 sequences of 4 (32 rows) 26 and 40,
-// 32 of one bf16 token 109 and 182.
+// would mostly be padding. Measured, few and chunk: one fp32 token at 32767 21 and 46 us, 8 sequences of 4 (32 rows) 25 and 42,
+// 32 of one bf16 token 110 and 229; 8 of 8 fp32 tokens over 2 KV heads of 128 18 and 41, 24 of one bf16 token over 8 of 64 46 and 156.
+// The call's largest token count decides for all its sequences: the single tokens beside a chunk go through k_paged_chunk.
 hipError_t launch_paged_attend(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* workspace, hipStream_t s) {
     if (a.n * (a.NH / a.NKV) <= 32) return launch_paged_few(a, D, bf16, n_cu, workspace, s);
     return launch_paged_chunk(a, D, bf16, n_cu, workspace, s);

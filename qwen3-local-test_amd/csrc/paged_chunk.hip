@@ -1,16 +1,19 @@
 // Attention of chunks of new tokens (more than 32 query rows a KV head) over a paged cache, on the matrix cores.
 //
-// The one-pass softmax of paged_few.hip for items of 128 or 256 query rows (KV head x sequence x tokens), eight waves of 16 or 32 rows
-// each: scores are K Q^T, so that a lane's scores are of one row and its weights are already the second product's operand
+// The one-pass softmax of paged_few.hip for items of 128 or 256 query rows (KV head x sequence x tokens), eight waves of 16 or 32
+// rows each: scores are K Q^T, so that a lane's scores are of one row and its weights are already the second product's operand
 // (O^T = V^T W^T); rows stay in registers, blocks of keys and values pass through rings in the LDS, each read by all waves.
 //
-// Bound by the matrix cores and, as near, by the LDS: a block of 32 keys is 2048 clocks of 16x16x32 products on every SIMD
-// (256 dims; fp32 rows: two parts, half the rows) and 256 KB of the LDS for eight waves, at 128 bytes a clock 2048 as well. It
-// takes 2990 clocks (fp32) or 3250 (bf16, 32 rows a wave); with half the LDS reads an fp32 chunk took 181 us in place of 224, with half
-// the products the bf16 one 115 in place of 138, without weights 130. Measured with 16 heads over 2 KV heads of 256: 2048 bf16
-// tokens behind 2048 128 to 130 us (103 GFLOP: 0.8 PFLOP/s), 1024 fp32 behind 7168 213 to 227 us (129 GFLOP: 0.6, twice that
-// in parts), 4096 bf16 in a window of 1024 93 to 97 us (73 GFLOP: 0.77), 61 fp32 behind 16384 49 to 51 us, at a clock of 1.9 GHz.
-// An item's rows cost some 13000 clocks to begin and 10000 to 25000 to write, where all workgroups do so at once.
+// Bound by the matrix cores and, as near, by the LDS: a block of 32 keys is 2048 clocks of 16x16x32 products on every SIMD for
+// fp32 rows of 256 dims (16 a wave, queries and weights in two parts), 3072 for bf16 rows (32 a wave, weights in two), and 256 KB of
+// the LDS for eight waves, at 128 bytes a clock 2048. It takes 2950 clocks (fp32) or 4270 to 4750 (bf16); with half the LDS reads
+// an fp32 chunk took 181 us in place of 224. Measured with 16 heads over 2 KV heads of 256: 2048 bf16 tokens behind 2048 162 to 165 us
+// (103 GFLOP: 0.63 PFLOP/s, 0.95 in parts; weights of one part, 11 bits, took 130), 1024 fp32 behind 7168 222 to 226 us (129 GFLOP:
+// 0.58, twice that in parts), 4096 bf16 in a window of 1024 118 to 120 us (73 GFLOP: 0.62, 0.93 in parts), 61 fp32 behind 16384
+// 50 to 51 us, at a clock of 1.8 to 1.9 GHz. A segment costs some 13000 clocks to begin, a partial 12000 to 13000, an item's rows 28000
+// to 35000 where all workgroups write theirs at once, up to 64000 with a join.
+//
+// 32 bf16 rows a wave of 256 dims spill 32 registers: none in the loop over the blocks, all around the writing of the rows.
 #include "paged.hpp"
 
 namespace qw {
@@ -56,7 +59,8 @@ __host__ __device__ inline ChPlan ch_plan(void* ws, int groups, int part_floats)
 //  - equal runs over all items, every item's first unit preceded by kSegment that stand for a segment's cost, their ends moved by up
 //    to a twelfth to an item's edge where one is that near: where there are more items than workgroups, or where the first way's run
 //    is longer by more than kUneven units. Measured on 2048 bf16 tokens behind 2048 (16 heads of 256, 128 items of 33 to 64 tiles):
-//    equal runs 131 us, with nothing for the segments 137; on 1024 fp32 tokens behind 7168 equal parts 224 us, equal runs 234.
+//    equal runs 165 us, with nothing for the segments 170, with eight units each 167; 6 prompts of up to 701 bf16 tokens 56, 87 and 57;
+//    2048 bf16 of 32 + 8 heads of 128 behind 2048 173, 175 and 182. On 1024 fp32 tokens behind 7168 equal parts 224 us, equal runs 234.
 constexpr int kSegment = 4, kUneven = 2;
 constexpr int64_t kItem = (int64_t)1 << 42;  // sums of units (2^20 of an item) count the items (less than 2^21) from this bit on
 __device__ __forceinline__ int64_t units_of(int64_t sum) { return sum & (kItem - 1); }
@@ -119,7 +123,8 @@ __global__ __launch_bounds__(THREADS) void k_paged_plan(PagedAttendArgs a, void*
     if (tid == 0) plan.unit[groups] = all;
 
     if (per == 1 && pairs * a.NKV <= groups && top > 0) {
-        const int part = least_run([&](int i) { return count[i]; }, pairs, a.NKV, groups, max(1, (int)((all + groups - 1) / groups)), top, lane);
+        const int part = least_run([&](int i) { return count[i]; }, pairs, a.NKV, groups, max(1, (int)((all + groups - 1) / groups)),
+                                   top, lane);
         if (part <= run + kUneven) {
             const int c = count[tid], k = parts_of(c, (float)part);
             int kincl = k;
@@ -163,7 +168,8 @@ __global__ __launch_bounds__(THREADS) void k_paged_plan(PagedAttendArgs a, void*
 }
 
 // The first way by every wave for itself, for calls of so few items that a second launch joins them: a lane a pair, then a lane a
-// run. What part w of all is: `first_key` tile of `count` and the next part's; false behind the last part.
+// run. Part w of all is key tiles [lo, hi) of KV head h and (sequence, query tile) `pair`; false behind the last part. `out`: where
+// the joining launch finds every pair's parts.
 struct Part {
     int h, pair, lo, hi;
 };
@@ -303,13 +309,14 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
         auto copy = [&](bool keys, int of) __attribute__((always_inline)) {
             if (D < 128 && keys != (wave < 4)) return;
             const int blk = __builtin_amdgcn_readlane(number, of - base), at = D >= 128 ? wave * PIECES : wave & 3;
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((keys ? a.c.k : a.c.v) + (int64_t)max(blk, 0) * BLKE, (short)0,
-                                                                               blk < 0 ? 0 : BLKE * 2, 0x00020000);
+            uint16_t* from = (keys ? a.c.k : a.c.v) + (int64_t)max(blk, 0) * BLKE;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(from, (short)0, blk < 0 ? 0 : BLKE * 2, 0x00020000);
             f16* to = (keys ? sk : sv) + (of & (kChRing - 1)) * BLKE + at * 512;
             const int l16 = lane_here() * 16;
 #pragma unroll
             for (int k = 0; k < PIECES; k++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + k * 512), 16, l16 + (at + k) * 1024, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + k * 512), 16,
+                                                         l16 + (at + k) * 1024, 0, 0, 0);
         };
         survey(0);
 
@@ -327,7 +334,8 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
             for (int kk = 0; kk < NKS; kk++)
 #pragma unroll
                 for (int k = 0; k < RAW; k++) {
-                    if constexpr (DT == 0) raw[nt][kk][k] = *reinterpret_cast<const raw_t*>(static_cast<const float*>(a.q) + base + 32 * kk + 4 * k);
+                    if constexpr (DT == 0)
+                        raw[nt][kk][k] = *reinterpret_cast<const raw_t*>(static_cast<const float*>(a.q) + base + 32 * kk + 4 * k);
                     else raw[nt][kk][k] = *reinterpret_cast<const raw_t*>(static_cast<const uint16_t*>(a.q) + base + 32 * kk);
                 }
         }
@@ -501,12 +509,15 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
             }
             int* arrived = plan.cnt + ((wg - own) * kChWaves + wave) * 2 + nt;
             // (the last to arrive need not store its own part)
-            if (joined || __builtin_amdgcn_readfirstlane(__hip_atomic_load(arrived, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) < parts - 1) {
+            if (joined ||
+                __builtin_amdgcn_readfirstlane(__hip_atomic_load(arrived, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) < parts - 1) {
                 const __amdgpu_buffer_rsrc_t rp = region(own);
 #pragma unroll
                 for (int dt = 0; dt < NDT; dt++)
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, mine[dt * 64]), rp, ((nt * NDT + dt) * 64 + lane) * 16, 0, kScDevice);
-                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{m, l}), rp, NT * NDT * 1024 + (nt * 64 + lane) * 8, 0, kScDevice);
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, mine[dt * 64]), rp,
+                                                           ((nt * NDT + dt) * 64 + lane) * 16, 0, kScDevice);
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{m, l}), rp,
+                                                      NT * NDT * 1024 + (nt * 64 + lane) * 8, 0, kScDevice);
                 if (joined) return;
                 __builtin_amdgcn_s_waitcnt(0x0F70);  // the partial is out before it is counted
                 int old = 0;
@@ -637,7 +648,8 @@ __global__ __launch_bounds__(64 * kChWaves, 1) void k_paged_chunk(PagedAttendArg
             check = !all;
         };
         // (the values of the block before the first)
-        for (int k = wave * 64 + lane_here(); k < BLKE / 8; k += 64 * kChWaves) *reinterpret_cast<u32x4*>(sv + (kChRing - 1) * BLKE + k * 8) = u32x4{};
+        for (int k = wave * 64 + lane_here(); k < BLKE / 8; k += 64 * kChWaves)
+            *reinterpret_cast<u32x4*>(sv + (kChRing - 1) * BLKE + k * 8) = u32x4{};
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0xC07F);
         landed<C::COPIES>();
@@ -827,9 +839,10 @@ hipError_t go(const PagedAttendArgs& a, int n_cu, void* ws, hipStream_t s) {
     using C = ChCfg<D, DT, NT>;
     const int groups = n_cu & ~7, tok = C::ROWS / (a.NH / a.NKV);
     const int64_t pairs = (int64_t)a.n_seq * ((a.n + tok - 1) / tok), items = pairs * a.NKV;
-    // Few items: every workgroup finds its part by itself, and a second launch joins them many workgroups at a time. Measured on 61 fp32
-    // tokens behind 16384 (16 heads of 256, 8 items) 53 us, with the plan and the last wave to arrive as the joiner 95; 1000 bf16 tokens
-    // from the first on (64 items) 55 and 61. With more items equal parts are too uneven: 2048 behind 2048 (128 items) 142 and 129.
+    // Few items: every workgroup finds its part by itself, and a second launch joins them many workgroups at a time. Measured on 61
+    // fp32 tokens behind 16384 (16 heads of 256, 8 items) 51 us, with the plan and the last wave to arrive as the joiner 94 (bf16 55
+    // and 208); 1000 bf16 tokens from the first on (64 items) 58 and 67; 2048 bf16 of 8 + 8 heads of 64 behind 2048 58 and 61. With more
+    // items equal parts are too uneven: 2048 behind 2048 (128 items) 188 and 165.
     const bool joined = items * 4 <= groups && pairs <= kJoinPairs;
     hipError_t e = hipSuccess;
     if (!joined) {
@@ -838,7 +851,8 @@ hipError_t go(const PagedAttendArgs& a, int n_cu, void* ws, hipStream_t s) {
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     auto kern = k_paged_chunk<D, DT, NT>;
-    if ((e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS)) != hipSuccess) return e;
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kern, dim3(groups), dim3(64 * kChWaves), C::LDS, s, a, ws, joined);
     if ((e = hipGetLastError()) != hipSuccess || !joined) return e;
     hipLaunchKernelGGL((k_paged_join_chunk<D, DT, NT>), dim3((unsigned)(items * kChWaves * NT * 4)), dim3(256), 0, s, a, ws, groups);
@@ -849,7 +863,8 @@ hipError_t go(const PagedAttendArgs& a, int n_cu, void* ws, hipStream_t s) {
 
 size_t paged_chunk_workspace(int D, int n_cu) {
     const size_t part = (size_t)kChWaves * (32 * D + 256) * sizeof(float);
-    return up256(2 * n_cu * part + n_cu * (sizeof(int4) + kChWaves * 2 * sizeof(int)) + (1 + n_cu) * sizeof(int64_t) + (1 + 2 * kJoinPairs) * sizeof(int));
+    return up256(2 * n_cu * part + n_cu * (sizeof(int4) + kChWaves * 2 * sizeof(int)) + (1 + n_cu) * sizeof(int64_t) +
+                 (1 + 2 * kJoinPairs) * sizeof(int));
 }
 
 hipError_t launch_paged_chunk(const PagedAttendArgs& a, int D, bool bf16, int n_cu, void* ws, hipStream_t s) {

@@ -7,10 +7,11 @@
 // Bound by memory: every page is read once, 4 D bytes a key and KV head. A wave holds one block of 32 keys and its values in
 // flight, copied straight to the LDS (128 KB a CU at 256 dims), and takes the next keys where the scores are done, the next
 // values where the weighted sums are. Measured with 16 heads over 2 KV heads of 256: 32 bf16 sequences of up to 16000 positions
-// 107 to 112 us (578 MB: 5.2 to 5.4 TB/s, a large copy's 5.1), 8 sequences of 4 fp32 tokens at up to 8190 27 us (2.8 TB/s), one token at 32767
-// 19.5 us (67 MB: 3.4 TB/s; kernel 16.7, joining 3.9), at 500 13.2 us: there the first workgroups' chain of loads (positions,
-// pages, blocks: 10000 clocks) and code that is not in the instruction cache yet. A workgroup's compute of 4 blocks takes
-// 5300 clocks, their bytes at the copy's rate 15000.
+// 110 to 116 us (578 MB: 5.0 to 5.2 TB/s, a large copy's 5.1), 8 sequences of 4 fp32 tokens at up to 8190 27 us (2.8 TB/s), one
+// token at 32767 19.8 us (67 MB: 3.4 TB/s; kernel 17, joining 3.9), at 500 13.3 us: there the first workgroups' chain of loads
+// (positions, pages, blocks: 10000 clocks) and code that is not in the instruction cache yet. A wave's block takes some 6300
+// clocks beside its waits (one tile of rows; scores 1200 in fp32, 750 in bf16), a workgroup's four at a time; their bytes
+// at the copy's rate take 15000.
 #include "paged.hpp"
 
 namespace qw {
@@ -23,8 +24,9 @@ constexpr int few_occ(int D) { return D == 256 ? 1 : 2; }  // workgroups a CU, a
 constexpr int kLdsBytes = 160 * 1024;                      // of a CU
 
 // Units of extra length that whole parts may cost a workgroup: about what a second segment's start does (8 us, of 3 a unit).
-// Measured with whole parts and with equal runs alone: 8 sequences of 4 fp32 tokens at up to 8190 26 and 33 us, 16 of one bf16
-// token behind a window of 4096 33 and 36; 32 sequences at up to 16000 take runs (their parts would be 20% longer).
+// Measured with whole parts and with equal runs alone: 8 sequences of 4 tokens at up to 8190 25 and 31 us (bf16 26 and 30), 16 of
+// one behind a window of 4096 30 and 34; 8 of 8 fp32 tokens over 2 KV heads of 128 18 and 20, 16 of one bf16 token there 28 and
+// 30, 24 over 8 of 64 46.1 and 45.6. Many sequences of different ages take runs (their parts would be 20% longer).
 constexpr int kFewSpare = 3;
 
 // Workspace: the partial rows of two segments a workgroup (its first and its last), [slot][row][D] and [slot][row]
