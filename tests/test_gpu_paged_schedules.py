@@ -154,6 +154,7 @@ FEW = [
     ("parts of one KV head", (QWEN3_NEXT, [33000, 20011, 30000], 4, 128, 0, 0), "parts", 3),
     ("runs, uneven ages", (QWEN3_NEXT, ragged(50, 16000, 1), 1, 128, 0, 0), "runs", 16),
     ("runs of a few tokens", (MANY, ragged(60, 9000, 2), 8, 64, 0, 0), "runs", 20),
+    ("runs of two tiles of 256 dims", (QWEN3_NEXT, ragged(70, 4000, 8), 4, 32, 0, 0), "runs", 8),
     ("runs behind a window", (MANY, ragged(50, 9000, 3), 2, 32, 7000, 70), "runs", 16),
     ("more sequences than lanes", (MANY, ragged(70, 3000, 4), 1, 64, 0, 0), "runs", 10),
     ("two and three a lane", (TINY, ragged(130, 3000, 5), 3, 32, 0, 0), "runs", 3),
