@@ -6,12 +6,12 @@
 //
 // Bound by the matrix cores and, as near, by the LDS: a block of 32 keys is 2048 clocks of 16x16x32 products on every SIMD for
 // fp32 rows of 256 dims (16 a wave, queries and weights in two parts), half as many again for bf16 rows (32 a wave, weights in
-// two), and 256 KB of the LDS for eight waves, at 128 bytes a clock 2048. It takes 2950 clocks (fp32) or 4270 to 4750 (bf16); with half the LDS reads
-// an fp32 chunk took 181 us in place of 224. Measured with 16 heads over 2 KV heads of 256: 2048 bf16 tokens behind 2048 162 to 165 us
-// (103 GFLOP: 0.63 PFLOP/s, 0.95 in parts; weights of one part, 11 bits, took 130), 1024 fp32 behind 7168 222 to 226 us (129 GFLOP:
-// 0.58, twice that in parts), 4096 bf16 in a window of 1024 118 to 120 us (73 GFLOP: 0.62, 0.93 in parts), 61 fp32 behind 16384
-// 50 to 51 us, at a clock of 1.8 to 1.9 GHz. A segment costs some 13000 clocks to begin, a partial 12000 to 13000, an item's rows 28000
-// to 35000 where all workgroups write theirs at once, up to 64000 with a join.
+// two), and 256 KB of the LDS for eight waves, at 128 bytes a clock 2048. It takes 2950 clocks (fp32) or 4270 to 4750 (bf16);
+// with half the LDS reads an fp32 chunk took 181 us in place of 224. Measured with 16 heads over 2 KV heads of 256: 2048 bf16
+// tokens behind 2048 162 to 169 us (103 GFLOP: 0.63 PFLOP/s, 0.95 in parts; weights of one part, 11 bits, took 130), 1024 fp32
+// behind 7168 222 to 230 us (129 GFLOP: 0.58, twice that in parts), 4096 bf16 in a window of 1024 118 to 122 us (73 GFLOP: 0.62,
+// 0.93 in parts), 61 fp32 behind 16384 50 to 52 us, at a clock of 1.8 to 1.9 GHz. A segment costs some 13000 clocks to begin, a
+// partial 12000 to 13000, an item's rows 28000 to 35000 where all workgroups write theirs at once, up to 64000 with a join.
 //
 // 32 bf16 rows a wave of 256 dims spill 32 registers: none in the loop over the blocks, all around the writing of the rows.
 #include "paged.hpp"
